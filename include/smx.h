@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define SMX_ABI_VERSION 11
+#define SMX_ABI_VERSION 12
 
 /* Return codes besides 0 and hipError_t values. */
 #define SMX_EINVAL 10001      /* an argument failed validation */
@@ -413,6 +413,114 @@ int smx_compute_slot_mapping(void* stream, const int32_t* query_start_loc, int32
                              const int64_t* positions, const int32_t* block_table,
                              int64_t* slot_mapping, int32_t num_tokens, int32_t max_tokens,
                              int32_t max_blocks, int32_t block_size);
+
+/*
+ * Causal attention of packed query rows over the paged cache: whole prompts,
+ * chunks behind a context, or a few drafted tokens a sequence.
+ *   q: [num_tokens, n_q, head_dim] bf16, q_stride elements from a token to the
+ *      next (a slice of a wider row is fine; heads are contiguous)
+ *   query_start_loc: [num_seqs + 1] int32, non-decreasing: sequence r's query
+ *      tokens are the rows query_start_loc[r] .. query_start_loc[r + 1] - 1
+ *      (entries past num_tokens count as num_tokens)
+ *   seq_lens: [num_seqs] int32, L_r = min(seq_lens[r], max_blocks *
+ *      block_size); the query tokens are the last n_r of the L_r tokens, whose
+ *      K and V are in the cache, so token i of them is at position
+ *      L_r - n_r + i and sees the tokens 0 .. that position
+ *   out: [num_tokens, n_q, head_dim] bf16 = RNE_bf16(softmax(scale q.k) v); 0
+ *      for a token that sees none (L_r < n_r); rows of no sequence are left
+ *      as they are.
+ * Scores, maxima and sums in fp32; probabilities are rounded to bf16 before
+ * they multiply V, the sum uses the unrounded values.  What a row does not see
+ * does not reach it, infinities and NaN included.  A block-table entry outside
+ * [0, num_blocks) is never dereferenced: the rows that see its tokens are NaN.
+ * head_dim 64 or 128, n_q a multiple of n_kv, block_size a power of two in
+ * [32, 4096]; q, caches and out 16-byte aligned, q_stride a multiple of 8.
+ * Where rows are too few to fill the chip the tokens are split over workgroups
+ * and merged by a second launch: workspace holds
+ * smx_prompt_attention_workspace(...) bytes (16-byte aligned; 0: none needed;
+ * -1: bad sizes).  Calls that can run at the same time need workspaces of their
+ * own.  Counterpart of the attention the reference leaves to vLLM's stock
+ * layer for x.shape[0] != 1 (src/spark_vllm_ascend/integration/model.py:50-61).
+ */
+int64_t smx_prompt_attention_workspace(int32_t num_tokens, int32_t num_seqs, int32_t max_blocks,
+                                       int32_t block_size, int32_t n_q, int32_t n_kv,
+                                       int32_t head_dim);
+int smx_prompt_attention(void* stream, const void* q, int64_t q_stride, const void* k_cache,
+                         const void* v_cache, const int32_t* block_table,
+                         const int32_t* query_start_loc, const int32_t* seq_lens,
+                         void* workspace, int64_t workspace_bytes, void* out, int32_t num_tokens,
+                         int32_t num_seqs, int32_t max_blocks, int32_t num_blocks,
+                         int32_t block_size, int32_t n_q, int32_t n_kv, int32_t head_dim,
+                         float scale);
+
+/*
+ * Decode attention (one token a sequence) of a batch whose sequences share
+ * their first P = min(prefix_len[0], prefix_blocks * block_size) tokens, whose
+ * K and V are read once for all of them:
+ *   prefix_table: [prefix_blocks] int32, the pages of tokens 0 .. P - 1
+ *   prefix_len: [1] int32, any length (its end may be inside a page)
+ *   block_table: [num_seqs, max_blocks] int32 by absolute position; entries
+ *      of tokens below P are not used
+ *   seq_lens: [num_seqs] int32, the whole length, prefix included: row r sees
+ *      the prefix's tokens below min(P, L_r) and its own tokens P .. L_r - 1
+ * q, out, rounding, invalid pages and limits as smx_prompt_attention (out is 0
+ * for seq_lens[r] <= 0).  workspace: smx_shared_prefix_attention_workspace
+ * bytes, always needed (two launches: partials, merge).  No counterpart in
+ * the reference, which decodes one sequence.
+ */
+int64_t smx_shared_prefix_attention_workspace(int32_t num_seqs, int32_t prefix_blocks,
+                                              int32_t max_blocks, int32_t block_size, int32_t n_q,
+                                              int32_t n_kv, int32_t head_dim);
+int smx_shared_prefix_attention(void* stream, const void* q, int64_t q_stride,
+                                const void* k_cache, const void* v_cache,
+                                const int32_t* prefix_table, const int32_t* prefix_len,
+                                const int32_t* block_table, const int32_t* seq_lens,
+                                void* workspace, int64_t workspace_bytes, void* out,
+                                int32_t num_seqs, int32_t prefix_blocks, int32_t max_blocks,
+                                int32_t num_blocks, int32_t block_size, int32_t n_q, int32_t n_kv,
+                                int32_t head_dim, float scale);
+
+/*
+ * Block tables, slots, positions and offsets of a step from request lengths
+ * on the device.  Request r has context_lens[r] tokens in the cache,
+ * num_pages[r] pages in its block-table row, and gets query_lens[r] more tokens
+ * (negative values count as 0).  It takes
+ *   need[r] = max(0, min(ceil((context + query) / block_size), max_blocks) - num_pages)
+ * pages in request order from the end of the free list free_pages[0 ..
+ * free_count[0] - 1] (num_free: its capacity): block num_pages[r] + j gets
+ * free_pages[free_count[0] - 1 - sum(need[0 .. r - 1]) - j], -1 once the list
+ * is used up.  Written:
+ *   block_table [num_reqs, max_blocks]: the entries of the pages taken (others
+ *      are left as they are); num_pages_out, free_count_out[0] (may be
+ *      num_pages and free_count): the pages each request then has, those left
+ *   query_start_loc [num_reqs + 1]: prefix sums of the query lengths;
+ *   seq_lens [num_reqs]: context + query (both stop at INT32_MAX; not in place)
+ *   positions, slot_mapping [max_tokens] int64: of query token j, the
+ *      (j - query_start_loc[r])-th of its request r, context_lens[r] + that,
+ *      and its slot page * block_size + position % block_size (-1 without a
+ *      page); past the last token 0 and -1.
+ * block_size a power of two up to 4096; num_reqs * max_blocks < 2^31.  The
+ * device-side form of the block manager's tables and of _slot_one / slot4_kernel
+ * (src/spark_vllm_ascend/integration/slot_mapping.py:8-33).
+ */
+int smx_request_tables(void* stream, const int32_t* query_lens, const int32_t* context_lens,
+                       const int32_t* num_pages, const int32_t* free_pages,
+                       const int32_t* free_count, int32_t* block_table, int32_t* num_pages_out,
+                       int32_t* free_count_out, int32_t* query_start_loc, int32_t* seq_lens,
+                       int64_t* positions, int64_t* slot_mapping, int32_t num_reqs,
+                       int32_t max_tokens, int32_t max_blocks, int32_t num_free,
+                       int32_t block_size);
+
+/*
+ * Gives pages back: request r keeps those of its first keep_lens[r] tokens (0:
+ * none), the others are appended to the free list in request and block order
+ * (what exceeds its capacity num_free is dropped), their table entries become
+ * -1, and num_pages and free_count are updated in place.
+ */
+int smx_release_pages(void* stream, const int32_t* keep_lens, int32_t* num_pages,
+                      int32_t* free_pages, int32_t* free_count, int32_t* block_table,
+                      int32_t num_reqs, int32_t max_blocks, int32_t num_free,
+                      int32_t block_size);
 
 /*
  * Q4_0 GEMM for m <= 16 activation rows (batched decode): y[m, n] = x[m, k]

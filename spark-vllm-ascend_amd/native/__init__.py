@@ -29,7 +29,7 @@ DEFAULT_RECORD = LIB_PATH.with_name("libsmx.validation.json")
 #: benchmark and the build check do (they are what validates and measures the
 #: library as built); a record named by SMX_VALIDATION_RECORD is still checked
 UNVALIDATED_ENV = "SMX_ALLOW_UNVALIDATED"
-ABI_VERSION = 11
+ABI_VERSION = 12
 SMX_EINVAL = 10001
 SMX_EUNSUPPORTED = 10002
 
@@ -62,6 +62,13 @@ SIGNATURES = {
     "smx_qknorm_rope_splitkv_decode_planned_merged": [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P,
                                                       _P, _I32, _I32, _I32, _I32, _I32, _I32,
                                                       _I32, _I32, _I32, _I32, _F32, _F32],
+    "smx_prompt_attention_workspace": [_I32] * 7,
+    "smx_prompt_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _P] + [_I32] * 8 + [_F32],
+    "smx_shared_prefix_attention_workspace": [_I32] * 7,
+    "smx_shared_prefix_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _P]
+                                   + [_I32] * 8 + [_F32],
+    "smx_request_tables": [_P] * 13 + [_I32] * 5,
+    "smx_release_pages": [_P] * 6 + [_I32] * 4,
     "smx_q4_0_gemm": [_P, _P, _P, _P, _I64, _I64, _I64],
     "smx_q4_0_gemm_rows": [_P, _P, _P, _P, _I64, _I64, _I64],
     "smx_q4_0_gemm_rows_preferred": [_I64, _I64, _I64],
@@ -111,6 +118,8 @@ RUNNER_FENCES_ACQUIRE_ONLY = 1
 
 # return types other than int
 RESTYPES = {"smx_argmax_parts": ctypes.c_int64,
+            "smx_prompt_attention_workspace": ctypes.c_int64,
+            "smx_shared_prefix_attention_workspace": ctypes.c_int64,
             "smx_q4_0_argmax_keys_size": ctypes.c_int64,
             "smx_q4_0_gemm_keys_per_row": ctypes.c_int64,
             "smx_q4_0_packed_bytes": ctypes.c_int64,

@@ -1,0 +1,759 @@
+// Attention of several query rows per sequence over the paged bf16 KV cache,
+// for gfx950: packed causal prompts (whole prompts, chunks behind a context,
+// drafted tokens) and decode batches whose sequences share a prefix.
+//
+// A query row is one (token, q head); the rows of one kv head read the same K
+// and V, so a workgroup takes 32 WM of them ("row = token * group + head in
+// the group") against one range of tokens.  With p = softmax of the scores a
+// row sees (token t is seen iff from <= t < the row's limit),
+//   S^T = K Q^T     v_mfma_f32_32x32x16_bf16, A = 32 tokens of K, B = 32 rows
+//   O^T = V^T P^T   the same instruction, A = 32 dims of V, B = P of 16 tokens
+// one online softmax a row: running maximum m and sum l in fp32, P rounded to
+// bf16 for the second product (the sum keeps the unrounded values, as split-KV
+// decode does).  Transposed products keep a row's scores in one lane pair: lane
+// 32 h + n holds row n's scores of tokens 8 a + 4 h + b (a, b < 4) of every 32,
+// so the maximum and the sum are in-lane but for one lane swap, and the B
+// operand of the second product is those registers as they stand, with V's
+// token order permuted to match: its A operand is two transposing LDS reads
+// (ds_read_b64_tr_b16) of 4 tokens each.
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "smx_common.h"
+#include "smx_launch.h"
+
+namespace smx {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(1))) const void global_void;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// (lo, hi) as one v_cvt_pk_bf16_f32
+__device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
+}
+
+// A dword of two bf16 values with those that are infinite or NaN replaced by 0.
+__device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
+  if ((w & 0x7f80u) == 0x7f80u) w &= 0xffff0000u;
+  if ((w & 0x7f800000u) == 0x7f800000u) w &= 0x0000ffffu;
+  return w;
+}
+
+struct RowsArgs {
+  const uint16_t* q;
+  const uint16_t* kc;
+  const uint16_t* vc;
+  const int32_t* table;         // [num_seqs, max_blocks]
+  const int32_t* query_start;   // [num_seqs + 1] (prompts)
+  const int32_t* prefix_table;  // [prefix_blocks] (shared prefix)
+  const int32_t* prefix_len;    // [1]
+  const int32_t* seq_lens;      // [num_seqs]
+  uint16_t* out;
+  float* part_o;    // [rows, slots, HD], where slots > 1
+  float* part_lse;  // [rows, slots], log2 units
+  int64_t q_stride;  // elements from a token's q to the next token's
+  int num_tokens, num_seqs, max_blocks, prefix_blocks, num_blocks, bs_log2, n_q, n_kv, group;
+  int splits;         // of a tile's tokens (prompts), of the prefix (shared prefix)
+  int suffix_splits;  // of each sequence's own tokens (shared prefix)
+  int tiles;          // row tiles the grid has room for
+  float scale_log2;
+};
+
+// What one workgroup computes: `rows` rows from row0 on (row -> token row / group
+// from token0 on, head kvh * group + row % group) over the tokens [from, to) of
+// the pages in `table`.  query_at: the position of token token0, or NO_QUERY
+// where every row is a sequence's one decode token.
+constexpr int NO_QUERY = INT_MIN;
+struct Item {
+  const int32_t* table;
+  int token0, row0, rows, from, to, slot, slots, query_at;
+};
+
+// HD: head_dim.  WM waves take 32 rows each, WN groups of them take every WN-th
+// tile of KT tokens; a group's tile of K and V is in LDS, two tiles deep.
+template <int HD, int WM, int WN, int KT>
+struct Shape {
+  static constexpr int M = 32 * WM, NT = 64 * WM * WN;
+  static constexpr int CH = HD / 8;                  // 16-byte chunks of a row
+  static constexpr int TILE = KT * CH;               // chunks of a K or V tile
+  static constexpr int GROUP = 2 * 2 * TILE;         // two buffers of K and V
+  static constexpr int JOIN = WN > 1 ? (WN - 1) * WM * (32 * HD + 64) / 4 : 0;
+  static constexpr int LDS = WN * GROUP > JOIN ? WN * GROUP : JOIN;
+  static constexpr int LOADS = TILE / 64 / WM;       // a wave's loads of a K (V) tile
+  static_assert(TILE % (64 * WM) == 0, "whole loads per wave");
+};
+
+// Chunk c of row r sits in slot c ^ k_swz(r) (K) or c ^ v_swz(r) (V) of its row, so
+// that the lanes of one LDS read are spread over all banks: K is read 16 bytes
+// a lane from 32 rows, V 8 bytes a lane, 64 bytes from each of 8 rows.
+template <int HD>
+__device__ __forceinline__ int k_swz(int r) {
+  return HD == 128 ? (r & 15) : ((r >> 1) & 7);
+}
+template <int HD>
+__device__ __forceinline__ int v_swz(int r) {
+  return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
+}
+
+template <int HD, int WM, int WN, int KT>
+__device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
+  using S = Shape<HD, WM, WN, KT>;
+  constexpr int KS = HD / 16, DT = HD / 32, NU = KT / 32, CH = S::CH;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int bs = 1 << A.bs_log2;
+  const int tok_stride = A.n_kv * HD;
+  const int64_t page_stride = (int64_t)tok_stride << A.bs_log2;
+
+  // ---- this lane's row
+  const int row = it.row0 + 32 * wm + n;
+  const bool valid = 32 * wm + n < it.rows;
+  const int tok = it.token0 + row / A.group, head = kvh * A.group + row % A.group;
+  // The row sees the tokens below lim: of a prompt up to its own position, of a
+  // decode row all of its sequence.  (A row past the tile's end is not stored: it
+  // sees everything, so that no tile is masked for it.)
+  int lim = it.to;
+  if (valid) {
+    const int len = it.query_at == NO_QUERY ? A.seq_lens[tok] : it.query_at + row / A.group + 1;
+    lim = min(max(len, 0), it.to);
+  }
+  u32x4 qf[KS];
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) {
+    qf[ks] = u32x4{0u, 0u, 0u, 0u};
+    if (valid)
+      qf[ks] = *reinterpret_cast<const u32x4*>(A.q + (int64_t)tok * A.q_stride + head * HD +
+                                               16 * ks + 8 * h);
+  }
+  int lim_min = lim;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o));
+  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+
+  // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile
+  const int first = it.from & ~(KT - 1);
+  const int ntiles = it.to > it.from ? (it.to - first + KT - 1) / KT : 0;
+  const int rounds = (ntiles + WN - 1) / WN;
+  u32x4* const lds = smem + wn * S::GROUP;
+  auto stage = [&](int buf, int base) {
+    u32x4* const kd = lds + buf * 2 * S::TILE;
+    // the pages of the tile's two halves; tokens past the end are those of the last one
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+      const int c0 = (i * WM + wm) * 64;  // first chunk of this load
+      const int r = c0 / CH + lane / CH;  // the lane's row of the tile
+      const int t = min(base + r, it.to - 1);
+      const int pg_raw = it.table[min(base + c0 / CH, it.to - 1) >> A.bs_log2];
+      const int pg = (unsigned)pg_raw < (unsigned)A.num_blocks ? pg_raw : 0;
+      const int64_t at = (int64_t)pg * page_stride + kvh * HD +
+                         (int64_t)(t & (bs - 1)) * tok_stride;
+      const int c = lane % CH;
+      __builtin_amdgcn_global_load_lds(
+          (global_void*)(A.kc + at + 8 * (c ^ k_swz<HD>(r))), (lds_void*)(kd + c0), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds(
+          (global_void*)(A.vc + at + 8 * (c ^ v_swz<HD>(r))), (lds_void*)(kd + S::TILE + c0), 16,
+          0, 0);
+    }
+  };
+
+  float m = -INFINITY;  // running maximum of the row's scores (unscaled)
+  float l = 0.f;        // running sum, this lane's tokens
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+
+  if (rounds > 0 && wn < ntiles) stage(0, first + wn * KT);
+  for (int rd = 0; rd < rounds; ++rd) {
+    const int tile = rd * WN + wn, base = first + tile * KT;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tile + WN < ntiles) stage((rd + 1) & 1, base + WN * KT);
+    if (tile >= ntiles) continue;
+    const u32x4* const kt = lds + (rd & 1) * 2 * S::TILE;
+    const uint16_t* const vt = reinterpret_cast<const uint16_t*>(kt + S::TILE);
+
+    // ---- scores: s[u][4 a + b] is token 32 u + 8 a + 4 h + b of row n
+    f32x16 s[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const u32x4 a = kt[(32 * u + n) * CH + ((2 * ks + h) ^ k_swz<HD>(n))];
+        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, qf[ks]), s[u],
+                                                       0, 0, 0);
+      }
+    }
+    // A table entry outside the cache is never dereferenced: its tokens' scores are
+    // NaN, and so is every row that sees one of them.
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int pg = it.table[min(base + 32 * u, it.to - 1) >> A.bs_log2];
+      if ((unsigned)pg >= (unsigned)A.num_blocks) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[u][i] = __builtin_nanf("");
+      }
+    }
+    const bool masked = base < it.from || base + KT > lim_min;  // for some row of the wave
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int t = base + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
+          s[u][i] = t >= it.from && t < lim ? s[u][i] : -INFINITY;
+        }
+    }
+    // ---- online softmax
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+    mx = fmaxf(m, xor_max<32>(mx));
+    const float ref = mx == -INFINITY ? 0.f : mx * A.scale_log2;
+    const float alpha = __builtin_amdgcn_exp2f(m * A.scale_log2 - ref);
+    m = mx;
+    l *= alpha;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+    uint32_t p[NU][8];
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], A.scale_log2, -ref));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], A.scale_log2, -ref));
+        l += p0;
+        l += p1;
+        p[u][i] = cvt_pk_bf16(p0, p1);
+      }
+    // ---- O^T += V^T P^T
+    const int vr = 4 * h + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    auto v_operand = [&](int kk, int d) -> u32x4 {  // V of 16 tokens, dims 32 d + n
+      u32x2 half[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = 16 * kk + 8 * j + vr;
+        const uint16_t* src = vt + (r * CH + ((4 * d + vc) ^ v_swz<HD>(r))) * 8 + 4 * (lane & 1);
+        half[j] = __builtin_bit_cast(u32x2,
+                                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src));
+      }
+      return u32x4{half[0].x, half[0].y, half[1].x, half[1].y};
+    };
+    // A masked token must not reach a row by 0 * infinity or 0 * NaN: where a
+    // tile that some row sees in part holds such values (0 * V tells), they are
+    // left out of the product and added to the rows that see them.
+    bool odd = false;
+    if (masked) {
+      f32x16 z;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) z[i] = 0.f;
+      const u32x4 none = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int kk = 0; kk < 2 * NU; ++kk)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, v_operand(kk, d)), __builtin_bit_cast(bf16x8, none), z,
+              0, 0, 0);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += z[i];
+      odd = __builtin_amdgcn_ballot_w64(sum != sum) != 0;
+    }
+    if (!odd) {
+#pragma unroll
+      for (int kk = 0; kk < 2 * NU; ++kk) {
+        const u32x4 b = {p[kk / 2][4 * (kk & 1)], p[kk / 2][4 * (kk & 1) + 1],
+                         p[kk / 2][4 * (kk & 1) + 2], p[kk / 2][4 * (kk & 1) + 3]};
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              __builtin_bit_cast(bf16x8, v_operand(kk, d)), __builtin_bit_cast(bf16x8, b), o[d],
+              0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < 2 * NU; ++kk) {
+        const u32x4 b = {p[kk / 2][4 * (kk & 1)], p[kk / 2][4 * (kk & 1) + 1],
+                         p[kk / 2][4 * (kk & 1) + 2], p[kk / 2][4 * (kk & 1) + 3]};
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          u32x4 a = v_operand(kk, d);
+          a = u32x4{finite_bf16x2(a.x), finite_bf16x2(a.y), finite_bf16x2(a.z),
+                    finite_bf16x2(a.w)};
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                         __builtin_bit_cast(bf16x8, b), o[d], 0,
+                                                         0, 0);
+        }
+      }
+      for (int r = 0; r < KT; ++r) {
+        const bool seen = base + r >= it.from && base + r < lim;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int dim = 32 * d + 8 * (i / 4) + 4 * h + i % 4;
+            const uint32_t v = vt[(r * CH + ((dim / 8) ^ v_swz<HD>(r))) * 8 + dim % 8];
+            if (seen && (v & 0x7f80u) == 0x7f80u) o[d][i] += bf16_bits_to_f32(v);
+          }
+      }
+    }
+  }
+
+  // ---- the lane pair's sums, then the WN groups' states
+  l = xor_sum<32>(l);
+  if constexpr (WN > 1) {
+    float* const jo = reinterpret_cast<float*>(smem);
+    __syncthreads();  // the tiles are read out
+    if (wn > 0) {
+      float* const dst = jo + ((wn - 1) * WM + wm) * (32 * HD + 64);
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dst[(16 * d + i) * 64 + lane] = o[d][i];
+      if (h == 0) {
+        dst[32 * HD + n] = m;
+        dst[32 * HD + 32 + n] = l;
+      }
+    }
+    __syncthreads();
+    if (wn > 0) return;  // nothing stored
+#pragma unroll
+    for (int w = 1; w < WN; ++w) {
+      const float* const src = jo + ((w - 1) * WM + wm) * (32 * HD + 64);
+      const float mo = src[32 * HD + n], lo = src[32 * HD + 32 + n];
+      const float mx = fmaxf(m, mo), ref = mx == -INFINITY ? 0.f : mx;
+      const float a = __builtin_amdgcn_exp2f((m - ref) * A.scale_log2);
+      const float b = __builtin_amdgcn_exp2f((mo - ref) * A.scale_log2);
+      m = mx;
+      l = l * a + lo * b;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * a + src[(16 * d + i) * 64 + lane] * b;
+    }
+  }
+  // l == 0 only where the row sees no token: its output is 0, its weight none
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t orow = (int64_t)tok * A.n_q + head;
+  if (valid && it.slots == 1) {
+    uint16_t* const dst = A.out + orow * HD;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int a = 0; a < 4; ++a)
+        st_agent(reinterpret_cast<u32x2*>(dst + 32 * d + 8 * a + 4 * h),
+                 u32x2{cvt_pk_bf16(o[d][4 * a] * inv, o[d][4 * a + 1] * inv),
+                       cvt_pk_bf16(o[d][4 * a + 2] * inv, o[d][4 * a + 3] * inv)});
+  } else if (valid) {
+    const int64_t prow = orow * it.slots + it.slot;
+    if (h == 0)
+      st_agent(A.part_lse + prow, l == 0.f ? -INFINITY : m * A.scale_log2 + log2f(l));
+    if (l != 0.f) {  // the merge reads no partial whose weight is none
+      float* const dst = A.part_o + prow * HD;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          st_agent_b128(dst + 32 * d + 8 * a + 4 * h,
+                        u32x4{__float_as_uint(o[d][4 * a] * inv),
+                              __float_as_uint(o[d][4 * a + 1] * inv),
+                              __float_as_uint(o[d][4 * a + 2] * inv),
+                              __float_as_uint(o[d][4 * a + 3] * inv)});
+    }
+  }
+  stores_done();
+}
+
+// Packed prompts.  Sequence r's queries are the tokens [query_start[r],
+// query_start[r + 1]), the last n of its L tokens: token i of them is at position
+// L - n + i and sees the tokens up to itself.  Grid: kv heads, row tiles (last
+// first: the longest come first), splits.  Which sequence a tile is of follows
+// from the prefix sums of the tile counts, 64 sequences at a time.
+template <int HD, int WM, int WN, int KT, int EU>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
+void prompt_attention_kernel(RowsArgs A) {
+  using S = Shape<HD, WM, WN, KT>;
+  __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
+  const int lane = threadIdx.x & 63;
+  const int kvh = blockIdx.x, tile = A.tiles - 1 - (int)blockIdx.y, split = blockIdx.z;
+  int done = 0, seq = -1, t_in = 0, q0 = 0, nq = 0;
+  for (int b = 0; b < A.num_seqs; b += 64) {
+    const int r = b + lane;
+    int s0 = 0, cnt = 0, nt = 0;
+    if (r < A.num_seqs) {
+      s0 = min(max(A.query_start[r], 0), A.num_tokens);
+      cnt = max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
+      nt = (int)(((int64_t)cnt * A.group + S::M - 1) / S::M);
+    }
+    int incl = nt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o);
+      if (lane >= o) incl += x;
+    }
+    const int total = __builtin_amdgcn_readlane(incl, 63);
+    if (tile < done + total) {
+      const int i = __ffsll((unsigned long long)__ballot(done + incl > tile)) - 1;
+      seq = b + i;
+      t_in = tile - done - (__builtin_amdgcn_readlane(incl, i) - __builtin_amdgcn_readlane(nt, i));
+      q0 = __builtin_amdgcn_readlane(s0, i);
+      nq = __builtin_amdgcn_readlane(cnt, i);
+      break;
+    }
+    done += total;
+  }
+  if (seq < 0) return;  // the grid has room for the most tiles there can be
+  const int cap = A.max_blocks << A.bs_log2;
+  const int L = min(max(A.seq_lens[seq], 0), cap);
+  Item it;
+  it.table = A.table + (int64_t)seq * A.max_blocks;
+  it.token0 = q0;
+  it.row0 = t_in * S::M;
+  it.rows = min(S::M, nq * A.group - it.row0);
+  const int ahead = L - nq;  // the position of the first query token
+  const int last = (it.row0 + it.rows - 1) / A.group;
+  const int range = max(ahead + last + 1, 0);
+  const int chunk = ((range + KT - 1) / KT + A.splits - 1) / A.splits * KT;
+  it.from = min(split * chunk, range);
+  it.to = min(it.from + chunk, range);
+  it.slot = split;
+  it.slots = A.splits;
+  it.query_at = ahead;
+  attend<HD, WM, WN, KT>(A, it, kvh, smem);
+}
+
+// Decode rows (one token a sequence) under a shared prefix.  Grid: kv heads,
+// items: first the prefix, row tiles of all sequences' rows times its splits,
+// then each sequence's own tokens [prefix, L) in its splits.
+template <int HD, int WM, int WN, int KT, int EU>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
+void shared_prefix_kernel(RowsArgs A) {
+  using S = Shape<HD, WM, WN, KT>;
+  __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
+  const int kvh = blockIdx.x;
+  const int prefix = min(max(A.prefix_len[0], 0), A.prefix_blocks << A.bs_log2);
+  const int cap = A.max_blocks << A.bs_log2;
+  Item it;
+  it.slots = A.splits + A.suffix_splits;
+  it.query_at = NO_QUERY;
+  const int y = blockIdx.y;
+  if (y < A.tiles * A.splits) {
+    const int split = y / A.tiles;
+    it.table = A.prefix_table;
+    it.token0 = 0;
+    it.row0 = (y % A.tiles) * S::M;
+    it.rows = min(S::M, A.num_seqs * A.group - it.row0);
+    const int chunk = ((prefix + KT - 1) / KT + A.splits - 1) / A.splits * KT;
+    it.from = min(split * chunk, prefix);
+    it.to = min(it.from + chunk, prefix);
+    it.slot = split;
+  } else {
+    const int gt = (A.group + S::M - 1) / S::M;  // row tiles of a sequence's group
+    int x = y - A.tiles * A.splits;
+    const int seq = x / (A.suffix_splits * gt);
+    x -= seq * A.suffix_splits * gt;
+    const int split = x / gt;
+    const int L = min(max(A.seq_lens[seq], 0), cap);
+    it.table = A.table + (int64_t)seq * A.max_blocks;
+    it.token0 = seq;
+    it.row0 = (x % gt) * S::M;
+    it.rows = min(S::M, A.group - it.row0);
+    const int span = max(L - prefix, 0);
+    // tiles are aligned to KT, so that a tile's halves of 32 tokens are within a page
+    const int first = prefix & ~(KT - 1);
+    const int tiles = span ? (L - first + KT - 1) / KT : 0;
+    const int chunk = (tiles + A.suffix_splits - 1) / A.suffix_splits * KT;
+    it.to = min(first + (split + 1) * chunk, max(L, prefix));
+    it.from = min(max(first + split * chunk, prefix), it.to);
+    it.slot = A.splits + split;
+  }
+  attend<HD, WM, WN, KT>(A, it, kvh, smem);
+}
+
+// out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a row's partials, a
+// wave a row: lane j holds the weights of slots j, j + 64, ..., every lane HD / 64
+// dims.  A partial of weight 0 is not read (it was not written).  Rows that are
+// of no sequence are left as they are.
+constexpr int MERGE_ROWS = 4;  // rows (waves) of a workgroup
+
+template <int HD>
+__global__ __launch_bounds__(64 * MERGE_ROWS) void rows_merge_kernel(
+    const float* part_o, const float* part_lse, uint16_t* out, const int32_t* query_start,
+    int num_seqs, int num_tokens, int n_q, int slots) {
+  constexpr int D = HD / 64;
+  const int lane = threadIdx.x & 63;
+  const int64_t row =
+      (int64_t)blockIdx.x * MERGE_ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tok = (int)(row / n_q);
+  if (tok >= num_tokens) return;
+  if (query_start && (tok < query_start[0] || tok >= query_start[num_seqs])) return;
+  const float* const lse = part_lse + row * slots;
+  const float* const po = part_o + row * slots * HD;
+  float top = -INFINITY;
+  bool bad = false;
+  for (int s = lane; s < slots; s += 64) {
+    top = fmaxf(top, lse[s]);
+    bad |= lse[s] != lse[s];
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  float sum = 0.f, acc[D] = {};
+  for (int s0 = 0; s0 < slots; s0 += 64) {
+    const float x = s0 + lane < slots ? lse[s0 + lane] : -INFINITY;
+    const float w = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
+    sum += w;
+    const int cnt = min(64, slots - s0);
+    for (int j = 0; j < cnt; ++j) {
+      const float wj = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
+      if (wj == 0.f) continue;
+#pragma unroll
+      for (int d = 0; d < D; ++d)
+        acc[d] = fmaf(wj, po[(int64_t)(s0 + j) * HD + D * lane + d], acc[d]);
+    }
+  }
+  sum = wave_sum(sum);
+  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  uint16_t* const dst = out + row * HD + D * lane;
+  float r[D];
+#pragma unroll
+  for (int d = 0; d < D; ++d) r[d] = bad ? __builtin_nanf("") : acc[d] * inv;
+  if constexpr (D == 2)
+    st_agent(reinterpret_cast<uint32_t*>(dst), cvt_pk_bf16(r[0], r[1]));
+  else
+    st_agent(dst, f32_to_bf16(r[0]));
+  stores_done();
+}
+
+int log2_of(int v) {
+  int b = 0;
+  while ((1 << b) < v) ++b;
+  return b;
+}
+
+template <int HD>
+int launch_merge(hipStream_t stream, const RowsArgs& a, int slots, bool prompts) {
+  const int64_t rows = (int64_t)a.num_tokens * a.n_q;
+  SMX_LAUNCH((rows_merge_kernel<HD>), dim3((unsigned)((rows + MERGE_ROWS - 1) / MERGE_ROWS)),
+             dim3(64 * MERGE_ROWS), 0, stream, a.part_o, a.part_lse, a.out,
+             prompts ? a.query_start : (const int32_t*)nullptr, a.num_seqs, a.num_tokens, a.n_q,
+             slots);
+  return (int)hipGetLastError();
+}
+
+// Rows of a workgroup and splits of a tile's tokens.
+struct Choice {
+  int wm, splits, suffix_splits, tiles;
+};
+
+Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
+  Choice c{};
+  c.wm = 4;
+  c.tiles = (int)((num_tokens * group + 32 * c.wm - 1) / (32 * c.wm) + num_seqs - 1);
+  c.splits = 1;
+  return c;
+}
+
+Choice choose_prefix(int64_t num_seqs, int64_t prefix_cap, int64_t cap, int group, int n_kv) {
+  Choice c{};
+  c.wm = 4;
+  c.tiles = (int)((num_seqs * group + 32 * c.wm - 1) / (32 * c.wm));
+  c.splits = 1;
+  c.suffix_splits = 1;
+  return c;
+}
+
+int64_t partial_bytes(int64_t rows, int64_t slots, int hd) {
+  if (slots == 1) return 0;
+  return rows * slots * (hd + 1) * 4;
+}
+
+template <int HD>
+int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
+  const dim3 grid(a.n_kv, c.tiles, c.splits);
+  SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
+  const int rc = (int)hipGetLastError();
+  return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, true);
+}
+
+template <int HD>
+int launch_prefix(hipStream_t stream, RowsArgs& a, const Choice& c) {
+  const int gt = (a.group + 32 * c.wm - 1) / (32 * c.wm);
+  const dim3 grid(a.n_kv, c.tiles * c.splits + a.num_seqs * c.suffix_splits * gt, 1);
+  SMX_LAUNCH((shared_prefix_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
+  const int rc = (int)hipGetLastError();
+  return rc ? rc : launch_merge<HD>(stream, a, c.splits + c.suffix_splits, false);
+}
+
+}  // namespace
+}  // namespace smx
+
+#include "smx_abi_util.h"
+
+#define SMX_ROWS_SIZES(num_tokens)                                                               \
+  SMX_REQUIRE(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");                  \
+  SMX_REQUIRE(n_kv >= 1 && n_kv <= 65535 && n_q >= n_kv && n_q % n_kv == 0,                      \
+              "n_q must be a multiple of n_kv");                                                 \
+  SMX_REQUIRE(block_size >= 32 && block_size <= 4096 && (block_size & (block_size - 1)) == 0,    \
+              "block_size must be a power of two in [32, 4096]");                                \
+  SMX_REQUIRE((int64_t)n_kv * head_dim * block_size < (1ll << 30),                               \
+              "a page must have fewer than 2^30 elements");                                      \
+  SMX_REQUIRE(max_blocks >= 1 && (int64_t)max_blocks * block_size <= INT32_MAX - 4096,           \
+              "max_blocks * block_size (a sequence's capacity) must fit in int32");              \
+  SMX_REQUIRE(num_seqs >= 1 && num_seqs <= 65535, "num_seqs must be in [1, 65535]");             \
+  SMX_REQUIRE(num_tokens >= 1 && (int64_t)(num_tokens) * n_q < (1ll << 30),                      \
+              "num_tokens * n_q must be in [1, 2^30)")
+
+#define SMX_ROWS_CHECKS()                                                                        \
+  SMX_REQUIRE(q && k_cache && v_cache && block_table && seq_lens && out,                         \
+              "null pointer argument");                                                          \
+  SMX_REQUIRE(num_blocks >= 1, "num_blocks must be >= 1");                                       \
+  SMX_REQUIRE(scale > 0.f && isfinite(scale), "scale must be positive and finite");              \
+  SMX_REQUIRE((uintptr_t)q % 16 == 0 && (uintptr_t)k_cache % 16 == 0 &&                          \
+                  (uintptr_t)v_cache % 16 == 0 && (uintptr_t)out % 16 == 0,                      \
+              "q, k_cache, v_cache and out must be 16-byte aligned");                            \
+  SMX_REQUIRE((uintptr_t)block_table % 4 == 0 && (uintptr_t)seq_lens % 4 == 0,                   \
+              "int arrays must be 4-byte aligned")
+
+extern "C" int64_t smx_prompt_attention_workspace(int32_t num_tokens, int32_t num_seqs,
+                                                  int32_t max_blocks, int32_t block_size,
+                                                  int32_t n_q, int32_t n_kv, int32_t head_dim) {
+  if (num_tokens < 1 || num_seqs < 1 || max_blocks < 1 || block_size < 1 || n_kv < 1 ||
+      n_q < n_kv || n_q % n_kv || head_dim < 1)
+    return -1;
+  const smx::Choice c = smx::choose_prompt(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
+                                           n_q / n_kv, n_kv);
+  return smx::partial_bytes((int64_t)num_tokens * n_q, c.splits, head_dim);
+}
+
+extern "C" int smx_prompt_attention(void* stream, const void* q, int64_t q_stride,
+                                    const void* k_cache, const void* v_cache,
+                                    const int32_t* block_table, const int32_t* query_start_loc,
+                                    const int32_t* seq_lens, void* workspace,
+                                    int64_t workspace_bytes, void* out, int32_t num_tokens,
+                                    int32_t num_seqs, int32_t max_blocks, int32_t num_blocks,
+                                    int32_t block_size, int32_t n_q, int32_t n_kv,
+                                    int32_t head_dim, float scale) {
+  SMX_ROWS_CHECKS();
+  SMX_ROWS_SIZES(num_tokens);
+  SMX_REQUIRE(query_start_loc && (uintptr_t)query_start_loc % 4 == 0,
+              "query_start_loc must be non-null and 4-byte aligned");
+  SMX_REQUIRE(q_stride >= (int64_t)n_q * head_dim && q_stride % 8 == 0,
+              "q_stride must be a multiple of 8 and hold n_q heads");
+  const smx::Choice c = smx::choose_prompt(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
+                                           n_q / n_kv, n_kv);
+  SMX_REQUIRE(c.tiles <= 65535, "too many row tiles for one launch");
+  const int64_t rows = (int64_t)num_tokens * n_q;
+  SMX_REQUIRE(c.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
+                                workspace_bytes >= smx::partial_bytes(rows, c.splits, head_dim)),
+              "workspace must be 16-byte aligned and hold smx_prompt_attention_workspace bytes");
+  smx::RowsArgs a{};
+  a.q = (const uint16_t*)q;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.table = block_table;
+  a.query_start = query_start_loc;
+  a.seq_lens = seq_lens;
+  a.out = (uint16_t*)out;
+  a.part_o = (float*)workspace;
+  a.part_lse = (float*)workspace + rows * c.splits * head_dim;
+  a.q_stride = q_stride;
+  a.num_tokens = num_tokens;
+  a.num_seqs = num_seqs;
+  a.max_blocks = max_blocks;
+  a.num_blocks = num_blocks;
+  a.bs_log2 = smx::log2_of(block_size);
+  a.n_q = n_q;
+  a.n_kv = n_kv;
+  a.group = n_q / n_kv;
+  a.splits = c.splits;
+  a.tiles = c.tiles;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  return head_dim == 128 ? smx::launch_prompt<128>((hipStream_t)stream, a, c)
+                         : smx::launch_prompt<64>((hipStream_t)stream, a, c);
+}
+
+extern "C" int64_t smx_shared_prefix_attention_workspace(int32_t num_seqs, int32_t prefix_blocks,
+                                                         int32_t max_blocks, int32_t block_size,
+                                                         int32_t n_q, int32_t n_kv,
+                                                         int32_t head_dim) {
+  if (num_seqs < 1 || prefix_blocks < 1 || max_blocks < 1 || block_size < 1 || n_kv < 1 ||
+      n_q < n_kv || n_q % n_kv || head_dim < 1)
+    return -1;
+  const smx::Choice c =
+      smx::choose_prefix(num_seqs, (int64_t)prefix_blocks * block_size,
+                         (int64_t)max_blocks * block_size, n_q / n_kv, n_kv);
+  return smx::partial_bytes((int64_t)num_seqs * n_q, c.splits + c.suffix_splits, head_dim);
+}
+
+extern "C" int smx_shared_prefix_attention(
+    void* stream, const void* q, int64_t q_stride, const void* k_cache, const void* v_cache,
+    const int32_t* prefix_table, const int32_t* prefix_len, const int32_t* block_table,
+    const int32_t* seq_lens, void* workspace, int64_t workspace_bytes, void* out,
+    int32_t num_seqs, int32_t prefix_blocks, int32_t max_blocks, int32_t num_blocks,
+    int32_t block_size, int32_t n_q, int32_t n_kv, int32_t head_dim, float scale) {
+  SMX_ROWS_CHECKS();
+  SMX_ROWS_SIZES(num_seqs);
+  SMX_REQUIRE(prefix_table && prefix_len && (uintptr_t)prefix_table % 4 == 0 &&
+                  (uintptr_t)prefix_len % 4 == 0,
+              "prefix_table and prefix_len must be non-null and 4-byte aligned");
+  SMX_REQUIRE(prefix_blocks >= 1 && (int64_t)prefix_blocks * block_size <= INT32_MAX - 4096,
+              "prefix_blocks * block_size must fit in int32");
+  SMX_REQUIRE(q_stride >= (int64_t)n_q * head_dim && q_stride % 8 == 0,
+              "q_stride must be a multiple of 8 and hold n_q heads");
+  const smx::Choice c =
+      smx::choose_prefix(num_seqs, (int64_t)prefix_blocks * block_size,
+                         (int64_t)max_blocks * block_size, n_q / n_kv, n_kv);
+  const int64_t rows = (int64_t)num_seqs * n_q;
+  const int slots = c.splits + c.suffix_splits;
+  SMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
+                  workspace_bytes >= smx::partial_bytes(rows, slots, head_dim),
+              "workspace must be 16-byte aligned and hold "
+              "smx_shared_prefix_attention_workspace bytes");
+  smx::RowsArgs a{};
+  a.q = (const uint16_t*)q;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.table = block_table;
+  a.prefix_table = prefix_table;
+  a.prefix_len = prefix_len;
+  a.seq_lens = seq_lens;
+  a.out = (uint16_t*)out;
+  a.part_o = (float*)workspace;
+  a.part_lse = (float*)workspace + rows * slots * head_dim;
+  a.q_stride = q_stride;
+  a.num_tokens = num_seqs;
+  a.num_seqs = num_seqs;
+  a.max_blocks = max_blocks;
+  a.prefix_blocks = prefix_blocks;
+  a.num_blocks = num_blocks;
+  a.bs_log2 = smx::log2_of(block_size);
+  a.n_q = n_q;
+  a.n_kv = n_kv;
+  a.group = n_q / n_kv;
+  a.splits = c.splits;
+  a.suffix_splits = c.suffix_splits;
+  a.tiles = c.tiles;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  return head_dim == 128 ? smx::launch_prefix<128>((hipStream_t)stream, a, c)
+                         : smx::launch_prefix<64>((hipStream_t)stream, a, c);
+}

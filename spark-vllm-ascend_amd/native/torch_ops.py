@@ -10,6 +10,8 @@ reference's custom ops do (src/spark_vllm_ascend/integration/head.py:8-9).
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import call, load
@@ -639,6 +641,199 @@ def compute_slot_mapping(query_start_loc: torch.Tensor, positions: torch.Tensor,
          pos_ptr, block_table.data_ptr(), out.data_ptr(), num_tokens,
          max(max_tokens, 1), block_table.shape[1], block_size)
     return out
+
+
+def _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out):
+    """The checks the row attentions share; returns out (allocated if None)."""
+    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dtype == BF16 and q.dim() == 3,
+          "q must be a bf16 GPU tensor [tokens, n_q, hd]")
+    _need(q.shape[0] >= 1 and q.shape[1] >= 1, "q must hold a token and a head")
+    n_q, hd = q.shape[1:]
+    _need(q.stride(2) == 1 and (n_q == 1 or q.stride(1) == hd)
+          and (q.shape[0] == 1 or q.stride(0) >= n_q * hd),
+          "a token's heads must be contiguous in q and its tokens apart")
+    _need(q.data_ptr() % 16 == 0 and (q.shape[0] == 1 or q.stride(0) % 8 == 0),
+          "q's tokens must be 16-byte aligned")
+    _check(k_cache, "k_cache", BF16, device=q.device)
+    _check(v_cache, "v_cache", BF16, device=q.device)
+    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
+          "the caches must be [blocks, block_size, n_kv, hd], both alike")
+    _need(hd == k_cache.shape[3], "head_dim mismatch between q and the cache")
+    _check(block_table, "block_table", torch.int32, device=q.device)
+    _need(block_table.dim() == 2, "block_table must be [seqs, max_blocks]")
+    _check(seq_lens, "seq_lens", torch.int32, block_table.shape[0], q.device)
+    if workspace is not None:
+        _check(workspace, "workspace", torch.uint8, device=q.device)
+    if out is None:
+        out = torch.empty(q.shape, dtype=BF16, device=q.device)
+    _check(out, "out", BF16, q.numel(), q.device)
+    return out
+
+
+def _q_stride(q: torch.Tensor) -> int:
+    return q.stride(0) if q.shape[0] > 1 else q.shape[1] * q.shape[2]
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _prompt_workspace_bytes(q, k_cache, block_table) -> int:
+    _, bs, n_kv, hd = k_cache.shape
+    return load().smx_prompt_attention_workspace(q.shape[0], block_table.shape[0],
+                                                 block_table.shape[1], bs, q.shape[1], n_kv, hd)
+
+
+def prompt_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor,
+                               block_table: torch.Tensor) -> torch.Tensor | None:
+    """The workspace prompt_attention uses for these sizes (uint8; None where it
+    uses none).  Calls that can overlap need one each."""
+    return _workspace(_prompt_workspace_bytes(q, k_cache, block_table), q.device)
+
+
+def prompt_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     block_table: torch.Tensor, query_start_loc: torch.Tensor,
+                     seq_lens: torch.Tensor, scale: float,
+                     workspace: torch.Tensor | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed query rows over the paged cache.  q [tokens, n_q,
+    hd] (tokens may be strided, a slice of the QKV rows); sequence r's queries
+    are the rows query_start_loc[r]..query_start_loc[r + 1] and the last of its
+    seq_lens[r] tokens, whose K and V the cache holds.  Rows of no sequence are
+    left as they are in `out`.  Without `workspace` (prompt_attention_workspace)
+    one is allocated where the call needs it."""
+    out = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
+    num_seqs, max_blocks = block_table.shape
+    _check(query_start_loc, "query_start_loc", torch.int32, num_seqs + 1, q.device)
+    num_blocks, bs, n_kv, hd = k_cache.shape
+    if workspace is None:
+        workspace = _workspace(_prompt_workspace_bytes(q, k_cache, block_table), q.device)
+    call("smx_prompt_attention", _stream(q), q.data_ptr(), _q_stride(q), k_cache.data_ptr(),
+         v_cache.data_ptr(), block_table.data_ptr(), query_start_loc.data_ptr(),
+         seq_lens.data_ptr(), _ptr(workspace), workspace.numel() if workspace is not None else 0,
+         out.data_ptr(), q.shape[0], num_seqs, max_blocks, num_blocks, bs, q.shape[1], n_kv, hd,
+         float(scale))
+    return out
+
+
+def _prefix_workspace_bytes(q, k_cache, prefix_table, block_table) -> int:
+    _, bs, n_kv, hd = k_cache.shape
+    return load().smx_shared_prefix_attention_workspace(
+        q.shape[0], prefix_table.numel(), block_table.shape[1], bs, q.shape[1], n_kv, hd)
+
+
+def shared_prefix_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor,
+                                      prefix_table: torch.Tensor,
+                                      block_table: torch.Tensor) -> torch.Tensor | None:
+    """The workspace shared_prefix_attention uses for these sizes (uint8)."""
+    return _workspace(_prefix_workspace_bytes(q, k_cache, prefix_table, block_table), q.device)
+
+
+def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                            prefix_table: torch.Tensor, prefix_len: torch.Tensor,
+                            block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                            workspace: torch.Tensor | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of sequences that share their first prefix_len[0] tokens
+    (pages prefix_table, int32 [blocks]), read once for all.  q [seqs, n_q, hd];
+    block_table [seqs, max_blocks] by absolute position (its entries below the
+    prefix are not used); seq_lens the whole lengths, prefix included."""
+    out = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
+    num_seqs, max_blocks = block_table.shape
+    _need(q.shape[0] == num_seqs, "q must have a row for each sequence of block_table")
+    _check(prefix_table, "prefix_table", torch.int32, device=q.device)
+    _need(prefix_table.dim() == 1 and prefix_table.numel() >= 1,
+          "prefix_table must be [prefix_blocks]")
+    _check(prefix_len, "prefix_len", torch.int32, 1, q.device)
+    num_blocks, bs, n_kv, hd = k_cache.shape
+    if workspace is None:
+        workspace = _workspace(_prefix_workspace_bytes(q, k_cache, prefix_table, block_table),
+                               q.device)
+    call("smx_shared_prefix_attention", _stream(q), q.data_ptr(), _q_stride(q),
+         k_cache.data_ptr(), v_cache.data_ptr(), prefix_table.data_ptr(), prefix_len.data_ptr(),
+         block_table.data_ptr(), seq_lens.data_ptr(), _ptr(workspace),
+         workspace.numel() if workspace is not None else 0, out.data_ptr(), num_seqs,
+         prefix_table.numel(), max_blocks, num_blocks, bs, q.shape[1], n_kv, hd, float(scale))
+    return out
+
+
+class RequestTables(NamedTuple):
+    """What request_tables() writes besides the block table."""
+    num_pages: torch.Tensor        # int32 [reqs]: pages each request now has
+    free_count: torch.Tensor       # int32 [1]: pages left in the free list
+    query_start_loc: torch.Tensor  # int32 [reqs + 1]
+    seq_lens: torch.Tensor         # int32 [reqs]
+    positions: torch.Tensor        # int64 [max_tokens], 0 past the last token
+    slot_mapping: torch.Tensor     # int64 [max_tokens], -1 past the last token
+
+
+def request_tables_out(num_pages: torch.Tensor, max_tokens: int) -> RequestTables:
+    """Buffers for request_tables(out=...).  A program that keeps its pages in
+    place passes _replace(num_pages=num_pages, free_count=free_count) of it."""
+    reqs, dev = num_pages.numel(), num_pages.device
+    i32 = dict(dtype=torch.int32, device=dev)
+    i64 = dict(dtype=torch.int64, device=dev)
+    return RequestTables(torch.empty(reqs, **i32), torch.empty(1, **i32),
+                         torch.empty(reqs + 1, **i32), torch.empty(reqs, **i32),
+                         torch.empty(max_tokens, **i64), torch.empty(max_tokens, **i64))
+
+
+def _pages_checks(num_pages, free_pages, free_count, block_table):
+    _check(num_pages, "num_pages", torch.int32)
+    reqs = num_pages.numel()
+    _need(reqs >= 1, "there must be a request")
+    _check(free_pages, "free_pages", torch.int32, device=num_pages.device)
+    _need(free_pages.numel() >= 1, "free_pages must have room for a page")
+    _check(free_count, "free_count", torch.int32, 1, num_pages.device)
+    _check(block_table, "block_table", torch.int32, device=num_pages.device)
+    _need(block_table.dim() == 2 and block_table.shape[0] == reqs and block_table.shape[1] >= 1,
+          "block_table must be [reqs, max_blocks]")
+    return reqs
+
+
+def request_tables(query_lens: torch.Tensor, context_lens: torch.Tensor,
+                   num_pages: torch.Tensor, free_pages: torch.Tensor, free_count: torch.Tensor,
+                   block_table: torch.Tensor, block_size: int, max_tokens: int | None = None,
+                   out: RequestTables | None = None) -> RequestTables:
+    """A step's block tables, offsets, lengths, positions and slots from the
+    requests' new and cached token counts, on the device.  Pages that block_table's
+    rows lack are taken from the end of the free list and written into the table;
+    num_pages and free_count are updated out of place, or in place where `out`
+    holds them.  max_tokens (without `out`): the size of positions and slots."""
+    reqs = _pages_checks(num_pages, free_pages, free_count, block_table)
+    dev = num_pages.device
+    _check(query_lens, "query_lens", torch.int32, reqs, dev)
+    _check(context_lens, "context_lens", torch.int32, reqs, dev)
+    if out is None:
+        _need(max_tokens is not None and max_tokens >= 1, "max_tokens or out is needed")
+        out = request_tables_out(num_pages, max_tokens)
+    else:
+        _check(out.num_pages, "out.num_pages", torch.int32, reqs, dev)
+        _check(out.free_count, "out.free_count", torch.int32, 1, dev)
+        _check(out.query_start_loc, "out.query_start_loc", torch.int32, reqs + 1, dev)
+        _check(out.seq_lens, "out.seq_lens", torch.int32, reqs, dev)
+        _check(out.positions, "out.positions", torch.int64, max_tokens, dev)
+        _check(out.slot_mapping, "out.slot_mapping", torch.int64, out.positions.numel(), dev)
+        _need(out.positions.numel() >= 1, "out.positions must hold a token")
+    call("smx_request_tables", _stream(num_pages), query_lens.data_ptr(),
+         context_lens.data_ptr(), num_pages.data_ptr(), free_pages.data_ptr(),
+         free_count.data_ptr(), block_table.data_ptr(), out.num_pages.data_ptr(),
+         out.free_count.data_ptr(), out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(),
+         out.positions.data_ptr(), out.slot_mapping.data_ptr(), reqs, out.positions.numel(),
+         block_table.shape[1], free_pages.numel(), block_size)
+    return out
+
+
+def release_pages(keep_lens: torch.Tensor, num_pages: torch.Tensor, free_pages: torch.Tensor,
+                  free_count: torch.Tensor, block_table: torch.Tensor, block_size: int) -> None:
+    """Give the pages beyond the first keep_lens[r] tokens of every request back to
+    the free list (0: all of a finished request's; fewer than its length: those
+    of rejected tokens).  Everything is updated in place."""
+    reqs = _pages_checks(num_pages, free_pages, free_count, block_table)
+    _check(keep_lens, "keep_lens", torch.int32, reqs, num_pages.device)
+    call("smx_release_pages", _stream(num_pages), keep_lens.data_ptr(), num_pages.data_ptr(),
+         free_pages.data_ptr(), free_count.data_ptr(), block_table.data_ptr(), reqs,
+         block_table.shape[1], free_pages.numel(), block_size)
 
 
 class PackedQ4_0:
