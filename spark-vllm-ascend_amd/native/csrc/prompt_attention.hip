@@ -47,6 +47,9 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
   return w;
 }
 
+constexpr float LAG = 8.f;        // log2 units
+constexpr float NO_REF = -1e30f;  // below every finite score's, and 2^(NO_REF - that) is 0
+
 struct RowsArgs {
   const uint16_t* q;
   const uint16_t* kc;
@@ -64,6 +67,7 @@ struct RowsArgs {
   int splits;         // of a tile's tokens (prompts), of the prefix (shared prefix)
   int suffix_splits;  // of each sequence's own tokens (shared prefix)
   int tiles;          // row tiles the grid has room for
+  int item0;          // the first item of this launch (shared prefix)
   float scale_log2;
 };
 
@@ -139,46 +143,78 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   for (int o = 1; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o));
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
 
-  // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile
+  // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile.  The
+  // pages of a tile's halves of 32 tokens (within a page each) are looked up a
+  // round before they are used; an entry outside the cache is never dereferenced.
   const int first = it.from & ~(KT - 1);
   const int ntiles = it.to > it.from ? (it.to - first + KT - 1) / KT : 0;
   const int rounds = (ntiles + WN - 1) / WN;
   u32x4* const lds = smem + wn * S::GROUP;
+  const int lrow = lane / CH, lc = lane % CH;  // the lane's row and chunk of a load
+  int page[NU];
+  auto look_up = [&](int base) {
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+      page[u] = it.table[min(base + 32 * u, it.to - 1) >> A.bs_log2];
+  };
   auto stage = [&](int buf, int base) {
     u32x4* const kd = lds + buf * 2 * S::TILE;
-    // the pages of the tile's two halves; tokens past the end are those of the last one
+    const bool whole = base + KT <= it.to;
 #pragma unroll
     for (int i = 0; i < S::LOADS; ++i) {
       const int c0 = (i * WM + wm) * 64;  // first chunk of this load
-      const int r = c0 / CH + lane / CH;  // the lane's row of the tile
-      const int t = min(base + r, it.to - 1);
-      const int pg_raw = it.table[min(base + c0 / CH, it.to - 1) >> A.bs_log2];
-      const int pg = (unsigned)pg_raw < (unsigned)A.num_blocks ? pg_raw : 0;
-      const int64_t at = (int64_t)pg * page_stride + kvh * HD +
-                         (int64_t)(t & (bs - 1)) * tok_stride;
-      const int c = lane % CH;
+      const int r0 = c0 / CH;             // first row
+      const int raw = NU == 2 && r0 >= 32 ? page[NU - 1] : page[0];
+      const int pg = (unsigned)raw < (unsigned)A.num_blocks ? raw : 0;
+      const int64_t at = (int64_t)pg * page_stride + kvh * HD;
+      // tokens past the end are the last one
+      const int t0 = whole ? base + r0 : min(base + r0, it.to - 1);
+      const uint32_t dr = whole ? lrow : min(lrow, it.to - 1 - t0);
+      const int64_t row_at = at + (int64_t)(t0 & (bs - 1)) * tok_stride;
+      const uint32_t lane_at = dr * (uint32_t)tok_stride;
+      const int r = r0 + lrow;
       __builtin_amdgcn_global_load_lds(
-          (global_void*)(A.kc + at + 8 * (c ^ k_swz<HD>(r))), (lds_void*)(kd + c0), 16, 0, 0);
+          (global_void*)(A.kc + row_at + (lane_at + 8 * (lc ^ k_swz<HD>(r)))),
+          (lds_void*)(kd + c0), 16, 0, 0);
       __builtin_amdgcn_global_load_lds(
-          (global_void*)(A.vc + at + 8 * (c ^ v_swz<HD>(r))), (lds_void*)(kd + S::TILE + c0), 16,
-          0, 0);
+          (global_void*)(A.vc + row_at + (lane_at + 8 * (lc ^ v_swz<HD>(r)))),
+          (lds_void*)(kd + S::TILE + c0), 16, 0, 0);
     }
   };
+  auto bad_pages = [&]() {
+    int bad = 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u) bad |= (unsigned)page[u] >= (unsigned)A.num_blocks ? 1 << u : 0;
+    return bad;
+  };
 
-  float m = -INFINITY;  // running maximum of the row's scores (unscaled)
-  float l = 0.f;        // running sum, this lane's tokens
+  // The exponents' reference of the row, log2 units: the running maximum, or up to
+  // LAG below it (NO_REF before the first token), and the running sum of
+  // 2^(score - ref) over this lane's tokens.
+  float ref = NO_REF, l = 0.f;
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
 
-  if (rounds > 0 && wn < ntiles) stage(0, first + wn * KT);
+  int bad_next = 0;
+  if (wn < ntiles) {
+    look_up(first + wn * KT);
+    stage(0, first + wn * KT);
+    bad_next = bad_pages();
+    look_up(first + (wn + WN) * KT);
+  }
   for (int rd = 0; rd < rounds; ++rd) {
     const int tile = rd * WN + wn, base = first + tile * KT;
+    const int bad = bad_next;
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    if (tile + WN < ntiles) stage((rd + 1) & 1, base + WN * KT);
+    if (tile + WN < ntiles) {
+      stage((rd + 1) & 1, base + WN * KT);
+      bad_next = bad_pages();
+      look_up(base + 2 * WN * KT);
+    }
     if (tile >= ntiles) continue;
     const u32x4* const kt = lds + (rd & 1) * 2 * S::TILE;
     const uint16_t* const vt = reinterpret_cast<const uint16_t*>(kt + S::TILE);
@@ -186,26 +222,26 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     // ---- scores: s[u][4 a + b] is token 32 u + 8 a + 4 h + b of row n
     f32x16 s[NU];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
         const u32x4 a = kt[(32 * u + n) * CH + ((2 * ks + h) ^ k_swz<HD>(n))];
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
                                                        __builtin_bit_cast(bf16x8, qf[ks]), s[u],
                                                        0, 0, 0);
       }
-    }
-    // A table entry outside the cache is never dereferenced: its tokens' scores are
-    // NaN, and so is every row that sees one of them.
+    // the scores of tokens without a page are NaN, and so is every row that sees one
+    if (bad) {
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int pg = it.table[min(base + 32 * u, it.to - 1) >> A.bs_log2];
-      if ((unsigned)pg >= (unsigned)A.num_blocks) {
+      for (int u = 0; u < NU; ++u)
+        if (bad >> u & 1) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[u][i] = __builtin_nanf("");
-      }
+          for (int i = 0; i < 16; ++i) s[u][i] = __builtin_nanf("");
+        }
     }
     const bool masked = base < it.from || base + KT > lim_min;  // for some row of the wave
     if (masked) {
@@ -223,15 +259,20 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-    mx = fmaxf(m, xor_max<32>(mx));
-    const float ref = mx == -INFINITY ? 0.f : mx * A.scale_log2;
-    const float alpha = __builtin_amdgcn_exp2f(m * A.scale_log2 - ref);
-    m = mx;
-    l *= alpha;
+    mx = xor_max<32>(mx) * A.scale_log2;
+    // The reference follows the maximum only once that has grown by LAG: p is then
+    // at most 2^LAG, which neither fp32 nor bf16 minds, and most tiles leave o and
+    // l as they are.
+    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG)) {
+      const float next = fmaxf(ref, mx);
+      const float alpha = __builtin_amdgcn_exp2f(ref - next);
+      ref = next;
+      l *= alpha;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+        for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+    }
     uint32_t p[NU][8];
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -329,7 +370,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
         for (int i = 0; i < 16; ++i) dst[(16 * d + i) * 64 + lane] = o[d][i];
       if (h == 0) {
-        dst[32 * HD + n] = m;
+        dst[32 * HD + n] = ref;
         dst[32 * HD + 32 + n] = l;
       }
     }
@@ -338,11 +379,10 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
     for (int w = 1; w < WN; ++w) {
       const float* const src = jo + ((w - 1) * WM + wm) * (32 * HD + 64);
-      const float mo = src[32 * HD + n], lo = src[32 * HD + 32 + n];
-      const float mx = fmaxf(m, mo), ref = mx == -INFINITY ? 0.f : mx;
-      const float a = __builtin_amdgcn_exp2f((m - ref) * A.scale_log2);
-      const float b = __builtin_amdgcn_exp2f((mo - ref) * A.scale_log2);
-      m = mx;
+      const float ro = src[32 * HD + n], lo = src[32 * HD + 32 + n];
+      const float next = fmaxf(ref, ro);
+      const float a = __builtin_amdgcn_exp2f(ref - next), b = __builtin_amdgcn_exp2f(ro - next);
+      ref = next;
       l = l * a + lo * b;
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -365,7 +405,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   } else if (valid) {
     const int64_t prow = orow * it.slots + it.slot;
     if (h == 0)
-      st_agent(A.part_lse + prow, l == 0.f ? -INFINITY : m * A.scale_log2 + log2f(l));
+      st_agent(A.part_lse + prow, l == 0.f ? -INFINITY : ref + log2f(l));
     if (l != 0.f) {  // the merge reads no partial whose weight is none
       float* const dst = A.part_o + prow * HD;
 #pragma unroll
@@ -380,6 +420,12 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     }
   }
   stores_done();
+}
+
+// Tokens of each of `splits` parts of `range` tokens, whole rounds of the tiles.
+template <int ROUND>
+__device__ __forceinline__ int chunk_of(int range, int splits) {
+  return ((range + ROUND - 1) / ROUND + splits - 1) / splits * ROUND;
 }
 
 // Packed prompts.  Sequence r's queries are the tokens [query_start[r],
@@ -431,7 +477,7 @@ void prompt_attention_kernel(RowsArgs A) {
   const int ahead = L - nq;  // the position of the first query token
   const int last = (it.row0 + it.rows - 1) / A.group;
   const int range = max(ahead + last + 1, 0);
-  const int chunk = ((range + KT - 1) / KT + A.splits - 1) / A.splits * KT;
+  const int chunk = chunk_of<WN * KT>(range, A.splits);
   it.from = min(split * chunk, range);
   it.to = min(it.from + chunk, range);
   it.slot = split;
@@ -454,14 +500,14 @@ void shared_prefix_kernel(RowsArgs A) {
   Item it;
   it.slots = A.splits + A.suffix_splits;
   it.query_at = NO_QUERY;
-  const int y = blockIdx.y;
+  const int y = A.item0 + (int)blockIdx.y;
   if (y < A.tiles * A.splits) {
     const int split = y / A.tiles;
     it.table = A.prefix_table;
     it.token0 = 0;
     it.row0 = (y % A.tiles) * S::M;
     it.rows = min(S::M, A.num_seqs * A.group - it.row0);
-    const int chunk = ((prefix + KT - 1) / KT + A.splits - 1) / A.splits * KT;
+    const int chunk = chunk_of<WN * KT>(prefix, A.splits);
     it.from = min(split * chunk, prefix);
     it.to = min(it.from + chunk, prefix);
     it.slot = split;
@@ -479,8 +525,7 @@ void shared_prefix_kernel(RowsArgs A) {
     const int span = max(L - prefix, 0);
     // tiles are aligned to KT, so that a tile's halves of 32 tokens are within a page
     const int first = prefix & ~(KT - 1);
-    const int tiles = span ? (L - first + KT - 1) / KT : 0;
-    const int chunk = (tiles + A.suffix_splits - 1) / A.suffix_splits * KT;
+    const int chunk = chunk_of<WN * KT>(span ? L - first : 0, A.suffix_splits);
     it.to = min(first + (split + 1) * chunk, max(L, prefix));
     it.from = min(max(first + split * chunk, prefix), it.to);
     it.slot = A.splits + split;
@@ -560,25 +605,47 @@ int launch_merge(hipStream_t stream, const RowsArgs& a, int slots, bool prompts)
   return (int)hipGetLastError();
 }
 
-// Rows of a workgroup and splits of a tile's tokens.
+// Shapes of a workgroup: WM waves of 32 rows by WN groups that share the tokens,
+// tiles of KT tokens.
+constexpr int SHAPE_WM[] = {1, 2, 4, 8};
+
+int tune(const char* name, int v) {
+  const char* e = tuning_env(name);
+  return e ? atoi(e) : v;
+}
+
 struct Choice {
-  int wm, splits, suffix_splits, tiles;
+  int shape, splits, suffix_splits, tiles;
 };
+
+constexpr int MAX_SPLITS = 64;
 
 Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Choice c{};
-  c.wm = 4;
-  c.tiles = (int)((num_tokens * group + 32 * c.wm - 1) / (32 * c.wm) + num_seqs - 1);
-  c.splits = 1;
+  const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
+  c.shape = tune("SMX_PA_SHAPE", rows <= 32 ? 0 : rows <= 64 ? 1 : 2);
+  const int m = 32 * SHAPE_WM[c.shape];
+  c.tiles = (int)((num_tokens * group + m - 1) / m + num_seqs - 1);
+  const int64_t wgs = (rows + m - 1) / m * num_seqs * n_kv;
+  const int64_t most = std::min<int64_t>(MAX_SPLITS, (cap + 255) / 256);
+  const int target = tune("SMX_PA_TARGET", 512);
+  c.splits = (int)std::max<int64_t>(1, std::min(most, target / wgs));
+  c.splits = tune("SMX_PA_SPLITS", c.splits);
   return c;
 }
 
 Choice choose_prefix(int64_t num_seqs, int64_t prefix_cap, int64_t cap, int group, int n_kv) {
   Choice c{};
-  c.wm = 4;
-  c.tiles = (int)((num_seqs * group + 32 * c.wm - 1) / (32 * c.wm));
-  c.splits = 1;
-  c.suffix_splits = 1;
+  const int64_t rows = num_seqs * group;
+  c.shape = tune("SMX_SP_SHAPE", rows <= 32 ? 0 : rows <= 64 ? 1 : rows <= 128 ? 2 : 3);
+  const int m = 32 * SHAPE_WM[c.shape];
+  c.tiles = (int)((rows + m - 1) / m);
+  const int target = tune("SMX_SP_TARGET", 512);
+  c.splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>({MAX_SPLITS, (prefix_cap + 127) / 128, target / (c.tiles * n_kv)}));
+  c.suffix_splits = (int)std::max<int64_t>(
+      1, std::min<int64_t>({MAX_SPLITS, (cap + 511) / 512,
+                            tune("SMX_SP_STARGET", 512) / (num_seqs * n_kv)}));
   return c;
 }
 
@@ -587,21 +654,44 @@ int64_t partial_bytes(int64_t rows, int64_t slots, int hd) {
   return rows * slots * (hd + 1) * 4;
 }
 
+#define SMX_ROWS_LAUNCH(kernel, shape, grid)                                                      \
+  do {                                                                                            \
+    if (shape == 0)                                                                               \
+      SMX_LAUNCH((kernel<HD, 1, 4, 32, 1>), grid, dim3(256), 0, stream, a);                       \
+    else if (shape == 1)                                                                          \
+      SMX_LAUNCH((kernel<HD, 2, 2, 64, 1>), grid, dim3(256), 0, stream, a);                       \
+    else if (shape == 2)                                                                          \
+      SMX_LAUNCH((kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);                       \
+    else                                                                                          \
+      SMX_LAUNCH((kernel<HD, 8, 1, 64, 2>), grid, dim3(512), 0, stream, a);                       \
+  } while (0)
+
 template <int HD>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  const dim3 grid(a.n_kv, c.tiles, c.splits);
-  SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
+  SMX_ROWS_LAUNCH(prompt_attention_kernel, c.shape, dim3(a.n_kv, c.tiles, c.splits));
   const int rc = (int)hipGetLastError();
   return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, true);
 }
 
+// One launch for the prefix and the sequences' own tokens where one shape suits
+// both, else one each.
 template <int HD>
 int launch_prefix(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  const int gt = (a.group + 32 * c.wm - 1) / (32 * c.wm);
-  const dim3 grid(a.n_kv, c.tiles * c.splits + a.num_seqs * c.suffix_splits * gt, 1);
-  SMX_LAUNCH((shared_prefix_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
-  const int rc = (int)hipGetLastError();
-  return rc ? rc : launch_merge<HD>(stream, a, c.splits + c.suffix_splits, false);
+  const int prefix_items = c.tiles * c.splits;
+  const bool one = c.shape == 0;
+  a.item0 = 0;
+  const int suffix_items = a.num_seqs * c.suffix_splits * ((a.group + 31) / 32);
+  SMX_ROWS_LAUNCH(shared_prefix_kernel, c.shape,
+                  dim3(a.n_kv, one ? prefix_items + suffix_items : prefix_items));
+  int rc = (int)hipGetLastError();
+  if (rc) return rc;
+  if (!one) {
+    a.item0 = prefix_items;
+    SMX_ROWS_LAUNCH(shared_prefix_kernel, 0, dim3(a.n_kv, suffix_items));
+    rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
+  return launch_merge<HD>(stream, a, c.splits + c.suffix_splits, false);
 }
 
 }  // namespace
