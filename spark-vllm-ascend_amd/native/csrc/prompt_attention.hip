@@ -20,6 +20,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "smx_common.h"
 #include "smx_launch.h"
@@ -33,6 +34,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) uint16_t lds_u16;
+typedef __attribute__((address_space(4))) int32_t constant_i32;
 
 // (lo, hi) as one v_cvt_pk_bf16_f32
 __device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
@@ -82,13 +86,14 @@ struct Item {
 };
 
 // HD: head_dim.  WM waves take 32 rows each, WN groups of them take every WN-th
-// tile of KT tokens; a group's tile of K and V is in LDS, two tiles deep.
-template <int HD, int WM, int WN, int KT>
+// tile of KT tokens; ST tiles of K and V a group are in LDS, one that is read and
+// ST - 1 that are on their way.
+template <int HD, int WM, int WN, int KT, int ST>
 struct Shape {
   static constexpr int M = 32 * WM, NT = 64 * WM * WN;
   static constexpr int CH = HD / 8;                  // 16-byte chunks of a row
   static constexpr int TILE = KT * CH;               // chunks of a K or V tile
-  static constexpr int GROUP = 2 * 2 * TILE;         // two buffers of K and V
+  static constexpr int GROUP = ST * 2 * TILE;        // the buffers of K and V
   static constexpr int JOIN = WN > 1 ? (WN - 1) * WM * (32 * HD + 64) / 4 : 0;
   static constexpr int LDS = WN * GROUP > JOIN ? WN * GROUP : JOIN;
   static constexpr int LOADS = TILE / 64 / WM;       // a wave's loads of a K (V) tile
@@ -107,9 +112,20 @@ __device__ __forceinline__ int v_swz(int r) {
   return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
 }
 
-template <int HD, int WM, int WN, int KT>
+// s_waitcnt operand: at most `vm` vector loads outstanding, no LDS operation
+constexpr int wait_vm(int vm) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4); }
+
+// Every wave of the workgroup is here.  (__syncthreads would also wait for all
+// vector loads.)
+__device__ __forceinline__ void meet() {
+  __asm__ volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __asm__ volatile("" ::: "memory");
+}
+
+template <int HD, int WM, int WN, int KT, int ST>
 __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
-  using S = Shape<HD, WM, WN, KT>;
+  using S = Shape<HD, WM, WN, KT, ST>;
   constexpr int KS = HD / 16, DT = HD / 32, NU = KT / 32, CH = S::CH;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -143,45 +159,55 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   for (int o = 1; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o));
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
 
-  // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile.  The
-  // pages of a tile's halves of 32 tokens (within a page each) are looked up a
-  // round before they are used; an entry outside the cache is never dereferenced.
+  // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile, by
+  // buffer loads into LDS whose resource is one half of 32 tokens (within a page):
+  // tokens past the end, and those of a table entry outside the cache, are past
+  // the resource's end and read as 0 without an access.  Pages are looked up a
+  // round before they are used, by scalar loads (the table is constant while the
+  // kernel runs), which do not queue behind the tiles' loads.
   const int first = it.from & ~(KT - 1);
   const int ntiles = it.to > it.from ? (it.to - first + KT - 1) / KT : 0;
   const int rounds = (ntiles + WN - 1) / WN;
-  u32x4* const lds = smem + wn * S::GROUP;
+  lds_u32x4* const lds = (lds_u32x4*)smem + wn * S::GROUP;
   const int lrow = lane / CH, lc = lane % CH;  // the lane's row and chunk of a load
-  int page[NU];
-  auto look_up = [&](int base) {
+  const int tok_bytes = 2 * tok_stride;
+  const constant_i32* const table = (const constant_i32*)it.table;
+  auto look_up = [&](int (&page)[NU], int base) {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
-      page[u] = it.table[min(base + 32 * u, it.to - 1) >> A.bs_log2];
+      page[u] = table[max(min(base + 32 * u, it.to - 1), 0) >> A.bs_log2];
   };
-  auto stage = [&](int buf, int base) {
-    u32x4* const kd = lds + buf * 2 * S::TILE;
-    const bool whole = base + KT <= it.to;
+  auto stage = [&](const uint16_t* cache, lds_u32x4* dst, const int (&page)[NU], int base,
+                   auto swz) {
+    __amdgpu_buffer_rsrc_t half[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      const int t = base + 32 * u;
+      const bool known = (unsigned)page[u] < (unsigned)A.num_blocks;
+      const int rows = known ? min(it.to - t, 32) : 0;
+      const uint16_t* const at = cache + (int64_t)(known ? page[u] : 0) * page_stride +
+                                 (t & (bs - 1)) * tok_stride + kvh * HD;
+      half[u] = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)at, 0, rows > 0 ? (rows - 1) * tok_bytes + 2 * HD : 0, 0x00027000);
+    }
 #pragma unroll
     for (int i = 0; i < S::LOADS; ++i) {
       const int c0 = (i * WM + wm) * 64;  // first chunk of this load
-      const int r0 = c0 / CH;             // first row
-      const int raw = NU == 2 && r0 >= 32 ? page[NU - 1] : page[0];
-      const int pg = (unsigned)raw < (unsigned)A.num_blocks ? raw : 0;
-      const int64_t at = (int64_t)pg * page_stride + kvh * HD;
-      // tokens past the end are the last one
-      const int t0 = whole ? base + r0 : min(base + r0, it.to - 1);
-      const uint32_t dr = whole ? lrow : min(lrow, it.to - 1 - t0);
-      const int64_t row_at = at + (int64_t)(t0 & (bs - 1)) * tok_stride;
-      const uint32_t lane_at = dr * (uint32_t)tok_stride;
-      const int r = r0 + lrow;
-      __builtin_amdgcn_global_load_lds(
-          (global_void*)(A.kc + row_at + (lane_at + 8 * (lc ^ k_swz<HD>(r)))),
-          (lds_void*)(kd + c0), 16, 0, 0);
-      __builtin_amdgcn_global_load_lds(
-          (global_void*)(A.vc + row_at + (lane_at + 8 * (lc ^ v_swz<HD>(r)))),
-          (lds_void*)(kd + S::TILE + c0), 16, 0, 0);
+      const int r0 = c0 / CH;             // its row
+      const int off = lrow * tok_bytes + 16 * (lc ^ swz(r0 + lrow));
+      const __amdgpu_buffer_rsrc_t src =
+          i * WM * 64 / CH >= 32 || (NU == 2 && r0 >= 32) ? half[NU - 1] : half[0];
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(dst + c0), 16, off,
+                                               (r0 & 31) * tok_bytes, 0, 0);
     }
   };
-  auto bad_pages = [&]() {
+  auto stage_k = [&](lds_u32x4* dst, const int (&page)[NU], int base) {
+    stage(A.kc, dst, page, base, [](int r) { return k_swz<HD>(r); });
+  };
+  auto stage_v = [&](lds_u32x4* dst, const int (&page)[NU], int base) {
+    stage(A.vc, dst, page, base, [](int r) { return v_swz<HD>(r); });
+  };
+  auto bad_pages = [&](const int (&page)[NU]) {
     int bad = 0;
 #pragma unroll
     for (int u = 0; u < NU; ++u) bad |= (unsigned)page[u] >= (unsigned)A.num_blocks ? 1 << u : 0;
@@ -197,30 +223,10 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  f32x16 s[NU];       // scores: s[u][4 a + b] is token 32 u + 8 a + 4 h + b of row n
+  uint32_t p[NU][8];  // and their 2^(score - ref), bf16 pairs
 
-  int bad_next = 0;
-  if (wn < ntiles) {
-    look_up(first + wn * KT);
-    stage(0, first + wn * KT);
-    bad_next = bad_pages();
-    look_up(first + (wn + WN) * KT);
-  }
-  for (int rd = 0; rd < rounds; ++rd) {
-    const int tile = rd * WN + wn, base = first + tile * KT;
-    const int bad = bad_next;
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (tile + WN < ntiles) {
-      stage((rd + 1) & 1, base + WN * KT);
-      bad_next = bad_pages();
-      look_up(base + 2 * WN * KT);
-    }
-    if (tile >= ntiles) continue;
-    const u32x4* const kt = lds + (rd & 1) * 2 * S::TILE;
-    const uint16_t* const vt = reinterpret_cast<const uint16_t*>(kt + S::TILE);
-
-    // ---- scores: s[u][4 a + b] is token 32 u + 8 a + 4 h + b of row n
-    f32x16 s[NU];
+  auto scores = [&](const lds_u32x4* kt) {
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -234,26 +240,25 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                                                        __builtin_bit_cast(bf16x8, qf[ks]), s[u],
                                                        0, 0, 0);
       }
+  };
+  // A plain tile: every row of the wave sees all of it, and its pages are known.  The
+  // others have code of their own, so that the accumulators are not moved at every
+  // tile where the paths join.
+  auto is_plain = [&](int base, int bad) {
+    return base >= it.from && base + KT <= lim_min && !bad;
+  };
+  auto softmax = [&](auto plain, int base, int bad) {
     // the scores of tokens without a page are NaN, and so is every row that sees one
-    if (bad) {
-#pragma unroll
-      for (int u = 0; u < NU; ++u)
-        if (bad >> u & 1) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[u][i] = __builtin_nanf("");
-        }
-    }
-    const bool masked = base < it.from || base + KT > lim_min;  // for some row of the wave
-    if (masked) {
+    if constexpr (!plain) {
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = base + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
-          s[u][i] = t >= it.from && t < lim ? s[u][i] : -INFINITY;
+          const float x = bad >> u & 1 ? __builtin_nanf("") : s[u][i];
+          s[u][i] = t >= it.from && t < lim ? x : -INFINITY;
         }
     }
-    // ---- online softmax
     float mx = s[0][0];
 #pragma unroll
     for (int u = 0; u < NU; ++u)
@@ -273,77 +278,80 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
     }
-    uint32_t p[NU][8];
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], A.scale_log2, -ref));
         const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], A.scale_log2, -ref));
-        l += p0;
-        l += p1;
+        part[2 * (i & 1)] += p0;
+        part[2 * (i & 1) + 1] += p1;
         p[u][i] = cvt_pk_bf16(p0, p1);
       }
-    // ---- O^T += V^T P^T
-    const int vr = 4 * h + ((lane & 15) >> 2), vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    auto v_operand = [&](int kk, int d) -> u32x4 {  // V of 16 tokens, dims 32 d + n
-      u32x2 half[2];
+    l += (part[0] + part[1]) + (part[2] + part[3]);
+  };
+  // O^T += V^T P^T
+  const int vr = 4 * h + ((lane & 15) >> 2), vcol = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  auto v_operand = [&](const lds_u16* vt, int kk, int d) -> u32x4 {  // 16 tokens, dims 32 d + n
+    u32x2 half[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int r = 16 * kk + 8 * j + vr;
-        const uint16_t* src = vt + (r * CH + ((4 * d + vc) ^ v_swz<HD>(r))) * 8 + 4 * (lane & 1);
-        half[j] = __builtin_bit_cast(u32x2,
-                                     __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src));
-      }
-      return u32x4{half[0].x, half[0].y, half[1].x, half[1].y};
-    };
-    // A masked token must not reach a row by 0 * infinity or 0 * NaN: where a
-    // tile that some row sees in part holds such values (0 * V tells), they are
-    // left out of the product and added to the rows that see them.
+    for (int j = 0; j < 2; ++j) {
+      const int r = 16 * kk + 8 * j + vr;
+      const lds_u16* src = vt + (r * CH + ((4 * d + vcol) ^ v_swz<HD>(r))) * 8 + 4 * (lane & 1);
+      half[j] = __builtin_bit_cast(u32x2,
+                                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)src));
+    }
+    return u32x4{half[0].x, half[0].y, half[1].x, half[1].y};
+  };
+  auto p_operand = [&](int kk) -> u32x4 {
+    return u32x4{p[kk / 2][4 * (kk & 1)], p[kk / 2][4 * (kk & 1) + 1],
+                 p[kk / 2][4 * (kk & 1) + 2], p[kk / 2][4 * (kk & 1) + 3]};
+  };
+  // A masked token must not reach a row by 0 * infinity or 0 * NaN: where a tile
+  // that some row sees in part holds such values (0 * V tells), they are left out
+  // of the product and added to the rows that see them.
+  auto odd_values = [&](const lds_u16* vt) {
+    f32x16 z;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i] = 0.f;
+    const u32x4 none = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int kk = 0; kk < 2 * NU; ++kk)
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+        z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            __builtin_bit_cast(bf16x8, v_operand(vt, kk, d)), __builtin_bit_cast(bf16x8, none), z,
+            0, 0, 0);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += z[i];
+    return __builtin_amdgcn_ballot_w64(sum != sum) != 0;
+  };
+  auto weigh = [&](auto plain, const lds_u32x4* vtile, int base) {
+    const lds_u16* const vt = (const lds_u16*)vtile;
     bool odd = false;
-    if (masked) {
-      f32x16 z;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) z[i] = 0.f;
-      const u32x4 none = u32x4{0u, 0u, 0u, 0u};
+    if constexpr (!plain) odd = odd_values(vt);
+    if (!odd) {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-          z = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, v_operand(kk, d)), __builtin_bit_cast(bf16x8, none), z,
-              0, 0, 0);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += z[i];
-      odd = __builtin_amdgcn_ballot_w64(sum != sum) != 0;
-    }
-    if (!odd) {
-#pragma unroll
-      for (int kk = 0; kk < 2 * NU; ++kk) {
-        const u32x4 b = {p[kk / 2][4 * (kk & 1)], p[kk / 2][4 * (kk & 1) + 1],
-                         p[kk / 2][4 * (kk & 1) + 2], p[kk / 2][4 * (kk & 1) + 3]};
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, v_operand(kk, d)), __builtin_bit_cast(bf16x8, b), o[d],
-              0, 0, 0);
-      }
+              __builtin_bit_cast(bf16x8, v_operand(vt, kk, d)),
+              __builtin_bit_cast(bf16x8, p_operand(kk)), o[d], 0, 0, 0);
     } else {
 #pragma unroll
-      for (int kk = 0; kk < 2 * NU; ++kk) {
-        const u32x4 b = {p[kk / 2][4 * (kk & 1)], p[kk / 2][4 * (kk & 1) + 1],
-                         p[kk / 2][4 * (kk & 1) + 2], p[kk / 2][4 * (kk & 1) + 3]};
+      for (int kk = 0; kk < 2 * NU; ++kk)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          u32x4 a = v_operand(kk, d);
+          u32x4 a = v_operand(vt, kk, d);
           a = u32x4{finite_bf16x2(a.x), finite_bf16x2(a.y), finite_bf16x2(a.z),
                     finite_bf16x2(a.w)};
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                         __builtin_bit_cast(bf16x8, b), o[d], 0,
-                                                         0, 0);
+                                                         __builtin_bit_cast(bf16x8, p_operand(kk)),
+                                                         o[d], 0, 0, 0);
         }
-      }
       for (int r = 0; r < KT; ++r) {
         const bool seen = base + r >= it.from && base + r < lim;
 #pragma unroll
@@ -354,6 +362,145 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
             const uint32_t v = vt[(r * CH + ((dim / 8) ^ v_swz<HD>(r))) * 8 + dim % 8];
             if (seen && (v & 0x7f80u) == 0x7f80u) o[d][i] += bf16_bits_to_f32(v);
           }
+      }
+    }
+  };
+
+  if constexpr (WM < 8) {
+    // One round after another: the loads of the tile ST - 1 rounds ahead into `next`,
+    // whose last readers are past the barrier, then the tile in `cur`.  Both are
+    // restrict so that the compiler does not wait for the loads into the one before
+    // it reads the other; the wait that counts is the one before the barrier.
+    int bad[ST];  // of the tiles in LDS, that of this round first
+    int page[NU];
+#pragma unroll
+    for (int i = 0; i < ST; ++i) bad[i] = 0;
+    look_up(page, first + wn * KT);
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) {
+      const int tile = i * WN + wn, base = first + tile * KT;
+      if (tile < ntiles) {
+        lds_u32x4* const dst = lds + i * 2 * S::TILE;
+        stage_k(dst, page, base);
+        stage_v(dst + S::TILE, page, base);
+        bad[i] = bad_pages(page);
+        look_up(page, base + WN * KT);
+      }
+    }
+    auto round = [&](auto plain, lds_u32x4* __restrict__ next, const lds_u32x4* __restrict__ cur,
+                     int tile) {
+      const int base = first + tile * KT, ahead = base + (ST - 1) * WN * KT;
+      if (tile + (ST - 1) * WN < ntiles) {
+        stage_k(next, page, ahead);
+        stage_v(next + S::TILE, page, ahead);
+        bad[ST - 1] = bad_pages(page);
+        look_up(page, ahead + WN * KT);
+      }
+      if (!plain && tile >= ntiles) return;
+      scores(cur);
+      softmax(plain, base, bad[0]);
+      weigh(plain, cur + S::TILE, base);
+    };
+    int at = 0, rd = 0;  // the buffer of this round's tile
+    auto step = [&](auto plain) {
+      // this wave's loads of the tile have arrived (those of later ones may be on
+      // their way), then every wave's have, and the last round's tile is read out
+      if (ST > 2 && (rd + ST - 2) * WN + wn < ntiles)
+        __builtin_amdgcn_s_waitcnt(wait_vm((ST - 2) * 2 * S::LOADS));
+      else
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+      meet();
+      const int before = at == 0 ? ST - 1 : at - 1;
+      round(plain, lds + before * 2 * S::TILE, lds + at * 2 * S::TILE, rd * WN + wn);
+      at = at == ST - 1 ? 0 : at + 1;
+#pragma unroll
+      for (int i = 0; i < ST - 1; ++i) bad[i] = bad[i + 1];
+      ++rd;
+    };
+    while (rd < rounds) {
+      while (rd * WN + wn < ntiles && is_plain(first + (rd * WN + wn) * KT, bad[0]))
+        step(std::true_type{});
+      if (rd < rounds) step(std::false_type{});
+    }
+  } else {
+    // Two groups of waves, one wave of each on every SIMD, in opposite phases: while
+    // one multiplies (the tile's scores and the last tile's weighted V, from LDS),
+    // the other does its softmax, so that neither the matrix nor the vector units
+    // wait for the other.  Barriers separate the slots: group g multiplies for tile i
+    // in slot 2 i + g and weighs it in slot 2 i + g + 1; tile i's K is read out
+    // after slot 2 i + 1, its V after slot 2 i + 3.  In slot 2 i all waves load
+    // K of tile i + ST - 1 and V of tile i + ST - 2, into the buffers read out last;
+    // they must have arrived before slot 2 (i + 1) where ST is 2, ST - 2 pairs of
+    // slots later otherwise.
+    constexpr int D = ST - 1;
+    const int g = wm / 4;
+    lds_u32x4* const vlds = lds + ST * S::TILE;
+    int kpage[NU], vpage[NU], bad[ST + 1];
+#pragma unroll
+    for (int i = 0; i <= ST; ++i) bad[i] = 0;
+    look_up(kpage, first);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) vpage[u] = kpage[u];
+    int kat = 0, vat = 0;  // the buffers that are loaded next
+    auto load = [&](int i) {  // K of tile i + D, V of tile i + D - 1
+      if (i + D - 1 >= 0 && i + D - 1 < ntiles) {
+        stage_v(vlds + vat * S::TILE, vpage, first + (i + D - 1) * KT);
+        vat = vat == ST - 1 ? 0 : vat + 1;
+      }
+      if (i + D < ntiles) {
+        stage_k(lds + kat * S::TILE, kpage, first + (i + D) * KT);
+        kat = kat == ST - 1 ? 0 : kat + 1;
+        bad[D] = bad_pages(kpage);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) vpage[u] = kpage[u];
+        look_up(kpage, first + (i + D + 1) * KT);
+      }
+    };
+    auto arrived = [&](int i) {  // what load(i - D + 1) asked for
+      if (D > 1 && i + D < ntiles)
+        __builtin_amdgcn_s_waitcnt(wait_vm((D - 1) * 2 * S::LOADS));
+      else
+        __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    };
+    int kr = 0, vrd = 0;  // the buffers that are read next
+    auto multiply = [&](const lds_u32x4* __restrict__ kt, const lds_u32x4* __restrict__ vt,
+                        int i) {
+      if (i > 0) weigh(std::false_type{}, vt, first + (i - 1) * KT);
+      if (i < ntiles) scores(kt);
+    };
+    if (ntiles > 0) {
+#pragma unroll
+      for (int i = -D; i < 0; ++i) {
+        load(i);
+#pragma unroll
+        for (int j = 0; j < D; ++j) bad[j] = bad[j + 1];
+      }
+      arrived(-1);
+      meet();
+      if (g == 1) {
+        load(0);
+        meet();
+      }
+      for (int i = 0;; ++i) {
+        if (g == 0) load(i);
+        __builtin_amdgcn_s_setprio(1);
+        multiply(lds + kr * S::TILE, vlds + vrd * S::TILE, i);
+        __builtin_amdgcn_s_setprio(0);
+        kr = kr == ST - 1 ? 0 : kr + 1;
+        if (i > 0) vrd = vrd == ST - 1 ? 0 : vrd + 1;
+        if (g == 1) arrived(i);
+        if (i == ntiles) {
+          if (g == 0) meet();
+          break;
+        }
+        meet();
+        const int bad_now = bad[0];
+#pragma unroll
+        for (int j = 0; j < D; ++j) bad[j] = bad[j + 1];
+        if (g == 1) load(i + 1);
+        softmax(std::false_type{}, first + i * KT, bad_now);
+        if (g == 0) arrived(i);
+        meet();
       }
     }
   }
@@ -433,10 +580,10 @@ __device__ __forceinline__ int chunk_of(int range, int splits) {
 // L - n + i and sees the tokens up to itself.  Grid: kv heads, row tiles (last
 // first: the longest come first), splits.  Which sequence a tile is of follows
 // from the prefix sums of the tile counts, 64 sequences at a time.
-template <int HD, int WM, int WN, int KT, int EU>
+template <int HD, int WM, int WN, int KT, int ST, int EU>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
 void prompt_attention_kernel(RowsArgs A) {
-  using S = Shape<HD, WM, WN, KT>;
+  using S = Shape<HD, WM, WN, KT, ST>;
   __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
   const int lane = threadIdx.x & 63;
   const int kvh = blockIdx.x, tile = A.tiles - 1 - (int)blockIdx.y, split = blockIdx.z;
@@ -483,16 +630,16 @@ void prompt_attention_kernel(RowsArgs A) {
   it.slot = split;
   it.slots = A.splits;
   it.query_at = ahead;
-  attend<HD, WM, WN, KT>(A, it, kvh, smem);
+  attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
 }
 
 // Decode rows (one token a sequence) under a shared prefix.  Grid: kv heads,
 // items: first the prefix, row tiles of all sequences' rows times its splits,
 // then each sequence's own tokens [prefix, L) in its splits.
-template <int HD, int WM, int WN, int KT, int EU>
+template <int HD, int WM, int WN, int KT, int ST, int EU>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
 void shared_prefix_kernel(RowsArgs A) {
-  using S = Shape<HD, WM, WN, KT>;
+  using S = Shape<HD, WM, WN, KT, ST>;
   __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
   const int kvh = blockIdx.x;
   const int prefix = min(max(A.prefix_len[0], 0), A.prefix_blocks << A.bs_log2);
@@ -530,7 +677,7 @@ void shared_prefix_kernel(RowsArgs A) {
     it.from = min(max(first + split * chunk, prefix), it.to);
     it.slot = A.splits + split;
   }
-  attend<HD, WM, WN, KT>(A, it, kvh, smem);
+  attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
 }
 
 // out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a row's partials, a
@@ -657,13 +804,13 @@ int64_t partial_bytes(int64_t rows, int64_t slots, int hd) {
 #define SMX_ROWS_LAUNCH(kernel, shape, grid)                                                      \
   do {                                                                                            \
     if (shape == 0)                                                                               \
-      SMX_LAUNCH((kernel<HD, 1, 4, 32, 1>), grid, dim3(256), 0, stream, a);                       \
+      SMX_LAUNCH((kernel<HD, 1, 4, 32, 2, 1>), grid, dim3(256), 0, stream, a);                    \
     else if (shape == 1)                                                                          \
-      SMX_LAUNCH((kernel<HD, 2, 2, 64, 1>), grid, dim3(256), 0, stream, a);                       \
+      SMX_LAUNCH((kernel<HD, 2, 2, 64, 2, 1>), grid, dim3(256), 0, stream, a);                    \
     else if (shape == 2)                                                                          \
-      SMX_LAUNCH((kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);                       \
+      SMX_LAUNCH((kernel<HD, 4, 1, 64, 2, 2>), grid, dim3(256), 0, stream, a);                    \
     else                                                                                          \
-      SMX_LAUNCH((kernel<HD, 8, 1, 64, 2>), grid, dim3(512), 0, stream, a);                       \
+      SMX_LAUNCH((kernel<HD, 8, 1, 64, 2, 2>), grid, dim3(512), 0, stream, a);                    \
   } while (0)
 
 template <int HD>
