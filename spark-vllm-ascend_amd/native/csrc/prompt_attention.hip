@@ -66,12 +66,15 @@ struct RowsArgs {
   uint16_t* out;
   float* part_o;    // [rows, slots, HD], where slots > 1
   float* part_lse;  // [rows, slots], log2 units
+  int32_t* counts;  // [rows] slots in use, of the prefix's and then [rows] of the suffix's
   int64_t q_stride;  // elements from a token's q to the next token's
   int num_tokens, num_seqs, max_blocks, prefix_blocks, num_blocks, bs_log2, n_q, n_kv, group;
-  int splits;         // of a tile's tokens (prompts), of the prefix (shared prefix)
-  int suffix_splits;  // of each sequence's own tokens (shared prefix)
-  int tiles;          // row tiles the grid has room for
-  int item0;          // the first item of this launch (shared prefix)
+  int splits;         // most parts of a tile's tokens (prompts), of the prefix (shared prefix)
+  int suffix_splits;  // most parts of a sequence's own tokens (shared prefix)
+  int tiles;          // row tiles: the most there can be (prompts), of the prefix's rows
+  int target;         // workgroups a kv head to aim at
+  int least;          // rounds of a part at least (prompts)
+  int zigzag;         // period of the order of the tiles (prompts)
   float scale_log2;
 };
 
@@ -83,6 +86,9 @@ constexpr int NO_QUERY = INT_MIN;
 struct Item {
   const int32_t* table;
   int token0, row0, rows, from, to, slot, slots, query_at;
+  int32_t* counts;  // where the first part's workgroup writes `parts` for its rows, or null
+  int parts;
+  bool direct;  // the only part of its rows: the output itself, no partial
 };
 
 // HD: head_dim.  WM waves take 32 rows each, WN groups of them take every WN-th
@@ -366,150 +372,70 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     }
   };
 
-  if constexpr (WM < 8) {
-    // One round after another: the loads of the tile ST - 1 rounds ahead into `next`,
-    // whose last readers are past the barrier, then the tile in `cur`.  Both are
-    // restrict so that the compiler does not wait for the loads into the one before
-    // it reads the other; the wait that counts is the one before the barrier.
-    int bad[ST];  // of the tiles in LDS, that of this round first
-    int page[NU];
+  // One round after another: the loads of the tile ST - 1 rounds ahead into `next`,
+  // whose last readers are past the barrier, then the tile in `cur`.  Both are
+  // restrict so that the compiler does not wait for the loads into the one before
+  // it reads the other; the wait that counts is the one before the barrier.
+  int bad[ST];  // of the tiles in LDS, that of this round first
+  int page[NU];
 #pragma unroll
-    for (int i = 0; i < ST; ++i) bad[i] = 0;
-    look_up(page, first + wn * KT);
+  for (int i = 0; i < ST; ++i) bad[i] = 0;
+  look_up(page, first + wn * KT);
 #pragma unroll
-    for (int i = 0; i < ST - 1; ++i) {
-      const int tile = i * WN + wn, base = first + tile * KT;
-      if (tile < ntiles) {
-        lds_u32x4* const dst = lds + i * 2 * S::TILE;
-        stage_k(dst, page, base);
-        stage_v(dst + S::TILE, page, base);
-        bad[i] = bad_pages(page);
-        look_up(page, base + WN * KT);
-      }
+  for (int i = 0; i < ST - 1; ++i) {
+    const int tile = i * WN + wn, base = first + tile * KT;
+    if (tile < ntiles) {
+      lds_u32x4* const dst = lds + i * 2 * S::TILE;
+      stage_k(dst, page, base);
+      stage_v(dst + S::TILE, page, base);
+      bad[i] = bad_pages(page);
+      look_up(page, base + WN * KT);
     }
-    auto round = [&](auto plain, lds_u32x4* __restrict__ next, const lds_u32x4* __restrict__ cur,
-                     int tile) {
-      const int base = first + tile * KT, ahead = base + (ST - 1) * WN * KT;
-      if (tile + (ST - 1) * WN < ntiles) {
-        stage_k(next, page, ahead);
-        stage_v(next + S::TILE, page, ahead);
-        bad[ST - 1] = bad_pages(page);
-        look_up(page, ahead + WN * KT);
-      }
-      if (!plain && tile >= ntiles) return;
-      scores(cur);
-      softmax(plain, base, bad[0]);
-      weigh(plain, cur + S::TILE, base);
-    };
-    int at = 0, rd = 0;  // the buffer of this round's tile
-    auto step = [&](auto plain) {
-      // this wave's loads of the tile have arrived (those of later ones may be on
-      // their way), then every wave's have, and the last round's tile is read out
-      if (ST > 2 && (rd + ST - 2) * WN + wn < ntiles)
-        __builtin_amdgcn_s_waitcnt(wait_vm((ST - 2) * 2 * S::LOADS));
-      else
-        __builtin_amdgcn_s_waitcnt(wait_vm(0));
-      meet();
-      const int before = at == 0 ? ST - 1 : at - 1;
-      round(plain, lds + before * 2 * S::TILE, lds + at * 2 * S::TILE, rd * WN + wn);
-      at = at == ST - 1 ? 0 : at + 1;
-#pragma unroll
-      for (int i = 0; i < ST - 1; ++i) bad[i] = bad[i + 1];
-      ++rd;
-    };
-    while (rd < rounds) {
-      while (rd * WN + wn < ntiles && is_plain(first + (rd * WN + wn) * KT, bad[0]))
-        step(std::true_type{});
-      if (rd < rounds) step(std::false_type{});
+  }
+  auto round = [&](auto plain, lds_u32x4* __restrict__ next, const lds_u32x4* __restrict__ cur,
+                   int tile) {
+    const int base = first + tile * KT, ahead = base + (ST - 1) * WN * KT;
+    // (a tile past the end is of no rows: a plain round loads nothing there, without
+    // the branch that would keep the addresses' arithmetic from the products' shadow)
+    if (plain || tile + (ST - 1) * WN < ntiles) {
+      stage_k(next, page, ahead);
+      stage_v(next + S::TILE, page, ahead);
+      bad[ST - 1] = bad_pages(page);
+      look_up(page, ahead + WN * KT);
     }
-  } else {
-    // Two groups of waves, one wave of each on every SIMD, in opposite phases: while
-    // one multiplies (the tile's scores and the last tile's weighted V, from LDS),
-    // the other does its softmax, so that neither the matrix nor the vector units
-    // wait for the other.  Barriers separate the slots: group g multiplies for tile i
-    // in slot 2 i + g and weighs it in slot 2 i + g + 1; tile i's K is read out
-    // after slot 2 i + 1, its V after slot 2 i + 3.  In slot 2 i all waves load
-    // K of tile i + ST - 1 and V of tile i + ST - 2, into the buffers read out last;
-    // they must have arrived before slot 2 (i + 1) where ST is 2, ST - 2 pairs of
-    // slots later otherwise.
-    constexpr int D = ST - 1;
-    const int g = wm / 4;
-    lds_u32x4* const vlds = lds + ST * S::TILE;
-    int kpage[NU], vpage[NU], bad[ST + 1];
+    if ((!plain && tile >= ntiles) || 32 * wm >= it.rows) return;
+    scores(cur);
+    softmax(plain, base, bad[0]);
+    weigh(plain, cur + S::TILE, base);
+  };
+  int at = 0, rd = 0;  // the buffer of this round's tile
+  auto step = [&](auto plain) {
+    // this wave's loads of the tile have arrived (those of later ones may be on
+    // their way), then every wave's have, and the last round's tile is read out
+    if (ST > 2 && (rd + ST - 2) * WN + wn < ntiles)
+      __builtin_amdgcn_s_waitcnt(wait_vm((ST - 2) * 2 * S::LOADS));
+    else
+      __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    meet();
+    const int before = at == 0 ? ST - 1 : at - 1;
+    round(plain, lds + before * 2 * S::TILE, lds + at * 2 * S::TILE, rd * WN + wn);
+    at = at == ST - 1 ? 0 : at + 1;
 #pragma unroll
-    for (int i = 0; i <= ST; ++i) bad[i] = 0;
-    look_up(kpage, first);
-#pragma unroll
-    for (int u = 0; u < NU; ++u) vpage[u] = kpage[u];
-    int kat = 0, vat = 0;  // the buffers that are loaded next
-    auto load = [&](int i) {  // K of tile i + D, V of tile i + D - 1
-      if (i + D - 1 >= 0 && i + D - 1 < ntiles) {
-        stage_v(vlds + vat * S::TILE, vpage, first + (i + D - 1) * KT);
-        vat = vat == ST - 1 ? 0 : vat + 1;
-      }
-      if (i + D < ntiles) {
-        stage_k(lds + kat * S::TILE, kpage, first + (i + D) * KT);
-        kat = kat == ST - 1 ? 0 : kat + 1;
-        bad[D] = bad_pages(kpage);
-#pragma unroll
-        for (int u = 0; u < NU; ++u) vpage[u] = kpage[u];
-        look_up(kpage, first + (i + D + 1) * KT);
-      }
-    };
-    auto arrived = [&](int i) {  // what load(i - D + 1) asked for
-      if (D > 1 && i + D < ntiles)
-        __builtin_amdgcn_s_waitcnt(wait_vm((D - 1) * 2 * S::LOADS));
-      else
-        __builtin_amdgcn_s_waitcnt(wait_vm(0));
-    };
-    int kr = 0, vrd = 0;  // the buffers that are read next
-    auto multiply = [&](const lds_u32x4* __restrict__ kt, const lds_u32x4* __restrict__ vt,
-                        int i) {
-      if (i > 0) weigh(std::false_type{}, vt, first + (i - 1) * KT);
-      if (i < ntiles) scores(kt);
-    };
-    if (ntiles > 0) {
-#pragma unroll
-      for (int i = -D; i < 0; ++i) {
-        load(i);
-#pragma unroll
-        for (int j = 0; j < D; ++j) bad[j] = bad[j + 1];
-      }
-      arrived(-1);
-      meet();
-      if (g == 1) {
-        load(0);
-        meet();
-      }
-      for (int i = 0;; ++i) {
-        if (g == 0) load(i);
-        __builtin_amdgcn_s_setprio(1);
-        multiply(lds + kr * S::TILE, vlds + vrd * S::TILE, i);
-        __builtin_amdgcn_s_setprio(0);
-        kr = kr == ST - 1 ? 0 : kr + 1;
-        if (i > 0) vrd = vrd == ST - 1 ? 0 : vrd + 1;
-        if (g == 1) arrived(i);
-        if (i == ntiles) {
-          if (g == 0) meet();
-          break;
-        }
-        meet();
-        const int bad_now = bad[0];
-#pragma unroll
-        for (int j = 0; j < D; ++j) bad[j] = bad[j + 1];
-        if (g == 1) load(i + 1);
-        softmax(std::false_type{}, first + i * KT, bad_now);
-        if (g == 0) arrived(i);
-        meet();
-      }
-    }
+    for (int i = 0; i < ST - 1; ++i) bad[i] = bad[i + 1];
+    ++rd;
+  };
+  while (rd < rounds) {
+    while (rd * WN + wn < ntiles && is_plain(first + (rd * WN + wn) * KT, bad[0]))
+      step(std::true_type{});
+    if (rd < rounds) step(std::false_type{});
   }
 
   // ---- the lane pair's sums, then the WN groups' states
   l = xor_sum<32>(l);
   if constexpr (WN > 1) {
     float* const jo = reinterpret_cast<float*>(smem);
-    __syncthreads();  // the tiles are read out
+    __builtin_amdgcn_s_waitcnt(wait_vm(0));
+    __syncthreads();  // the tiles are read out, nothing is on its way into them
     if (wn > 0) {
       float* const dst = jo + ((wn - 1) * WM + wm) * (32 * HD + 64);
 #pragma unroll
@@ -522,7 +448,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       }
     }
     __syncthreads();
-    if (wn > 0) return;  // nothing stored
+    if (wn > 0) return;
 #pragma unroll
     for (int w = 1; w < WN; ++w) {
       const float* const src = jo + ((w - 1) * WM + wm) * (32 * HD + 64);
@@ -537,10 +463,15 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
         for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * a + src[(16 * d + i) * 64 + lane] * b;
     }
   }
+  // The row again, from its number: not kept in registers through the rounds.
+  int row_again = row;
+  __asm__ volatile("" : "+v"(row_again));
+  const int64_t orow = (int64_t)(it.token0 + row_again / A.group) * A.n_q + kvh * A.group +
+                       row_again % A.group;
   // l == 0 only where the row sees no token: its output is 0, its weight none
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t orow = (int64_t)tok * A.n_q + head;
-  if (valid && it.slots == 1) {
+  if (valid && it.direct) {
+    if (h == 0 && it.counts) st_agent(it.counts + orow, 0);  // nothing to merge
     uint16_t* const dst = A.out + orow * HD;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -551,6 +482,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                        cvt_pk_bf16(o[d][4 * a + 2] * inv, o[d][4 * a + 3] * inv)});
   } else if (valid) {
     const int64_t prow = orow * it.slots + it.slot;
+    if (h == 0 && it.counts) st_agent(it.counts + orow, it.parts);
     if (h == 0)
       st_agent(A.part_lse + prow, l == 0.f ? -INFINITY : ref + log2f(l));
     if (l != 0.f) {  // the merge reads no partial whose weight is none
@@ -566,164 +498,329 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                               __float_as_uint(o[d][4 * a + 3] * inv)});
     }
   }
-  stores_done();
 }
 
-// Tokens of each of `splits` parts of `range` tokens, whole rounds of the tiles.
-template <int ROUND>
-__device__ __forceinline__ int chunk_of(int range, int splits) {
-  return ((range + ROUND - 1) / ROUND + splits - 1) / splits * ROUND;
+// The largest of a wave's values, for every lane.
+__device__ __forceinline__ int wave_max_i32(int v) {
+  auto dpp = [](int x, auto ctrl) {
+    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR1>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR2>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_HALF_MIRROR>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_MIRROR>{}));
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)b[0], (int)b[1]);
 }
 
-// Packed prompts.  Sequence r's queries are the tokens [query_start[r],
-// query_start[r + 1]), the last n of its L tokens: token i of them is at position
-// L - n + i and sees the tokens up to itself.  Grid: kv heads, row tiles (last
-// first: the longest come first), splits.  Which sequence a tile is of follows
-// from the prefix sums of the tile counts, 64 sequences at a time.
-template <int HD, int WM, int WN, int KT, int ST, int EU>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
-void prompt_attention_kernel(RowsArgs A) {
-  using S = Shape<HD, WM, WN, KT, ST>;
-  __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
+// The end of a part that begins at `from`, at most `end`.
+__device__ __forceinline__ int part_end(int from, int chunk, int end) {
+  return (int)min((int64_t)from + chunk, (int64_t)end);
+}
+
+// Where a workgroup stands in a launch's work: segment seg (a sequence, or the
+// prefix), item x of its tiles times parts, the segment's parts of `chunk` tokens.
+struct Place {
+  int seg, x, parts, chunk;
+};
+
+// Finds item `item` of segments whose row tiles and rounds (of ROUND tokens) seg_of
+// gives, 64 at a time, a lane each.  With max_parts > 1 every segment's tokens
+// are cut into parts of one length, the least (of at least `least` rounds) that
+// makes about `target` items of all segments and at most max_parts of any, so
+// that the workgroups are alike whatever the lengths: every workgroup derives
+// it from the lengths.
+template <int ROUND, typename Seg>
+__device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, int target,
+                                          int max_parts, int least, Place& place) {
   const int lane = threadIdx.x & 63;
-  const int kvh = blockIdx.x, tile = A.tiles - 1 - (int)blockIdx.y, split = blockIdx.z;
-  int done = 0, seq = -1, t_in = 0, q0 = 0, nq = 0;
-  for (int b = 0; b < A.num_seqs; b += 64) {
-    const int r = b + lane;
-    int s0 = 0, cnt = 0, nt = 0;
-    if (r < A.num_seqs) {
-      s0 = min(max(A.query_start[r], 0), A.num_tokens);
-      cnt = max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
-      nt = (int)(((int64_t)cnt * A.group + S::M - 1) / S::M);
+  int chunk = INT_MAX / ROUND;  // in rounds
+  int tiles0 = 0, rounds0 = 0;
+  if (lane < num_segs) seg_of(lane, tiles0, rounds0);
+  if (max_parts > 1) {
+    float work = wave_sum((float)tiles0 * (float)rounds0);
+    int top = wave_max_i32(rounds0);
+    for (int b = 64; b < num_segs; b += 64) {
+      int tiles = 0, rounds = 0;
+      if (b + lane < num_segs) seg_of(b + lane, tiles, rounds);
+      work += wave_sum((float)tiles * (float)rounds);
+      top = max(top, wave_max_i32(rounds));
     }
-    int incl = nt;
+    chunk = max(max((int)fminf(ceilf(work / (float)target), 1e9f),
+                    (top + max_parts - 1) / max_parts), least);
+    // every segment rounds up: a little longer parts where that made too many
+    for (int i = 0; i < 3 && num_segs <= 64; ++i) {
+      const float items = wave_sum((float)tiles0 * (float)max(1, (rounds0 + chunk - 1) / chunk));
+      if (items <= (float)target || chunk >= top) break;
+      chunk = max(chunk + 1, min((int)fminf((float)chunk * items / (float)target, 1e9f), top));
+    }
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+  }
+  int done = 0;
+  for (int b = 0; b < num_segs; b += 64) {
+    int tiles = tiles0, rounds = rounds0;
+    if (b > 0) {
+      tiles = rounds = 0;
+      if (b + lane < num_segs) seg_of(b + lane, tiles, rounds);
+    }
+    const int parts = max(1, (rounds + chunk - 1) / chunk);
+    const int items = tiles * parts;
+    int incl = items;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int x = __shfl_up(incl, o);
       if (lane >= o) incl += x;
     }
     const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (tile < done + total) {
-      const int i = __ffsll((unsigned long long)__ballot(done + incl > tile)) - 1;
-      seq = b + i;
-      t_in = tile - done - (__builtin_amdgcn_readlane(incl, i) - __builtin_amdgcn_readlane(nt, i));
-      q0 = __builtin_amdgcn_readlane(s0, i);
-      nq = __builtin_amdgcn_readlane(cnt, i);
-      break;
+    if (item < done + total) {
+      const int i = __ffsll((unsigned long long)__ballot(done + incl > item)) - 1;
+      place.seg = b + i;
+      place.x = item - done - (__builtin_amdgcn_readlane(incl, i) -
+                               __builtin_amdgcn_readlane(items, i));
+      place.parts = __builtin_amdgcn_readlane(parts, i);
+      place.chunk = chunk * ROUND;
+      return true;
     }
     done += total;
   }
-  if (seq < 0) return;  // the grid has room for the most tiles there can be
+  return false;
+}
+
+// Packed prompts.  Sequence r's queries are the tokens [query_start[r],
+// query_start[r + 1]), the last n of its L tokens: token i of them is at position
+// L - n + i and sees the tokens up to itself.  Grid: kv heads, items.
+template <int HD, int WM, int WN, int KT, int ST>
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
+void prompt_attention_kernel(RowsArgs A) {
+  using S = Shape<HD, WM, WN, KT, ST>;
+  __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
+  constexpr int ROUND = WN * KT;
+  const int kvh = blockIdx.x;
   const int cap = A.max_blocks << A.bs_log2;
-  const int L = min(max(A.seq_lens[seq], 0), cap);
+  auto queries = [&](int r, int& s0) {
+    s0 = min(max(A.query_start[r], 0), A.num_tokens);
+    return max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
+  };
+  auto length = [&](int r) { return min(max(A.seq_lens[r], 0), cap); };
+  auto seg_of = [&](int r, int& tiles, int& rounds) {
+    int s0;
+    const int cnt = queries(r, s0);
+    tiles = (int)(((int64_t)cnt * A.group + S::M - 1) / S::M);
+    rounds = tiles ? (int)(((int64_t)length(r) + ROUND - 1) / ROUND) : 0;
+  };
+  // Whole tiles: the last (longest) first, every other run of `zigzag` of them in
+  // turned order, so that a compute unit that starts with a long tile of one run
+  // gets a short one of the next.
+  int item = blockIdx.y;
+  if (A.splits == 1) {
+    const int run = item / A.zigzag, i = item % A.zigzag;
+    const int here = min(A.zigzag, A.tiles - run * A.zigzag);
+    item = A.tiles - 1 - (run * A.zigzag + (run & 1 ? here - 1 - i : i));
+  }
+  Place place;
+  // (the grid has room for the most items there can be)
+  if (!find_item<ROUND>(seg_of, A.num_seqs, item, A.target, A.splits, A.least, place)) return;
+  const int seq = place.seg;
+  int q0;
+  const int nq = queries(seq, q0), L = length(seq);
+  const int tiles = (int)(((int64_t)nq * A.group + S::M - 1) / S::M);
+  const int split = place.x / tiles;
   Item it;
   it.table = A.table + (int64_t)seq * A.max_blocks;
   it.token0 = q0;
-  it.row0 = t_in * S::M;
+  it.row0 = (place.x - split * tiles) * S::M;
   it.rows = min(S::M, nq * A.group - it.row0);
   const int ahead = L - nq;  // the position of the first query token
   const int last = (it.row0 + it.rows - 1) / A.group;
   const int range = max(ahead + last + 1, 0);
-  const int chunk = chunk_of<WN * KT>(range, A.splits);
-  it.from = min(split * chunk, range);
-  it.to = min(it.from + chunk, range);
+  it.from = part_end(0, split * place.chunk, range);
+  it.to = part_end(it.from, place.chunk, range);
   it.slot = split;
   it.slots = A.splits;
   it.query_at = ahead;
+  it.counts = split == 0 && A.splits > 1 ? A.counts : nullptr;
+  it.parts = place.parts;
+  it.direct = place.parts == 1;
   attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
+  stores_done();
 }
 
-// Decode rows (one token a sequence) under a shared prefix.  Grid: kv heads,
-// items: first the prefix, row tiles of all sequences' rows times its splits,
-// then each sequence's own tokens [prefix, L) in its splits.
-template <int HD, int WM, int WN, int KT, int ST, int EU>
-__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(EU)))
+// Decode rows (one token a sequence) under a shared prefix: the prefix with the
+// rows of all sequences, and each sequence's own tokens [prefix, L).  Grid: kv
+// heads, items.  Up to 64 rows the prefix and the sequences are segments of one
+// work list in parts of one length.  More (BIG): the prefix's items come first,
+// workgroups of 128 rows, one a compute unit, bound by the matrix units; the
+// sequences' items, bound by memory, run beside them.
+template <int HD, bool BIG>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void shared_prefix_kernel(RowsArgs A) {
+  constexpr int WM = 2, WN = 2, KT = 32, ST = 2;
   using S = Shape<HD, WM, WN, KT, ST>;
+  using B = Shape<HD, 4, 1, 64, 2>;  // the prefix's where BIG
+  static_assert(B::LDS <= S::LDS, "one LDS array serves both");
   __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
+  constexpr int ROUND = WN * KT;
   const int kvh = blockIdx.x;
   const int prefix = min(max(A.prefix_len[0], 0), A.prefix_blocks << A.bs_log2);
   const int cap = A.max_blocks << A.bs_log2;
+  const int64_t rows = (int64_t)A.num_seqs * A.n_q;
   Item it;
   it.slots = A.splits + A.suffix_splits;
   it.query_at = NO_QUERY;
-  const int y = A.item0 + (int)blockIdx.y;
-  if (y < A.tiles * A.splits) {
-    const int split = y / A.tiles;
+  it.direct = false;
+  auto prefix_item = [&](int split, int tile, int m, int chunk, int parts) {
     it.table = A.prefix_table;
     it.token0 = 0;
-    it.row0 = (y % A.tiles) * S::M;
-    it.rows = min(S::M, A.num_seqs * A.group - it.row0);
-    const int chunk = chunk_of<WN * KT>(prefix, A.splits);
-    it.from = min(split * chunk, prefix);
-    it.to = min(it.from + chunk, prefix);
+    it.row0 = tile * m;
+    it.rows = min(m, A.num_seqs * A.group - it.row0);
+    it.from = part_end(0, split * chunk, prefix);
+    it.to = part_end(it.from, chunk, prefix);
     it.slot = split;
-  } else {
-    const int gt = (A.group + S::M - 1) / S::M;  // row tiles of a sequence's group
-    int x = y - A.tiles * A.splits;
-    const int seq = x / (A.suffix_splits * gt);
-    x -= seq * A.suffix_splits * gt;
-    const int split = x / gt;
-    const int L = min(max(A.seq_lens[seq], 0), cap);
-    it.table = A.table + (int64_t)seq * A.max_blocks;
-    it.token0 = seq;
-    it.row0 = (x % gt) * S::M;
-    it.rows = min(S::M, A.group - it.row0);
-    const int span = max(L - prefix, 0);
-    // tiles are aligned to KT, so that a tile's halves of 32 tokens are within a page
+    it.counts = split > 0 ? nullptr : A.counts;
+    it.parts = parts;
+  };
+  auto prefix_part = [&]() {  // the item of a BIG launch's first tiles * splits
+    const int rounds = (prefix + 63) / 64;
+    const int chunk = max((rounds + A.splits - 1) / A.splits, 1);
+    const int parts = max((rounds + chunk - 1) / chunk, 1);
+    const int split = blockIdx.y / A.tiles;
+    if (split >= parts) return;
+    prefix_item(split, blockIdx.y - split * A.tiles, B::M, chunk * 64, parts);
+    attend<HD, 4, 1, 64, 2>(A, it, kvh, smem);
+  };
+  auto listed_part = [&](int item) {
+    const int group_tiles = (A.group + S::M - 1) / S::M;
+    // a sequence's tiles are aligned, so that a tile's halves of 32 tokens are within a page
     const int first = prefix & ~(KT - 1);
-    const int chunk = chunk_of<WN * KT>(span ? L - first : 0, A.suffix_splits);
-    it.to = min(first + (split + 1) * chunk, max(L, prefix));
-    it.from = min(max(first + split * chunk, prefix), it.to);
-    it.slot = A.splits + split;
-  }
-  attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
+    auto length = [&](int r) { return min(max(A.seq_lens[r], 0), cap); };
+    constexpr int SEG0 = BIG ? 1 : 0;  // segment 0 is the prefix, r + 1 sequence r
+    auto seg_of = [&](int i, int& tiles, int& rounds) {
+      const int s = SEG0 + i;
+      tiles = s == 0 ? A.tiles : group_tiles;
+      const int L = s == 0 ? prefix : length(s - 1);
+      const int span = s == 0 ? prefix : L > prefix ? L - first : 0;
+      rounds = (span + ROUND - 1) / ROUND;
+    };
+    Place place;
+    if (!find_item<ROUND>(seg_of, A.num_seqs + 1 - SEG0, item, A.target, A.suffix_splits, 1,
+                          place))
+      return;
+    const int seg = SEG0 + place.seg;
+    const int tiles = seg == 0 ? A.tiles : group_tiles;
+    const int split = place.x / tiles, tile = place.x - split * tiles;
+    if (seg == 0) {
+      prefix_item(split, tile, S::M, place.chunk, place.parts);
+    } else {
+      const int L = length(seg - 1);
+      it.table = A.table + (int64_t)(seg - 1) * A.max_blocks;
+      it.token0 = seg - 1;
+      it.row0 = tile * S::M;
+      it.rows = min(S::M, A.group - it.row0);
+      const int end = max(L, prefix);
+      const int begin = part_end(first, split * place.chunk, end);
+      it.from = max(begin, prefix);
+      it.to = max(part_end(begin, place.chunk, end), it.from);
+      it.slot = A.splits + split;
+      it.counts = split > 0 ? nullptr : A.counts + rows;
+      it.parts = place.parts;
+    }
+    attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
+  };
+  const int big = BIG ? A.tiles * A.splits : 0;
+  if (BIG && (int)blockIdx.y < big)
+    prefix_part();
+  else
+    listed_part((int)blockIdx.y - big);
+  stores_done();
 }
 
-// out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a row's partials, a
-// wave a row: lane j holds the weights of slots j, j + 64, ..., every lane HD / 64
-// dims.  A partial of weight 0 is not read (it was not written).  Rows that are
-// of no sequence are left as they are.
-constexpr int MERGE_ROWS = 4;  // rows (waves) of a workgroup
+// out = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max) over a row's partials: the
+// counts[row] first slots and the counts[rows + row] from slot `second` on.  WPR
+// waves a row take chunks of MCH partials in turn, lane j of a wave the weight of
+// partial j of its chunk, every lane HD / 64 dims; all of a chunk's loads are
+// issued before the first is used.  A partial of weight 0 may not have been
+// written and is left out.  Rows that are of no sequence, and rows of one part
+// (no partials: counts 0), stay as they are.
+constexpr int MCH = 16;
 
-template <int HD>
-__global__ __launch_bounds__(64 * MERGE_ROWS) void rows_merge_kernel(
-    const float* part_o, const float* part_lse, uint16_t* out, const int32_t* query_start,
-    int num_seqs, int num_tokens, int n_q, int slots) {
-  constexpr int D = HD / 64;
+template <int HD, int WPR>
+__global__ __launch_bounds__(256) void rows_merge_kernel(
+    const float* part_o, const float* part_lse, const int32_t* counts, uint16_t* out,
+    const int32_t* query_start, int num_seqs, int num_tokens, int n_q, int slots, int second) {
+  constexpr int D = HD / 64, ROWS = 4 / WPR;
+  __shared__ float top_s[4], sum_s[4], acc_s[4][HD];
+  __shared__ int bad_s[4];
   const int lane = threadIdx.x & 63;
-  const int64_t row =
-      (int64_t)blockIdx.x * MERGE_ROWS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v = wave % WPR;
+  const int64_t rows = (int64_t)num_tokens * n_q;
+  const int64_t row = (int64_t)blockIdx.x * ROWS + wave / WPR;
+  if (row >= rows) return;
   const int tok = (int)(row / n_q);
-  if (tok >= num_tokens) return;
   if (query_start && (tok < query_start[0] || tok >= query_start[num_seqs])) return;
+  const int c0 = min(max(counts[row], 0), second);
+  const int c1 = second < slots ? min(max(counts[rows + row], 0), slots - second) : 0;
+  const int cnt = c0 + c1;
+  if (cnt == 0) return;  // written by the only part
+  auto slot = [&](int i) { return i < c0 ? i : second + i - c0; };
   const float* const lse = part_lse + row * slots;
-  const float* const po = part_o + row * slots * HD;
-  float top = -INFINITY;
+  const float* const po = part_o + row * slots * HD + D * lane;
+  float top = -INFINITY, sum = 0.f, acc[D] = {};
   bool bad = false;
-  for (int s = lane; s < slots; s += 64) {
-    top = fmaxf(top, lse[s]);
-    bad |= lse[s] != lse[s];
-  }
+  for (int i0 = v * MCH; i0 < cnt; i0 += WPR * MCH) {
+    const int last = min(MCH, cnt - i0) - 1;
+    const float x = lse[slot(i0 + min(lane, last))];
+    float pv[MCH][D];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  float sum = 0.f, acc[D] = {};
-  for (int s0 = 0; s0 < slots; s0 += 64) {
-    const float x = s0 + lane < slots ? lse[s0 + lane] : -INFINITY;
-    const float w = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top);
-    sum += w;
-    const int cnt = min(64, slots - s0);
-    for (int j = 0; j < cnt; ++j) {
+    for (int j = 0; j < MCH; ++j) {
+      const float* const src = po + (int64_t)slot(i0 + min(j, last)) * HD;
+#pragma unroll
+      for (int d = 0; d < D; ++d) pv[j][d] = src[d];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const float mine = lane <= last ? x : -INFINITY;
+    bad |= __builtin_amdgcn_ballot_w64(mine != mine) != 0;
+    const float next = fmaxf(top, wave_max(mine));
+    const float w = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - next);
+    const float a = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - next);
+    sum = sum * a + wave_sum(w);
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] *= a;
+#pragma unroll
+    for (int j = 0; j < MCH; ++j) {
       const float wj = __builtin_bit_cast(
           float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), j));
-      if (wj == 0.f) continue;
 #pragma unroll
-      for (int d = 0; d < D; ++d)
-        acc[d] = fmaf(wj, po[(int64_t)(s0 + j) * HD + D * lane + d], acc[d]);
+      for (int d = 0; d < D; ++d) acc[d] = wj == 0.f ? acc[d] : fmaf(wj, pv[j][d], acc[d]);
+    }
+    top = next;
+  }
+  if constexpr (WPR > 1) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc_s[wave][D * lane + d] = acc[d];
+    if (lane == 0) {
+      top_s[wave] = top;
+      sum_s[wave] = sum;
+      bad_s[wave] = bad;
+    }
+    __syncthreads();
+    if (v != 0) return;
+    const float mine = top;
+    for (int w = 1; w < WPR; ++w) top = fmaxf(top, top_s[wave + w]);
+    const float a = mine == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mine - top);
+    sum *= a;
+#pragma unroll
+    for (int d = 0; d < D; ++d) acc[d] *= a;
+    for (int w = 1; w < WPR; ++w) {
+      const float t = top_s[wave + w];
+      const float b = t == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(t - top);
+      sum = fmaf(b, sum_s[wave + w], sum);
+      bad |= bad_s[wave + w] != 0;
+#pragma unroll
+      for (int d = 0; d < D; ++d) acc[d] = fmaf(b, acc_s[wave + w][D * lane + d], acc[d]);
     }
   }
-  sum = wave_sum(sum);
-  bad = __builtin_amdgcn_ballot_w64(bad) != 0;
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   uint16_t* const dst = out + row * HD + D * lane;
   float r[D];
@@ -743,40 +840,46 @@ int log2_of(int v) {
 }
 
 template <int HD>
-int launch_merge(hipStream_t stream, const RowsArgs& a, int slots, bool prompts) {
+int launch_merge(hipStream_t stream, const RowsArgs& a, int slots, int second, bool prompts) {
   const int64_t rows = (int64_t)a.num_tokens * a.n_q;
-  SMX_LAUNCH((rows_merge_kernel<HD>), dim3((unsigned)((rows + MERGE_ROWS - 1) / MERGE_ROWS)),
-             dim3(64 * MERGE_ROWS), 0, stream, a.part_o, a.part_lse, a.out,
-             prompts ? a.query_start : (const int32_t*)nullptr, a.num_seqs, a.num_tokens, a.n_q,
-             slots);
+  const int32_t* const start = prompts ? a.query_start : nullptr;
+  if (slots > MCH)
+    SMX_LAUNCH((rows_merge_kernel<HD, 4>), dim3((unsigned)rows), dim3(256), 0, stream, a.part_o,
+               a.part_lse, a.counts, a.out, start, a.num_seqs, a.num_tokens, a.n_q, slots, second);
+  else
+    SMX_LAUNCH((rows_merge_kernel<HD, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream,
+               a.part_o, a.part_lse, a.counts, a.out, start, a.num_seqs, a.num_tokens, a.n_q,
+               slots, second);
   return (int)hipGetLastError();
 }
-
-// Shapes of a workgroup: WM waves of 32 rows by WN groups that share the tokens,
-// tiles of KT tokens.
-constexpr int SHAPE_WM[] = {1, 2, 4, 8};
 
 int tune(const char* name, int v) {
   const char* e = tuning_env(name);
   return e ? atoi(e) : v;
 }
 
-struct Choice {
-  int shape, splits, suffix_splits, tiles;
-};
+constexpr int MAX_PARTS = 64;
 
-constexpr int MAX_SPLITS = 64;
+struct Choice {
+  int m, splits, suffix_splits, tiles, target;
+};
 
 Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
-  c.shape = tune("SMX_PA_SHAPE", rows <= 32 ? 0 : rows <= 64 ? 1 : 2);
-  const int m = 32 * SHAPE_WM[c.shape];
-  c.tiles = (int)((num_tokens * group + m - 1) / m + num_seqs - 1);
-  const int64_t wgs = (rows + m - 1) / m * num_seqs * n_kv;
-  const int64_t most = std::min<int64_t>(MAX_SPLITS, (cap + 255) / 256);
-  const int target = tune("SMX_PA_TARGET", 512);
-  c.splits = (int)std::max<int64_t>(1, std::min(most, target / wgs));
+  auto tiles = [&](int m) { return (rows + m - 1) / m * num_seqs; };  // of even lengths
+  c.splits = 1;
+  c.m = tiles(128) * n_kv >= 512 ? 128 : 64;
+  const bool few = c.m == 64 && tiles(64) * n_kv < 400 && cap >= 1024;
+  if (few && rows > 1024) c.m = 128;
+  c.m = tune("SMX_PA_M", c.m);
+  c.tiles = (int)((num_tokens * group + c.m - 1) / c.m + num_seqs - 1);
+  c.target = std::max(1, tune("SMX_PA_TARGET", 512) / n_kv);
+  if (few) {
+    const int64_t even = (c.target + tiles(c.m) - 1) / tiles(c.m);
+    const int64_t most = num_seqs == 1 ? even : num_tokens * group <= 1024 ? 4 * even : 2 * even;
+    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, MAX_PARTS, cap / 256}));
+  }
   c.splits = tune("SMX_PA_SPLITS", c.splits);
   return c;
 }
@@ -784,61 +887,71 @@ Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int grou
 Choice choose_prefix(int64_t num_seqs, int64_t prefix_cap, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = num_seqs * group;
-  c.shape = tune("SMX_SP_SHAPE", rows <= 32 ? 0 : rows <= 64 ? 1 : rows <= 128 ? 2 : 3);
-  const int m = 32 * SHAPE_WM[c.shape];
-  c.tiles = (int)((rows + m - 1) / m);
-  const int target = tune("SMX_SP_TARGET", 512);
-  c.splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>({MAX_SPLITS, (prefix_cap + 127) / 128, target / (c.tiles * n_kv)}));
-  c.suffix_splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>({MAX_SPLITS, (cap + 511) / 512,
-                            tune("SMX_SP_STARGET", 512) / (num_seqs * n_kv)}));
+  c.m = tune("SMX_SP_M", rows <= 64 ? 64 : 128);
+  c.tiles = (int)((rows + c.m - 1) / c.m);
+  const int64_t prefix_parts = std::max<int64_t>(1, prefix_cap / 64);
+  const int64_t suffix_parts = std::max<int64_t>(1, cap / 64);
+  if (c.m == 64) {  // one work list, parts of one length
+    c.target = std::max(1, tune("SMX_SP_TARGET", 512) / n_kv);
+    c.suffix_splits = (int)std::min<int64_t>(
+        {MAX_PARTS, c.target, std::max(prefix_parts, suffix_parts)});
+    c.splits = c.suffix_splits;
+  } else {
+    const int64_t wgs = tune("SMX_SP_TARGET", 256) / n_kv;
+    c.splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>({wgs / c.tiles, MAX_PARTS, prefix_parts}));
+    c.target = std::max(1, tune("SMX_SP_STARGET", 1024) / n_kv);
+    const int64_t even = (c.target + num_seqs - 1) / num_seqs;
+    c.suffix_splits = (int)std::min<int64_t>({4 * even, MAX_PARTS, suffix_parts});
+  }
   return c;
 }
 
 int64_t partial_bytes(int64_t rows, int64_t slots, int hd) {
   if (slots == 1) return 0;
-  return rows * slots * (hd + 1) * 4;
+  return rows * (slots * (hd + 1) + 2) * 4;
 }
 
-#define SMX_ROWS_LAUNCH(kernel, shape, grid)                                                      \
-  do {                                                                                            \
-    if (shape == 0)                                                                               \
-      SMX_LAUNCH((kernel<HD, 1, 4, 32, 2, 1>), grid, dim3(256), 0, stream, a);                    \
-    else if (shape == 1)                                                                          \
-      SMX_LAUNCH((kernel<HD, 2, 2, 64, 2, 1>), grid, dim3(256), 0, stream, a);                    \
-    else if (shape == 2)                                                                          \
-      SMX_LAUNCH((kernel<HD, 4, 1, 64, 2, 2>), grid, dim3(256), 0, stream, a);                    \
-    else                                                                                          \
-      SMX_LAUNCH((kernel<HD, 8, 1, 64, 2, 2>), grid, dim3(512), 0, stream, a);                    \
-  } while (0)
+void set_workspace(RowsArgs& a, void* workspace, int64_t rows, int slots, int hd) {
+  a.part_o = (float*)workspace;
+  a.part_lse = a.part_o + rows * slots * hd;
+  a.counts = (int32_t*)(a.part_lse + rows * slots);
+}
+
+// Tiles times parts: at most the target (whose parts' length comes from a sum in
+// fp32, so perhaps one more) and one more part of every tile.
+int items_bound(int64_t tiles, int target, int splits) {
+  return (int)std::min<int64_t>(tiles * splits, target + tiles + 1);
+}
 
 template <int HD>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  SMX_ROWS_LAUNCH(prompt_attention_kernel, c.shape, dim3(a.n_kv, c.tiles, c.splits));
+  a.zigzag = a.num_seqs == 1 ? std::max(1, 256 / a.n_kv) : 1 << 30;
+  a.target = c.target;
+  a.least = tune("SMX_PA_LEAST", 256) / 64;
+  const dim3 grid(a.n_kv, items_bound(c.tiles, c.target, c.splits));
+  if (c.m == 64)
+    SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2>), grid, dim3(256), 0, stream, a);
+  else
+    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
   const int rc = (int)hipGetLastError();
-  return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, true);
+  return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, c.splits, true);
 }
 
-// One launch for the prefix and the sequences' own tokens where one shape suits
-// both, else one each.
 template <int HD>
 int launch_prefix(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  const int prefix_items = c.tiles * c.splits;
-  const bool one = c.shape == 0;
-  a.item0 = 0;
-  const int suffix_items = a.num_seqs * c.suffix_splits * ((a.group + 31) / 32);
-  SMX_ROWS_LAUNCH(shared_prefix_kernel, c.shape,
-                  dim3(a.n_kv, one ? prefix_items + suffix_items : prefix_items));
-  int rc = (int)hipGetLastError();
-  if (rc) return rc;
-  if (!one) {
-    a.item0 = prefix_items;
-    SMX_ROWS_LAUNCH(shared_prefix_kernel, 0, dim3(a.n_kv, suffix_items));
-    rc = (int)hipGetLastError();
-    if (rc) return rc;
-  }
-  return launch_merge<HD>(stream, a, c.splits + c.suffix_splits, false);
+  const int64_t own = a.num_seqs * (int64_t)((a.group + 63) / 64);
+  a.target = c.target;
+  if (c.m == 64)
+    SMX_LAUNCH((shared_prefix_kernel<HD, false>),
+               dim3(a.n_kv, items_bound(c.tiles + own, c.target, c.splits)), dim3(256), 0, stream,
+               a);
+  else
+    SMX_LAUNCH((shared_prefix_kernel<HD, true>),
+               dim3(a.n_kv, c.tiles * c.splits + items_bound(own, c.target, c.suffix_splits)),
+               dim3(256), 0, stream, a);
+  const int rc = (int)hipGetLastError();
+  return rc ? rc : launch_merge<HD>(stream, a, c.splits + c.suffix_splits, c.splits, false);
 }
 
 }  // namespace
@@ -911,8 +1024,7 @@ extern "C" int smx_prompt_attention(void* stream, const void* q, int64_t q_strid
   a.query_start = query_start_loc;
   a.seq_lens = seq_lens;
   a.out = (uint16_t*)out;
-  a.part_o = (float*)workspace;
-  a.part_lse = (float*)workspace + rows * c.splits * head_dim;
+  smx::set_workspace(a, workspace, rows, c.splits, head_dim);
   a.q_stride = q_stride;
   a.num_tokens = num_tokens;
   a.num_seqs = num_seqs;
@@ -975,8 +1087,7 @@ extern "C" int smx_shared_prefix_attention(
   a.prefix_len = prefix_len;
   a.seq_lens = seq_lens;
   a.out = (uint16_t*)out;
-  a.part_o = (float*)workspace;
-  a.part_lse = (float*)workspace + rows * slots * head_dim;
+  smx::set_workspace(a, workspace, rows, slots, head_dim);
   a.q_stride = q_stride;
   a.num_tokens = num_seqs;
   a.num_seqs = num_seqs;

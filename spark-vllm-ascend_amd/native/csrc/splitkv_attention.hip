@@ -529,17 +529,6 @@ void splitkv_decode_kernel(
   stores_done();
 }
 
-// Max / sum over the 64 lanes of a wave (every lane gets the result).
-__device__ __forceinline__ float wave_max(float v) {
-  v = fmaxf(v, dpp_f32<DPP_QUAD_XOR1>(v));
-  v = fmaxf(v, dpp_f32<DPP_QUAD_XOR2>(v));
-  v = fmaxf(v, dpp_f32<DPP_ROW_HALF_MIRROR>(v));
-  v = fmaxf(v, dpp_f32<DPP_ROW_MIRROR>(v));
-  v = xor_max<16>(v);
-  v = xor_max<32>(v);
-  return v;
-}
-
 // Log-sum-exp merge (merge_attention, src/spark_vllm_ascend/kernels/
 // vector.py:61-78): w_s = exp(lse_s - max), out = sum_s w_s o_s / sum_s w_s.
 // One workgroup of nw waves per (64 dims of a q head, sequence); wave v folds

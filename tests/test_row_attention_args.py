@@ -76,4 +76,5 @@ def test_workspace_sizes():
         assert lib.smx_shared_prefix_attention_workspace(*bad[:1], 1, *bad[2:]) == -1 or bad[1] == 0
     for seqs, hd in ((1, 128), (64, 64)):
         n = lib.smx_shared_prefix_attention_workspace(seqs, 256, 300, 128, 32, 8, hd)
-        assert n > 0 and n % (seqs * 32 * (hd + 1) * 4) == 0
+        slots = (n / (seqs * 32 * 4) - 2) / (hd + 1)  # partials, lse, two counts a row
+        assert n > 0 and slots == int(slots) >= 2
