@@ -159,24 +159,37 @@ __global__ __launch_bounds__(NT) void request_tables_kernel(TablesArgs A) {
 }
 
 // Positions and slots of the tokens, a thread a token, from the tables that
-// request_tables_kernel left.
+// request_tables_kernel left.  With up to LOCAL requests their offsets are read
+// into LDS at once, so that the bisection's steps are LDS reads and not a chain
+// of loads (24000 tokens of 256 requests: 3.9 us, 2.9 so).
+constexpr int LOCAL = 1024;
+
+template <bool IN_LDS>
 __global__ __launch_bounds__(256) void request_tokens_kernel(
     const int32_t* query_start, const int32_t* context, const int32_t* table, int64_t* positions,
     int64_t* slots, int num_reqs, int max_tokens, int max_blocks, int bs_log2) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= max_tokens) return;
-  int64_t pos = 0, slot = -1;
-  if (j < query_start[num_reqs]) {
-    const int i = last_le(query_start, num_reqs, j);
-    pos = (int64_t)max(context[i], 0) + (j - query_start[i]);
-    const int64_t blk = pos >> bs_log2;
-    if (blk < max_blocks) {
-      const int page = table[(int64_t)i * max_blocks + blk];
-      if (page >= 0) slot = ((int64_t)page << bs_log2) + (pos & ((1 << bs_log2) - 1));
-    }
+  __shared__ int32_t start_s[IN_LDS ? LOCAL + 1 : 1];
+  const int32_t* start = query_start;
+  if constexpr (IN_LDS) {
+    for (int r = threadIdx.x; r <= num_reqs; r += 256) start_s[r] = query_start[r];
+    __syncthreads();
+    start = start_s;
   }
-  st_agent(reinterpret_cast<uint64_t*>(positions) + j, (uint64_t)pos);
-  st_agent(reinterpret_cast<uint64_t*>(slots) + j, (uint64_t)slot);
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j < max_tokens) {
+    int64_t pos = 0, slot = -1;
+    if (j < start[num_reqs]) {
+      const int i = last_le(start, num_reqs, j);
+      pos = (int64_t)max(context[i], 0) + (j - start[i]);
+      const int64_t blk = pos >> bs_log2;
+      if (blk < max_blocks) {
+        const int page = table[(int64_t)i * max_blocks + blk];
+        if (page >= 0) slot = ((int64_t)page << bs_log2) + (pos & ((1 << bs_log2) - 1));
+      }
+    }
+    st_agent(reinterpret_cast<uint64_t*>(positions) + j, (uint64_t)pos);
+    st_agent(reinterpret_cast<uint64_t*>(slots) + j, (uint64_t)slot);
+  }
   stores_done();
 }
 
@@ -261,8 +274,9 @@ extern "C" int smx_request_tables(void* stream, const int32_t* query_lens,
                     num_pages_out, free_count_out, query_start_loc, seq_lens, positions,
                     slot_mapping, num_reqs, max_tokens, max_blocks, num_free, 0, 0};
   while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
+  // One workgroup deals a few thousand tokens out in about a launch's time.
   a.with_tokens = num_reqs <= 1024 && max_tokens <= 4096;
-  if (num_reqs <= 256 && max_tokens <= 256)
+  if (num_reqs <= 256 && (max_tokens <= 256 || !a.with_tokens))
     SMX_LAUNCH((smx::request_tables_kernel<256>), dim3(1), dim3(256), 0, (hipStream_t)stream, a);
   else
     SMX_LAUNCH((smx::request_tables_kernel<1024>), dim3(1), dim3(1024), 0, (hipStream_t)stream,
@@ -270,9 +284,15 @@ extern "C" int smx_request_tables(void* stream, const int32_t* query_lens,
   if (!a.with_tokens) {
     const int rc = (int)hipGetLastError();
     if (rc) return rc;
-    SMX_LAUNCH(smx::request_tokens_kernel, dim3((unsigned)(((int64_t)max_tokens + 255) / 256)),
-               dim3(256), 0, (hipStream_t)stream, query_start_loc, context_lens, block_table,
-               positions, slot_mapping, num_reqs, max_tokens, max_blocks, a.bs_log2);
+    const dim3 grid((unsigned)(((int64_t)max_tokens + 255) / 256));
+    if (num_reqs <= smx::LOCAL)
+      SMX_LAUNCH((smx::request_tokens_kernel<true>), grid, dim3(256), 0, (hipStream_t)stream,
+                 query_start_loc, context_lens, block_table, positions, slot_mapping, num_reqs,
+                 max_tokens, max_blocks, a.bs_log2);
+    else
+      SMX_LAUNCH((smx::request_tokens_kernel<false>), grid, dim3(256), 0, (hipStream_t)stream,
+                 query_start_loc, context_lens, block_table, positions, slot_mapping, num_reqs,
+                 max_tokens, max_blocks, a.bs_log2);
   }
   return (int)hipGetLastError();
 }

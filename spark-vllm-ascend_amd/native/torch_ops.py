@@ -10,8 +10,6 @@ reference's custom ops do (src/spark_vllm_ascend/integration/head.py:8-9).
 """
 from __future__ import annotations
 
-from typing import NamedTuple
-
 import torch
 
 from . import call, load
@@ -643,52 +641,69 @@ def compute_slot_mapping(query_start_loc: torch.Tensor, positions: torch.Tensor,
     return out
 
 
+def _plain(t: torch.Tensor, dtype: torch.dtype, index: int) -> bool:
+    """Whether t is a contiguous `dtype` tensor on GPU `index` (get_device() is -1 on
+    the CPU): half of _check's time for the calls that a step makes of small work,
+    with _check only to say what is wrong."""
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
+def _all_plain(index: int, dtype: torch.dtype, **tensors: torch.Tensor) -> None:
+    """Refuses the first of `tensors` that is not _plain."""
+    for name, t in tensors.items():
+        _need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
+        if index < 0 or not _plain(t, dtype, index):
+            _check(t, name, dtype, device=torch.device("cuda", max(index, 0)))
+            raise ValueError(f"{name} is not a valid argument")
+
+
 def _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out):
-    """The checks the row attentions share; returns out (allocated if None)."""
-    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dtype == BF16 and q.dim() == 3,
+    """The checks the row attentions share -> (out, allocated if None; sizes)."""
+    _need(isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is BF16 and q.dim() == 3,
           "q must be a bf16 GPU tensor [tokens, n_q, hd]")
-    _need(q.shape[0] >= 1 and q.shape[1] >= 1, "q must hold a token and a head")
-    n_q, hd = q.shape[1:]
-    _need(q.stride(2) == 1 and (n_q == 1 or q.stride(1) == hd)
-          and (q.shape[0] == 1 or q.stride(0) >= n_q * hd),
+    tokens, n_q, hd = q.shape
+    step, head_step, unit = q.stride()
+    _need(tokens >= 1 and n_q >= 1, "q must hold a token and a head")
+    if tokens == 1:
+        step = n_q * hd
+    _need(unit == 1 and (n_q == 1 or head_step == hd) and step >= n_q * hd,
           "a token's heads must be contiguous in q and its tokens apart")
-    _need(q.data_ptr() % 16 == 0 and (q.shape[0] == 1 or q.stride(0) % 8 == 0),
-          "q's tokens must be 16-byte aligned")
-    _check(k_cache, "k_cache", BF16, device=q.device)
-    _check(v_cache, "v_cache", BF16, device=q.device)
-    _need(k_cache.dim() == 4 and v_cache.shape == k_cache.shape,
+    _need(q.data_ptr() % 16 == 0 and step % 8 == 0, "q's tokens must be 16-byte aligned")
+    i = q.get_device()
+    if not (_plain(k_cache, BF16, i) and _plain(v_cache, BF16, i)
+            and _plain(block_table, torch.int32, i) and _plain(seq_lens, torch.int32, i)):
+        _all_plain(i, BF16, k_cache=k_cache, v_cache=v_cache)
+        _all_plain(i, torch.int32, block_table=block_table, seq_lens=seq_lens)
+    shape = k_cache.shape
+    _need(len(shape) == 4 and v_cache.shape == shape,
           "the caches must be [blocks, block_size, n_kv, hd], both alike")
-    _need(hd == k_cache.shape[3], "head_dim mismatch between q and the cache")
-    _check(block_table, "block_table", torch.int32, device=q.device)
+    num_blocks, bs, n_kv, cache_hd = shape
+    _need(hd == cache_hd, "head_dim mismatch between q and the cache")
     _need(block_table.dim() == 2, "block_table must be [seqs, max_blocks]")
-    _check(seq_lens, "seq_lens", torch.int32, block_table.shape[0], q.device)
-    if workspace is not None:
-        _check(workspace, "workspace", torch.uint8, device=q.device)
+    num_seqs, max_blocks = block_table.shape
+    _need(seq_lens.numel() == num_seqs, "seq_lens must have an entry for each row of block_table")
+    if workspace is not None and not _plain(workspace, torch.uint8, i):
+        _all_plain(i, torch.uint8, workspace=workspace)
     if out is None:
-        out = torch.empty(q.shape, dtype=BF16, device=q.device)
-    _check(out, "out", BF16, q.numel(), q.device)
-    return out
-
-
-def _q_stride(q: torch.Tensor) -> int:
-    return q.stride(0) if q.shape[0] > 1 else q.shape[1] * q.shape[2]
+        out = torch.empty((tokens, n_q, hd), dtype=BF16, device=q.device)
+    elif not _plain(out, BF16, i):
+        _all_plain(i, BF16, out=out)
+    _need(out.numel() == tokens * n_q * hd, "out must have q's elements")
+    return out, step, (num_seqs, max_blocks, num_blocks, bs, n_q, n_kv, hd)
 
 
 def _workspace(nbytes: int, device) -> torch.Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
-def _prompt_workspace_bytes(q, k_cache, block_table) -> int:
-    _, bs, n_kv, hd = k_cache.shape
-    return load().smx_prompt_attention_workspace(q.shape[0], block_table.shape[0],
-                                                 block_table.shape[1], bs, q.shape[1], n_kv, hd)
-
-
 def prompt_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor,
                                block_table: torch.Tensor) -> torch.Tensor | None:
     """The workspace prompt_attention uses for these sizes (uint8; None where it
     uses none).  Calls that can overlap need one each."""
-    return _workspace(_prompt_workspace_bytes(q, k_cache, block_table), q.device)
+    _, bs, n_kv, hd = k_cache.shape
+    return _workspace(load().smx_prompt_attention_workspace(
+        q.shape[0], block_table.shape[0], block_table.shape[1], bs, q.shape[1], n_kv, hd),
+        q.device)
 
 
 def prompt_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -702,31 +717,27 @@ def prompt_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     seq_lens[r] tokens, whose K and V the cache holds.  Rows of no sequence are
     left as they are in `out`.  Without `workspace` (prompt_attention_workspace)
     one is allocated where the call needs it."""
-    out = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
-    num_seqs, max_blocks = block_table.shape
-    _check(query_start_loc, "query_start_loc", torch.int32, num_seqs + 1, q.device)
-    num_blocks, bs, n_kv, hd = k_cache.shape
+    out, step, sizes = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
+    if not _plain(query_start_loc, torch.int32, q.get_device()):
+        _all_plain(q.get_device(), torch.int32, query_start_loc=query_start_loc)
+    _need(query_start_loc.numel() == sizes[0] + 1, "query_start_loc must have num_seqs + 1 entries")
     if workspace is None:
-        workspace = _workspace(_prompt_workspace_bytes(q, k_cache, block_table), q.device)
-    call("smx_prompt_attention", _stream(q), q.data_ptr(), _q_stride(q), k_cache.data_ptr(),
+        workspace = prompt_attention_workspace(q, k_cache, block_table)
+    call("smx_prompt_attention", _stream(q), q.data_ptr(), step, k_cache.data_ptr(),
          v_cache.data_ptr(), block_table.data_ptr(), query_start_loc.data_ptr(),
          seq_lens.data_ptr(), _ptr(workspace), workspace.numel() if workspace is not None else 0,
-         out.data_ptr(), q.shape[0], num_seqs, max_blocks, num_blocks, bs, q.shape[1], n_kv, hd,
-         float(scale))
+         out.data_ptr(), q.shape[0], *sizes, float(scale))
     return out
-
-
-def _prefix_workspace_bytes(q, k_cache, prefix_table, block_table) -> int:
-    _, bs, n_kv, hd = k_cache.shape
-    return load().smx_shared_prefix_attention_workspace(
-        q.shape[0], prefix_table.numel(), block_table.shape[1], bs, q.shape[1], n_kv, hd)
 
 
 def shared_prefix_attention_workspace(q: torch.Tensor, k_cache: torch.Tensor,
                                       prefix_table: torch.Tensor,
                                       block_table: torch.Tensor) -> torch.Tensor | None:
     """The workspace shared_prefix_attention uses for these sizes (uint8)."""
-    return _workspace(_prefix_workspace_bytes(q, k_cache, prefix_table, block_table), q.device)
+    _, bs, n_kv, hd = k_cache.shape
+    return _workspace(load().smx_shared_prefix_attention_workspace(
+        q.shape[0], prefix_table.numel(), block_table.shape[1], bs, q.shape[1], n_kv, hd),
+        q.device)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -738,38 +749,61 @@ def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     (pages prefix_table, int32 [blocks]), read once for all.  q [seqs, n_q, hd];
     block_table [seqs, max_blocks] by absolute position (its entries below the
     prefix are not used); seq_lens the whole lengths, prefix included."""
-    out = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
-    num_seqs, max_blocks = block_table.shape
-    _need(q.shape[0] == num_seqs, "q must have a row for each sequence of block_table")
-    _check(prefix_table, "prefix_table", torch.int32, device=q.device)
+    out, step, sizes = _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out)
+    _need(q.shape[0] == sizes[0], "q must have a row for each sequence of block_table")
+    i = q.get_device()
+    if not (_plain(prefix_table, torch.int32, i) and _plain(prefix_len, torch.int32, i)):
+        _all_plain(i, torch.int32, prefix_table=prefix_table, prefix_len=prefix_len)
     _need(prefix_table.dim() == 1 and prefix_table.numel() >= 1,
           "prefix_table must be [prefix_blocks]")
-    _check(prefix_len, "prefix_len", torch.int32, 1, q.device)
-    num_blocks, bs, n_kv, hd = k_cache.shape
+    _need(prefix_len.numel() == 1, "prefix_len must have 1 element")
     if workspace is None:
-        workspace = _workspace(_prefix_workspace_bytes(q, k_cache, prefix_table, block_table),
-                               q.device)
-    call("smx_shared_prefix_attention", _stream(q), q.data_ptr(), _q_stride(q),
-         k_cache.data_ptr(), v_cache.data_ptr(), prefix_table.data_ptr(), prefix_len.data_ptr(),
+        workspace = shared_prefix_attention_workspace(q, k_cache, prefix_table, block_table)
+    call("smx_shared_prefix_attention", _stream(q), q.data_ptr(), step, k_cache.data_ptr(),
+         v_cache.data_ptr(), prefix_table.data_ptr(), prefix_len.data_ptr(),
          block_table.data_ptr(), seq_lens.data_ptr(), _ptr(workspace),
-         workspace.numel() if workspace is not None else 0, out.data_ptr(), num_seqs,
-         prefix_table.numel(), max_blocks, num_blocks, bs, q.shape[1], n_kv, hd, float(scale))
+         workspace.numel() if workspace is not None else 0, out.data_ptr(), sizes[0],
+         prefix_table.numel(), *sizes[1:], float(scale))
     return out
 
 
-class RequestTables(NamedTuple):
-    """What request_tables() writes besides the block table."""
-    num_pages: torch.Tensor        # int32 [reqs]: pages each request now has
-    free_count: torch.Tensor       # int32 [1]: pages left in the free list
-    query_start_loc: torch.Tensor  # int32 [reqs + 1]
-    seq_lens: torch.Tensor         # int32 [reqs]
-    positions: torch.Tensor        # int64 [max_tokens], 0 past the last token
-    slot_mapping: torch.Tensor     # int64 [max_tokens], -1 past the last token
+class RequestTables:
+    """What request_tables() writes besides the block table; the buffers are checked
+    once, here.
+      num_pages        int32 [reqs]: pages each request now has
+      free_count       int32 [1]: pages left in the free list
+      query_start_loc  int32 [reqs + 1]
+      seq_lens         int32 [reqs]
+      positions        int64 [max_tokens], 0 past the last token
+      slot_mapping     int64 [max_tokens], -1 past the last token"""
+
+    __slots__ = ("num_pages", "free_count", "query_start_loc", "seq_lens", "positions",
+                 "slot_mapping", "reqs", "max_tokens", "index")
+
+    def __init__(self, num_pages, free_count, query_start_loc, seq_lens, positions,
+                 slot_mapping):
+        _check(num_pages, "num_pages", torch.int32)
+        reqs, dev = num_pages.numel(), num_pages.device
+        _check(free_count, "free_count", torch.int32, 1, dev)
+        _check(query_start_loc, "query_start_loc", torch.int32, reqs + 1, dev)
+        _check(seq_lens, "seq_lens", torch.int32, reqs, dev)
+        _check(positions, "positions", torch.int64, device=dev)
+        _check(slot_mapping, "slot_mapping", torch.int64, positions.numel(), dev)
+        _need(reqs >= 1 and positions.numel() >= 1, "there must be a request and a token")
+        self.num_pages, self.free_count = num_pages, free_count
+        self.query_start_loc, self.seq_lens = query_start_loc, seq_lens
+        self.positions, self.slot_mapping = positions, slot_mapping
+        self.reqs, self.max_tokens, self.index = reqs, positions.numel(), num_pages.get_device()
+
+    def replace(self, **buffers) -> "RequestTables":
+        """The same with some buffers others."""
+        return RequestTables(**{**{n: getattr(self, n) for n in self.__slots__[:6]}, **buffers})
 
 
 def request_tables_out(num_pages: torch.Tensor, max_tokens: int) -> RequestTables:
     """Buffers for request_tables(out=...).  A program that keeps its pages in
-    place passes _replace(num_pages=num_pages, free_count=free_count) of it."""
+    place takes .replace(num_pages=num_pages, free_count=free_count) of it."""
+    _need(max_tokens >= 1, "max_tokens must be >= 1")
     reqs, dev = num_pages.numel(), num_pages.device
     i32 = dict(dtype=torch.int32, device=dev)
     i64 = dict(dtype=torch.int64, device=dev)
@@ -778,17 +812,22 @@ def request_tables_out(num_pages: torch.Tensor, max_tokens: int) -> RequestTable
                          torch.empty(max_tokens, **i64), torch.empty(max_tokens, **i64))
 
 
-def _pages_checks(num_pages, free_pages, free_count, block_table):
-    _check(num_pages, "num_pages", torch.int32)
+def _pages_checks(num_pages, free_pages, free_count, block_table, lens, lens_name):
+    _need(isinstance(num_pages, torch.Tensor), "num_pages must be a tensor")
+    i = num_pages.get_device()
+    if i < 0 or not (_plain(num_pages, torch.int32, i) and _plain(free_pages, torch.int32, i)
+                     and _plain(free_count, torch.int32, i)
+                     and _plain(block_table, torch.int32, i) and _plain(lens, torch.int32, i)):
+        _all_plain(i, torch.int32, num_pages=num_pages, free_pages=free_pages,
+                   free_count=free_count, block_table=block_table, **{lens_name: lens})
     reqs = num_pages.numel()
-    _need(reqs >= 1, "there must be a request")
-    _check(free_pages, "free_pages", torch.int32, device=num_pages.device)
+    _need(reqs >= 1 and lens.numel() == reqs, f"{lens_name} must have an entry for each request")
     _need(free_pages.numel() >= 1, "free_pages must have room for a page")
-    _check(free_count, "free_count", torch.int32, 1, num_pages.device)
-    _check(block_table, "block_table", torch.int32, device=num_pages.device)
-    _need(block_table.dim() == 2 and block_table.shape[0] == reqs and block_table.shape[1] >= 1,
+    _need(free_count.numel() == 1, "free_count must have 1 element")
+    shape = block_table.shape
+    _need(len(shape) == 2 and shape[0] == reqs and shape[1] >= 1,
           "block_table must be [reqs, max_blocks]")
-    return reqs
+    return reqs, shape[1], i
 
 
 def request_tables(query_lens: torch.Tensor, context_lens: torch.Tensor,
@@ -800,27 +839,23 @@ def request_tables(query_lens: torch.Tensor, context_lens: torch.Tensor,
     rows lack are taken from the end of the free list and written into the table;
     num_pages and free_count are updated out of place, or in place where `out`
     holds them.  max_tokens (without `out`): the size of positions and slots."""
-    reqs = _pages_checks(num_pages, free_pages, free_count, block_table)
-    dev = num_pages.device
-    _check(query_lens, "query_lens", torch.int32, reqs, dev)
-    _check(context_lens, "context_lens", torch.int32, reqs, dev)
+    reqs, max_blocks, i = _pages_checks(num_pages, free_pages, free_count, block_table,
+                                        query_lens, "query_lens")
+    if not (isinstance(context_lens, torch.Tensor) and _plain(context_lens, torch.int32, i)
+            and context_lens.numel() == reqs):
+        _check(context_lens, "context_lens", torch.int32, reqs, num_pages.device)
     if out is None:
-        _need(max_tokens is not None and max_tokens >= 1, "max_tokens or out is needed")
+        _need(max_tokens is not None, "max_tokens or out is needed")
         out = request_tables_out(num_pages, max_tokens)
-    else:
-        _check(out.num_pages, "out.num_pages", torch.int32, reqs, dev)
-        _check(out.free_count, "out.free_count", torch.int32, 1, dev)
-        _check(out.query_start_loc, "out.query_start_loc", torch.int32, reqs + 1, dev)
-        _check(out.seq_lens, "out.seq_lens", torch.int32, reqs, dev)
-        _check(out.positions, "out.positions", torch.int64, max_tokens, dev)
-        _check(out.slot_mapping, "out.slot_mapping", torch.int64, out.positions.numel(), dev)
-        _need(out.positions.numel() >= 1, "out.positions must hold a token")
+    _need(isinstance(out, RequestTables) and out.reqs == reqs and out.index == i
+          and max_tokens in (None, out.max_tokens),
+          "out must be RequestTables of these requests and max_tokens")
     call("smx_request_tables", _stream(num_pages), query_lens.data_ptr(),
          context_lens.data_ptr(), num_pages.data_ptr(), free_pages.data_ptr(),
          free_count.data_ptr(), block_table.data_ptr(), out.num_pages.data_ptr(),
          out.free_count.data_ptr(), out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(),
-         out.positions.data_ptr(), out.slot_mapping.data_ptr(), reqs, out.positions.numel(),
-         block_table.shape[1], free_pages.numel(), block_size)
+         out.positions.data_ptr(), out.slot_mapping.data_ptr(), reqs, out.max_tokens, max_blocks,
+         free_pages.numel(), block_size)
     return out
 
 
@@ -829,11 +864,11 @@ def release_pages(keep_lens: torch.Tensor, num_pages: torch.Tensor, free_pages: 
     """Give the pages beyond the first keep_lens[r] tokens of every request back to
     the free list (0: all of a finished request's; fewer than its length: those
     of rejected tokens).  Everything is updated in place."""
-    reqs = _pages_checks(num_pages, free_pages, free_count, block_table)
-    _check(keep_lens, "keep_lens", torch.int32, reqs, num_pages.device)
+    reqs, max_blocks, _ = _pages_checks(num_pages, free_pages, free_count, block_table, keep_lens,
+                                        "keep_lens")
     call("smx_release_pages", _stream(num_pages), keep_lens.data_ptr(), num_pages.data_ptr(),
-         free_pages.data_ptr(), free_count.data_ptr(), block_table.data_ptr(), reqs,
-         block_table.shape[1], free_pages.numel(), block_size)
+         free_pages.data_ptr(), free_count.data_ptr(), block_table.data_ptr(), reqs, max_blocks,
+         free_pages.numel(), block_size)
 
 
 class PackedQ4_0:

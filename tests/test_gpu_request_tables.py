@@ -41,7 +41,7 @@ def _check(query, context, width, bs, free, max_tokens, seed=0, capacity=None, i
     ops = _ops()
     out = ops.request_tables_out(n, max_tokens)
     if in_place:
-        out = out._replace(num_pages=n, free_count=c)
+        out = out.replace(num_pages=n, free_count=c)
     got = ops.request_tables(_i32(query), _i32(context), n, fp, c, t, bs, out=out)
     want = tables64(query, context, held, left, len(left), table, bs, max_tokens)
     for name, a, b in zip(("table", "num_pages", "free_count", "query_start_loc", "seq_lens",
@@ -125,7 +125,7 @@ def test_random_steps_with_releases():
     lens = [0] * S
     for step in range(25):
         query = [min(r.choice([0, 1, 1, 5, 40]), width * bs - x) for x in lens]
-        out = ops.request_tables_out(n, 400)._replace(num_pages=n, free_count=c)
+        out = ops.request_tables_out(n, 400).replace(num_pages=n, free_count=c)
         got = ops.request_tables(_i32(query), _i32(lens), n, fp, c, t, bs, out=out)
         lens = [a + b for a, b in zip(lens, query)]
         assert got.seq_lens.tolist() == lens
@@ -173,7 +173,7 @@ def test_captured_and_replayed():
     n, t = _i32([0] * S), torch.full((S, width), -1, dtype=torch.int32, device="cuda")
     fp, c = _i32(list(range(500))), _i32([500])
     query, context = _i32([0] * S), _i32([0] * S)
-    out = ops.request_tables_out(n, 6000)._replace(num_pages=n, free_count=c)
+    out = ops.request_tables_out(n, 6000).replace(num_pages=n, free_count=c)
     call = lambda: ops.request_tables(query, context, n, fp, c, t, bs, out=out)  # noqa: E731
     call()
     torch.cuda.synchronize()
@@ -209,5 +209,5 @@ def test_wrapper_refusals():
     with pytest.raises(pkg("native").SmxError):
         ops.request_tables(**{**ok, "block_size": 24})
     with pytest.raises(pkg("native").SmxError):  # lengths are not updated in place
-        out = ops.request_tables_out(ok["num_pages"], 2)._replace(seq_lens=ok["context_lens"])
+        out = ops.request_tables_out(ok["num_pages"], 2).replace(seq_lens=ok["context_lens"])
         ops.request_tables(**{**ok, "max_tokens": None, "out": out})
