@@ -13,7 +13,9 @@ vLLM's AttentionBackend / AttentionImpl method names:
   SplitKVDecodeImpl.forward(layer, query, key, value, kv_cache,
       attn_metadata, output=None)
       writes key/value at slot_mapping, runs split-KV decode and the LSE
-      merge (HIP kernels), returns [num_tokens, n_q * head_dim] bf16.
+      merge (HIP kernels), returns [num_tokens, n_q * head_dim] bf16; with
+      the metadata's query_start_loc or prefix_table, causal attention of
+      packed rows or decode under a shared prefix instead.
   SplitKVDecodeBackend.plan(attn_metadata, block_size, num_heads, head_size)
       once per step for a batch: cuts the live tokens into per-sequence
       splits of one length (a device kernel), which every layer's forward
@@ -45,6 +47,15 @@ class SplitKVDecodeMetadata:
     num_items: int = 0            # a plan's split budget (SplitKVDecodeBackend.plan)
     plan: torch.Tensor | None = None  # int32 [num_items + num_seqs, 64] plan records
     plan_positions: torch.Tensor | None = None  # the positions the plan's records carry
+    # packed query rows (prompts, chunks, drafted tokens): int32 [num_seqs + 1]
+    query_start_loc: torch.Tensor | None = None
+    # decode under a prefix that all sequences share: its pages int32 [blocks] and
+    # length int32 [1]
+    prefix_table: torch.Tensor | None = None
+    prefix_len: torch.Tensor | None = None
+    # the workspace of prompt_attention / shared_prefix_attention, which the layers of
+    # a pass can share (None: each call allocates its own)
+    workspace: torch.Tensor | None = None
 
 
 def choose_num_splits(capacity: int, tokens_per_split: int = 128, num_seqs: int = 1) -> int:
@@ -109,14 +120,34 @@ class SplitKVDecodeImpl:
     def forward(self, layer, query: torch.Tensor, key: torch.Tensor | None,
                 value: torch.Tensor | None, kv_cache: torch.Tensor,
                 attn_metadata: SplitKVDecodeMetadata, output: torch.Tensor | None = None):
-        """query [num_seqs, n_q*hd] (one decode token per sequence)."""
+        """query [num_seqs, n_q*hd]: one decode token per sequence; with
+        attn_metadata.query_start_loc [num_tokens, n_q*hd]: packed rows of any number
+        of tokens per sequence (rows of none are left as they are in `output`, 0
+        without it); with attn_metadata.prefix_table one decode token per
+        sequence under a shared prefix, read once for all."""
         k_cache, v_cache = kv_cache[0], kv_cache[1]
+        packed, shared = attn_metadata.query_start_loc, attn_metadata.prefix_table
+        if packed is not None and shared is not None:
+            raise ValueError("packed query rows and a shared prefix do not go together")
         num_seqs = attn_metadata.seq_lens.numel()
         if key is not None and value is not None:
             torch_ops.reshape_and_cache(key.reshape(-1, self.num_kv_heads, self.head_size),
                                         value.reshape(-1, self.num_kv_heads, self.head_size),
                                         k_cache, v_cache, attn_metadata.slot_mapping)
+        if packed is not None:
+            q = query.reshape(-1, self.num_heads, self.head_size)
+            out = torch.zeros_like(q) if output is None else output.view(q.shape)
+            torch_ops.prompt_attention(q, k_cache, v_cache, attn_metadata.block_tables, packed,
+                                       attn_metadata.seq_lens, self.scale,
+                                       workspace=attn_metadata.workspace, out=out)
+            return out.view(-1, self.num_heads * self.head_size)
         q = query.reshape(num_seqs, self.num_heads, self.head_size)
+        if shared is not None:
+            out = torch_ops.shared_prefix_attention(
+                q, k_cache, v_cache, shared, attn_metadata.prefix_len, attn_metadata.block_tables,
+                attn_metadata.seq_lens, self.scale, workspace=attn_metadata.workspace,
+                out=None if output is None else output.view(q.shape))
+            return out.view(num_seqs, self.num_heads * self.head_size)
         po, pl = split_partials(num_seqs, attn_metadata.num_splits, self.num_heads,
                                 self.head_size, query.device)
         out = output.view(num_seqs, self.num_heads, self.head_size) if output is not None else None

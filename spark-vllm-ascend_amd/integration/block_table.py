@@ -8,12 +8,18 @@ multi-sequence decode this module keeps the host side of that: a free list of
 physical pages, each sequence's pages in order, and the device block table
 ``[max_seqs, max_blocks]`` int32 the attention kernel reads (unused entries
 are -1).  Slots for a step come from ``torch_ops.compute_slot_mapping``.
+
+DeviceBlockTables keeps all of that on the device instead, where the lengths
+may be known there alone (drafted tokens accepted by a kernel, steps in a
+captured graph): a step is one or two launches (``torch_ops.request_tables``).
 """
 from __future__ import annotations
 
 from collections import deque
 
 import torch
+
+from ..native import torch_ops
 
 
 class BlockManager:
@@ -106,3 +112,42 @@ class BlockManager:
                     positions=pos.to(dev),
                     seq_lens=(pos + 1).to(torch.int32).to(dev),
                     query_start_loc=torch.arange(len(seq_ids) + 1, dtype=torch.int32).to(dev))
+
+
+class DeviceBlockTables:
+    """Pages, block tables and lengths of up to `max_seqs` requests, on the device:
+    request r is row r.  Nothing is read back: a request that finds the free list
+    empty gets -1 entries and slots (its tokens are not kept), which num_pages
+    (below ceil(len / block_size)) tells.  Steps follow one another on a stream."""
+
+    def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_blocks_per_seq: int,
+                 max_tokens: int, device):
+        if min(num_blocks, block_size, max_seqs, max_blocks_per_seq, max_tokens) < 1:
+            raise ValueError("sizes must be >= 1")
+        self.block_size = block_size
+        i32 = dict(dtype=torch.int32, device=device)
+        self.block_table = torch.full((max_seqs, max_blocks_per_seq), -1, **i32)
+        self.num_pages = torch.zeros(max_seqs, **i32)
+        self.lens = torch.zeros(max_seqs, **i32)
+        # pages are taken from the end: 0 first
+        self.free_pages = torch.arange(num_blocks - 1, -1, -1, **i32)
+        self.free_count = torch.full((1,), num_blocks, **i32)
+        self._out = torch_ops.request_tables_out(self.num_pages, max_tokens).replace(
+            num_pages=self.num_pages, free_count=self.free_count)
+
+    def step(self, query_lens: torch.Tensor) -> torch_ops.RequestTables:
+        """query_lens (int32 [max_seqs], on the device) more tokens a request: takes
+        their pages and gives the step's query_start_loc, seq_lens, positions and
+        slot_mapping (buffers of this object, valid until the next step)."""
+        out = torch_ops.request_tables(query_lens, self.lens, self.num_pages, self.free_pages,
+                                       self.free_count, self.block_table, self.block_size,
+                                       out=self._out)
+        self.lens.copy_(out.seq_lens)
+        return out
+
+    def keep(self, lens: torch.Tensor) -> None:
+        """Takes every request back to its first lens[r] tokens (int32 [max_seqs], at
+        most its length; 0 ends it): pages no longer needed are free again."""
+        torch_ops.release_pages(lens, self.num_pages, self.free_pages, self.free_count,
+                                self.block_table, self.block_size)
+        torch.minimum(self.lens, lens.clamp(min=0), out=self.lens)

@@ -14,6 +14,12 @@ under the namespace ``smx``:
   smx::add_rmsnorm(x, residual, gamma, eps) -> (y, residual_out)
   smx::splitkv_decode_attention(q, k_cache, v_cache, block_table, seq_lens,
                                 num_splits, scale) -> out   bf16 [seqs, n_q, hd]
+  smx::prompt_attention(q, k_cache, v_cache, block_table, query_start_loc,
+                        seq_lens, scale) -> out       bf16 [tokens, n_q, hd],
+      rows of no sequence 0
+  smx::shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len,
+                               block_table, seq_lens, scale) -> out
+                                                       bf16 [seqs, n_q, hd]
   smx::argmax(logits) -> ids                           int64 [rows]
   smx::layer_run(x, residual, positions, layer_name) -> (y, residual_out)
       one decoder layer's decode step over the layers layer_run.install()
@@ -82,6 +88,30 @@ def register() -> None:
     @splitkv_decode_attention.register_fake
     def _(q, k_cache, v_cache, block_table, seq_lens, num_splits, scale):
         return torch.empty_like(q)
+
+    @torch.library.custom_op(f"{_NS}::prompt_attention", mutates_args=())
+    def prompt_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         block_table: torch.Tensor, query_start_loc: torch.Tensor,
+                         seq_lens: torch.Tensor, scale: float) -> torch.Tensor:
+        q = q.contiguous()
+        return torch_ops.prompt_attention(q, k_cache, v_cache, block_table, query_start_loc,
+                                          seq_lens, scale, out=torch.zeros_like(q))
+
+    @prompt_attention.register_fake
+    def _(q, k_cache, v_cache, block_table, query_start_loc, seq_lens, scale):
+        return q.new_empty(q.shape)
+
+    @torch.library.custom_op(f"{_NS}::shared_prefix_attention", mutates_args=())
+    def shared_prefix_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                prefix_table: torch.Tensor, prefix_len: torch.Tensor,
+                                block_table: torch.Tensor, seq_lens: torch.Tensor,
+                                scale: float) -> torch.Tensor:
+        return torch_ops.shared_prefix_attention(q.contiguous(), k_cache, v_cache, prefix_table,
+                                                 prefix_len, block_table, seq_lens, scale)
+
+    @shared_prefix_attention.register_fake
+    def _(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, scale):
+        return q.new_empty(q.shape)
 
     @torch.library.custom_op(f"{_NS}::argmax", mutates_args=())
     def argmax(logits: torch.Tensor) -> torch.Tensor:

@@ -40,6 +40,10 @@ Kernel sequence (HIP launches):
           its linears were packed, Q4_0LinearMethod.pack): QKV GEMM -> fused planned split-KV + merge
           -> o_proj GEMM -> add + RMSNorm -> gate|up GEMM with SwiGLU -> down
           GEMM -> add + RMSNorm(next norm).
+  Packed rows (the metadata's query_start_loc: prompts, chunks, drafted
+          tokens; any T): prompt_layer (integration/prompt.py), its positions
+          the argument, its slots metadata.slot_mapping -> add +
+          RMSNorm(next norm).
 Other calls -- no published metadata, more than 16 rows, or rows that are
 not one decode token per sequence (prefill) -- go to the stock layer, as the
 reference's op runs vLLM's attention, post-attention norm, MLP and next norm
@@ -60,6 +64,7 @@ import torch
 from ..native import torch_ops
 from .attention import SplitKVDecodeMetadata, split_partials
 from .linear import gemm_weight
+from .prompt import PromptRows, prompt_layer
 
 _layers: dict = {}
 _metadata: SplitKVDecodeMetadata | None = None
@@ -157,6 +162,25 @@ def _check_plan_positions(md: SplitKVDecodeMetadata, positions: torch.Tensor) ->
         raise ValueError("positions differ from those the step's plan was built with")
 
 
+def _packed_rows(e: _Entry, md: SplitKVDecodeMetadata, x: torch.Tensor, residual: torch.Tensor,
+                 positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The layer over packed rows (the metadata has a query_start_loc)."""
+    c = e.cfg
+    if x.dim() != 2 or x.shape[1] != c.hidden or x.dtype != torch.bfloat16:
+        raise ValueError(f"x must be bf16 [T, {c.hidden}], got {x.dtype} {tuple(x.shape)}")
+    if tuple(residual.shape) != tuple(x.shape) or residual.dtype != torch.bfloat16:
+        raise ValueError("residual must be bf16 of x's shape")
+    T = x.shape[0]
+    for t, name in ((positions, "positions"), (md.slot_mapping, "slot_mapping")):
+        if t.numel() != T or t.dtype != torch.int64:
+            raise ValueError(f"{name} must be int64 [T]")
+    rows = PromptRows(md.block_tables, md.query_start_loc, md.seq_lens, positions.contiguous(),
+                      md.slot_mapping, md.workspace)
+    d, res = prompt_layer(c, e.layer, e.cos_sin, e.scale, e.act_lut, x.contiguous(),
+                          residual.contiguous(), rows)
+    return torch_ops.add_rmsnorm(d, res, e.next_norm, c.eps)
+
+
 def layer_run(x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor,
               layer_name: str) -> tuple[torch.Tensor, torch.Tensor]:
     """One decoder layer's decode step; see the module docstring."""
@@ -165,6 +189,8 @@ def layer_run(x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor,
     e = _layers[layer_name]
     md = _metadata
     T = x.shape[0] if x.dim() == 2 else -1
+    if md is not None and md.query_start_loc is not None:
+        return _packed_rows(e, md, x, residual, positions)
     decode = md is not None and 1 <= T <= 16 and md.seq_lens.numel() == T
     if not decode:
         if e.stock is not None:  # prefill and unpublished metadata: the stock layer

@@ -43,6 +43,7 @@ from ..native import torch_ops
 from .attention import choose_num_splits, choose_plan
 from .head import TiedQ4_0Head
 from .linear import Q4_0Linear, gemm_weight
+from .prompt import PromptRows, prompt_layer
 from .weights import synthetic_q4_0
 
 
@@ -427,6 +428,70 @@ class DecodeModel:
         st.slot_mapping.copy_(st.block_table[:, 0].to(torch.int64) * self.cfg.block_size)
         self.head.embed(st.ids, out=self.x)
 
+    def prefill(self, prompt, chunk_tokens: int = 8192) -> torch.Tensor:
+        """Takes the prompt(s) in through the layers' packed rows (prompt_layer)
+        instead of one token a step: their K and V are in the cache, and the state
+        is as after the step that fed each sequence's last prompt token, so that
+        step() (or a captured graph, or the runner) goes on with the first generated
+        one.  prompt as for reset(); passes of at most chunk_tokens rows, the
+        sequences' in turn.  Returns the last tokens' logits [batch, vocab]
+        (self.logits)."""
+        if chunk_tokens < 1:
+            raise ValueError("chunk_tokens must be >= 1")
+        c, st, ops, dev = self.cfg, self.state, torch_ops, self.device
+        self.reset(prompt)
+        lens = st.forced_len.tolist()
+        i32 = dict(dtype=torch.int32, device=dev)
+        # the sequences have their pages already: none is taken from this list
+        pages = torch.full((self.batch,), st.block_table.shape[1], **i32)
+        free, none = torch.full((1,), -1, **i32), torch.zeros(1, **i32)
+        done = [0] * self.batch
+        while sum(done) < sum(lens):
+            n, room = [], chunk_tokens
+            for length, at in zip(lens, done):
+                n.append(min(length - at, room))
+                room -= n[-1]
+            total = sum(n)
+            tables = ops.request_tables(torch.tensor(n, **i32), torch.tensor(done, **i32), pages,
+                                        free, none, st.block_table, c.block_size,
+                                        max_tokens=total)
+            ids = torch.cat([st.forced[r, at:at + k] for r, (at, k) in enumerate(zip(done, n))])
+            x = self.head.embed(ids)
+            rows = PromptRows(st.block_table, tables.query_start_loc, tables.seq_lens,
+                              tables.positions, tables.slot_mapping,
+                              ops.prompt_attention_workspace(
+                                  x.new_empty((total, c.n_q, c.head_dim)),
+                                  self.layers[0].kv_cache[0], st.block_table))
+            residual = None
+            for L in self.layers:
+                h, residual = ops.add_rmsnorm(x, residual, L.input_norm, c.eps)
+                x, residual = prompt_layer(c, L, self.cos_sin, self.scale, self.act_lut, h,
+                                           residual, rows)
+            done = [at + k for at, k in zip(done, n)]
+            # the last rows of the sequences that this pass finished
+            ended = [r for r in range(self.batch) if n[r] and done[r] == lens[r]]
+            if ended:
+                last = torch.tensor([sum(n[:r + 1]) - 1 for r in ended], device=dev)
+                h, _ = ops.add_rmsnorm(x[last], residual[last], self.final_norm, c.eps)
+                self.h[torch.tensor(ended, device=dev)] = h
+        if self.batch == 1:
+            ops.q4_0_gemv(self.h, self.head.q4_0_head, c.vocab, c.hidden, out=self.logits)
+        else:
+            head = self.head_packed if self.head_packed is not None else self.head.q4_0_head
+            ops.q4_0_gemm(self.h, head, c.vocab, c.hidden, out=self.logits)
+        ops.argmax(self.logits, out=st.next_ids)
+        # the state of the step that feeds the last prompt token, then its end
+        last = st.forced_len.to(torch.int64) - 1
+        at = torch.arange(self.max_len, device=dev)[None]
+        st.tokens.copy_(torch.where(at <= last[:, None], st.forced, -1))
+        st.ids.copy_(st.forced.gather(1, last[:, None]).view(-1))
+        st.positions.copy_(last)
+        ops.decode_advance(st.next_ids, st.ids, st.positions, st.seq_lens, st.slot_mapping,
+                           st.block_table, c.block_size, tokens_out=st.tokens,
+                           forced_ids=st.forced, forced_len=st.forced_len,
+                           embed_table=self.head.weight, embed_out=self.x)
+        return self.logits
+
     def fill_kv(self, seed: int) -> None:
         """Seeded N(0, 1) bf16 values in every layer's whole KV cache (K and V
         planes), generated on the device: a cache with realistic contents
@@ -453,22 +518,31 @@ class DecodeModel:
                                      dtype=torch.int64))
         self.head.embed(st.ids, out=self.x)
 
-    def generate(self, prompt, new_tokens: int, fences: str | None = None) -> torch.Tensor:
+    def generate(self, prompt, new_tokens: int, fences: str | None = None,
+                 prefill: bool = False) -> torch.Tensor:
         """Greedy decode: feeds the prompt(s), then new_tokens generated
         tokens.  Returns the token ids by position (prompt followed by
         generated): [total] for batch 1, else [batch, longest total].  With
         fences, the steps run on the recorded step runner (record_runner)
-        with that fence mode, all of them in one replay."""
+        with that fence mode, all of them in one replay.  With prefill, the
+        prompts are taken in by prefill() and every sequence gets new_tokens
+        (of ragged prompts, a shorter one's positions past its own are -1;
+        without prefill its generated tokens go on to the longest's total)."""
         prompts = list(prompt) if isinstance(prompt, (list, tuple)) else [prompt] * self.batch
         total = max(int(torch.as_tensor(p).numel()) for p in prompts) + new_tokens
         if total > self.max_len:
             raise ValueError("prompt + new_tokens exceeds max_len")
-        self.reset(prompt)
-        if fences is not None:
-            if total > 1:
-                self.run_steps(total - 1, fences)
+        if prefill and new_tokens > 0:
+            self.prefill(prompt)
+            steps = new_tokens - 1
         else:
-            for _ in range(total - 1):
+            self.reset(prompt)
+            steps = total - 1
+        if fences is not None:
+            if steps > 0:
+                self.run_steps(steps, fences)
+        else:
+            for _ in range(steps):
                 self.step()
         torch.cuda.synchronize(self.device)
         out = self.state.tokens[:, :total].clone()
