@@ -52,7 +52,7 @@ __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
 }
 
 constexpr float LAG = 8.f;        // log2 units
-constexpr float NO_REF = -1e30f;  // below every finite score's, and 2^(NO_REF - that) is 0
+constexpr float NO_REF = -3e38f;  // before the first token: below the scores of any use
 
 struct RowsArgs {
   const uint16_t* q;
@@ -129,10 +129,13 @@ __device__ __forceinline__ void meet() {
   __asm__ volatile("" ::: "memory");
 }
 
-template <int HD, int WM, int WN, int KT, int ST>
+// BS: the least block_size, 32 or 64: a tile is looked up and addressed by NP pieces
+// of BT tokens that are within a page.
+template <int HD, int WM, int WN, int KT, int ST, int BS>
 __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
   using S = Shape<HD, WM, WN, KT, ST>;
   constexpr int KS = HD / 16, DT = HD / 32, NU = KT / 32, CH = S::CH;
+  constexpr int BT = KT < BS ? KT : BS, NP = KT / BT;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WM, wn = wave / WM;
@@ -166,11 +169,12 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   lim_min = __builtin_amdgcn_readfirstlane(lim_min);
 
   // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile, by
-  // buffer loads into LDS whose resource is one half of 32 tokens (within a page):
-  // tokens past the end, and those of a table entry outside the cache, are past
-  // the resource's end and read as 0 without an access.  Pages are looked up a
-  // round before they are used, by scalar loads (the table is constant while the
-  // kernel runs), which do not queue behind the tiles' loads.
+  // buffer loads into LDS whose resource is one piece of BT tokens: tokens past the
+  // end, and those of a table entry outside the cache, are past the resource's end
+  // and read as 0 without an access.  Pages are looked up a round before they are
+  // used, by scalar loads (the table is constant while the kernel runs), which do
+  // not queue behind the tiles' loads.  (Whole tiles of 64 by one resource where
+  // pages allow it: a third less scalar arithmetic, 8192-token prompt 541 us, 531.)
   const int first = it.from & ~(KT - 1);
   const int ntiles = it.to > it.from ? (it.to - first + KT - 1) / KT : 0;
   const int rounds = (ntiles + WN - 1) / WN;
@@ -178,22 +182,22 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   const int lrow = lane / CH, lc = lane % CH;  // the lane's row and chunk of a load
   const int tok_bytes = 2 * tok_stride;
   const constant_i32* const table = (const constant_i32*)it.table;
-  auto look_up = [&](int (&page)[NU], int base) {
+  auto look_up = [&](int (&page)[NP], int base) {
 #pragma unroll
-    for (int u = 0; u < NU; ++u)
-      page[u] = table[max(min(base + 32 * u, it.to - 1), 0) >> A.bs_log2];
+    for (int u = 0; u < NP; ++u)
+      page[u] = table[max(min(base + BT * u, it.to - 1), 0) >> A.bs_log2];
   };
-  auto stage = [&](const uint16_t* cache, lds_u32x4* dst, const int (&page)[NU], int base,
+  auto stage = [&](const uint16_t* cache, lds_u32x4* dst, const int (&page)[NP], int base,
                    auto swz) {
-    __amdgpu_buffer_rsrc_t half[NU];
+    __amdgpu_buffer_rsrc_t piece[NP];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      const int t = base + 32 * u;
+    for (int u = 0; u < NP; ++u) {
+      const int t = base + BT * u;
       const bool known = (unsigned)page[u] < (unsigned)A.num_blocks;
-      const int rows = known ? min(it.to - t, 32) : 0;
+      const int rows = known ? min(it.to - t, BT) : 0;
       const uint16_t* const at = cache + (int64_t)(known ? page[u] : 0) * page_stride +
                                  (t & (bs - 1)) * tok_stride + kvh * HD;
-      half[u] = __builtin_amdgcn_make_buffer_rsrc(
+      piece[u] = __builtin_amdgcn_make_buffer_rsrc(
           (void*)at, 0, rows > 0 ? (rows - 1) * tok_bytes + 2 * HD : 0, 0x00027000);
     }
 #pragma unroll
@@ -202,21 +206,21 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       const int r0 = c0 / CH;             // its row
       const int off = lrow * tok_bytes + 16 * (lc ^ swz(r0 + lrow));
       const __amdgpu_buffer_rsrc_t src =
-          i * WM * 64 / CH >= 32 || (NU == 2 && r0 >= 32) ? half[NU - 1] : half[0];
+          NP > 1 && (i * WM * 64 / CH >= BT || r0 >= BT) ? piece[NP - 1] : piece[0];
       __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_void*)(dst + c0), 16, off,
-                                               (r0 & 31) * tok_bytes, 0, 0);
+                                               (r0 & (BT - 1)) * tok_bytes, 0, 0);
     }
   };
-  auto stage_k = [&](lds_u32x4* dst, const int (&page)[NU], int base) {
+  auto stage_k = [&](lds_u32x4* dst, const int (&page)[NP], int base) {
     stage(A.kc, dst, page, base, [](int r) { return k_swz<HD>(r); });
   };
-  auto stage_v = [&](lds_u32x4* dst, const int (&page)[NU], int base) {
+  auto stage_v = [&](lds_u32x4* dst, const int (&page)[NP], int base) {
     stage(A.vc, dst, page, base, [](int r) { return v_swz<HD>(r); });
   };
-  auto bad_pages = [&](const int (&page)[NU]) {
+  auto bad_pages = [&](const int (&page)[NP]) {
     int bad = 0;
 #pragma unroll
-    for (int u = 0; u < NU; ++u) bad |= (unsigned)page[u] >= (unsigned)A.num_blocks ? 1 << u : 0;
+    for (int u = 0; u < NP; ++u) bad |= (unsigned)page[u] >= (unsigned)A.num_blocks ? 1 << u : 0;
     return bad;
   };
 
@@ -261,7 +265,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = base + 32 * u + 8 * (i / 4) + 4 * h + i % 4;
-          const float x = bad >> u & 1 ? __builtin_nanf("") : s[u][i];
+          const float x = bad >> (NP == NU ? u : 0) & 1 ? __builtin_nanf("") : s[u][i];
           s[u][i] = t >= it.from && t < lim ? x : -INFINITY;
         }
     }
@@ -377,7 +381,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   // restrict so that the compiler does not wait for the loads into the one before
   // it reads the other; the wait that counts is the one before the barrier.
   int bad[ST];  // of the tiles in LDS, that of this round first
-  int page[NU];
+  int page[NP];
 #pragma unroll
   for (int i = 0; i < ST; ++i) bad[i] = 0;
   look_up(page, first + wn * KT);
@@ -591,7 +595,7 @@ __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, in
 // Packed prompts.  Sequence r's queries are the tokens [query_start[r],
 // query_start[r + 1]), the last n of its L tokens: token i of them is at position
 // L - n + i and sees the tokens up to itself.  Grid: kv heads, items.
-template <int HD, int WM, int WN, int KT, int ST>
+template <int HD, int WM, int WN, int KT, int ST, int BS>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
 void prompt_attention_kernel(RowsArgs A) {
   using S = Shape<HD, WM, WN, KT, ST>;
@@ -643,7 +647,7 @@ void prompt_attention_kernel(RowsArgs A) {
   it.counts = split == 0 && A.splits > 1 ? A.counts : nullptr;
   it.parts = place.parts;
   it.direct = place.parts == 1;
-  attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
+  attend<HD, WM, WN, KT, ST, BS>(A, it, kvh, smem);
   stores_done();
 }
 
@@ -653,7 +657,7 @@ void prompt_attention_kernel(RowsArgs A) {
 // work list in parts of one length.  More (BIG): the prefix's items come first,
 // workgroups of 128 rows, one a compute unit, bound by the matrix units; the
 // sequences' items, bound by memory, run beside them.
-template <int HD, bool BIG>
+template <int HD, bool BIG, int BS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void shared_prefix_kernel(RowsArgs A) {
   constexpr int WM = 2, WN = 2, KT = 32, ST = 2;
@@ -688,7 +692,7 @@ void shared_prefix_kernel(RowsArgs A) {
     const int split = blockIdx.y / A.tiles;
     if (split >= parts) return;
     prefix_item(split, blockIdx.y - split * A.tiles, B::M, chunk * 64, parts);
-    attend<HD, 4, 1, 64, 2>(A, it, kvh, smem);
+    attend<HD, 4, 1, 64, 2, BS>(A, it, kvh, smem);
   };
   auto listed_part = [&](int item) {
     const int group_tiles = (A.group + S::M - 1) / S::M;
@@ -726,7 +730,7 @@ void shared_prefix_kernel(RowsArgs A) {
       it.counts = split > 0 ? nullptr : A.counts + rows;
       it.parts = place.parts;
     }
-    attend<HD, WM, WN, KT, ST>(A, it, kvh, smem);
+    attend<HD, WM, WN, KT, ST, 32>(A, it, kvh, smem);
   };
   const int big = BIG ? A.tiles * A.splits : 0;
   if (BIG && (int)blockIdx.y < big)
@@ -858,49 +862,71 @@ int tune(const char* name, int v) {
   return e ? atoi(e) : v;
 }
 
-constexpr int MAX_PARTS = 64;
+// How a call is cut, from its sizes (lengths are on the device).  512 workgroups of
+// 64 KB of LDS and 256 threads fill the chip once.
+constexpr int FILL = 512, MAX_PARTS = 64;
 
 struct Choice {
-  int m, splits, suffix_splits, tiles, target;
+  int m;  // rows of a workgroup: 64 (two waves share them, two groups the tokens) or 128
+  int splits, suffix_splits, tiles, target;
 };
 
+// 128 rows multiply faster (a K tile read from L2 serves twice the rows), 64 fill
+// the chip sooner and halve the longest workgroup.  us at 32 / 8 heads of 128,
+// rows of 64 / of 128: a prompt of 512 tokens 13.3 / 17.9, 1024 22.1 / 27.9, 1500
+// 37.7 / 42.9, 2048 53.8 / 52.1, 2500 82 / 73; 16 prompts to 300 20.6 / 19.1.  Short
+// prompts of many sequences are bound by the latency of a workgroup: 12 of 83 tokens
+// 18.9 / 14.9, 31 of 62 22.7 / 18.3.
+//
+// Cutting a tile's tokens into parts pays for its second launch (about 4 us) where
+// few workgroups have long ranges.  us whole / cut: 512 tokens behind 2000 58.7 /
+// 43.5, 4 sequences of 200 behind 8000 142 / 157; 29 of up to 7 tokens behind 2300 to
+// 6900, whose longest would run alone, 137 / 98, but 23 of up to 11 behind 2821, bound
+// by memory already, 51 / 59.  Short tables stay whole: 10 sequences of one token
+// behind 642, 8 / 1 heads, 14.4 / 12.2, 3 prompts to 529 14.3 / 20.6.  A part is at
+// least 256 tokens: 300 behind 1500 31.5 at 512, 32.2 at 256, 35.6 at 1024, one token
+// behind 900 14.6 at 512, 12.3 at 256.
 Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
   auto tiles = [&](int m) { return (rows + m - 1) / m * num_seqs; };  // of even lengths
   c.splits = 1;
-  c.m = tiles(128) * n_kv >= 512 ? 128 : 64;
-  const bool few = c.m == 64 && tiles(64) * n_kv < 400 && cap >= 1024;
-  if (few && rows > 1024) c.m = 128;
-  c.m = tune("SMX_PA_M", c.m);
+  c.m = tiles(128) * n_kv >= FILL ? 128 : 64;
+  const bool few = c.m == 64 && cap >= (rows <= 64 ? 768 : 1024) &&
+                   tiles(64) * n_kv < (rows <= 64 && cap < 4096 ? 160 : 400);
+  if (few ? rows > 1024 : rows > 64 && rows <= 512 && tiles(64) * n_kv >= 256) c.m = 128;
+  c.m = tune("SMX_PA_M", c.m) < 128 ? 64 : 128;
   c.tiles = (int)((num_tokens * group + c.m - 1) / c.m + num_seqs - 1);
-  c.target = std::max(1, tune("SMX_PA_TARGET", 512) / n_kv);
+  c.target = std::max(1, FILL / n_kv);
   if (few) {
     const int64_t even = (c.target + tiles(c.m) - 1) / tiles(c.m);
     const int64_t most = num_seqs == 1 ? even : num_tokens * group <= 1024 ? 4 * even : 2 * even;
     c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, MAX_PARTS, cap / 256}));
   }
-  c.splits = tune("SMX_PA_SPLITS", c.splits);
+  c.splits = std::clamp(tune("SMX_PA_SPLITS", c.splits), 1, MAX_PARTS);
   return c;
 }
 
+// Rows of 128 for the prefix (its own workgroups, one a compute unit) where that is
+// much work; else one list of 64-row workgroups for the prefix and the sequences.
+// us, list / own: 64 sequences (256 rows) under 2000 tokens 25.6 / 30.2, 8000 32.8 /
+// 32.1, 32700 134 / 90; 24 (96 rows) under 4000 16.9 / 19.3, 16000 28.6 / 25.2.
 Choice choose_prefix(int64_t num_seqs, int64_t prefix_cap, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = num_seqs * group;
-  c.m = tune("SMX_SP_M", rows <= 64 ? 64 : 128);
+  c.m = tune("SMX_SP_M", rows > 64 && rows * prefix_cap >= 1500000 ? 128 : 64) < 128 ? 64 : 128;
   c.tiles = (int)((rows + c.m - 1) / c.m);
   const int64_t prefix_parts = std::max<int64_t>(1, prefix_cap / 64);
   const int64_t suffix_parts = std::max<int64_t>(1, cap / 64);
-  if (c.m == 64) {  // one work list, parts of one length
-    c.target = std::max(1, tune("SMX_SP_TARGET", 512) / n_kv);
+  if (c.m == 64) {
+    c.target = std::max(1, FILL / n_kv);
     c.suffix_splits = (int)std::min<int64_t>(
         {MAX_PARTS, c.target, std::max(prefix_parts, suffix_parts)});
     c.splits = c.suffix_splits;
   } else {
-    const int64_t wgs = tune("SMX_SP_TARGET", 256) / n_kv;
     c.splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({wgs / c.tiles, MAX_PARTS, prefix_parts}));
-    c.target = std::max(1, tune("SMX_SP_STARGET", 1024) / n_kv);
+        1, std::min<int64_t>({FILL / 2 / n_kv / c.tiles, MAX_PARTS, prefix_parts}));
+    c.target = std::max(1, 2 * FILL / n_kv);
     const int64_t even = (c.target + num_seqs - 1) / num_seqs;
     c.suffix_splits = (int)std::min<int64_t>({4 * even, MAX_PARTS, suffix_parts});
   }
@@ -920,36 +946,43 @@ void set_workspace(RowsArgs& a, void* workspace, int64_t rows, int slots, int hd
 
 // Tiles times parts: at most the target (whose parts' length comes from a sum in
 // fp32, so perhaps one more) and one more part of every tile.
-int items_bound(int64_t tiles, int target, int splits) {
-  return (int)std::min<int64_t>(tiles * splits, target + tiles + 1);
+int64_t items_bound(int64_t tiles, int target, int splits) {
+  return std::min<int64_t>(tiles * splits, target + tiles + 1);
 }
 
 template <int HD>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
   a.zigzag = a.num_seqs == 1 ? std::max(1, 256 / a.n_kv) : 1 << 30;
   a.target = c.target;
-  a.least = tune("SMX_PA_LEAST", 256) / 64;
-  const dim3 grid(a.n_kv, items_bound(c.tiles, c.target, c.splits));
+  a.least = 256 / 64;
+  const dim3 grid(a.n_kv, (unsigned)items_bound(c.tiles, c.target, c.splits));
   if (c.m == 64)
-    SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2>), grid, dim3(256), 0, stream, a);
+    SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2, 32>), grid, dim3(256), 0, stream, a);
+  else if (a.bs_log2 > 5)
+    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 64>), grid, dim3(256), 0, stream, a);
   else
-    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2>), grid, dim3(256), 0, stream, a);
+    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 32>), grid, dim3(256), 0, stream, a);
   const int rc = (int)hipGetLastError();
   return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, c.splits, true);
 }
 
+// Workgroups a kv head of the shared-prefix launch.
+int64_t prefix_items(int64_t num_seqs, int64_t group, const Choice& c) {
+  const int64_t own = num_seqs * ((group + 63) / 64);
+  return c.m == 64 ? items_bound(c.tiles + own, c.target, c.splits)
+                   : (int64_t)c.tiles * c.splits + items_bound(own, c.target, c.suffix_splits);
+}
+
 template <int HD>
 int launch_prefix(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  const int64_t own = a.num_seqs * (int64_t)((a.group + 63) / 64);
   a.target = c.target;
+  const dim3 grid(a.n_kv, (unsigned)prefix_items(a.num_seqs, a.group, c));
   if (c.m == 64)
-    SMX_LAUNCH((shared_prefix_kernel<HD, false>),
-               dim3(a.n_kv, items_bound(c.tiles + own, c.target, c.splits)), dim3(256), 0, stream,
-               a);
+    SMX_LAUNCH((shared_prefix_kernel<HD, false, 32>), grid, dim3(256), 0, stream, a);
+  else if (a.bs_log2 > 5)
+    SMX_LAUNCH((shared_prefix_kernel<HD, true, 64>), grid, dim3(256), 0, stream, a);
   else
-    SMX_LAUNCH((shared_prefix_kernel<HD, true>),
-               dim3(a.n_kv, c.tiles * c.splits + items_bound(own, c.target, c.suffix_splits)),
-               dim3(256), 0, stream, a);
+    SMX_LAUNCH((shared_prefix_kernel<HD, true, 32>), grid, dim3(256), 0, stream, a);
   const int rc = (int)hipGetLastError();
   return rc ? rc : launch_merge<HD>(stream, a, c.splits + c.suffix_splits, c.splits, false);
 }
@@ -1011,7 +1044,8 @@ extern "C" int smx_prompt_attention(void* stream, const void* q, int64_t q_strid
               "q_stride must be a multiple of 8 and hold n_q heads");
   const smx::Choice c = smx::choose_prompt(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
                                            n_q / n_kv, n_kv);
-  SMX_REQUIRE(c.tiles <= 65535, "too many row tiles for one launch");
+  SMX_REQUIRE(smx::items_bound(c.tiles, c.target, c.splits) <= 65535,
+              "too many row tiles for one launch");
   const int64_t rows = (int64_t)num_tokens * n_q;
   SMX_REQUIRE(c.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
                                 workspace_bytes >= smx::partial_bytes(rows, c.splits, head_dim)),
@@ -1074,6 +1108,8 @@ extern "C" int smx_shared_prefix_attention(
                          (int64_t)max_blocks * block_size, n_q / n_kv, n_kv);
   const int64_t rows = (int64_t)num_seqs * n_q;
   const int slots = c.splits + c.suffix_splits;
+  SMX_REQUIRE(smx::prefix_items(num_seqs, n_q / n_kv, c) <= 65535,
+              "too many row tiles for one launch");
   SMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
                   workspace_bytes >= smx::partial_bytes(rows, slots, head_dim),
               "workspace must be 16-byte aligned and hold "
