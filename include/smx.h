@@ -499,7 +499,7 @@ int smx_shared_prefix_attention(void* stream, const void* q, int64_t q_stride,
  *      (j - query_start_loc[r])-th of its request r, context_lens[r] + that,
  *      and its slot page * block_size + position % block_size (-1 without a
  *      page); past the last token 0 and -1.
- * block_size a power of two up to 4096; num_reqs * max_blocks < 2^31.  The
+ * block_size a power of two up to 4096; num_reqs * max_blocks <= 2^31 - 4097.  The
  * device-side form of the block manager's tables and of _slot_one / slot4_kernel
  * (src/spark_vllm_ascend/integration/slot_mapping.py:8-33).
  */

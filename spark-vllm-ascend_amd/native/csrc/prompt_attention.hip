@@ -182,10 +182,12 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   const int lrow = lane / CH, lc = lane % CH;  // the lane's row and chunk of a load
   const int tok_bytes = 2 * tok_stride;
   const constant_i32* const table = (const constant_i32*)it.table;
+  // (an empty range may lie past the table's end, with a prefix longer than it)
+  const int table_end = it.to > it.from ? it.to - 1 : 0;
   auto look_up = [&](int (&page)[NP], int base) {
 #pragma unroll
     for (int u = 0; u < NP; ++u)
-      page[u] = table[max(min(base + BT * u, it.to - 1), 0) >> A.bs_log2];
+      page[u] = table[min(base + BT * u, table_end) >> A.bs_log2];
   };
   auto stage = [&](const uint16_t* cache, lds_u32x4* dst, const int (&page)[NP], int base,
                    auto swz) {

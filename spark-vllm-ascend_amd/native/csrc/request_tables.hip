@@ -242,8 +242,8 @@ __global__ __launch_bounds__(NT) void release_pages_kernel(const int32_t* keep, 
 
 #define SMX_TABLES_CHECKS()                                                                      \
   SMX_REQUIRE(num_reqs >= 1 && num_reqs <= 65535, "num_reqs must be in [1, 65535]");             \
-  SMX_REQUIRE(max_blocks >= 1 && (int64_t)num_reqs * max_blocks <= INT_MAX,                      \
-              "num_reqs * max_blocks must fit in int32");                                        \
+  SMX_REQUIRE(max_blocks >= 1 && (int64_t)num_reqs * max_blocks <= INT_MAX - 4096,               \
+              "num_reqs * max_blocks must be at most 2^31 - 4097");                              \
   SMX_REQUIRE(num_free >= 1, "the free list must have room for a page");                         \
   SMX_REQUIRE(block_size >= 1 && block_size <= 4096 && (block_size & (block_size - 1)) == 0,     \
               "block_size must be a power of two in [1, 4096]")

@@ -100,6 +100,15 @@ def test_no_prefix_and_a_prefix_past_its_table():
     _check(case, what="prefix_len past the table")
 
 
+@pytest.mark.parametrize("seqs", [3, 40])
+def test_a_prefix_longer_than_the_own_tables(seqs):
+    """All sequences end within the prefix, whose last page is past their tables'."""
+    q, k, v, ptable, plen, table, lens = _case(11, 3000, [1] * seqs, 8, 2, 128, 32)
+    table = table[:, :4].contiguous()
+    lens = torch.arange(seqs, dtype=torch.int32) * 7 % 129
+    _check((q, k, v, ptable, plen, table, lens), what="narrow tables")
+
+
 @pytest.mark.parametrize("bad", [math.inf, math.nan])
 def test_what_a_row_does_not_see_does_not_reach_it(bad):
     """Behind every sequence's end, behind the prefix's end in its last page, and in

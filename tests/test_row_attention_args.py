@@ -51,7 +51,8 @@ def test_shared_prefix_attention_refuses(change):
 @pytest.mark.parametrize("change", [{k: None} for k in list(T)[:12]]
                          + [dict(query=18), dict(pos=20), dict(slots=12), dict(reqs=0),
                             dict(reqs=1 << 17), dict(tokens=0), dict(max_blocks=0),
-                            dict(reqs=60000, max_blocks=1 << 20), dict(num_free=0), dict(bs=0),
+                            dict(reqs=60000, max_blocks=1 << 20),
+                            dict(reqs=1, max_blocks=2 ** 31 - 1), dict(num_free=0), dict(bs=0),
                             dict(bs=24), dict(bs=8192), dict(lens=32, query=32)], ids=str)
 def test_request_tables_refuses(change):
     base = dict(T, lens=48)
