@@ -457,11 +457,14 @@ class DecodeModel:
                                         max_tokens=total)
             ids = torch.cat([st.forced[r, at:at + k] for r, (at, k) in enumerate(zip(done, n))])
             x = self.head.embed(ids)
-            rows = PromptRows(st.block_table, tables.query_start_loc, tables.seq_lens,
-                              tables.positions, tables.slot_mapping,
+            # no wider than the pass needs: prompt_attention goes by the capacity
+            blocks = -(-max(at + k for at, k in zip(done, n)) // c.block_size)
+            table = st.block_table[:, :blocks].contiguous()
+            rows = PromptRows(table, tables.query_start_loc, tables.seq_lens, tables.positions,
+                              tables.slot_mapping,
                               ops.prompt_attention_workspace(
                                   x.new_empty((total, c.n_q, c.head_dim)),
-                                  self.layers[0].kv_cache[0], st.block_table))
+                                  self.layers[0].kv_cache[0], table))
             residual = None
             for L in self.layers:
                 h, residual = ops.add_rmsnorm(x, residual, L.input_norm, c.eps)

@@ -75,6 +75,7 @@ struct RowsArgs {
   int target;         // workgroups a kv head to aim at
   int least;          // rounds of a part at least (prompts)
   int zigzag;         // period of the order of the tiles (prompts)
+  float gain;         // of find_item (prompts)
   float scale_log2;
 };
 
@@ -537,25 +538,33 @@ struct Place {
 // are cut into parts of one length, the least (of at least `least` rounds) that
 // makes about `target` items of all segments and at most max_parts of any, so
 // that the workgroups are alike whatever the lengths: every workgroup derives
-// it from the lengths.
+// it from the lengths.  Unless that saves `gain` rounds of the longest item (a
+// round beside another workgroup's takes 1.45 of one alone), or the items read
+// memory at its rate as they are (`memory`), nothing is cut.
 template <int ROUND, typename Seg>
 __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, int target,
-                                          int max_parts, int least, Place& place) {
+                                          int max_parts, int least, float gain, bool memory,
+                                          Place& place) {
   const int lane = threadIdx.x & 63;
   int chunk = INT_MAX / ROUND;  // in rounds
   int tiles0 = 0, rounds0 = 0;
   if (lane < num_segs) seg_of(lane, tiles0, rounds0);
   if (max_parts > 1) {
-    float work = wave_sum((float)tiles0 * (float)rounds0);
+    float work = wave_sum((float)tiles0 * (float)rounds0), all = wave_sum((float)tiles0);
     int top = wave_max_i32(rounds0);
     for (int b = 64; b < num_segs; b += 64) {
       int tiles = 0, rounds = 0;
       if (b + lane < num_segs) seg_of(b + lane, tiles, rounds);
       work += wave_sum((float)tiles * (float)rounds);
+      all += wave_sum((float)tiles);
       top = max(top, wave_max_i32(rounds));
     }
     chunk = max(max((int)fminf(ceilf(work / (float)target), 1e9f),
                     (top + max_parts - 1) / max_parts), least);
+    const float alone = all / (float)target;
+    if ((float)top * (1.f - 1.45f * alone) < gain ||
+        (memory && alone > 0.31f && (float)top * all < 1.3f * work))
+      chunk = max(chunk, top);
     // every segment rounds up: a little longer parts where that made too many
     for (int i = 0; i < 3 && num_segs <= 64; ++i) {
       const float items = wave_sum((float)tiles0 * (float)max(1, (rounds0 + chunk - 1) / chunk));
@@ -627,7 +636,9 @@ void prompt_attention_kernel(RowsArgs A) {
   }
   Place place;
   // (the grid has room for the most items there can be)
-  if (!find_item<ROUND>(seg_of, A.num_seqs, item, A.target, A.splits, A.least, place)) return;
+  if (!find_item<ROUND>(seg_of, A.num_seqs, item, A.target, A.splits, A.least,
+                        A.gain, A.gain < 14.f, place))
+    return;
   const int seq = place.seg;
   int q0;
   const int nq = queries(seq, q0), L = length(seq);
@@ -711,7 +722,7 @@ void shared_prefix_kernel(RowsArgs A) {
     };
     Place place;
     if (!find_item<ROUND>(seg_of, A.num_seqs + 1 - SEG0, item, A.target, A.suffix_splits, 1,
-                          place))
+                          0.f, false, place))
       return;
     const int seg = SEG0 + place.seg;
     const int tiles = seg == 0 ? A.tiles : group_tiles;
@@ -871,39 +882,46 @@ constexpr int FILL = 512, MAX_PARTS = 64;
 struct Choice {
   int m;  // rows of a workgroup: 64 (two waves share them, two groups the tokens) or 128
   int splits, suffix_splits, tiles, target;
+  float gain;
 };
 
-// 128 rows multiply faster (a K tile read from L2 serves twice the rows), 64 fill
-// the chip sooner and halve the longest workgroup.  us at 32 / 8 heads of 128,
-// rows of 64 / of 128: a prompt of 512 tokens 13.3 / 17.9, 1024 22.1 / 27.9, 1500
-// 37.7 / 42.9, 2048 53.8 / 52.1, 2500 82 / 73; 16 prompts to 300 20.6 / 19.1.  Short
-// prompts of many sequences are bound by the latency of a workgroup: 12 of 83 tokens
-// 18.9 / 14.9, 31 of 62 22.7 / 18.3.
+// 128 rows a workgroup multiply faster (a K tile read from L2 serves twice the
+// rows), 64 fill the chip sooner and halve the longest workgroup.  us at 32 / 8
+// heads of 128, rows of 64 / of 128: a prompt of 1000 tokens 22 / 27, 1500 35 / 38,
+// 2048 54 / 50, 3000 103 / 85; behind a context, where all ranges are about as long,
+// 128 from one filling on (1000 behind 3000, 40 / 8 heads 114 / 100, 32 / 8 74 / 83).
+// Sequences of 65 to 128 rows are one tile of 128: 20 of 28 tokens 11.5 / 9.7.
 //
-// Cutting a tile's tokens into parts pays for its second launch (about 4 us) where
-// few workgroups have long ranges.  us whole / cut: 512 tokens behind 2000 58.7 /
-// 43.5, 4 sequences of 200 behind 8000 142 / 157; 29 of up to 7 tokens behind 2300 to
-// 6900, whose longest would run alone, 137 / 98, but 23 of up to 11 behind 2821, bound
-// by memory already, 51 / 59.  Short tables stay whole: 10 sequences of one token
-// behind 642, 8 / 1 heads, 14.4 / 12.2, 3 prompts to 529 14.3 / 20.6.  A part is at
-// least 256 tokens: 300 behind 1500 31.5 at 512, 32.2 at 256, 35.6 at 1024, one token
-// behind 900 14.6 at 512, 12.3 at 256.
+// Cutting tiles' tokens into parts costs partials and a second launch, about 11 us
+// (14 rounds of 64 tokens), 5 where a tile has few rows, and two workgroups a
+// compute unit take 1.45 of a round alone: it pays for long ranges of few
+// workgroups.  us whole / cut: 300 tokens behind 16000 201 / 116 (rows of 64), 64
+// behind 1000 20 / 14, 1000 behind 3000, 8 / 1 heads 55 / 36, but 16 / 16 heads
+// 56.6 / 56.9 and 512 behind 2000 38 / 41.  (The tables' capacity stands for the
+// lengths here, find_item asks again with them.)  Sequences of few rows read memory
+// at its rate from 160 workgroups on: 23 of up to 11 tokens behind 2821 51 / 59; only
+// uneven ones are cut then, 29 of up to 7 behind 2300 to 6900 137 / 98.  Cut for long
+// contexts 128 rows are better: 509 behind 16000 170 / 153, 500 behind 4000 60 / 60.
+// Parts are of at least 256 tokens: 300 behind 1500 31.5 at 512, 32.2 at 256, one
+// token behind 900 14.6 at 512, 12.3 at 256.
 Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
-  auto tiles = [&](int m) { return (rows + m - 1) / m * num_seqs; };  // of even lengths
-  c.splits = 1;
-  c.m = tiles(128) * n_kv >= FILL ? 128 : 64;
-  const bool few = c.m == 64 && cap >= (rows <= 64 ? 768 : 1024) &&
-                   tiles(64) * n_kv < (rows <= 64 && cap < 4096 ? 160 : 400);
-  if (few ? rows > 1024 : rows > 64 && rows <= 512 && tiles(64) * n_kv >= 256) c.m = 128;
+  auto groups = [&](int m) { return (rows + m - 1) / m * num_seqs * n_kv; };  // of even lengths
+  const bool behind = cap > 2 * ((num_tokens + num_seqs - 1) / num_seqs);
+  c.m = groups(64) > (behind ? FILL : 800) || (rows > 64 && rows <= 128 && groups(64) >= 256)
+            ? 128 : 64;
+  c.gain = 6.f + 8.f * std::min<int64_t>(rows, 64) / 64;
+  const bool few = (float)(cap / 64) * (1.f - 1.45f * groups(64) / FILL) >= c.gain &&
+                   !(rows <= 64 && cap < 4096 && groups(64) >= 160);
+  if (few && rows > 1024 && cap >= 8192) c.m = 128;
   c.m = tune("SMX_PA_M", c.m) < 128 ? 64 : 128;
   c.tiles = (int)((num_tokens * group + c.m - 1) / c.m + num_seqs - 1);
   c.target = std::max(1, FILL / n_kv);
   if (few) {
-    const int64_t even = (c.target + tiles(c.m) - 1) / tiles(c.m);
+    const int64_t even = (FILL + groups(c.m) - 1) / groups(c.m);
     const int64_t most = num_seqs == 1 ? even : num_tokens * group <= 1024 ? 4 * even : 2 * even;
-    c.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, MAX_PARTS, cap / 256}));
+    c.splits = (int)std::min<int64_t>({most, MAX_PARTS, cap / 256});
   }
   c.splits = std::clamp(tune("SMX_PA_SPLITS", c.splits), 1, MAX_PARTS);
   return c;
@@ -957,6 +975,7 @@ int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
   a.zigzag = a.num_seqs == 1 ? std::max(1, 256 / a.n_kv) : 1 << 30;
   a.target = c.target;
   a.least = 256 / 64;
+  a.gain = c.gain;
   const dim3 grid(a.n_kv, (unsigned)items_bound(c.tiles, c.target, c.splits));
   if (c.m == 64)
     SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2, 32>), grid, dim3(256), 0, stream, a);
