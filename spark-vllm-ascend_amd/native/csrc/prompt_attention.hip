@@ -130,6 +130,21 @@ __device__ __forceinline__ void meet() {
   __asm__ volatile("" ::: "memory");
 }
 
+// The largest of a wave's values, for every lane.
+__device__ __forceinline__ int wave_max_i32(int v) {
+  auto dpp = [](int x, auto ctrl) {
+    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR1>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR2>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_HALF_MIRROR>{}));
+  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_MIRROR>{}));
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return max((int)b[0], (int)b[1]);
+}
+
 // BS: the least block_size, 32 or 64: a tile is looked up and addressed by NP pieces
 // of BT tokens that are within a page.
 template <int HD, int WM, int WN, int KT, int ST, int BS>
@@ -164,10 +179,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       qf[ks] = *reinterpret_cast<const u32x4*>(A.q + (int64_t)tok * A.q_stride + head * HD +
                                                16 * ks + 8 * h);
   }
-  int lim_min = lim;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) lim_min = min(lim_min, __shfl_xor(lim_min, o));
-  lim_min = __builtin_amdgcn_readfirstlane(lim_min);
+  const int lim_min = __builtin_amdgcn_readfirstlane(-wave_max_i32(-lim));
 
   // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile, by
   // buffer loads into LDS whose resource is one piece of BT tokens: tokens past the
@@ -437,9 +449,9 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     if (rd < rounds) step(std::false_type{});
   }
 
-  // ---- the lane pair's sums, then the WN groups' states
+  // ---- the lane pair's sums, then the WN groups' states (of one tile the first's only)
   l = xor_sum<32>(l);
-  if constexpr (WN > 1) {
+  if (WN > 1 && ntiles > 1) {
     float* const jo = reinterpret_cast<float*>(smem);
     __builtin_amdgcn_s_waitcnt(wait_vm(0));
     __syncthreads();  // the tiles are read out, nothing is on its way into them
@@ -470,6 +482,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
         for (int i = 0; i < 16; ++i) o[d][i] = o[d][i] * a + src[(16 * d + i) * 64 + lane] * b;
     }
   }
+  if (WN > 1 && wn > 0) return;  // (a single tile: the first group's)
   // The row again, from its number: not kept in registers through the rounds.
   int row_again = row;
   __asm__ volatile("" : "+v"(row_again));
@@ -505,21 +518,6 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                               __float_as_uint(o[d][4 * a + 3] * inv)});
     }
   }
-}
-
-// The largest of a wave's values, for every lane.
-__device__ __forceinline__ int wave_max_i32(int v) {
-  auto dpp = [](int x, auto ctrl) {
-    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
-  };
-  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR1>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR2>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_HALF_MIRROR>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_MIRROR>{}));
-  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-  v = max((int)a[0], (int)a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-  return max((int)b[0], (int)b[1]);
 }
 
 // The end of a part that begins at `from`, at most `end`.

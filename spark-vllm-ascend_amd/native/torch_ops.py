@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import torch
 
-from . import call, load
+from . import SMX_EINVAL, SmxError, call, load
 
 BF16 = torch.bfloat16
 
@@ -721,12 +721,19 @@ def prompt_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     if not _plain(query_start_loc, torch.int32, q.get_device()):
         _all_plain(q.get_device(), torch.int32, query_start_loc=query_start_loc)
     _need(query_start_loc.numel() == sizes[0] + 1, "query_start_loc must have num_seqs + 1 entries")
+    args = (_stream(q), q.data_ptr(), step, k_cache.data_ptr(), v_cache.data_ptr(),
+            block_table.data_ptr(), query_start_loc.data_ptr(), seq_lens.data_ptr())
+    rest = (out.data_ptr(), q.shape[0], *sizes, float(scale))
     if workspace is None:
-        workspace = prompt_attention_workspace(q, k_cache, block_table)
-    call("smx_prompt_attention", _stream(q), q.data_ptr(), step, k_cache.data_ptr(),
-         v_cache.data_ptr(), block_table.data_ptr(), query_start_loc.data_ptr(),
-         seq_lens.data_ptr(), _ptr(workspace), workspace.numel() if workspace is not None else 0,
-         out.data_ptr(), q.shape[0], *sizes, float(scale))
+        # most prompts need none: the call that refuses is cheaper than asking each time
+        try:
+            call("smx_prompt_attention", *args, None, 0, *rest)
+            return out
+        except SmxError as e:
+            workspace = prompt_attention_workspace(q, k_cache, block_table)
+            if e.code != SMX_EINVAL or workspace is None:
+                raise
+    call("smx_prompt_attention", *args, workspace.data_ptr(), workspace.numel(), *rest)
     return out
 
 
