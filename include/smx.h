@@ -436,7 +436,9 @@ int smx_compute_slot_mapping(void* stream, const int32_t* query_start_loc, int32
  * head_dim 64 or 128, n_q a multiple of n_kv, block_size a power of two in
  * [32, 4096]; q, caches and out 16-byte aligned, q_stride a multiple of 8.
  * Where rows are too few to fill the chip the tokens are split over workgroups
- * and merged by a second launch: workspace holds
+ * and merged by a second launch, in parts of one length that follows from all of
+ * the call's lengths (so a sequence's last bit may change with its neighbours;
+ * equal calls give equal results): workspace holds
  * smx_prompt_attention_workspace(...) bytes (16-byte aligned; 0: none needed;
  * -1: bad sizes).  Calls that can run at the same time need workspaces of their
  * own.  Counterpart of the attention the reference leaves to vLLM's stock

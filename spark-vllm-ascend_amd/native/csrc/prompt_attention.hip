@@ -536,9 +536,9 @@ struct Place {
 // are cut into parts of one length, the least (of at least `least` rounds) that
 // makes about `target` items of all segments and at most max_parts of any, so
 // that the workgroups are alike whatever the lengths: every workgroup derives
-// it from the lengths.  Unless that saves `gain` rounds of the longest item (a
-// round beside another workgroup's takes 1.45 of one alone), or the items read
-// memory at its rate as they are (`memory`), nothing is cut.
+// it from the lengths.  Nothing is cut where that would not save `gain` rounds of
+// the longest item (a round beside another workgroup's takes 1.45 of one alone), or
+// where the items read memory at its rate as they are (`memory`).
 template <int ROUND, typename Seg>
 __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, int target,
                                           int max_parts, int least, float gain, bool memory,
@@ -720,7 +720,7 @@ void shared_prefix_kernel(RowsArgs A) {
     };
     Place place;
     if (!find_item<ROUND>(seg_of, A.num_seqs + 1 - SEG0, item, A.target, A.suffix_splits, 1,
-                          0.f, false, place))
+                          -INFINITY, false, place))
       return;
     const int seg = SEG0 + place.seg;
     const int tiles = seg == 0 ? A.tiles : group_tiles;
