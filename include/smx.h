@@ -427,8 +427,8 @@ int smx_compute_slot_mapping(void* stream, const int32_t* query_start_loc, int32
  *      K and V are in the cache, so token i of them is at position
  *      L_r - n_r + i and sees the tokens 0 .. that position
  *   out: [num_tokens, n_q, head_dim] bf16 = RNE_bf16(softmax(scale q.k) v); 0
- *      for a token that sees none (L_r < n_r); rows of no sequence are left
- *      as they are.
+ *      for a token that sees none (L_r < n_r) or only scores of -infinity; rows
+ *      of no sequence are left as they are.
  * Scores, maxima and sums in fp32; probabilities are rounded to bf16 before
  * they multiply V, the sum uses the unrounded values.  What a row does not see
  * does not reach it, infinities and NaN included.  A block-table entry outside

@@ -68,6 +68,43 @@ def test_matches_float64(case):
     assert_rows(got[mine], ref[mine], mag[mine], str(case))
 
 
+@pytest.mark.parametrize("n,ctx,n_q,n_kv,spare", [
+    ([200], [0], 16, 4, 90), ([5, 3], [10, 3000], 32, 8, 60), ([1] * 22, [700] * 22, 8, 8, 60),
+    ([1] * 22, [700] * 21 + [2100], 8, 8, 60), ([30, 400], [5000, 2], 8, 1, 0),
+    ([300], [9000], 8, 2, 0), ([70, 90, 128], [0, 3, 0], 128, 32, 1)])
+def test_lengths_far_below_the_capacity_and_uneven(n, ctx, n_q, n_kv, spare):
+    """Both sides of the rules that cut a tile's tokens: by the tables' capacity on
+    the host, by the lengths on the device (heads of 64, 128 tokens a page)."""
+    case = _case(16, n, ctx, n_q, n_kv, 64, 128, spare=spare)
+    print(n, ctx, flush=True)
+    assert_rows(_run(*case, 0.1), *prompt64(*case, 0.1)[:2], f"{n} {ctx}")
+
+
+def test_one_capture_cuts_and_does_not():
+    """One captured call whose replays take whole tiles and cut ones in turn: what the
+    other form left in the workspace does not matter."""
+    q, k, v, table, start, lens = [x.cuda() for x in _case(17, [24], [5000], 8, 2, 128, 64)]
+    ops = _ops()
+    ws = ops.prompt_attention_workspace(q, k, table)
+    assert ws is not None
+    ws.fill_(255)
+    out = torch.empty_like(q)
+    call = lambda: ops.prompt_attention(q, k, v, table, start, lens, 0.1, workspace=ws, out=out)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    cpu = [x.cpu() for x in (q, k, v, table, start)]
+    for length in (100, 5024, 24, 4000, 0, 300):
+        lens.fill_(length)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref, mag, _ = prompt64(*cpu, torch.tensor([length], dtype=torch.int32), 0.1)
+        assert_rows(out, ref, mag, f"length {length}")
+
+
 def test_many_sequences():
     """More sequences than one round of the tile search, most of them tiny."""
     n = [(7 * i) % 5 for i in range(150)]
