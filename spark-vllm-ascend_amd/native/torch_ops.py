@@ -685,7 +685,9 @@ def _rows_checks(q, k_cache, v_cache, block_table, seq_lens, workspace, out):
     if workspace is not None and not _plain(workspace, torch.uint8, i):
         _all_plain(i, torch.uint8, workspace=workspace)
     if out is None:
-        out = torch.empty((tokens, n_q, hd), dtype=BF16, device=q.device)
+        # (empty_like: 0.9 us, an empty of the sizes 1.5)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(
+            (tokens, n_q, hd), dtype=BF16, device=q.device)
     elif not _plain(out, BF16, i):
         _all_plain(i, BF16, out=out)
     _need(out.numel() == tokens * n_q * hd, "out must have q's elements")

@@ -78,6 +78,22 @@ def test_exact(case, in_place):
     _check(*case, in_place=in_place)
 
 
+@pytest.mark.parametrize("names", [("free_count",), ("num_pages",)])
+def test_half_in_place(names):
+    """One of the two updated in place, the other not, over many tokens."""
+    query, context = [900, 0, 5000, 1], [3, 700, 64, 31]
+    table, held, left = _state(4, context, 90, 64, 100)
+    t, n, c, fp = _i32(table.tolist()), _i32(held), _i32([len(left)]), _i32(left)
+    own = dict(free_count=c, num_pages=n)
+    ops = _ops()
+    out = ops.request_tables_out(n, 6000).replace(**{k: own[k] for k in names})
+    got = ops.request_tables(_i32(query), _i32(context), n, fp, c, t, 64, out=out)
+    want = tables64(query, context, held, left, len(left), table, 64, 6000)
+    for a, b in zip((t, got.num_pages, got.free_count, got.query_start_loc, got.seq_lens,
+                     got.positions, got.slot_mapping), want):
+        assert np.array_equal(a.cpu().numpy().reshape(-1), np.array(b).reshape(-1)), names
+
+
 def test_list_used_up_and_row_full():
     """Requests past the end of the free list get -1, and so do tokens past the
     table's row; pages there are not taken."""
