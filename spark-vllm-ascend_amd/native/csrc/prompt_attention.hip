@@ -601,7 +601,18 @@ __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, in
   return false;
 }
 
-// Packed prompts.  Sequence r's queries are the tokens [query_start[r],
+// Shapes.  Rounds of 64 tokens: a workgroup of 64 rows takes 0.85 us alone on its
+// compute unit and 1.2 beside another (heads of 64: 0.6 alone), one of 128 rows 1.3
+// and 2.07, so 128 rows multiply 1.16 times as fast where the chip is full.  64 KB of
+// LDS and at most 256 registers let two be resident.  Two waves a SIMD from two
+// workgroups overlap matrix and vector work by themselves; 8 waves a workgroup (256
+// rows, or four token groups) were slower on full chips.
+//
+// Packed prompts.  Bound by the matrix units at the chip's power where there are many
+// rows: one prompt of 8192 tokens, 32 / 8 heads of 128, 515 us = 1070 TFLOP/s, a large
+// library product 1406; by the longest workgroups where all are resident (2048 tokens
+// 49 us); by memory for a few drafted tokens (8 x 5 behind 300 to 8000: 21.6 us, 4.5
+// TB/s).  Sequence r's queries are the tokens [query_start[r],
 // query_start[r + 1]), the last n of its L tokens: token i of them is at position
 // L - n + i and sees the tokens up to itself.  Grid: kv heads, items.
 template <int HD, int WM, int WN, int KT, int ST, int BS>
@@ -625,7 +636,8 @@ void prompt_attention_kernel(RowsArgs A) {
   };
   // Whole tiles: the last (longest) first, every other run of `zigzag` of them in
   // turned order, so that a compute unit that starts with a long tile of one run
-  // gets a short one of the next.
+  // gets a short one of the next (one prompt of 2048 tokens 50.8 us without, 48.5,
+  // 4096 149 and 146; from more than two fillings on not: 8192 515, 522).
   int item = blockIdx.y;
   if (A.splits == 1) {
     const int run = item / A.zigzag, i = item % A.zigzag;
@@ -667,7 +679,8 @@ void prompt_attention_kernel(RowsArgs A) {
 // heads, items.  Up to 64 rows the prefix and the sequences are segments of one
 // work list in parts of one length.  More (BIG): the prefix's items come first,
 // workgroups of 128 rows, one a compute unit, bound by the matrix units; the
-// sequences' items, bound by memory, run beside them.
+// sequences' items, bound by memory, run beside them.  64 sequences of 100 to 2048
+// tokens under 32700: 82 us, 400 TFLOP/s and 3.7 TB/s at once; 8 under 4096 11 us.
 template <int HD, bool BIG, int BS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void shared_prefix_kernel(RowsArgs A) {
@@ -755,7 +768,8 @@ void shared_prefix_kernel(RowsArgs A) {
 // counts[row] first slots and the counts[rows + row] from slot `second` on.  WPR
 // waves a row take chunks of MCH partials in turn, lane j of a wave the weight of
 // partial j of its chunk, every lane HD / 64 dims; all of a chunk's loads are
-// issued before the first is used.  A partial of weight 0 may not have been
+// issued before the first is used (64 partials of 256 rows 3.8 us; with one wave a
+// row 4.9).  A partial of weight 0 may not have been
 // written and is left out.  Rows that are of no sequence, and rows of one part
 // (no partials: counts 0), stay as they are.
 constexpr int MCH = 16;
@@ -970,7 +984,8 @@ int64_t items_bound(int64_t tiles, int target, int splits) {
 
 template <int HD>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  a.zigzag = a.num_seqs == 1 ? std::max(1, 256 / a.n_kv) : 1 << 30;
+  a.zigzag = a.num_seqs == 1 && (int64_t)c.tiles * a.n_kv <= 2 * FILL ? std::max(1, 256 / a.n_kv)
+                                                                      : 1 << 30;
   a.target = c.target;
   a.least = 256 / 64;
   a.gain = c.gain;

@@ -89,7 +89,7 @@ __device__ __forceinline__ int last_le(const int32_t* first, int n, int k) {
 // One workgroup takes the requests NT at a time.  with_tokens: positions and slots
 // too (all requests then fit one round), by more workgroups where there are many
 // tokens: each makes the sums again, from inputs that nothing overwrites meanwhile,
-// the first alone writes what is not of a token.  24000 tokens of 256 requests: one
+// and deals out its share of the pages and tokens; the first alone writes the rest.  24000 tokens of 256 requests: one
 // such launch 4.3 us, the sums and then request_tokens_kernel 6.2 (in a graph; 6.1 and
 // 9.5 with the host's calls).
 template <int NT>
@@ -128,14 +128,15 @@ __global__ __launch_bounds__(NT) void request_tables_kernel(TablesArgs A) {
     pages_s[tid] = pages;
     ctx_s[tid] = ctx;
     __syncthreads();
-    for (int k = tid; writes && k < tp; k += NT) {
+    const int64_t step = (int64_t)gridDim.x * NT;
+    for (int64_t k0 = (int64_t)blockIdx.x * NT + tid; k0 < tp; k0 += step) {
+      const int k = (int)k0;
       const int i = last_le(first_s, here, taken + k);
       const int at = count - 1 - (taken + k);
       st_agent(A.table + (int64_t)(r0 + i) * A.max_blocks + pages_s[i] + (taken + k - first_s[i]),
                at >= 0 ? A.free_pages[at] : -1);
     }
     if (A.with_tokens) {
-      const int64_t step = (int64_t)gridDim.x * NT;
       for (int64_t j0 = (int64_t)blockIdx.x * NT + tid; j0 < A.max_tokens; j0 += step) {
         const int j = (int)j0;
         int64_t pos = 0, slot = -1;
@@ -202,6 +203,9 @@ __global__ __launch_bounds__(256) void request_tokens_kernel(
   stores_done();
 }
 
+// Bound by the chain of a page's reads (bisection in LDS, its entry), NT pages at a
+// time: 8192 pages of 256 requests 9.7 us.
+//
 // Gives back the pages beyond the first keep[r] tokens of every request, in request
 // and block order: they are appended to the free list, their table entries become -1.
 template <int NT>
@@ -292,7 +296,10 @@ extern "C" int smx_request_tables(void* stream, const int32_t* query_lens,
   const bool several = num_reqs <= 1024 && apart(num_pages, num_pages_out, num_reqs) &&
                        apart(free_count, free_count_out, 1);
   a.with_tokens = num_reqs <= 1024 && (max_tokens <= 4096 || several);
-  const int nt = num_reqs <= 256 && (max_tokens <= 256 || several || !a.with_tokens) ? 256 : 1024;
+  // (tokens and pages by 256 threads a workgroup if those are all or there are more)
+  const bool pages = max_tokens / block_size > 256;
+  const int nt = num_reqs <= 256 && (max_tokens <= 256 || several || !(a.with_tokens || pages))
+                     ? 256 : 1024;
   const int64_t parts = several ? std::min<int64_t>(((int64_t)max_tokens + nt - 1) / nt, 2048) : 1;
   if (nt == 256)
     SMX_LAUNCH((smx::request_tables_kernel<256>), dim3((unsigned)parts), dim3(256), 0,
@@ -328,7 +335,9 @@ extern "C" int smx_release_pages(void* stream, const int32_t* keep_lens, int32_t
   SMX_TABLES_CHECKS();
   int bs_log2 = 0;
   while ((1 << bs_log2) < block_size) ++bs_log2;
-  if (num_reqs <= 256)
+  // (us by 256 threads / by 1024, half of the table's pages given back: 16 rows of 8
+  // entries 2.6 / 2.9, 16 of 64 3.3 / 3.1, 64 of 32 4.7 / 3.1, 256 of 64 29.3 / 9.7)
+  if (num_reqs <= 256 && num_reqs * max_blocks <= 512)
     SMX_LAUNCH((smx::release_pages_kernel<256>), dim3(1), dim3(256), 0, (hipStream_t)stream,
                keep_lens, num_pages, free_pages, free_count, block_table, num_reqs, max_blocks,
                num_free, bs_log2);
