@@ -35,6 +35,7 @@ struct TablesArgs {
   int64_t* positions;
   int64_t* slots;
   int num_reqs, max_tokens, max_blocks, num_free, bs_log2, with_tokens;
+  int parts;  // workgroups of the launch (the step runner passes no implicit arguments)
 };
 
 // Inclusive prefix sums of two values over a workgroup of NT threads; *ta and *tb
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(NT) void request_tables_kernel(TablesArgs A) {
     pages_s[tid] = pages;
     ctx_s[tid] = ctx;
     __syncthreads();
-    const int64_t step = (int64_t)gridDim.x * NT;
+    const int64_t step = (int64_t)A.parts * NT;
     for (int64_t k0 = (int64_t)blockIdx.x * NT + tid; k0 < tp; k0 += step) {
       const int k = (int)k0;
       const int i = last_le(first_s, here, taken + k);
@@ -285,7 +286,7 @@ extern "C" int smx_request_tables(void* stream, const int32_t* query_lens,
   SMX_REQUIRE(max_tokens >= 1, "max_tokens must be >= 1");
   smx::TablesArgs a{query_lens, context_lens, num_pages, free_pages, free_count, block_table,
                     num_pages_out, free_count_out, query_start_loc, seq_lens, positions,
-                    slot_mapping, num_reqs, max_tokens, max_blocks, num_free, 0, 0};
+                    slot_mapping, num_reqs, max_tokens, max_blocks, num_free, 0, 0, 1};
   while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
   // One workgroup deals a few thousand tokens out in about a launch's time.  Several
   // must not see its outputs in their inputs.
@@ -300,12 +301,12 @@ extern "C" int smx_request_tables(void* stream, const int32_t* query_lens,
   const bool pages = max_tokens / block_size > 256;
   const int nt = num_reqs <= 256 && (max_tokens <= 256 || several || !(a.with_tokens || pages))
                      ? 256 : 1024;
-  const int64_t parts = several ? std::min<int64_t>(((int64_t)max_tokens + nt - 1) / nt, 2048) : 1;
+  if (several) a.parts = (int)std::min<int64_t>(((int64_t)max_tokens + nt - 1) / nt, 2048);
   if (nt == 256)
-    SMX_LAUNCH((smx::request_tables_kernel<256>), dim3((unsigned)parts), dim3(256), 0,
+    SMX_LAUNCH((smx::request_tables_kernel<256>), dim3((unsigned)a.parts), dim3(256), 0,
                (hipStream_t)stream, a);
   else
-    SMX_LAUNCH((smx::request_tables_kernel<1024>), dim3((unsigned)parts), dim3(1024), 0,
+    SMX_LAUNCH((smx::request_tables_kernel<1024>), dim3((unsigned)a.parts), dim3(1024), 0,
                (hipStream_t)stream, a);
   if (!a.with_tokens) {
     const int rc = (int)hipGetLastError();
