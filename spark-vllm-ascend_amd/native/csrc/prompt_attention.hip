@@ -520,6 +520,23 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   }
 }
 
+// Inclusive prefix sums of a wave's values: within rows of 16 lanes, then the rows'
+// totals handed on (all by DPP; shuffles through LDS took 0.3 us of a workgroup's start).
+__device__ __forceinline__ int wave_scan_i32(int v) {
+  auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf,
+                                     false);
+  };
+  using std::integral_constant;
+  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
+  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31
+  return v;
+}
+
 // The end of a part that begins at `from`, at most `end`.
 __device__ __forceinline__ int part_end(int from, int chunk, int end) {
   return (int)min((int64_t)from + chunk, (int64_t)end);
@@ -580,12 +597,7 @@ __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, in
     }
     const int parts = max(1, (rounds + chunk - 1) / chunk);
     const int items = tiles * parts;
-    int incl = items;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(incl, o);
-      if (lane >= o) incl += x;
-    }
+    const int incl = wave_scan_i32(items);
     const int total = __builtin_amdgcn_readlane(incl, 63);
     if (item < done + total) {
       const int i = __ffsll((unsigned long long)__ballot(done + incl > item)) - 1;
@@ -628,11 +640,12 @@ void prompt_attention_kernel(RowsArgs A) {
     return max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
   };
   auto length = [&](int r) { return min(max(A.seq_lens[r], 0), cap); };
+  int my_q0 = 0, my_nq = 0, my_len = 0;  // of sequence `lane` where there are up to 64
   auto seg_of = [&](int r, int& tiles, int& rounds) {
-    int s0;
-    const int cnt = queries(r, s0);
-    tiles = (int)(((int64_t)cnt * A.group + S::M - 1) / S::M);
-    rounds = tiles ? (int)(((int64_t)length(r) + ROUND - 1) / ROUND) : 0;
+    my_nq = queries(r, my_q0);
+    my_len = length(r);
+    tiles = (int)(((int64_t)my_nq * A.group + S::M - 1) / S::M);
+    rounds = tiles ? (int)(((int64_t)my_len + ROUND - 1) / ROUND) : 0;
   };
   // Whole tiles: the last (longest) first, every other run of `zigzag` of them in
   // turned order, so that a compute unit that starts with a long tile of one run
@@ -650,8 +663,15 @@ void prompt_attention_kernel(RowsArgs A) {
                         A.gain, A.gain < 14.f, place))
     return;
   const int seq = place.seg;
-  int q0;
-  const int nq = queries(seq, q0), L = length(seq);
+  int q0, nq, L;
+  if (A.num_seqs <= 64) {  // (a second look in memory is a round trip)
+    q0 = __builtin_amdgcn_readlane(my_q0, seq);
+    nq = __builtin_amdgcn_readlane(my_nq, seq);
+    L = __builtin_amdgcn_readlane(my_len, seq);
+  } else {
+    nq = queries(seq, q0);
+    L = length(seq);
+  }
   const int tiles = (int)(((int64_t)nq * A.group + S::M - 1) / S::M);
   const int split = place.x / tiles;
   Item it;
@@ -724,11 +744,12 @@ void shared_prefix_kernel(RowsArgs A) {
     const int first = prefix & ~(KT - 1);
     auto length = [&](int r) { return min(max(A.seq_lens[r], 0), cap); };
     constexpr int SEG0 = BIG ? 1 : 0;  // segment 0 is the prefix, r + 1 sequence r
+    int my_len = 0;  // of segment `lane` where there are up to 64
     auto seg_of = [&](int i, int& tiles, int& rounds) {
       const int s = SEG0 + i;
       tiles = s == 0 ? A.tiles : group_tiles;
-      const int L = s == 0 ? prefix : length(s - 1);
-      const int span = s == 0 ? prefix : L > prefix ? L - first : 0;
+      my_len = s == 0 ? prefix : length(s - 1);
+      const int span = s == 0 ? prefix : my_len > prefix ? my_len - first : 0;
       rounds = (span + ROUND - 1) / ROUND;
     };
     Place place;
@@ -741,7 +762,8 @@ void shared_prefix_kernel(RowsArgs A) {
     if (seg == 0) {
       prefix_item(split, tile, S::M, place.chunk, place.parts);
     } else {
-      const int L = length(seg - 1);
+      const int L = A.num_seqs + 1 - SEG0 <= 64 ? __builtin_amdgcn_readlane(my_len, place.seg)
+                                               : length(seg - 1);
       it.table = A.table + (int64_t)(seg - 1) * A.max_blocks;
       it.token0 = seg - 1;
       it.row0 = tile * S::M;
