@@ -520,23 +520,6 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   }
 }
 
-// Inclusive prefix sums of a wave's values: within rows of 16 lanes, then the rows'
-// totals handed on (all by DPP; shuffles through LDS took 0.3 us of a workgroup's start).
-__device__ __forceinline__ int wave_scan_i32(int v) {
-  auto add = [&](auto ctrl, auto rows) {
-    v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf,
-                                     false);
-  };
-  using std::integral_constant;
-  add(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});  // row_shr:1
-  add(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
-  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // row_bcast:15
-  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // row_bcast:31
-  return v;
-}
-
 // The end of a part that begins at `from`, at most `end`.
 __device__ __forceinline__ int part_end(int from, int chunk, int end) {
   return (int)min((int64_t)from + chunk, (int64_t)end);

@@ -44,15 +44,10 @@ template <int NT>
 __device__ __forceinline__ void scan2(int64_t& a, int& b, int64_t* ta, int* tb, int64_t* wa,
                                       int* wb) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t x = __shfl_up(a, o);
-    const int y = __shfl_up(b, o);
-    if (lane >= o) {
-      a += x;
-      b += y;
-    }
-  }
+  // (a < 2^31 in two parts, whose sums fit 32 bits)
+  const int lo = wave_scan_i32((int)(a & 0xffffff)), hi = wave_scan_i32((int)(a >> 24));
+  a = ((int64_t)hi << 24) + lo;
+  b = wave_scan_i32(b);
   __syncthreads();  // the last round's totals have been read
   if (lane == 63) {
     wa[wave] = a;
@@ -91,7 +86,7 @@ __device__ __forceinline__ int last_le(const int32_t* first, int n, int k) {
 // too (all requests then fit one round), by more workgroups where there are many
 // tokens: each makes the sums again, from inputs that nothing overwrites meanwhile,
 // and deals out its share of the pages and tokens; the first alone writes the rest.  24000 tokens of 256 requests: one
-// such launch 4.3 us, the sums and then request_tokens_kernel 6.2 (in a graph; 6.1 and
+// such launch 4.0 us, the sums and then request_tokens_kernel 6.0 (in a graph; 6.1 and
 // 9.5 with the host's calls).
 template <int NT>
 __global__ __launch_bounds__(NT) void request_tables_kernel(TablesArgs A) {

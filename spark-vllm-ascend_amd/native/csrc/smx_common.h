@@ -221,6 +221,22 @@ __device__ __forceinline__ float xor_max(float v) {
   return fmaxf(a, b);
 }
 
+// v plus the value of another lane by DPP (nothing for lanes without one).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add_i32(int v) {
+  return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+// Inclusive prefix sums of a wave's values: within rows of 16 lanes (row_shr), then
+// the rows' totals handed on (row_bcast).  Shuffles would go through LDS.
+__device__ __forceinline__ int wave_scan_i32(int v) {
+  v = dpp_add_i32<0x111, 0xf>(v);
+  v = dpp_add_i32<0x112, 0xf>(v);
+  v = dpp_add_i32<0x114, 0xf>(v);
+  v = dpp_add_i32<0x118, 0xf>(v);
+  v = dpp_add_i32<0x142, 0xa>(v);
+  return dpp_add_i32<0x143, 0xc>(v);
+}
+
 // Full-wave reductions.
 __device__ __forceinline__ float wave_sum(float v) {
   v += dpp_f32<DPP_QUAD_XOR1>(v);
