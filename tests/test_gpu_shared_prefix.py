@@ -68,6 +68,14 @@ def test_matches_float64(case, entries):
     _check(_case(1, *case, own_prefix_entries=entries), what=str(case))
 
 
+@pytest.mark.parametrize("seqs,prefix", [(64, 70), (70, 333), (130, 40), (100, 3900)])
+def test_many_sequences(seqs, prefix):
+    """More segments than one round of the search for a workgroup's item holds, with
+    one list of them and with workgroups of the prefix's own (100 under 3900)."""
+    suffix = [(37 * i) % 90 for i in range(seqs)]
+    _check(_case(12, prefix, suffix, 8, 2, 64, 32), what=f"{seqs} under {prefix}")
+
+
 def test_agrees_with_split_kv_decode():
     """The framework's decode attention over the same whole sequences: two
     evaluations of one function, each within the derived bound of it."""
