@@ -11,7 +11,8 @@ are -1).  Slots for a step come from ``torch_ops.compute_slot_mapping``.
 
 DeviceBlockTables keeps all of that on the device instead, where the lengths
 may be known there alone (drafted tokens accepted by a kernel, steps in a
-captured graph): a step is one or two launches (``torch_ops.request_tables``).
+captured graph): a step is one or two launches of ``torch_ops.request_tables``
+and five small ones that count what it kept, ``keep`` is three.
 """
 from __future__ import annotations
 
@@ -116,14 +117,23 @@ class BlockManager:
 
 class DeviceBlockTables:
     """Pages, block tables and lengths of up to `max_seqs` requests, on the device:
-    request r is row r.  Nothing is read back: a request that finds the free list
-    empty gets -1 entries and slots (its tokens are not kept), which num_pages
-    (below ceil(len / block_size)) tells.  Steps follow one another on a stream."""
+    request r is row r, a page is one request's.  Steps follow one another on a stream.
+
+    Nothing is read back, so a step is not refused where there is no room: a token
+    without a page (the free list is used up, or the row's max_blocks_per_seq pages
+    are full) has slot -1, one past max_tokens has none at all, and neither is
+    counted: `lens` are the tokens that the cache holds, and a step after it goes on
+    from there (the same tokens can be given again).  In the step itself attention
+    gives NaN to the rows that see a token whose entry in the table is -1; a
+    request must not be given more tokens than its row holds, since prompt_attention
+    takes its rows for the last of the row's capacity then."""
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_blocks_per_seq: int,
                  max_tokens: int, device):
         if min(num_blocks, block_size, max_seqs, max_blocks_per_seq, max_tokens) < 1:
             raise ValueError("sizes must be >= 1")
+        if max_blocks_per_seq * block_size + max_tokens > 2 ** 31 - 1:
+            raise ValueError("a row's capacity and max_tokens must fit in int32 together")
         self.block_size = block_size
         i32 = dict(dtype=torch.int32, device=device)
         self.block_table = torch.full((max_seqs, max_blocks_per_seq), -1, **i32)
@@ -134,20 +144,30 @@ class DeviceBlockTables:
         self.free_count = torch.full((1,), num_blocks, **i32)
         self._out = torch_ops.request_tables_out(self.num_pages, max_tokens).replace(
             num_pages=self.num_pages, free_count=self.free_count)
+        self._ends = torch.zeros(max_seqs + 1, **i32)
+        self._room = torch.zeros(max_seqs, **i32)
 
     def step(self, query_lens: torch.Tensor) -> torch_ops.RequestTables:
         """query_lens (int32 [max_seqs], on the device) more tokens a request: takes
-        their pages and gives the step's query_start_loc, seq_lens, positions and
+        their pages and gives the step's query_start_loc, seq_lens (with the tokens
+        past max_tokens left out, those without a page not), positions and
         slot_mapping (buffers of this object, valid until the next step)."""
         out = torch_ops.request_tables(query_lens, self.lens, self.num_pages, self.free_pages,
                                        self.free_count, self.block_table, self.block_size,
                                        out=self._out)
-        self.lens.copy_(out.seq_lens)
+        # The next step's context is what the cache holds: the tokens that have an entry
+        # in slot_mapping, as far as the request's pages go.  (A lost token counted
+        # would have its place filled later by a page with another's K and V.)
+        torch.clamp(out.query_start_loc, max=out.max_tokens, out=self._ends)
+        torch.sub(self._ends[1:], self._ends[:-1], out=self._room)
+        torch.add(self.lens, self._room, out=out.seq_lens)
+        torch.mul(self.num_pages, self.block_size, out=self._room)
+        torch.minimum(out.seq_lens, self._room, out=self.lens)
         return out
 
     def keep(self, lens: torch.Tensor) -> None:
-        """Takes every request back to its first lens[r] tokens (int32 [max_seqs], at
-        most its length; 0 ends it): pages no longer needed are free again."""
+        """Takes every request back to its first lens[r] tokens (int32 [max_seqs]; one
+        past its length keeps it, 0 ends it): pages no longer needed are free again."""
         torch_ops.release_pages(lens, self.num_pages, self.free_pages, self.free_count,
                                 self.block_table, self.block_size)
         torch.minimum(self.lens, lens.clamp(min=0), out=self.lens)
