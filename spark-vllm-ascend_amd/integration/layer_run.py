@@ -44,10 +44,11 @@ Kernel sequence (HIP launches):
           tokens; any T): prompt_layer (integration/prompt.py), its positions
           the argument, its slots metadata.slot_mapping -> add +
           RMSNorm(next norm).
-Other calls -- no published metadata, more than 16 rows, or rows that are
-not one decode token per sequence (prefill) -- go to the stock layer, as the
-reference's op runs vLLM's attention, post-attention norm, MLP and next norm
-for ``x.shape[0] != 1`` or missing metadata (:50-61): install() takes the
+Other calls -- no published metadata, more than 16 rows, rows that are not
+one decode token per sequence (prefill), or a shared prefix (the metadata's
+prefix_table) -- go to the stock layer, as the reference's op runs vLLM's
+attention, post-attention norm, MLP and next norm for ``x.shape[0] != 1``
+or missing metadata (:50-61): install() takes the
 stock layer as a callable ``stock_layer(index, x, residual, positions) ->
 (y, residual_out)`` with the same contract as layer_run.  Without one, such
 calls raise.  With several sequences the positions and KV slots come from
@@ -189,15 +190,22 @@ def layer_run(x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor,
     e = _layers[layer_name]
     md = _metadata
     T = x.shape[0] if x.dim() == 2 else -1
+    # the kernels of a decode step read every token by the rows' own block tables
+    shared = md is not None and md.prefix_table is not None
     if md is not None and md.query_start_loc is not None:
+        if shared:
+            raise ValueError("packed query rows and a shared prefix do not go together")
         return _packed_rows(e, md, x, residual, positions)
-    decode = md is not None and 1 <= T <= 16 and md.seq_lens.numel() == T
+    decode = md is not None and not shared and 1 <= T <= 16 and md.seq_lens.numel() == T
     if not decode:
-        if e.stock is not None:  # prefill and unpublished metadata: the stock layer
+        if e.stock is not None:  # prefill, unpublished metadata, a shared prefix
             return e.stock(e.index, x, residual, positions)
         if md is None:
             raise RuntimeError("no attention metadata published: call set_attention_metadata() "
                                "for this step (or install a stock layer)")
+        if shared:
+            raise ValueError("layer_run does not decode under a shared prefix "
+                             "(SplitKVDecodeImpl.forward does); install a stock layer for it")
     c, L = e.cfg, e.layer
     if x.dim() != 2 or x.shape[1] != c.hidden or x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bf16 [T, {c.hidden}], got {x.dtype} {tuple(x.shape)}")
