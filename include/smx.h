@@ -484,9 +484,10 @@ int smx_shared_prefix_attention(void* stream, const void* q, int64_t q_stride,
 
 /*
  * Block tables, slots, positions and offsets of a step from request lengths
- * on the device.  Request r has context_lens[r] tokens in the cache,
- * num_pages[r] pages in its block-table row, and gets query_lens[r] more tokens
- * (negative values count as 0).  It takes
+ * on the device.  Request r has context_lens[r] tokens in the cache, num_pages[r]
+ * pages in its block-table row, and gets query_lens[r] more tokens (negative
+ * values count as 0).  (A token that an earlier step gave no slot is not in the
+ * cache: counted, its place would get a page that it was never written to.)  It takes
  *   need[r] = max(0, min(ceil((context + query) / block_size), max_blocks) - num_pages)
  * pages in request order from the end of the free list free_pages[0 ..
  * free_count[0] - 1] (num_free: its capacity): block num_pages[r] + j gets
@@ -517,7 +518,9 @@ int smx_request_tables(void* stream, const int32_t* query_lens, const int32_t* c
  * Gives pages back: request r keeps those of its first keep_lens[r] tokens (0:
  * none), the others are appended to the free list in request and block order
  * (what exceeds its capacity num_free is dropped), their table entries become
- * -1, and num_pages and free_count are updated in place.
+ * -1, and num_pages and free_count are updated in place.  A page belongs to one
+ * row: one that several rows list is appended once for each that gives it back,
+ * so pages that requests share (a prefix's) stay out of the rows given here.
  */
 int smx_release_pages(void* stream, const int32_t* keep_lens, int32_t* num_pages,
                       int32_t* free_pages, int32_t* free_count, int32_t* block_table,

@@ -538,7 +538,11 @@ struct Place {
 // that the workgroups are alike whatever the lengths: every workgroup derives
 // it from the lengths.  Nothing is cut where that would not save `gain` rounds of
 // the longest item (a round beside another workgroup's takes 1.45 of one alone), or
-// where the items read memory at its rate as they are (`memory`).
+// where the items read memory at its rate as they are (`memory`: few rows a
+// sequence): from 160 of 512 workgroups on, none 1.3 times as long as the average.  us
+// whole / cut of sequences of 5 tokens behind 5000, a fourth of them r times the
+// average: 16 (128 workgroups) r = 1 97 / 63; 20 (160) 110 / 91, behind 2500
+// 38 / 41; 29 (232) 122 / 130, r = 1.15 133 / 130, 1.3 146 / 140, 1.5 160 / 131.
 template <int ROUND, typename Seg>
 __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, int target,
                                           int max_parts, int least, float gain, bool memory,
@@ -603,11 +607,12 @@ __device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, in
 // workgroups overlap matrix and vector work by themselves; 8 waves a workgroup (256
 // rows, or four token groups) were slower on full chips.
 //
-// Packed prompts.  Bound by the matrix units at the chip's power where there are many
-// rows: one prompt of 8192 tokens, 32 / 8 heads of 128, 515 us = 1070 TFLOP/s, a large
-// library product 1406; by the longest workgroups where all are resident (2048 tokens
-// 49 us); by memory for a few drafted tokens (8 x 5 behind 300 to 8000: 21.6 us, 4.5
-// TB/s).  Sequence r's queries are the tokens [query_start[r],
+// Packed prompts.  Bound by matrix and vector work in turn where there are many rows:
+// one prompt of 8192 tokens, 32 / 8 heads of 128, 515 to 545 us = 1070 to 1010 TFLOP/s,
+// a large library product 1406; of 1.05 million cycles at 1.94 GHz the matrix units
+// are busy for 0.53, other vector instructions issue for 0.42.  By the longest
+// workgroups where all are resident (2048 tokens 50 us); by memory for a few drafted
+// tokens (8 x 5 behind 300 to 8000: 20 us, 4.9 TB/s).  Sequence r's queries are the tokens [query_start[r],
 // query_start[r + 1]), the last n of its L tokens: token i of them is at position
 // L - n + i and sees the tokens up to itself.  Grid: kv heads, items.
 template <int HD, int WM, int WN, int KT, int ST, int BS>
@@ -642,6 +647,7 @@ void prompt_attention_kernel(RowsArgs A) {
   }
   Place place;
   // (the grid has room for the most items there can be)
+  // (a gain below 14 is choose_prompt's for fewer than 64 rows a sequence)
   if (!find_item<ROUND>(seg_of, A.num_seqs, item, A.target, A.splits, A.least,
                         A.gain, A.gain < 14.f, place))
     return;
@@ -681,9 +687,10 @@ void prompt_attention_kernel(RowsArgs A) {
 // rows of all sequences, and each sequence's own tokens [prefix, L).  Grid: kv
 // heads, items.  Up to 64 rows the prefix and the sequences are segments of one
 // work list in parts of one length.  More (BIG): the prefix's items come first,
-// workgroups of 128 rows, one a compute unit, bound by the matrix units; the
-// sequences' items, bound by memory, run beside them.  64 sequences of 100 to 2048
-// tokens under 32700: 82 us, 400 TFLOP/s and 3.7 TB/s at once; 8 under 4096 11 us.
+// workgroups of 128 rows, one a compute unit, bound by a round's chain alone on its
+// unit; the sequences' items, bound by memory, run beside them.  64 sequences of 100
+// to 2048 tokens under 32700: 80 us, 440 TFLOP/s and 3.9 TB/s at once, the matrix
+// units busy for a fifth of it; 8 under 4096 9.8 us.
 template <int HD, bool BIG, int BS>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void shared_prefix_kernel(RowsArgs A) {
@@ -907,7 +914,10 @@ struct Choice {
 // heads of 128, rows of 64 / of 128: a prompt of 1000 tokens 22 / 27, 1500 35 / 38,
 // 2048 54 / 50, 3000 103 / 85; behind a context, where all ranges are about as long,
 // 128 from one filling on (1000 behind 3000, 40 / 8 heads 114 / 100, 32 / 8 74 / 83).
-// Sequences of 65 to 128 rows are one tile of 128: 20 of 28 tokens 11.5 / 9.7.
+// Sequences of 65 to 128 rows are one tile of 128, so that fewer workgroups share a
+// compute unit: 28 tokens of 12 sequences (192 workgroups of 64) 7.2 / 8.6, 16 (256) 7.6 /
+// 8.7, 20 (320) 9.4 / 9.1, 40 (640) 14.9 / 13.5; behind 600 12 15.9 / 20.0, 16 17.2 /
+// 20.7, 20 21.3 / 21.2, 40 34.5 / 32.5.
 //
 // Cutting tiles' tokens into parts costs partials and a second launch, about 11 us
 // (14 rounds of 64 tokens), 5 where a tile has few rows, and two workgroups a
@@ -917,7 +927,12 @@ struct Choice {
 // 56.6 / 56.9 and 512 behind 2000 38 / 41.  (The tables' capacity stands for the
 // lengths here, find_item asks again with them.)  Sequences of few rows read memory
 // at its rate from 160 workgroups on: 23 of up to 11 tokens behind 2821 51 / 59; only
-// uneven ones are cut then, 29 of up to 7 behind 2300 to 6900 137 / 98.  Cut for long
+// uneven ones are cut then (find_item), and those of a small capacity not even asked:
+// 20 of 5 behind 2500 38 / 41, a fourth of them 1.3 times that 47 / 41, 29 such 57 / 63
+// and 65 / 63.  Lengths below the longest take fewer parts, so the longest may take 2
+// or 4 times the parts of even ones: 1, 2, 4 times 8 of 5 behind 300 to 8000
+// 32.0, 29.6, 29.8; 60 each behind 500, 12000, 900, 700 47.1, 33.6, 32.2; 200 each
+// behind 500, 12000, 900 91.8, 75.7, 79.6.  Cut for long
 // contexts 128 rows are better: 509 behind 16000 170 / 153, 500 behind 4000 60 / 60.
 // Parts are of at least 256 tokens: 300 behind 1500 31.5 at 512, 32.2 at 256, one
 // token behind 900 14.6 at 512, 12.3 at 256.
@@ -948,6 +963,9 @@ Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int grou
 // much work; else one list of 64-row workgroups for the prefix and the sequences.
 // us, list / own: 64 sequences (256 rows) under 2000 tokens 25.6 / 30.2, 8000 32.8 /
 // 32.1, 32700 134 / 90; 24 (96 rows) under 4000 16.9 / 19.3, 16000 28.6 / 25.2.
+// Beside the prefix's own workgroups a long sequence may take 4 times the parts of
+// even ones: 1, 2, 4 times 64 of 100 to 2048 under 32700 93, 88, 88, 48 of 1 to 6000
+// under 16000 60, 52, 48, one of 7000 among 31 of 100 46, 36, 33, 40 of 1 to 600 52, 53, 54.
 Choice choose_prefix(int64_t num_seqs, int64_t prefix_cap, int64_t cap, int group, int n_kv) {
   Choice c{};
   const int64_t rows = num_seqs * group;

@@ -887,7 +887,8 @@ def release_pages(keep_lens: torch.Tensor, num_pages: torch.Tensor, free_pages: 
                   free_count: torch.Tensor, block_table: torch.Tensor, block_size: int) -> None:
     """Give the pages beyond the first keep_lens[r] tokens of every request back to
     the free list (0: all of a finished request's; fewer than its length: those
-    of rejected tokens).  Everything is updated in place."""
+    of rejected tokens).  Everything is updated in place.  A page belongs to one
+    request: one that several rows list would be in the free list several times."""
     reqs, max_blocks, _ = _pages_checks(num_pages, free_pages, free_count, block_table, keep_lens,
                                         "keep_lens")
     call("smx_release_pages", _stream(num_pages), keep_lens.data_ptr(), num_pages.data_ptr(),
