@@ -220,3 +220,35 @@ def test_attention_after_the_list_ran_out():
     kept[1] = [x[:0] for x in kept[1]]
     step([3, 2])
     step([1, 100], lost=(0, 39))  # 69 of its 100 rows, 30 in the one page it has
+
+
+@pytest.mark.gpu
+def test_captured_steps_short_of_room():
+    """A captured step and keep, replayed on other lengths: the same tables, lengths and
+    slots as another object's eager steps, where room runs out too."""
+    mod = pkg("integration.block_table")
+    S, r = 5, random.Random(9)
+    a, b = (mod.DeviceBlockTables(13, 8, S, 5, 40, "cuda") for _ in range(2))
+    query, keep = (torch.zeros(S, dtype=torch.int32, device="cuda") for _ in range(2))
+    outs = []
+
+    def run():
+        outs.append(a.step(query))
+        a.keep(keep)
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in range(12):
+        query.copy_(torch.tensor([r.choice([0, 1, 1, 9, 30]) for _ in range(S)]))
+        keep.copy_(torch.tensor([r.choice([0, 7, 100, 100, 100]) for _ in range(S)]))
+        graph.replay()
+        want = b.step(query)
+        b.keep(keep)
+        torch.cuda.synchronize()
+        for name in ("query_start_loc", "seq_lens", "positions", "slot_mapping"):
+            assert torch.equal(getattr(outs[-1], name), getattr(want, name)), (i, name)
+        for name in ("lens", "num_pages", "block_table", "free_count"):
+            assert torch.equal(getattr(a, name), getattr(b, name)), (i, name)
