@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define SMX_ABI_VERSION 12
+#define SMX_ABI_VERSION 13
 
 /* Return codes besides 0 and hipError_t values. */
 #define SMX_EINVAL 10001      /* an argument failed validation */
@@ -661,6 +661,128 @@ int smx_decode_advance(void* stream, int64_t* next_ids,
                        int32_t block_size, int32_t max_len,
                        const void* embed_table, void* embed_out, int64_t vocab,
                        int64_t hidden);
+
+/*
+ * The paged KV cache held in 4 bits.  Blocks of 32 channels of one head of a token share
+ * an fp16 scale d and hold codes c of 0..15 for the values d (c - 8), the block format of
+ * the Q4_0 weights (src/spark_vllm_ascend/integration/weights.py:34-40): m the block's
+ * first value of largest magnitude, d = fp16(m / -8) kept within +-65504, c =
+ * floor(x / d + 8.5) kept within 0..15 (8 where d is 0: |m| below 2^-22); a block with a
+ * NaN has the scale NaN and codes 0, an infinity becomes the block's largest value.
+ *   codes  [2][num_blocks][n_kv][block_size][head_dim / 2] bytes, K first
+ *   scales [2][num_blocks][n_kv][block_size][head_dim / 32] fp16
+ * both 16-byte aligned; the order of the codes of a row is the kernels' own
+ * (native/csrc/q4_cache.h), their values are read with smx_q4_kv_read.  head_dim 64 or
+ * 128, block_size a power of two in [32, 4096].  The reference's caches are bf16
+ * (kernels/qkv.py:192-198,226-236) and so are smx_reshape_and_cache's.
+ *
+ * smx_q4_reshape_and_cache: smx_reshape_and_cache into it; a token's heads are contiguous,
+ * tokens key_stride (value_stride) elements apart, a multiple of 8.
+ * smx_q4_qknorm_rope_kv_write: smx_qknorm_rope_kv_write into it (head_dim 128).
+ * smx_q4_kv_read: the values of the tokens at slot_mapping as fp32 [num_tokens, n_kv,
+ * head_dim], exactly; 0 for slots outside the cache.
+ */
+int smx_q4_reshape_and_cache(void* stream, const void* key, int64_t key_stride,
+                             const void* value, int64_t value_stride, void* codes, void* scales,
+                             const int64_t* slot_mapping, int32_t num_tokens, int32_t n_kv,
+                             int32_t head_dim, int32_t num_blocks, int32_t block_size);
+int smx_q4_qknorm_rope_kv_write(void* stream, const void* qkv, const void* q_gamma,
+                                const void* k_gamma, const void* cos_sin,
+                                const int64_t* positions, const int64_t* slot_mapping,
+                                void* q_out, void* codes, void* scales, int32_t num_tokens,
+                                int32_t n_q, int32_t n_kv, int32_t head_dim, int32_t num_blocks,
+                                int32_t block_size, int32_t max_position, float eps);
+int smx_q4_kv_read(void* stream, const void* codes, const void* scales,
+                   const int64_t* slot_mapping, void* key, void* value, int32_t num_tokens,
+                   int32_t n_kv, int32_t head_dim, int32_t num_blocks, int32_t block_size);
+
+/*
+ * smx_prompt_attention over a cache held in 4 bits: the same rows, masks and table rules
+ * (rows that see a token whose table entry is outside the cache are NaN, rows that see
+ * none 0, rows of no sequence stay as they are).  query_start_loc may be NULL where
+ * num_tokens is num_seqs: row r is sequence r's newest token, a decode step.  The cache's
+ * values are not rounded; scores, sums and outputs are fp32, the weights of the second
+ * product (softmax weight times V's scale) bf16.
+ */
+int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_seqs, int32_t max_blocks,
+                                   int32_t block_size, int32_t n_q, int32_t n_kv,
+                                   int32_t head_dim);
+int smx_q4_attention(void* stream, const void* q, int64_t q_stride, const void* codes,
+                     const void* scales, const int32_t* block_table,
+                     const int32_t* query_start_loc, const int32_t* seq_lens, void* workspace,
+                     int64_t workspace_bytes, void* out, int32_t num_tokens, int32_t num_seqs,
+                     int32_t max_blocks, int32_t num_blocks, int32_t block_size, int32_t n_q,
+                     int32_t n_kv, int32_t head_dim, float scale);
+
+/*
+ * Beam search's selection.  Sequence s has the rows s * beams + b of logits (bf16 or fp32
+ * by element_size 2 or 4, rows stride elements apart) and of scores (fp32).  Its
+ * continuations score
+ *   scores[b] + logits[b][v] - log sum_u exp(logits[b][u])
+ * taken in 64 bits; the best `width` in order, ties to the lowest b * vocab + v, go to
+ * parents (the row), tokens and out_scores [seqs, width].  Where there are fewer the rest
+ * is -1, -1 and -inf.  A logit of -inf or NaN is never chosen; logits of +inf share the
+ * probability; a row whose score is -inf or NaN offers nothing.  A row with done[row] != 0
+ * (done may be NULL) offers pad_id at its own score and nothing else.
+ * beams and width in [1, 64], vocab in [1, 2^24].  out_scores may be scores where width
+ * is beams.  The reference samples one sequence greedily (integration/head.py:12-31).
+ */
+int64_t smx_beam_select_workspace(int32_t seqs, int32_t beams, int32_t width, int32_t vocab,
+                                  int32_t element_size);
+int smx_beam_select(void* stream, const void* logits, int64_t stride, int32_t element_size,
+                    const float* scores, const uint8_t* done, void* workspace,
+                    int64_t workspace_bytes, int32_t* parents, int64_t* tokens,
+                    float* out_scores, int32_t seqs, int32_t beams, int32_t width, int32_t vocab,
+                    int32_t pad_id);
+
+/*
+ * Block tables of the rows that a step goes on with.  New row j continues old row
+ * parents[j] (outside [0, num_rows): it is empty), the first lens[parents[j]] tokens of
+ * it: it lists the same pages, so rows of one parent share them.  A last page that is not
+ * full is not shared: it stays with its parent's first child, if none of the other rows
+ * that go on lists it, and the other children get a page of their own from the end of
+ * the free list, in the order of the rows; copies[j] is (page, that page), else
+ * (-1, -1), for smx_copy_pages.  Where the free list is used up the row is cut to its
+ * whole pages (num_pages_out, lens_out tell).  Pages that old rows listed and no new row
+ * does are appended to what is left of the free list, in ascending order; its entries
+ * past free_count_out become -1.  A page listed by a row must not be in the free list.
+ * parents, lens, num_pages, num_pages_out and lens_out are [num_rows], the tables
+ * [num_rows, max_blocks], the free lists [num_free], copies [num_rows, 2].
+ * block_table_out, num_pages_out and lens_out are apart from all inputs; free_pages_out
+ * may be free_pages, free_count_out free_count.  num_rows <= 8192, num_blocks <= 262144.
+ * A finished row is freed by not being a parent; smx_release_pages is for tables whose
+ * rows share no page.
+ */
+int smx_fork_pages(void* stream, const int32_t* parents, const int32_t* lens,
+                   const int32_t* num_pages, const int32_t* free_pages,
+                   const int32_t* free_count, const int32_t* block_table,
+                   int32_t* block_table_out, int32_t* num_pages_out, int32_t* lens_out,
+                   int32_t* free_pages_out, int32_t* free_count_out, int32_t* copies,
+                   int32_t num_rows, int32_t max_blocks, int32_t num_blocks, int32_t num_free,
+                   int32_t block_size);
+
+/*
+ * Moves the pages in use to the front of the pool.  With U pages listed (by any number of
+ * rows, among their num_pages first entries), the k-th of them that is U or more moves
+ * to the k-th unlisted page below U: moves[k] = (from, to), for smx_copy_pages, the rest
+ * of moves [num_blocks / 2, 2] is (-1, -1).  block_table_out (it may be block_table)
+ * lists the new places, -1 past a row's pages; free_pages [num_blocks] becomes
+ * num_blocks - 1, ..., U and then -1, free_count num_blocks - U.
+ */
+int smx_compact_pages(void* stream, const int32_t* num_pages, const int32_t* block_table,
+                      int32_t* block_table_out, int32_t* free_pages, int32_t* free_count,
+                      int32_t* moves, int32_t num_rows, int32_t max_blocks, int32_t num_blocks);
+
+/*
+ * Copies page src to page dst in every plane, for each of num_pairs pairs (src, dst); a
+ * pair with an entry outside [0, num_blocks) is skipped.  planes [num_planes, 2] is device
+ * memory: the address of a plane's page 0 (16-byte aligned) and the bytes of a page (a
+ * multiple of 16, at most max_page_bytes); page p of a plane is p pages further on.  No
+ * page may be the dst of two pairs, or the dst of one and the src of another.
+ */
+int smx_copy_pages(void* stream, const int64_t* planes, int32_t num_planes,
+                   int64_t max_page_bytes, const int32_t* pairs, int32_t num_pairs,
+                   int32_t num_blocks);
 
 /*
  * Step runner: records the kernel launches that the C-ABI calls made on the

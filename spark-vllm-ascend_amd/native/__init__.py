@@ -29,7 +29,7 @@ DEFAULT_RECORD = LIB_PATH.with_name("libsmx.validation.json")
 #: benchmark and the build check do (they are what validates and measures the
 #: library as built); a record named by SMX_VALIDATION_RECORD is still checked
 UNVALIDATED_ENV = "SMX_ALLOW_UNVALIDATED"
-ABI_VERSION = 12
+ABI_VERSION = 13
 SMX_EINVAL = 10001
 SMX_EUNSUPPORTED = 10002
 
@@ -100,6 +100,16 @@ SIGNATURES = {
     "smx_q4_0_add_rmsnorm_gemv_gelu": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _F32],
     "smx_q4_0_add_rmsnorm_gemv_argmax": [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _F32],
     "smx_q4_0_argmax_keys_size": [_I64, _I64],
+    "smx_q4_reshape_and_cache": [_P, _P, _I64, _P, _I64, _P, _P, _P] + [_I32] * 5,
+    "smx_q4_qknorm_rope_kv_write": [_P] * 10 + [_I32] * 7 + [_F32],
+    "smx_q4_kv_read": [_P] * 6 + [_I32] * 5,
+    "smx_q4_attention_workspace": [_I32] * 7,
+    "smx_q4_attention": [_P, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _P] + [_I32] * 8 + [_F32],
+    "smx_beam_select_workspace": [_I32] * 5,
+    "smx_beam_select": [_P, _P, _I64, _I32, _P, _P, _P, _I64, _P, _P, _P] + [_I32] * 5,
+    "smx_fork_pages": [_P] * 13 + [_I32] * 5,
+    "smx_compact_pages": [_P] * 7 + [_I32] * 3,
+    "smx_copy_pages": [_P, _P, _I32, _I64, _P, _I32, _I32],
     "smx_runner_create": [ctypes.POINTER(ctypes.c_char_p), _I32, ctypes.POINTER(_P)],
     "smx_runner_begin": [_P],
     "smx_runner_end": [_P],
@@ -120,6 +130,8 @@ RUNNER_FENCES_ACQUIRE_ONLY = 1
 RESTYPES = {"smx_argmax_parts": ctypes.c_int64,
             "smx_prompt_attention_workspace": ctypes.c_int64,
             "smx_shared_prefix_attention_workspace": ctypes.c_int64,
+            "smx_q4_attention_workspace": ctypes.c_int64,
+            "smx_beam_select_workspace": ctypes.c_int64,
             "smx_q4_0_argmax_keys_size": ctypes.c_int64,
             "smx_q4_0_gemm_keys_per_row": ctypes.c_int64,
             "smx_q4_0_packed_bytes": ctypes.c_int64,

@@ -1,0 +1,427 @@
+// Pages of the cache that several rows of the block tables share (gfx950): block tables of
+// the rows that a step goes on with (beams of a search, samples of a prompt), pages moved
+// to the front of the pool, and the copies of pages that both ask for.
+//
+// Who holds a page is read off the tables: a page is in use where a row lists it among its
+// num_pages first, and free again once no row does.  No counts are kept, so that there
+// are none to go wrong.  A workgroup collects the pages in bit sets in LDS (32768 pages
+// a 4 KB set); nothing of a call is left for the next.
+#include <limits.h>
+
+#include <algorithm>
+
+#include "smx_common.h"
+#include "smx_launch.h"
+
+namespace smx {
+namespace {
+
+constexpr int NT = 1024;
+constexpr int MAX_PAGES = 1 << 18;
+
+// A row's first `kept` pages go to its children; the tail, a last page that is not full,
+// to the first of them alone.
+struct ForkArgs {
+  const int32_t* parents;
+  const int32_t* lens;
+  const int32_t* num_pages;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  const int32_t* table;
+  int32_t* table_out;
+  int32_t* num_pages_out;
+  int32_t* lens_out;
+  int32_t* free_pages_out;
+  int32_t* free_count_out;
+  int32_t* copies;  // [rows, 2]
+  int rows, max_blocks, num_blocks, num_free, bs_log2;
+};
+
+__device__ __forceinline__ void set_bit(uint32_t* set, int i) {
+  atomicOr(set + (i >> 5), 1u << (i & 31));
+}
+__device__ __forceinline__ bool get_bit(const uint32_t* set, int i) {
+  return set[i >> 5] >> (i & 31) & 1;
+}
+
+// Inclusive prefix sums over a workgroup; *total the sum.
+__device__ __forceinline__ int scan(int v, int* total, int* waves) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  v = wave_scan_i32(v);
+  __syncthreads();  // the last call's sums have been read
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  int sum = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w == wave) v += sum;
+    sum += waves[w];
+  }
+  *total = sum;
+  return v;
+}
+
+// A row's pages, tokens and pages kept.
+__device__ __forceinline__ void row_sizes(const ForkArgs& A, int r, int& pages, int& len,
+                                          int& kept) {
+  pages = min(max(A.num_pages[r], 0), A.max_blocks);
+  len = (int)min((int64_t)max(A.lens[r], 0), (int64_t)pages << A.bs_log2);
+  kept = (int)(((int64_t)len + (1 << A.bs_log2) - 1) >> A.bs_log2);
+}
+
+// Workgroup 0 does all but the tables' whole columns, which the others copy: 4 rows each,
+// a wave a row.
+template <int PAGES, int ROWS>
+__global__ __launch_bounds__(NT) void fork_pages_kernel(ForkArgs A) {
+  __shared__ uint32_t listed[PAGES / 32];  // by an old row, and by no new one in the end
+  __shared__ uint32_t live[PAGES / 32];    // among the kept pages of a row with children
+  __shared__ uint32_t twice[PAGES / 32];   // the same by two rows
+  __shared__ int first_s[ROWS];            // a row's first child, INT_MAX: none
+  __shared__ int waves[NT / 64];
+  const int tid = threadIdx.x;
+  const int bs = 1 << A.bs_log2;
+  if (blockIdx.x > 0) {
+    const int j = (blockIdx.x - 1) * (NT / 64) + (tid >> 6), lane = tid & 63;
+    if (j < A.rows) {
+      const int r = A.parents[j];
+      const bool ok = r >= 0 && r < A.rows;
+      int pages, len, kept = 0, tail = -1;
+      if (ok) {
+        row_sizes(A, r, pages, len, kept);
+        if (len & (bs - 1)) tail = kept - 1;  // workgroup 0 writes it
+      }
+      const int32_t* const src = A.table + (int64_t)(ok ? r : 0) * A.max_blocks;
+      int32_t* const dst = A.table_out + (int64_t)j * A.max_blocks;
+      for (int b = lane; b < A.max_blocks; b += 64)
+        if (b != tail) st_agent(dst + b, b < kept ? src[b] : -1);
+    }
+    stores_done();
+    return;
+  }
+  for (int i = tid; i < PAGES / 32; i += NT) listed[i] = live[i] = twice[i] = 0;
+  for (int i = tid; i < A.rows; i += NT) first_s[i] = INT_MAX;
+  __syncthreads();
+  for (int j = tid; j < A.rows; j += NT) {
+    const int r = A.parents[j];
+    if (r >= 0 && r < A.rows) atomicMin(first_s + r, j);
+  }
+  __syncthreads();
+  // a wave a row
+  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
+    int pages, len, kept;
+    row_sizes(A, r, pages, len, kept);
+    const bool parent = first_s[r] != INT_MAX;
+    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
+    for (int b = tid & 63; b < pages; b += 64) {
+      const int p = src[b];
+      if ((unsigned)p >= (unsigned)A.num_blocks) continue;
+      set_bit(listed, p);
+      if (parent && b < kept) {
+        const uint32_t bit = 1u << (p & 31);
+        if (atomicOr(live + (p >> 5), bit) & bit) set_bit(twice, p);
+      }
+    }
+  }
+  __syncthreads();
+  // ---- copies, in the order of the new rows, from the end of the free list
+  const int count = min(max(A.free_count[0], 0), A.num_free);
+  int taken = 0;
+  for (int j0 = 0; j0 < A.rows; j0 += NT) {
+    const int j = j0 + tid;
+    int kept = 0, len = 0, page = -1;
+    bool tail = false, copy = false;
+    if (j < A.rows) {
+      const int r = A.parents[j];
+      if (r >= 0 && r < A.rows) {
+        int pages;
+        row_sizes(A, r, pages, len, kept);
+        tail = len & (bs - 1);
+        if (tail) {
+          page = A.table[(int64_t)r * A.max_blocks + kept - 1];
+          copy = (unsigned)page < (unsigned)A.num_blocks &&
+                 (first_s[r] != j || get_bit(twice, page));
+        }
+      }
+    }
+    int all;
+    const int at = count - taken - scan(copy, &all, waves);
+    if (j < A.rows) {
+      int src = -1, dst = -1;
+      if (copy) {
+        // (an entry of the free list outside the pool is no page)
+        dst = at >= 0 ? A.free_pages[at] : -1;
+        if ((unsigned)dst >= (unsigned)A.num_blocks) dst = -1;
+        if (dst >= 0) src = page;
+      }
+      if (tail)
+        st_agent(A.table_out + (int64_t)j * A.max_blocks + kept - 1, copy ? dst : page);
+      if (copy && dst < 0) {  // no room: the row ends with its whole pages
+        --kept;
+        len = kept << A.bs_log2;
+      }
+      st_agent(A.num_pages_out + j, kept);
+      st_agent(A.lens_out + j, len);
+      st_agent(A.copies + 2 * j, src);
+      st_agent(A.copies + 2 * j + 1, dst);
+    }
+    taken += all;
+  }
+  // ---- pages that no new row lists: `live` is now what the new rows list, which their
+  // first child lists (the pages of the free list apart): whole pages, and a tail that it
+  // has no copy of.
+  __syncthreads();
+  for (int i = tid; i < PAGES / 32; i += NT) live[i] = 0;
+  __syncthreads();
+  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
+    if (first_s[r] == INT_MAX) continue;
+    int pages, len, kept;
+    row_sizes(A, r, pages, len, kept);
+    const int whole = len >> A.bs_log2;
+    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
+    for (int b = tid & 63; b < kept; b += 64) {
+      const int p = src[b];
+      if ((unsigned)p < (unsigned)A.num_blocks && (b < whole || !get_bit(twice, p)))
+        set_bit(live, p);
+    }
+  }
+  __syncthreads();
+  const int left = max(count - taken, 0);
+  for (int i = tid; i < left; i += NT)
+    if (A.free_pages_out != A.free_pages) st_agent(A.free_pages_out + i, A.free_pages[i]);
+  int given = 0;
+  for (int w0 = 0; w0 * 32 < A.num_blocks; w0 += NT) {
+    const int w = w0 + tid;
+    uint32_t bits = w < PAGES / 32 ? listed[w] & ~live[w] : 0;
+    int all;
+    int at = left + given + scan(__popc(bits), &all, waves) - __popc(bits);
+    while (bits) {
+      if (at < A.num_free) st_agent(A.free_pages_out + at, w * 32 + __ffs(bits) - 1);
+      bits &= bits - 1;
+      ++at;
+    }
+    given += all;
+  }
+  const int now = min(left + given, A.num_free);
+  for (int i = now + tid; i < A.num_free; i += NT) st_agent(A.free_pages_out + i, -1);
+  if (tid == 0) st_agent(A.free_count_out, now);
+  stores_done();
+}
+
+struct CompactArgs {
+  const int32_t* num_pages;
+  const int32_t* table;
+  int32_t* table_out;
+  int32_t* free_pages;  // [num_blocks]
+  int32_t* free_count;
+  int32_t* moves;  // [num_blocks / 2, 2]
+  int rows, max_blocks, num_blocks;
+};
+
+// With U pages in use, those from U on move to the unused ones below it, in order: the
+// k-th such page to the k-th such place.  Both ranks come from the sums of the set's words.
+template <int PAGES>
+__global__ __launch_bounds__(NT) void compact_pages_kernel(CompactArgs A) {
+  __shared__ uint32_t used[PAGES / 32];
+  __shared__ int32_t before[PAGES / 32];  // pages in use before a word's
+  __shared__ int waves[NT / 64];
+  const int tid = threadIdx.x;
+  const int words = (A.num_blocks + 31) / 32;
+  for (int i = tid; i < words; i += NT) used[i] = 0;
+  __syncthreads();
+  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
+    const int pages = min(max(A.num_pages[r], 0), A.max_blocks);
+    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
+    for (int b = tid & 63; b < pages; b += 64) {
+      const int p = src[b];
+      if ((unsigned)p < (unsigned)A.num_blocks) set_bit(used, p);
+    }
+  }
+  __syncthreads();
+  int total = 0;
+  for (int w0 = 0; w0 < words; w0 += NT) {
+    const int w = w0 + tid;
+    const int c = w < words ? __popc(used[w]) : 0;
+    int all;
+    const int upto = scan(c, &all, waves);
+    if (w < words) before[w] = total + upto - c;
+    total += all;
+  }
+  __syncthreads();
+  auto rank_of = [&](int p) {  // pages in use below p
+    return before[p >> 5] + __popc(used[p >> 5] & ((1u << (p & 31)) - 1));
+  };
+  const int kept = total > 0 ? rank_of(total - 1) + get_bit(used, total - 1) : 0;  // below `total`
+  auto hole = [&](int k) {  // the k-th unused page
+    int lo = 0, hi = words;  // the last word with at most k unused pages before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (32 * mid - before[mid] <= k)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    uint32_t free_bits = ~used[lo];
+    for (int i = k - (32 * lo - before[lo]); i > 0; --i) free_bits &= free_bits - 1;
+    return 32 * lo + __ffs(free_bits) - 1;
+  };
+  const int moved = total - kept;  // pages in use from `total` on
+  for (int w = (total >> 5) + tid; w < words; w += NT) {
+    uint32_t bits = used[w];
+    if (w == total >> 5) bits &= ~0u << (total & 31);
+    for (; bits; bits &= bits - 1) {
+      const int p = 32 * w + __ffs(bits) - 1, k = rank_of(p) - kept;
+      st_agent(A.moves + 2 * k, p);
+      st_agent(A.moves + 2 * k + 1, hole(k));
+    }
+  }
+  for (int i = 2 * moved + tid; i < 2 * (A.num_blocks / 2); i += NT) st_agent(A.moves + i, -1);
+  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
+    const int pages = min(max(A.num_pages[r], 0), A.max_blocks);
+    for (int b = tid & 63; b < A.max_blocks; b += 64) {
+      const int64_t at = (int64_t)r * A.max_blocks + b;
+      int p = b < pages ? A.table[at] : -1;
+      if ((unsigned)p >= (unsigned)A.num_blocks)
+        p = -1;
+      else if (p >= total)
+        p = hole(rank_of(p) - kept);
+      st_agent(A.table_out + at, p);
+    }
+  }
+  for (int i = tid; i < A.num_blocks; i += NT)
+    st_agent(A.free_pages + i, i < A.num_blocks - total ? A.num_blocks - 1 - i : -1);
+  if (tid == 0) st_agent(A.free_count, A.num_blocks - total);
+  stores_done();
+}
+
+// One plane of a cache: its pages are `bytes` each, one after another from `base`.
+struct PagePlane {
+  uint64_t base;
+  int64_t bytes;
+};
+
+// Copies page src to page dst in every plane for each pair (src, dst); a pair with an
+// entry outside the pool is skipped.  Bound by memory.  Grid: pieces, planes, pairs.
+constexpr int PIECE = 16384;  // bytes a workgroup copies
+
+__global__ __launch_bounds__(256) void copy_pages_kernel(const PagePlane* __restrict__ planes,
+                                                         const int32_t* __restrict__ pairs,
+                                                         int num_blocks) {
+  const int src = pairs[2 * blockIdx.z], dst = pairs[2 * blockIdx.z + 1];
+  if ((unsigned)src >= (unsigned)num_blocks || (unsigned)dst >= (unsigned)num_blocks ||
+      src == dst)
+    return;
+  const PagePlane pl = planes[blockIdx.y];
+  const uint8_t* const from = (const uint8_t*)pl.base + src * pl.bytes;
+  uint8_t* const to = (uint8_t*)pl.base + dst * pl.bytes;
+  u32x4 v[4];
+  const int64_t at = (int64_t)blockIdx.x * PIECE + threadIdx.x * 16;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i * 4096 < pl.bytes) v[i] = *reinterpret_cast<const u32x4*>(from + at + i * 4096);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (at + i * 4096 < pl.bytes) st_agent_b128(to + at + i * 4096, v[i]);
+  stores_done();
+}
+
+}  // namespace
+}  // namespace smx
+
+#include "smx_abi_util.h"
+
+#define SMX_PAGES_CHECKS()                                                                       \
+  SMX_REQUIRE(num_rows >= 1 && num_rows <= 8192, "num_rows must be in [1, 8192]");               \
+  SMX_REQUIRE(max_blocks >= 1 && (int64_t)num_rows * max_blocks <= INT_MAX - 4096,               \
+              "num_rows * max_blocks must be at most 2^31 - 4097");                              \
+  SMX_REQUIRE(num_blocks >= 1 && num_blocks <= smx::MAX_PAGES,                                   \
+              "num_blocks must be in [1, 262144]")
+
+namespace {
+// Whether [a, a + bytes) and [b, b + bytes) are apart.
+bool apart(const void* a, const void* b, int64_t bytes) {
+  return (uintptr_t)a + bytes <= (uintptr_t)b || (uintptr_t)b + bytes <= (uintptr_t)a;
+}
+}  // namespace
+
+extern "C" int smx_fork_pages(void* stream, const int32_t* parents, const int32_t* lens,
+                              const int32_t* num_pages, const int32_t* free_pages,
+                              const int32_t* free_count, const int32_t* block_table,
+                              int32_t* block_table_out, int32_t* num_pages_out, int32_t* lens_out,
+                              int32_t* free_pages_out, int32_t* free_count_out, int32_t* copies,
+                              int32_t num_rows, int32_t max_blocks, int32_t num_blocks,
+                              int32_t num_free, int32_t block_size) {
+  SMX_REQUIRE(parents && lens && num_pages && free_pages && free_count && block_table &&
+                  block_table_out && num_pages_out && lens_out && free_pages_out &&
+                  free_count_out && copies,
+              "null pointer argument");
+  SMX_REQUIRE(((uintptr_t)parents | (uintptr_t)lens | (uintptr_t)num_pages |
+               (uintptr_t)free_pages | (uintptr_t)free_count | (uintptr_t)block_table |
+               (uintptr_t)block_table_out | (uintptr_t)num_pages_out | (uintptr_t)lens_out |
+               (uintptr_t)free_pages_out | (uintptr_t)free_count_out | (uintptr_t)copies) % 4 == 0,
+              "int32 arrays must be 4-byte aligned");
+  SMX_PAGES_CHECKS();
+  SMX_REQUIRE(num_free >= 1, "the free list must have room for a page");
+  SMX_REQUIRE(block_size >= 1 && block_size <= 4096 && (block_size & (block_size - 1)) == 0,
+              "block_size must be a power of two in [1, 4096]");
+  // (a new row reads another old one's: the workgroups run side by side)
+  const int64_t row_bytes = 4 * (int64_t)num_rows, table_bytes = row_bytes * max_blocks;
+  SMX_REQUIRE(apart(block_table, block_table_out, table_bytes),
+              "block_table_out must be apart from block_table");
+  for (const int32_t* in : {parents, lens, num_pages})
+    for (const int32_t* out : {num_pages_out, lens_out})
+      SMX_REQUIRE(apart(in, out, row_bytes),
+                  "num_pages_out and lens_out must be apart from parents, lens and num_pages");
+  SMX_REQUIRE(free_pages == free_pages_out || apart(free_pages, free_pages_out, 4 * (int64_t)num_free),
+              "free_pages_out must be free_pages or apart from it");
+  smx::ForkArgs a{parents, lens, num_pages, free_pages, free_count, block_table, block_table_out,
+                  num_pages_out, lens_out, free_pages_out, free_count_out, copies, num_rows,
+                  max_blocks, num_blocks, num_free, 0};
+  while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
+  const dim3 grid(1 + (num_rows + smx::NT / 64 - 1) / (smx::NT / 64));
+  const auto kernel = num_blocks <= 32768 && num_rows <= 2048
+      ? smx::fork_pages_kernel<32768, 2048> : smx::fork_pages_kernel<smx::MAX_PAGES, 8192>;
+  SMX_LAUNCH(kernel, grid, dim3(smx::NT), 0, (hipStream_t)stream, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int smx_compact_pages(void* stream, const int32_t* num_pages,
+                                 const int32_t* block_table, int32_t* block_table_out,
+                                 int32_t* free_pages, int32_t* free_count, int32_t* moves,
+                                 int32_t num_rows, int32_t max_blocks, int32_t num_blocks) {
+  SMX_REQUIRE(num_pages && block_table && block_table_out && free_pages && free_count && moves,
+              "null pointer argument");
+  SMX_REQUIRE(((uintptr_t)num_pages | (uintptr_t)block_table | (uintptr_t)block_table_out |
+               (uintptr_t)free_pages | (uintptr_t)free_count | (uintptr_t)moves) % 4 == 0,
+              "int32 arrays must be 4-byte aligned");
+  SMX_PAGES_CHECKS();
+  SMX_REQUIRE(block_table == block_table_out ||
+                  apart(block_table, block_table_out, 4 * (int64_t)num_rows * max_blocks),
+              "block_table_out must be block_table or apart from it");
+  const smx::CompactArgs a{num_pages, block_table, block_table_out, free_pages, free_count, moves,
+                           num_rows, max_blocks, num_blocks};
+  const auto kernel = num_blocks <= 32768 ? smx::compact_pages_kernel<32768>
+                                          : smx::compact_pages_kernel<smx::MAX_PAGES>;
+  SMX_LAUNCH(kernel, dim3(1), dim3(smx::NT), 0, (hipStream_t)stream, a);
+  return (int)hipGetLastError();
+}
+
+extern "C" int smx_copy_pages(void* stream, const int64_t* planes, int32_t num_planes,
+                              int64_t max_page_bytes, const int32_t* pairs, int32_t num_pairs,
+                              int32_t num_blocks) {
+  SMX_REQUIRE(planes && pairs, "null pointer argument");
+  SMX_REQUIRE((uintptr_t)planes % 8 == 0 && (uintptr_t)pairs % 4 == 0,
+              "planes must be 8-byte aligned, pairs 4-byte");
+  SMX_REQUIRE(num_planes >= 1 && num_planes <= 65535, "num_planes must be in [1, 65535]");
+  SMX_REQUIRE(num_pairs >= 1 && num_pairs <= smx::MAX_PAGES, "num_pairs must be in [1, 262144]");
+  SMX_REQUIRE(num_blocks >= 1, "num_blocks must be >= 1");
+  SMX_REQUIRE(max_page_bytes >= 16 && max_page_bytes <= (1ll << 31), "max_page_bytes out of range");
+  const unsigned pieces = (unsigned)((max_page_bytes + smx::PIECE - 1) / smx::PIECE);
+  for (int32_t at = 0; at < num_pairs; at += 65535) {
+    const dim3 grid(pieces, num_planes, std::min(num_pairs - at, 65535));
+    SMX_LAUNCH(smx::copy_pages_kernel, grid, dim3(256), 0, (hipStream_t)stream,
+               reinterpret_cast<const smx::PagePlane*>(planes), pairs + 2 * at, num_blocks);
+    const int rc = (int)hipGetLastError();
+    if (rc) return rc;
+  }
+  return 0;
+}

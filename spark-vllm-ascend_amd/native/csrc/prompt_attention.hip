@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "row_items.h"
 #include "smx_common.h"
 #include "smx_launch.h"
 
@@ -37,12 +38,6 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
 typedef __attribute__((address_space(4))) int32_t constant_i32;
-
-// (lo, hi) as one v_cvt_pk_bf16_f32
-__device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
-}
 
 // A dword of two bf16 values with those that are infinite or NaN replaced by 0.
 __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
@@ -128,21 +123,6 @@ __device__ __forceinline__ void meet() {
   __asm__ volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   __asm__ volatile("" ::: "memory");
-}
-
-// The largest of a wave's values, for every lane.
-__device__ __forceinline__ int wave_max_i32(int v) {
-  auto dpp = [](int x, auto ctrl) {
-    return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, 0xf, 0xf, false);
-  };
-  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR1>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_QUAD_XOR2>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_HALF_MIRROR>{}));
-  v = max(v, dpp(v, std::integral_constant<int, DPP_ROW_MIRROR>{}));
-  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
-  v = max((int)a[0], (int)a[1]);
-  const auto b = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
-  return max((int)b[0], (int)b[1]);
 }
 
 // BS: the least block_size, 32 or 64: a tile is looked up and addressed by NP pieces
@@ -518,86 +498,6 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                               __float_as_uint(o[d][4 * a + 3] * inv)});
     }
   }
-}
-
-// The end of a part that begins at `from`, at most `end`.
-__device__ __forceinline__ int part_end(int from, int chunk, int end) {
-  return (int)min((int64_t)from + chunk, (int64_t)end);
-}
-
-// Where a workgroup stands in a launch's work: segment seg (a sequence, or the
-// prefix), item x of its tiles times parts, the segment's parts of `chunk` tokens.
-struct Place {
-  int seg, x, parts, chunk;
-};
-
-// Finds item `item` of segments whose row tiles and rounds (of ROUND tokens) seg_of
-// gives, 64 at a time, a lane each.  With max_parts > 1 every segment's tokens
-// are cut into parts of one length, the least (of at least `least` rounds) that
-// makes about `target` items of all segments and at most max_parts of any, so
-// that the workgroups are alike whatever the lengths: every workgroup derives
-// it from the lengths.  Nothing is cut where that would not save `gain` rounds of
-// the longest item (a round beside another workgroup's takes 1.45 of one alone), or
-// where the items read memory at its rate as they are (`memory`: few rows a
-// sequence): from 160 of 512 workgroups on, none 1.3 times as long as the average.  us
-// whole / cut of sequences of 5 tokens behind 5000, a fourth of them r times the
-// average: 16 (128 workgroups) r = 1 97 / 63; 20 (160) 110 / 91, behind 2500
-// 38 / 41; 29 (232) 122 / 130, r = 1.15 133 / 130, 1.3 146 / 140, 1.5 160 / 131.
-template <int ROUND, typename Seg>
-__device__ __forceinline__ bool find_item(Seg seg_of, int num_segs, int item, int target,
-                                          int max_parts, int least, float gain, bool memory,
-                                          Place& place) {
-  const int lane = threadIdx.x & 63;
-  int chunk = INT_MAX / ROUND;  // in rounds
-  int tiles0 = 0, rounds0 = 0;
-  if (lane < num_segs) seg_of(lane, tiles0, rounds0);
-  if (max_parts > 1) {
-    float work = wave_sum((float)tiles0 * (float)rounds0), all = wave_sum((float)tiles0);
-    int top = wave_max_i32(rounds0);
-    for (int b = 64; b < num_segs; b += 64) {
-      int tiles = 0, rounds = 0;
-      if (b + lane < num_segs) seg_of(b + lane, tiles, rounds);
-      work += wave_sum((float)tiles * (float)rounds);
-      all += wave_sum((float)tiles);
-      top = max(top, wave_max_i32(rounds));
-    }
-    chunk = max(max((int)fminf(ceilf(work / (float)target), 1e9f),
-                    (top + max_parts - 1) / max_parts), least);
-    const float alone = all / (float)target;
-    if ((float)top * (1.f - 1.45f * alone) < gain ||
-        (memory && alone > 0.31f && (float)top * all < 1.3f * work))
-      chunk = max(chunk, top);
-    // every segment rounds up: a little longer parts where that made too many
-    for (int i = 0; i < 3 && num_segs <= 64; ++i) {
-      const float items = wave_sum((float)tiles0 * (float)max(1, (rounds0 + chunk - 1) / chunk));
-      if (items <= (float)target || chunk >= top) break;
-      chunk = max(chunk + 1, min((int)fminf((float)chunk * items / (float)target, 1e9f), top));
-    }
-    chunk = __builtin_amdgcn_readfirstlane(chunk);
-  }
-  int done = 0;
-  for (int b = 0; b < num_segs; b += 64) {
-    int tiles = tiles0, rounds = rounds0;
-    if (b > 0) {
-      tiles = rounds = 0;
-      if (b + lane < num_segs) seg_of(b + lane, tiles, rounds);
-    }
-    const int parts = max(1, (rounds + chunk - 1) / chunk);
-    const int items = tiles * parts;
-    const int incl = wave_scan_i32(items);
-    const int total = __builtin_amdgcn_readlane(incl, 63);
-    if (item < done + total) {
-      const int i = __ffsll((unsigned long long)__ballot(done + incl > item)) - 1;
-      place.seg = b + i;
-      place.x = item - done - (__builtin_amdgcn_readlane(incl, i) -
-                               __builtin_amdgcn_readlane(items, i));
-      place.parts = __builtin_amdgcn_readlane(parts, i);
-      place.chunk = chunk * ROUND;
-      return true;
-    }
-    done += total;
-  }
-  return false;
 }
 
 // Shapes.  Rounds of 64 tokens: a workgroup of 64 rows takes 0.85 us alone on its
@@ -1045,6 +945,23 @@ int launch_prefix(hipStream_t stream, RowsArgs& a, const Choice& c) {
 }
 
 }  // namespace
+
+int merge_rows(hipStream_t stream, int head_dim, const float* part_o, const float* part_lse,
+               const int32_t* counts, void* out, const int32_t* query_start, int num_seqs,
+               int num_tokens, int n_q, int slots) {
+  RowsArgs a{};
+  a.part_o = const_cast<float*>(part_o);
+  a.part_lse = const_cast<float*>(part_lse);
+  a.counts = const_cast<int32_t*>(counts);
+  a.out = (uint16_t*)out;
+  a.query_start = query_start;
+  a.num_seqs = num_seqs;
+  a.num_tokens = num_tokens;
+  a.n_q = n_q;
+  return head_dim == 128 ? launch_merge<128>(stream, a, slots, slots, true)
+                         : launch_merge<64>(stream, a, slots, slots, true);
+}
+
 }  // namespace smx
 
 #include "smx_abi_util.h"

@@ -5,6 +5,7 @@
 // latency-cheap (one workgroup per row, vector loads, wave reductions).
 #include <math.h>
 
+#include "qknorm_rope.h"
 #include "smx_common.h"
 #include "smx_launch.h"
 
@@ -161,8 +162,8 @@ __global__ __launch_bounds__(256) void qknorm_rope_kv_vec_kernel(
     const int64_t* __restrict__ positions, const int64_t* __restrict__ slot_mapping,
     uint16_t* __restrict__ q_out, uint16_t* __restrict__ k_cache, uint16_t* __restrict__ v_cache,
     uint32_t items, int n_q, int n_kv, int64_t cache_slots, int max_position, float eps) {
-  constexpr int HD = 128, HALF = 64;
-  const int j = threadIdx.x & 15, dim = 8 * (j & 7);
+  constexpr int HD = 128;
+  const int j = threadIdx.x & 15;
   const uint32_t raw = blockIdx.x * 16u + (threadIdx.x >> 4);
   // lanes past the end work on the last item (the row moves below need every
   // lane) and store nothing
@@ -170,44 +171,9 @@ __global__ __launch_bounds__(256) void qknorm_rope_kv_vec_kernel(
   const uint32_t nh = (uint32_t)(n_q + 2 * n_kv);
   const uint32_t t = item / nh;
   const int h = (int)(item - t * nh);
-  const u32x4 own = *reinterpret_cast<const u32x4*>(qkv + (int64_t)item * HD + 8 * j);
   const int64_t slot = slot_mapping[t];
-  int64_t pos = positions[t];
-  const uint16_t* gam = h < n_q ? q_gamma : k_gamma;
-  const u32x4 gv = *reinterpret_cast<const u32x4*>(gam + 8 * j);
-  pos = pos < 0 ? 0 : (pos >= max_position ? max_position - 1 : pos);
-  const u32x4 cv = *reinterpret_cast<const u32x4*>(cos_sin + pos * HD + dim);
-  const u32x4 sv = *reinterpret_cast<const u32x4*>(cos_sin + pos * HD + HALF + dim);
-  auto other_half = [](uint32_t v) {  // lane j ^ 8's register
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, DPP_ROW_ROR8, 0xf, 0xf, false);
-  };
-  u32x4 val = own;
-  // (every head of a wave is a V head, or all lanes stay: the row moves need them)
-  if (__builtin_amdgcn_ballot_w64(h < n_q + n_kv) != 0) {
-    const bool lo = j < 8;
-    float sq[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t p = other_half(own[i]);
-      const uint32_t aw = lo ? own[i] : p, bw = lo ? p : own[i];
-      sq[2 * i] = bf16_lo(aw) * bf16_lo(aw) + bf16_lo(bw) * bf16_lo(bw);
-      sq[2 * i + 1] = bf16_hi(aw) * bf16_hi(aw) + bf16_hi(bw) * bf16_hi(bw);
-    }
-    const float ss = sum8(((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7])));
-    const float inv = 1.0f / sqrtf(ss / (float)HD + eps);
-    const uint32_t flip = lo ? 0x80008000u : 0u;  // u = a c - b s, v = b c + a s
-    uint32_t r[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // the rounded norm of this half, and the other half's from lane j ^ 8
-      const uint32_t nw = pack_bf16x2(bf16_lo(own[i]) * inv * bf16_lo(gv[i]),
-                                      bf16_hi(own[i]) * inv * bf16_hi(gv[i]));
-      const uint32_t ow = other_half(nw), sw = sv[i] ^ flip;
-      r[i] = pack_bf16x2(fmaf(bf16_lo(nw), bf16_lo(cv[i]), bf16_lo(ow) * bf16_lo(sw)),
-                         fmaf(bf16_hi(nw), bf16_hi(cv[i]), bf16_hi(ow) * bf16_hi(sw)));
-    }
-    if (h < n_q + n_kv) val = u32x4{r[0], r[1], r[2], r[3]};
-  }
+  const u32x4 val = qknorm_rope_chunk(qkv + (int64_t)item * HD, h < n_q ? q_gamma : k_gamma,
+                                      cos_sin, positions[t], h < n_q + n_kv, j, max_position, eps);
   const bool write_kv = slot >= 0 && slot < cache_slots;
   uint16_t* dst;
   if (h < n_q) {

@@ -896,6 +896,429 @@ def release_pages(keep_lens: torch.Tensor, num_pages: torch.Tensor, free_pages: 
          free_pages.numel(), block_size)
 
 
+class Q4KVCache:
+    """A paged KV cache held in 4 bits (smx_q4_reshape_and_cache): blocks of 32 channels of
+    a token's head share an fp16 scale d and hold codes of 0..15 for d * (code - 8).
+      codes   uint8 [2, num_blocks, n_kv, block_size, head_dim / 2], K first
+      scales  fp16 [2, num_blocks, n_kv, block_size, head_dim / 32]
+    4.5 bits a value.  The order of a row's codes is the kernels' own: q4_kv_read gives
+    the values."""
+
+    __slots__ = ("codes", "scales", "num_blocks", "n_kv", "block_size", "head_dim", "index")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        _check(codes, "codes", torch.uint8)
+        _need(codes.dim() == 5 and codes.shape[0] == 2,
+              "codes must be [2, num_blocks, n_kv, block_size, head_dim / 2]")
+        _, self.num_blocks, self.n_kv, self.block_size, half = codes.shape
+        self.head_dim = 2 * half
+        _need(self.head_dim in (64, 128), "head_dim must be 64 or 128")
+        _check(scales, "scales", torch.float16, device=codes.device)
+        _need(scales.shape == (*codes.shape[:4], half // 16),
+              "scales must be [2, num_blocks, n_kv, block_size, head_dim / 32]")
+        self.codes, self.scales, self.index = codes, scales, codes.get_device()
+
+    def planes(self) -> list[torch.Tensor]:
+        """The tensors of a PageSet(page_dim=1)."""
+        return [self.codes, self.scales]
+
+
+def q4_kv_cache(num_blocks: int, block_size: int, n_kv: int, head_dim: int,
+                device) -> Q4KVCache:
+    """An empty cache in 4 bits."""
+    _need(min(num_blocks, n_kv) >= 1, "num_blocks and n_kv must be >= 1")
+    _need(32 <= block_size <= 4096 and block_size & (block_size - 1) == 0,
+          "block_size must be a power of two in [32, 4096]")
+    _need(head_dim in (64, 128), "head_dim must be 64 or 128")
+    shape = (2, num_blocks, n_kv, block_size)
+    return Q4KVCache(torch.zeros((*shape, head_dim // 2), dtype=torch.uint8, device=device),
+                     torch.zeros((*shape, head_dim // 32), dtype=torch.float16, device=device))
+
+
+def _q4_cache(cache, index: int) -> Q4KVCache:
+    if not isinstance(cache, Q4KVCache):
+        raise ValueError("cache must be a Q4KVCache")
+    if cache.index != index:
+        raise ValueError("the cache must be on the other tensors' device")
+    return cache
+
+
+def reshape_and_cache_q4(key: torch.Tensor, value: torch.Tensor, cache: Q4KVCache,
+                         slot_mapping: torch.Tensor) -> None:
+    """reshape_and_cache into a cache in 4 bits.  key, value [tokens, n_kv, hd]: a token's
+    heads are contiguous, tokens may be strided (a slice of the QKV rows)."""
+    _need(isinstance(slot_mapping, torch.Tensor), "slot_mapping must be a tensor")
+    i = slot_mapping.get_device()
+    c = _q4_cache(cache, i)
+    _check(slot_mapping, "slot_mapping", torch.int64)
+    tokens = slot_mapping.numel()
+    steps = []
+    for t, name in ((key, "key"), (value, "value")):
+        if not (isinstance(t, torch.Tensor) and t.dtype is BF16 and t.get_device() == i):
+            raise ValueError(f"{name} must be a bf16 tensor on slot_mapping's device")
+        if tuple(t.shape) != (tokens, c.n_kv, c.head_dim):
+            raise ValueError(f"{name} must be [tokens, n_kv, head_dim]")
+        step, head_step, unit = t.stride()
+        if not (unit == 1 and (c.n_kv == 1 or head_step == c.head_dim)):
+            raise ValueError(f"a token's heads must be contiguous in {name}")
+        if tokens <= 1:
+            step = c.n_kv * c.head_dim
+        if step < c.n_kv * c.head_dim or step % 8 or t.data_ptr() % 16:
+            raise ValueError(f"{name}'s tokens must be apart and 16-byte aligned")
+        steps.append(step)
+    if tokens == 0:
+        return
+    call("smx_q4_reshape_and_cache", _stream(slot_mapping), key.data_ptr(), steps[0],
+         value.data_ptr(), steps[1], c.codes.data_ptr(), c.scales.data_ptr(),
+         slot_mapping.data_ptr(), tokens, c.n_kv, c.head_dim, c.num_blocks, c.block_size)
+
+
+def q4_kv_read(cache: Q4KVCache, slot_mapping: torch.Tensor,
+               out: tuple[torch.Tensor, torch.Tensor] | None = None):
+    """The (key, value) that a cache in 4 bits holds for the tokens at slot_mapping, exactly:
+    fp32 [tokens, n_kv, hd]; 0 for slots outside it."""
+    _check(slot_mapping, "slot_mapping", torch.int64)
+    c = _q4_cache(cache, slot_mapping.get_device())
+    shape = (slot_mapping.numel(), c.n_kv, c.head_dim)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=torch.float32, device=slot_mapping.device)
+                    for _ in range(2))
+    n = shape[0] * shape[1] * shape[2]
+    for t, name in zip(out, ("out[0]", "out[1]")):
+        _check(t, name, torch.float32, n, slot_mapping.device)
+    if n:
+        call("smx_q4_kv_read", _stream(slot_mapping), c.codes.data_ptr(), c.scales.data_ptr(),
+             slot_mapping.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), *shape, c.num_blocks,
+             c.block_size)
+    return out
+
+
+def qknorm_rope_kv_write_q4(qkv: torch.Tensor, q_gamma: torch.Tensor, k_gamma: torch.Tensor,
+                            cos_sin: torch.Tensor, positions: torch.Tensor,
+                            slot_mapping: torch.Tensor, cache: Q4KVCache, n_q: int, n_kv: int,
+                            eps: float, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """qknorm_rope_kv_write into a cache in 4 bits."""
+    _check(positions, "positions", torch.int64)
+    dev = positions.device
+    c = _q4_cache(cache, positions.get_device())
+    _need(c.n_kv == n_kv, "cache kv-head count mismatch")
+    hd, num_tokens = c.head_dim, positions.numel()
+    _check(qkv, "qkv", BF16, num_tokens * (n_q + 2 * n_kv) * hd, dev)
+    _check(q_gamma, "q_gamma", BF16, hd, dev)
+    _check(k_gamma, "k_gamma", BF16, hd, dev)
+    _check(cos_sin, "cos_sin", BF16, device=dev)
+    _need(cos_sin.dim() == 2 and cos_sin.shape[1] == hd, "cos_sin must be [max_position, head_dim]")
+    _check(slot_mapping, "slot_mapping", torch.int64, num_tokens, dev)
+    if q_out is None:
+        q_out = torch.empty((num_tokens, n_q, hd), dtype=BF16, device=dev)
+    _check(q_out, "q_out", BF16, num_tokens * n_q * hd, dev)
+    call("smx_q4_qknorm_rope_kv_write", _stream(positions), qkv.data_ptr(), q_gamma.data_ptr(),
+         k_gamma.data_ptr(), cos_sin.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(),
+         q_out.data_ptr(), c.codes.data_ptr(), c.scales.data_ptr(), num_tokens, n_q, n_kv, hd,
+         c.num_blocks, c.block_size, cos_sin.shape[0], float(eps))
+    return q_out
+
+
+def q4_attention_workspace(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
+                           query_start_loc: torch.Tensor | None = None) -> torch.Tensor | None:
+    """The workspace q4_attention uses for these sizes (uint8; None where it uses none).
+    Calls that can overlap need one each."""
+    return _workspace(load().smx_q4_attention_workspace(
+        q.shape[0], block_table.shape[0], block_table.shape[1], cache.block_size, q.shape[1],
+        cache.n_kv, cache.head_dim), q.device)
+
+
+def q4_attention(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
+                 seq_lens: torch.Tensor, scale: float,
+                 query_start_loc: torch.Tensor | None = None,
+                 workspace: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """prompt_attention over a cache in 4 bits: sequence r's queries are the rows
+    query_start_loc[r]..query_start_loc[r + 1] of q [tokens, n_q, hd] (tokens may be
+    strided), the last of its seq_lens[r] tokens.  Without query_start_loc row r is
+    sequence r's newest token: a decode step.  Rows of no sequence are left as they are
+    in `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
+    needs it."""
+    if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is BF16 and q.dim() == 3):
+        raise ValueError("q must be a bf16 GPU tensor [tokens, n_q, hd]")
+    tokens, n_q, hd = q.shape
+    step, head_step, unit = q.stride()
+    if tokens < 1 or n_q < 1:
+        raise ValueError("q must hold a token and a head")
+    if tokens == 1:
+        step = n_q * hd
+    if not (unit == 1 and (n_q == 1 or head_step == hd) and step >= n_q * hd):
+        raise ValueError("a token's heads must be contiguous in q and its tokens apart")
+    if q.data_ptr() % 16 or step % 8:
+        raise ValueError("q's tokens must be 16-byte aligned")
+    i = q.get_device()
+    c = _q4_cache(cache, i)
+    if hd != c.head_dim:
+        raise ValueError("head_dim mismatch between q and the cache")
+    _all_plain(i, torch.int32, block_table=block_table, seq_lens=seq_lens)
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [seqs, max_blocks]")
+    num_seqs, max_blocks = block_table.shape
+    if seq_lens.numel() != num_seqs:
+        raise ValueError("seq_lens must have an entry for each row of block_table")
+    if query_start_loc is None:
+        if tokens != num_seqs:
+            raise ValueError("without query_start_loc q must have a row for each sequence")
+    else:
+        _all_plain(i, torch.int32, query_start_loc=query_start_loc)
+        if query_start_loc.numel() != num_seqs + 1:
+            raise ValueError("query_start_loc must have num_seqs + 1 entries")
+    if out is None:
+        out = torch.empty((tokens, n_q, hd), dtype=BF16, device=q.device)
+    else:
+        _all_plain(i, BF16, out=out)
+        if out.numel() != tokens * n_q * hd:
+            raise ValueError("out must have q's elements")
+    if workspace is None:
+        workspace = q4_attention_workspace(q, c, block_table, query_start_loc)
+    else:
+        _all_plain(i, torch.uint8, workspace=workspace)
+    call("smx_q4_attention", _stream(q), q.data_ptr(), step, c.codes.data_ptr(),
+         c.scales.data_ptr(), block_table.data_ptr(), _ptr(query_start_loc), seq_lens.data_ptr(),
+         _ptr(workspace), workspace.numel() if workspace is not None else 0, out.data_ptr(),
+         tokens, num_seqs, max_blocks, c.num_blocks, c.block_size, n_q, c.n_kv, hd, float(scale))
+    return out
+
+
+class BeamSelection:
+    """What beam_select() writes, [seqs, width], the best first:
+      parents  int32: the row of logits it continues, -1 where there is none
+      tokens   int64, -1 where there is none
+      scores   fp32, -inf where there is none"""
+
+    __slots__ = ("parents", "tokens", "scores")
+
+    def __init__(self, parents, tokens, scores):
+        _check(parents, "parents", torch.int32)
+        _need(parents.dim() == 2, "parents must be [seqs, width]")
+        _check(tokens, "tokens", torch.int64, parents.numel(), parents.device)
+        _check(scores, "scores", torch.float32, parents.numel(), parents.device)
+        _need(tokens.shape == parents.shape and scores.shape == parents.shape,
+              "parents, tokens and scores must be [seqs, width]")
+        self.parents, self.tokens, self.scores = parents, tokens, scores
+
+
+def beam_select_out(seqs: int, width: int, device) -> BeamSelection:
+    """Buffers for beam_select(out=...)."""
+    return BeamSelection(torch.empty((seqs, width), dtype=torch.int32, device=device),
+                         torch.empty((seqs, width), dtype=torch.int64, device=device),
+                         torch.empty((seqs, width), dtype=torch.float32, device=device))
+
+
+def beam_select_workspace(logits: torch.Tensor, beams: int, width: int) -> torch.Tensor | None:
+    """The workspace beam_select uses for these sizes (uint8).  Calls that can overlap need
+    one each."""
+    return _workspace(load().smx_beam_select_workspace(
+        logits.shape[0] // max(beams, 1), beams, width, logits.shape[1], logits.element_size()),
+        logits.device)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, width: int,
+                done: torch.Tensor | None = None, pad_id: int = 0,
+                workspace: torch.Tensor | None = None,
+                out: BeamSelection | None = None) -> BeamSelection:
+    """The `width` best continuations of each sequence's `beams` rows of logits [seqs *
+    beams, vocab] (bf16 or fp32; rows may be strided) by scores[row] + log softmax(logits
+    [row]), scores fp32 [rows]: in order, ties to the lowest beam and token.  Logits of
+    -inf and NaN are never chosen, rows whose score is -inf offer nothing.  A row that is
+    done (bool [rows]) offers pad_id at its own score.  Without `workspace`
+    (beam_select_workspace) one is allocated."""
+    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dim() == 2
+            and logits.dtype in (BF16, torch.float32)):
+        raise ValueError("logits must be a bf16 or fp32 GPU tensor [rows, vocab]")
+    rows, vocab = logits.shape
+    step, unit = logits.stride()
+    if not (1 <= beams <= 64 and 1 <= width <= 64):
+        raise ValueError("beams and width must be in [1, 64]")
+    if rows < 1 or rows % beams or vocab < 1:
+        raise ValueError("logits must have `beams` rows for each sequence")
+    if rows == 1:
+        step = vocab
+    if not ((unit == 1 or vocab == 1) and step >= vocab):
+        raise ValueError("a row's logits must be contiguous and rows apart")
+    i = logits.get_device()
+    _all_plain(i, torch.float32, scores=scores)
+    if scores.numel() != rows:
+        raise ValueError("scores must have an entry for each row of logits")
+    if done is not None:
+        _all_plain(i, torch.bool, done=done)
+        if done.numel() != rows:
+            raise ValueError("done must have an entry for each row of logits")
+    if not 0 <= pad_id < vocab:
+        raise ValueError("pad_id must be a token")
+    if out is None:
+        out = beam_select_out(rows // beams, width, logits.device)
+    elif not (isinstance(out, BeamSelection) and out.parents.shape == (rows // beams, width)
+              and out.parents.get_device() == i):
+        raise ValueError("out must be a BeamSelection of these sequences and width")
+    if workspace is None:
+        workspace = beam_select_workspace(logits, beams, width)
+    else:
+        _all_plain(i, torch.uint8, workspace=workspace)
+    call("smx_beam_select", _stream(logits), logits.data_ptr(), step, logits.element_size(),
+         scores.data_ptr(), _ptr(done), workspace.data_ptr(), workspace.numel(),
+         out.parents.data_ptr(), out.tokens.data_ptr(), out.scores.data_ptr(), rows // beams,
+         beams, width, vocab, pad_id)
+    return out
+
+
+class ForkedPages:
+    """What fork_pages() writes:
+      block_table  int32 [rows, max_blocks], -1 past a row's pages
+      num_pages    int32 [rows]
+      lens         int32 [rows]
+      free_pages   int32 [any]: the free list, -1 past its end
+      free_count   int32 [1]
+      copies       int32 [rows, 2]: (page, its copy) for copy_pages, else -1"""
+
+    __slots__ = ("block_table", "num_pages", "lens", "free_pages", "free_count", "copies")
+
+    def __init__(self, block_table, num_pages, lens, free_pages, free_count, copies):
+        _check(block_table, "block_table", torch.int32)
+        _need(block_table.dim() == 2, "block_table must be [rows, max_blocks]")
+        rows, dev = block_table.shape[0], block_table.device
+        _check(num_pages, "num_pages", torch.int32, rows, dev)
+        _check(lens, "lens", torch.int32, rows, dev)
+        _check(free_pages, "free_pages", torch.int32, device=dev)
+        _check(free_count, "free_count", torch.int32, 1, dev)
+        _check(copies, "copies", torch.int32, 2 * rows, dev)
+        self.block_table, self.num_pages, self.lens = block_table, num_pages, lens
+        self.free_pages, self.free_count, self.copies = free_pages, free_count, copies
+
+
+def fork_pages_out(block_table: torch.Tensor, free_pages: torch.Tensor) -> ForkedPages:
+    """Buffers for fork_pages(out=...) of a table and free list of these sizes."""
+    rows, dev = block_table.shape[0], block_table.device
+    i32 = dict(dtype=torch.int32, device=dev)
+    return ForkedPages(torch.empty_like(block_table), torch.empty(rows, **i32),
+                       torch.empty(rows, **i32), torch.empty_like(free_pages),
+                       torch.empty(1, **i32), torch.empty((rows, 2), **i32))
+
+
+def fork_pages(parents: torch.Tensor, lens: torch.Tensor, num_pages: torch.Tensor,
+               free_pages: torch.Tensor, free_count: torch.Tensor, block_table: torch.Tensor,
+               num_blocks: int, block_size: int, out: ForkedPages | None = None) -> ForkedPages:
+    """Block tables of the rows that a step goes on with: new row j continues the first
+    lens[parents[j]] tokens of old row parents[j] (outside the rows: it is empty).  Rows of
+    one parent share its pages, but for a last page that is not full: the first child keeps
+    it, the others get pages from the end of the free list, into which copy_pages(...,
+    copies) copies it before they are written.  Pages that no new row lists are free again.
+    A row whose copy finds no page is cut to its whole pages (see lens).  int32 throughout;
+    `out` may hold free_pages and free_count themselves, the rest is apart from the inputs."""
+    reqs, max_blocks, i = _pages_checks(num_pages, free_pages, free_count, block_table, lens,
+                                        "lens")
+    _all_plain(i, torch.int32, parents=parents)
+    if parents.numel() != reqs:
+        raise ValueError("parents must have an entry for each row of block_table")
+    if out is None:
+        out = fork_pages_out(block_table, free_pages)
+    elif not (isinstance(out, ForkedPages) and out.block_table.shape == block_table.shape
+              and out.free_pages.numel() == free_pages.numel()
+              and out.block_table.get_device() == i):
+        raise ValueError("out must be ForkedPages of this table and free list")
+    call("smx_fork_pages", _stream(num_pages), parents.data_ptr(), lens.data_ptr(),
+         num_pages.data_ptr(), free_pages.data_ptr(), free_count.data_ptr(),
+         block_table.data_ptr(), out.block_table.data_ptr(), out.num_pages.data_ptr(),
+         out.lens.data_ptr(), out.free_pages.data_ptr(), out.free_count.data_ptr(),
+         out.copies.data_ptr(), reqs, max_blocks, num_blocks, free_pages.numel(), block_size)
+    return out
+
+
+class CompactedPages:
+    """What compact_pages() writes:
+      block_table  int32 [rows, max_blocks], -1 past a row's pages
+      free_pages   int32 [num_blocks]: the free list, -1 past its end
+      free_count   int32 [1]
+      moves        int32 [num_blocks // 2, 2]: (from, to) for copy_pages, then -1"""
+
+    __slots__ = ("block_table", "free_pages", "free_count", "moves")
+
+    def __init__(self, block_table, free_pages, free_count, moves):
+        _check(block_table, "block_table", torch.int32)
+        _need(block_table.dim() == 2, "block_table must be [rows, max_blocks]")
+        dev = block_table.device
+        _check(free_pages, "free_pages", torch.int32, device=dev)
+        _check(free_count, "free_count", torch.int32, 1, dev)
+        _check(moves, "moves", torch.int32, free_pages.numel() // 2 * 2, dev)
+        self.block_table, self.free_pages = block_table, free_pages
+        self.free_count, self.moves = free_count, moves
+
+
+def compact_pages(num_pages: torch.Tensor, block_table: torch.Tensor, num_blocks: int,
+                  out: CompactedPages | None = None) -> CompactedPages:
+    """Moves the pages that block_table's rows list (each its num_pages first entries; rows
+    may share pages) to the front of the pool: the table with the new places, the free
+    list of all pages behind them, and the moves for copy_pages, which must be done before
+    the table is used.  `out` may hold block_table itself."""
+    _need(isinstance(num_pages, torch.Tensor), "num_pages must be a tensor")
+    i = num_pages.get_device()
+    _all_plain(i, torch.int32, num_pages=num_pages, block_table=block_table)
+    rows = num_pages.numel()
+    if not (block_table.dim() == 2 and block_table.shape[0] == rows >= 1
+            and block_table.shape[1] >= 1):
+        raise ValueError("block_table must be [rows, max_blocks]")
+    _need(num_blocks >= 2, "num_blocks must be >= 2")
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=num_pages.device)
+        out = CompactedPages(torch.empty_like(block_table), torch.empty(num_blocks, **i32),
+                             torch.empty(1, **i32), torch.empty((num_blocks // 2, 2), **i32))
+    elif not (isinstance(out, CompactedPages) and out.block_table.shape == block_table.shape
+              and out.free_pages.numel() == num_blocks and out.block_table.get_device() == i):
+        raise ValueError("out must be CompactedPages of this table and num_blocks")
+    call("smx_compact_pages", _stream(num_pages), num_pages.data_ptr(), block_table.data_ptr(),
+         out.block_table.data_ptr(), out.free_pages.data_ptr(), out.free_count.data_ptr(),
+         out.moves.data_ptr(), rows, block_table.shape[1], num_blocks)
+    return out
+
+
+class PageSet:
+    """The caches whose pages copy_pages copies together: tensors on one GPU whose
+    dimension page_dim counts the pages ([2, num_blocks, ...] caches: 1), as many in each.
+    Built once; it keeps the tensors."""
+
+    __slots__ = ("tensors", "planes", "num_planes", "page_bytes", "num_blocks", "index")
+
+    def __init__(self, tensors: list[torch.Tensor], page_dim: int = 1):
+        _need(len(tensors) >= 1, "there must be a tensor")
+        planes, self.num_blocks = [], None
+        for n, t in enumerate(tensors):
+            _need(isinstance(t, torch.Tensor), f"tensors[{n}] must be a tensor")
+            _check(t, f"tensors[{n}]", t.dtype, device=tensors[0].device)
+            _need(0 <= page_dim < t.dim() and t.numel() > 0,
+                  f"tensors[{n}] must have pages in dimension {page_dim}")
+            pages = t.shape[page_dim]
+            self.num_blocks = pages if self.num_blocks is None else self.num_blocks
+            _need(pages == self.num_blocks, "the tensors must have as many pages each")
+            size = t.element_size() * t.stride(page_dim)
+            _need(size % 16 == 0 and t.data_ptr() % 16 == 0,
+                  f"tensors[{n}]'s pages must be whole and aligned 16 bytes")
+            count = t.numel() * t.element_size() // (size * pages)
+            planes += [[t.data_ptr() + k * size * pages, size] for k in range(count)]
+        self.tensors = list(tensors)
+        self.planes = torch.tensor(planes, dtype=torch.int64).to(tensors[0].device)
+        self.num_planes, self.page_bytes = len(planes), max(b for _, b in planes)
+        self.index = tensors[0].get_device()
+
+
+def copy_pages(pages: PageSet, pairs: torch.Tensor) -> None:
+    """Copies page src to page dst of every cache of `pages` for each row (src, dst) of
+    pairs (int32 [n, 2]); rows with an entry outside the pool are skipped.  No page may be
+    the dst of two rows, or the dst of one and the src of another."""
+    if not isinstance(pages, PageSet):
+        raise ValueError("pages must be a PageSet")
+    _all_plain(pages.index, torch.int32, pairs=pairs)
+    if not (pairs.dim() == 2 and pairs.shape[1] == 2):
+        raise ValueError("pairs must be [n, 2]")
+    if pairs.shape[0]:
+        call("smx_copy_pages", _stream(pairs), pages.planes.data_ptr(), pages.num_planes,
+             pages.page_bytes, pairs.data_ptr(), pairs.shape[0], pages.num_blocks)
+
+
 class PackedQ4_0:
     """A Q4_0 matrix in the packed layout of the MFMA GEMMs (smx_q4_0_repack):
     ``data`` uint8 [packed_bytes], the [n, k] matrix it holds (gated: the

@@ -1,0 +1,292 @@
+"""Attention over a KV cache held in 4 bits (torch_ops.q4_attention) against float64
+attention over the values that it holds."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from _rows import FP32, U, attend64
+from _util import pkg
+from oracle import q4_kv
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+
+
+def _ops():
+    return pkg("native.torch_ops")
+
+
+class Case:
+    """Random inputs on the CPU: q, a cache of N(0, 1) values, table, start, lens."""
+
+    def __init__(self, seed, n, ctx, n_q, n_kv, hd, bs, pad=0, spare=1):
+        g = torch.Generator().manual_seed(seed)
+        lens = [a + b for a, b in zip(n, ctx)]
+        per = -(-max(max(lens), 1) // bs) + spare
+        blocks = len(n) * per + 3
+        kv = torch.randn((2, blocks, n_kv, bs, hd), generator=g).to(BF16).float().numpy()
+        cd = [q4_kv.quantise(kv[i]) for i in range(2)]
+        self.codes = torch.from_numpy(np.stack([q4_kv.pack(c, i == 0)
+                                                for i, (c, _) in enumerate(cd)]))
+        self.scales = torch.from_numpy(np.stack([d for _, d in cd]))
+        self.q = torch.randn((sum(n) + pad, n_q, hd), generator=g).to(BF16)
+        self.table = torch.randperm(blocks, generator=g)[:len(n) * per].to(torch.int32).view(
+            len(n), per)
+        self.start = torch.tensor([sum(n[:i]) for i in range(len(n) + 1)], dtype=torch.int32)
+        self.lens = torch.tensor(lens, dtype=torch.int32)
+        self.scale = 1 / math.sqrt(hd)
+
+    def run(self, decode=False, **kw):
+        q, codes, scales, table, lens, start = (x.cuda() for x in (
+            self.q, self.codes, self.scales, self.table, self.lens, self.start))
+        return _ops().q4_attention(q, _ops().Q4KVCache(codes, scales), table, lens, self.scale,
+                                   query_start_loc=None if decode else start, **kw)
+
+    def reference(self):
+        """(out, sum p |v|, sum p |d|, row is of a sequence)"""
+        codes, scales = self.codes.numpy(), self.scales.numpy()
+        k, v = (torch.from_numpy(q4_kv.plane_values(codes, scales, i)) for i in range(2))
+        d = torch.from_numpy(np.repeat(scales[1].astype(np.float64), 32, -1).transpose(0, 2, 1, 3))
+        bs = k.shape[1]
+        cap = self.table.shape[1] * bs
+        out, mag, unit = (torch.zeros(self.q.shape, dtype=torch.float64) for _ in range(3))
+        mine = torch.zeros(self.q.shape[0], dtype=torch.bool)
+        for r in range(len(self.lens)):
+            a, b = (min(int(self.start[r + i]), self.q.shape[0]) for i in range(2))
+            if b <= a:
+                continue
+            mine[a:b] = True
+            L = min(max(int(self.lens[r]), 0), cap)
+            if L == 0:
+                continue
+            seen = torch.arange(L)[None] <= torch.arange(L - (b - a), L)[:, None]
+            kk, vv, dd = (x[self.table[r, :-(-L // bs)].long()].flatten(0, 1)[:L]
+                          for x in (k, v, d))
+            out[a:b], mag[a:b] = attend64(self.q[a:b].double(), kk, vv, self.scale, seen)
+            unit[a:b] = attend64(self.q[a:b].double(), kk, dd, self.scale, seen)[1]
+        return out, mag, unit, mine
+
+    def check(self, got, what="", rows=None):
+        """The output's rounding to bf16 and the weights' (U), what fp32 adds to the scores
+        (FP32; a score's products are of 16 + code, below 31, where _rows counts |v|, and
+        sums of 32 in one instruction), and to sums of weights times 16 + code, up to 31
+        times the weight's scale: one for every 32 tokens of a wave's quarter of them
+        and 8 to join, half a step of fp32 (2^-24) doubled for the products inside."""
+        ref, mag, unit, mine = self.reference()
+        got = got.double().cpu()
+        rows = mine if rows is None else rows
+        assert torch.isfinite(got[rows]).all(), f"{what}: not finite"
+        chain = int(self.lens.max().clamp(min=0)) / 32 + 8
+        bound = (U * ref.abs() + (U + FP32) * mag + 31 * 2.0 ** -23 * chain * unit + 1e-30)
+        over = ((got - ref).abs() / bound)[rows]
+        assert over.numel() == 0 or over.max() <= 1.0, f"{what}: {over.max():.3g} of the bound"
+
+
+CASES = [
+    # n, ctx, n_q, n_kv, hd, bs, pad
+    ([1], [0], 4, 1, 128, 32, 0),
+    ([1], [0], 1, 1, 64, 32, 0),
+    ([1], [512], 32, 8, 128, 128, 0),
+    ([1, 1, 1, 1], [0, 31, 63, 64], 32, 8, 128, 32, 0),
+    ([1, 1, 1], [255, 256, 5000], 14, 2, 64, 64, 0),
+    ([17], [0], 32, 8, 128, 128, 0),
+    ([33, 1, 0, 65, 2], [0, 0, 0, 0, 0], 8, 2, 128, 32, 7),
+    ([0, 0, 5], [3, 0, 1], 6, 6, 64, 32, 1),
+    ([200], [0], 14, 2, 64, 32, 0),
+    ([130], [71], 10, 2, 128, 64, 0),
+    ([5, 5, 5], [100, 641, 1003], 32, 8, 128, 128, 0),
+    ([1, 1, 1, 1], [0, 31, 32, 900], 32, 8, 128, 128, 2),
+    ([3], [2000], 8, 1, 128, 256, 0),
+    ([77, 130], [64, 0], 40, 8, 128, 128, 0),
+    ([257], [0], 64, 1, 64, 32, 0),
+    ([9], [500], 100, 1, 64, 64, 0),
+    ([2], [300], 34, 2, 128, 4096, 0),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
+def test_matches_float64(case):
+    n, ctx, n_q, n_kv, hd, bs, pad = case
+    print(f"case {case}", flush=True)
+    c = Case(1, n, ctx, n_q, n_kv, hd, bs, pad)
+    out = torch.full(c.q.shape, 7.0, dtype=BF16, device="cuda")
+    assert c.run(out=out) is out
+    mine = c.reference()[3]
+    assert torch.equal(out.cpu()[~mine], torch.full_like(c.q[~mine], 7.0)), "rows of no sequence"
+    c.check(out, str(case))
+
+
+@pytest.mark.parametrize("ctx,n_q,n_kv,hd,bs", [([0], 4, 1, 128, 32), ([513], 32, 8, 128, 128),
+                                                ([0, 77, 3000, 255, 256], 32, 8, 128, 64),
+                                                ([40] * 70, 7, 1, 64, 32),
+                                                ([9000, 1], 16, 16, 64, 128)])
+def test_decode_steps(ctx, n_q, n_kv, hd, bs):
+    """Without query_start_loc: one row a sequence, the same as with it."""
+    print(len(ctx), n_q, n_kv, hd, bs, flush=True)
+    c = Case(3, [1] * len(ctx), ctx, n_q, n_kv, hd, bs)
+    got = c.run(decode=True)
+    c.check(got)
+    assert torch.equal(got, c.run())
+
+
+def test_rows_that_see_nothing_are_zero():
+    """seq_lens below the number of query tokens (and 0, and negative)."""
+    c = Case(4, [3, 2, 1, 4], [0, 0, 0, 0], 8, 2, 64, 32)
+    c.lens = torch.tensor([1, 0, -5, 2], dtype=torch.int32)
+    got = c.run()
+    c.check(got)
+    for row in (0, 1, 3, 4, 5, 6, 7):
+        assert not got[row].any()
+    assert got[2].any() and got[9].any()
+
+
+@pytest.mark.parametrize("n,ctx", [([1], [40]), ([6], [90]), ([40], [30])])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_what_is_not_seen_does_not_count(n, ctx, hd):
+    """NaN and infinite scales and any codes behind the last token of a page, on pages that no
+    sequence lists and at later tokens of other rows' pages."""
+    c = Case(5, n + [2], ctx + [3], 8, 2, hd, 32)
+    clean = c.run()
+    bs = 32
+    for r in range(2):
+        L = int(c.lens[r])
+        for b in range(c.table.shape[1]):
+            lo = max(0, min(bs, L - b * bs))
+            page = int(c.table[r, b])
+            c.scales[:, page, :, lo:] = math.nan if b % 2 else math.inf
+            c.codes[:, page, :, lo:] = 0xff
+    listed = set(c.table.flatten().tolist())
+    for page in range(c.codes.shape[1]):
+        if page not in listed:
+            c.scales[:, page] = math.nan
+    assert torch.equal(clean.view(torch.int16), c.run().view(torch.int16))
+
+
+def test_later_tokens_do_not_reach_earlier_rows():
+    """A prompt whose last token's K and V are NaN: only the row that sees it is NaN."""
+    c = Case(6, [50], [0], 4, 1, 128, 32)
+    page, at = int(c.table[0, 49 // 32]), 49 % 32
+    for plane in range(2):
+        save = c.scales[plane, page, :, at].clone()
+        c.scales[plane, page, :, at] = math.nan
+        got = c.run().cpu()
+        assert got[49].isnan().all()
+        assert torch.isfinite(got[:49]).all()
+        c.scales[plane, page, :, at] = save
+
+
+@pytest.mark.parametrize("bad", [-1, 10 ** 6])
+def test_entries_outside_the_cache(bad):
+    """Rows that see a token whose table entry is outside the cache are NaN, the others are
+    what they were."""
+    c = Case(7, [100, 3], [0, 60], 8, 2, 128, 32)
+    clean = c.run().cpu()
+    c.table[0, 2] = bad  # tokens 64..95
+    c.table[1, 2:] = bad  # (entries past the length are not looked at)
+    c.lens[1] = 63
+    c.lens[1] = 64
+    got = c.run().cpu()
+    assert got[64:100].isnan().all()
+    assert torch.equal(got[:64], clean[:64])
+    assert torch.isfinite(got[100:]).all()
+
+
+def test_strided_queries_and_streams():
+    """Queries as a slice of the QKV rows; a call on another stream."""
+    c = Case(8, [5, 20], [100, 0], 8, 2, 64, 32)
+    want = c.run()
+    wide = torch.zeros((25, 12, 64), dtype=BF16, device="cuda")
+    wide[:, :8] = c.q.cuda()
+    ops = _ops()
+    cache = ops.Q4KVCache(c.codes.cuda(), c.scales.cuda())
+    args = [cache, c.table.cuda(), c.lens.cuda(), c.scale]
+    start = c.start.cuda()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.q4_attention(wide[:, :8], *args, query_start_loc=start)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_capture_with_lengths_that_change():
+    """One captured call: lengths from 0 to the capacity, whole and cut, a poisoned
+    workspace between the replays."""
+    ops = _ops()
+    c = Case(9, [1, 1, 1], [6000, 4000, 3], 32, 8, 128, 128)
+    q, table, lens = c.q.cuda(), c.table.cuda(), c.lens.cuda()
+    cache = ops.Q4KVCache(c.codes.cuda(), c.scales.cuda())
+    ws = ops.q4_attention_workspace(q, cache, table)
+    assert ws is not None
+    out = torch.empty_like(q)
+    call = lambda: ops.q4_attention(q, cache, table, lens, c.scale, workspace=ws, out=out)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for now in ([1, 2, 3], [6001, 4001, 4], [0, 64, 65], [300, 6000, 0], [5, 255, 257]):
+        c.lens = torch.tensor(now, dtype=torch.int32)
+        lens.copy_(c.lens)
+        ws.fill_(255)
+        out.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(out, str(now))
+
+
+def test_a_long_cache():
+    """Offsets past 2^31 and 2^32 bytes: pages at both ends of a cache of 5 GB of codes."""
+    ops = _ops()
+    bs, n_kv, hd = 128, 8, 128
+    blocks = 38200
+    try:
+        codes = torch.zeros((2, blocks, n_kv, bs, hd // 2), dtype=torch.uint8, device="cuda")
+        scales = torch.zeros((2, blocks, n_kv, bs, hd // 32), dtype=torch.float16, device="cuda")
+    except torch.OutOfMemoryError:
+        pytest.skip("needs 6 GB")
+    c = Case(10, [1, 1], [300, 200], 32, n_kv, hd, bs)
+    used = c.table.flatten().unique().long()
+    far = blocks - 1 - torch.arange(used.numel())  # page by page at the end
+    far[0] = 0
+    codes[:, far.cuda()] = c.codes[:, used].cuda()
+    scales[:, far.cuda()] = c.scales[:, used].cuda()
+    new = torch.zeros(c.codes.shape[1], dtype=torch.int64)
+    new[used] = far
+    cache = ops.Q4KVCache(codes, scales)
+    got = ops.q4_attention(c.q.cuda(), cache, new[c.table.long()].to(torch.int32).cuda(),
+                           c.lens.cuda(), c.scale)
+    assert torch.equal(got, c.run(decode=True))
+    # a write and a read of the last slot
+    key = torch.randn((1, n_kv, hd), device="cuda").to(BF16)
+    slot = torch.tensor([blocks * bs - 1], device="cuda")
+    ops.reshape_and_cache_q4(key, key, cache, slot)
+    small = ops.q4_kv_cache(1, bs, n_kv, hd, "cuda")
+    ops.reshape_and_cache_q4(key, key, small, slot * 0)
+    for a, b in zip(ops.q4_kv_read(cache, slot), ops.q4_kv_read(small, slot * 0)):
+        assert torch.equal(a, b)
+
+
+def test_refusals():
+    ops = _ops()
+    c = Case(11, [1, 1], [5, 9], 8, 2, 64, 32)
+    q, table, lens, start = c.q.cuda(), c.table.cuda(), c.lens.cuda(), c.start.cuda()
+    cache = ops.Q4KVCache(c.codes.cuda(), c.scales.cuda())
+    f = lambda **k: ops.q4_attention(*({**dict(q=q, cache=cache, block_table=table, seq_lens=lens,  # noqa: E731
+                                               scale=0.1), **k}.values()))
+    f()
+    bad = [dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(q=q[:, :, :32]),
+           dict(q=q.transpose(0, 1)), dict(cache=None), dict(cache=(cache.codes, cache.scales)),
+           dict(block_table=table.long()), dict(block_table=table[0]),
+           dict(block_table=table.cpu()), dict(seq_lens=lens[:1]), dict(seq_lens=lens.long()),
+           dict(q=q[:1]), dict(s=start[:2]), dict(s=start.long()), dict(s=start, w=torch.empty(4)),
+           dict(s=start, w=None, out=torch.empty_like(q)[:1])]
+    for i, change in enumerate(bad):
+        with pytest.raises(ValueError):
+            f(**change)
+            print("not refused:", i)
+    for change in (dict(scale=0.0), dict(scale=math.nan), dict(q=q[:, :7].contiguous())):
+        with pytest.raises(pkg("native").SmxError):
+            f(**change)
