@@ -72,6 +72,8 @@ struct RowsArgs {
   int zigzag;         // period of the order of the tiles (prompts)
   float gain;         // of find_item (prompts)
   float scale_log2;
+  const uint8_t* codes;    // the cache, where it is held in 4 bits (q4_cache.h)
+  const uint16_t* scales;
 };
 
 // What one workgroup computes: `rows` rows from row0 on (row -> token row / group
@@ -127,7 +129,12 @@ __device__ __forceinline__ void meet() {
 
 // BS: the least block_size, 32 or 64: a tile is looked up and addressed by NP pieces
 // of BT tokens that are within a page.
-template <int HD, int WM, int WN, int KT, int ST, int BS>
+// Q4: the cache is held in 4 bits; tiles are loaded into registers a round ahead and
+// written to LDS as bf16 values.  (These are rounded, to 8 significant bits of the 15 of d
+// (c - 8): with codes multiplied as they are, as decode steps do, the scales' products take
+// as many instructions for every row as the rest of its softmax, which would be most of
+// a prompt's time.)
+template <int HD, int WM, int WN, int KT, int ST, int BS, bool Q4 = false>
 __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
   using S = Shape<HD, WM, WN, KT, ST>;
   constexpr int KS = HD / 16, DT = HD / 32, NU = KT / 32, CH = S::CH;
@@ -211,6 +218,71 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   };
   auto stage_v = [&](lds_u32x4* dst, const int (&page)[NP], int base) {
     stage(A.vc, dst, page, base, [](int r) { return v_swz<HD>(r); });
+  };
+  // A cache in 4 bits: a lane has a quarter of a token's row, K's dwords of every block's
+  // eight channels 8 (lane & 3) .., and V's NB dwords in channel order, of one block.
+  constexpr int NB = HD / 32, RB = HD / 2;
+  uint32_t kq[NB], vq[NB], kd[NB / 2], vd = 0;
+  const int qtok = (wm * 64 + lane) >> 2, qg = lane & 3;
+  auto fetch = [&](const int (&page)[NP], int base) {
+    static_assert(!Q4 || (KT == 16 * WM && ST == 2), "a quarter of a row a lane, two buffers");
+    const int u = NP > 1 && 16 * wm >= BT ? NP - 1 : 0;
+    const int t = base + BT * u;
+    const bool known = (unsigned)page[u] < (unsigned)A.num_blocks;
+    const int rows = known ? max(min(it.to - t, BT), 0) : 0;
+    const int64_t row = (((int64_t)(known ? page[u] : 0) * A.n_kv + kvh) << A.bs_log2) +
+                        (t & (bs - 1));
+    const int64_t plane = (int64_t)A.num_blocks * A.n_kv << A.bs_log2;
+    const int at = qtok - BT * u;
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      const int64_t r = v ? row + plane : row;
+      const auto codes = __builtin_amdgcn_make_buffer_rsrc((void*)(A.codes + r * RB), 0, rows * RB,
+                                                           0x00027000);
+      const auto scales = __builtin_amdgcn_make_buffer_rsrc((void*)(A.scales + r * NB), 0,
+                                                            rows * 2 * NB, 0x00027000);
+      uint32_t* const w = v ? vq : kq;
+      if constexpr (NB == 4) {
+        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(codes, at * RB + 16 * qg, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = x[i];
+      } else {
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(codes, at * RB + 8 * qg, 0, 0);
+        w[0] = x[0];
+        w[1] = x[1];
+      }
+      if (v) {
+        vd = __builtin_amdgcn_raw_buffer_load_b16(scales, at * 2 * NB + 2 * (NB * qg / 4), 0, 0);
+      } else if constexpr (NB == 4) {
+        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(scales, at * 2 * NB, 0, 0);
+        kd[0] = x[0];
+        kd[1] = x[1];
+      } else {
+        kd[0] = __builtin_amdgcn_raw_buffer_load_b32(scales, at * 2 * NB, 0, 0);
+      }
+    }
+  };
+  // Eight values of scale d as bf16: bytes of half-bytes 0, 2, 4, 6 (lo) and 1, 3, 5, 7 (hi).
+  auto widen = [](uint32_t w, float d, bool key) -> u32x4 {
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    const float off = -8.f * d;
+    auto val = [&](uint32_t x, int i) { return fmaf((float)((x >> (8 * i)) & 0xffu), d, off); };
+    if (key)
+      return u32x4{cvt_pk_bf16(val(lo, 0), val(lo, 2)), cvt_pk_bf16(val(hi, 0), val(hi, 2)),
+                   cvt_pk_bf16(val(lo, 1), val(lo, 3)), cvt_pk_bf16(val(hi, 1), val(hi, 3))};
+    return u32x4{cvt_pk_bf16(val(lo, 0), val(hi, 0)), cvt_pk_bf16(val(lo, 1), val(hi, 1)),
+                 cvt_pk_bf16(val(lo, 2), val(hi, 2)), cvt_pk_bf16(val(lo, 3), val(hi, 3))};
+  };
+  auto fill = [&](lds_u32x4* dst) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const float d = f16_bits_to_f32(kd[b / 2] >> (16 * (b & 1)) & 0xffffu);
+      dst[qtok * CH + ((4 * b + qg) ^ k_swz<HD>(qtok))] = widen(kq[b], d, true);
+    }
+    const float d = f16_bits_to_f32(vd);
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+      dst[S::TILE + qtok * CH + ((NB * qg + j) ^ v_swz<HD>(qtok))] = widen(vq[j], d, false);
   };
   auto bad_pages = [&](const int (&page)[NP]) {
     int bad = 0;
@@ -376,12 +448,23 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   // restrict so that the compiler does not wait for the loads into the one before
   // it reads the other; the wait that counts is the one before the barrier.
   int bad[ST];  // of the tiles in LDS, that of this round first
-  int page[NP];
+  int page[NP], bad_fetched = 0;
 #pragma unroll
   for (int i = 0; i < ST; ++i) bad[i] = 0;
   look_up(page, first + wn * KT);
+  if constexpr (Q4) {
+    if (wn < ntiles) {
+      fetch(page, first + wn * KT);
+      bad[0] = bad_pages(page);
+      look_up(page, first + (wn + WN) * KT);
+      fill(lds);
+      fetch(page, first + (wn + WN) * KT);  // (past the end: of no rows, without an access)
+      bad_fetched = bad_pages(page);
+      look_up(page, first + (wn + 2 * WN) * KT);
+    }
+  }
 #pragma unroll
-  for (int i = 0; i < ST - 1; ++i) {
+  for (int i = 0; i < (Q4 ? 0 : ST - 1); ++i) {
     const int tile = i * WN + wn, base = first + tile * KT;
     if (tile < ntiles) {
       lds_u32x4* const dst = lds + i * 2 * S::TILE;
@@ -397,10 +480,18 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     // (a tile past the end is of no rows: a plain round loads nothing there, without
     // the branch that would keep the addresses' arithmetic from the products' shadow)
     if (plain || tile + (ST - 1) * WN < ntiles) {
-      stage_k(next, page, ahead);
-      stage_v(next + S::TILE, page, ahead);
-      bad[ST - 1] = bad_pages(page);
-      look_up(page, ahead + WN * KT);
+      if constexpr (Q4) {
+        fill(next);
+        bad[1] = bad_fetched;
+        fetch(page, ahead + WN * KT);
+        bad_fetched = bad_pages(page);
+        look_up(page, ahead + 2 * WN * KT);
+      } else {
+        stage_k(next, page, ahead);
+        stage_v(next + S::TILE, page, ahead);
+        bad[ST - 1] = bad_pages(page);
+        look_up(page, ahead + WN * KT);
+      }
     }
     if ((!plain && tile >= ntiles) || 32 * wm >= it.rows) return;
     scores(cur);
@@ -411,7 +502,9 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   auto step = [&](auto plain) {
     // this wave's loads of the tile have arrived (those of later ones may be on
     // their way), then every wave's have, and the last round's tile is read out
-    if (ST > 2 && (rd + ST - 2) * WN + wn < ntiles)
+    if (Q4)
+      __builtin_amdgcn_s_waitcnt(wait_vm(63));  // its writes to LDS; the next tile's loads go on
+    else if (ST > 2 && (rd + ST - 2) * WN + wn < ntiles)
       __builtin_amdgcn_s_waitcnt(wait_vm((ST - 2) * 2 * S::LOADS));
     else
       __builtin_amdgcn_s_waitcnt(wait_vm(0));
@@ -515,7 +608,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 // tokens (8 x 5 behind 300 to 8000: 20 us, 4.9 TB/s).  Sequence r's queries are the tokens [query_start[r],
 // query_start[r + 1]), the last n of its L tokens: token i of them is at position
 // L - n + i and sees the tokens up to itself.  Grid: kv heads, items.
-template <int HD, int WM, int WN, int KT, int ST, int BS>
+template <int HD, int WM, int WN, int KT, int ST, int BS, bool Q4>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
 void prompt_attention_kernel(RowsArgs A) {
   using S = Shape<HD, WM, WN, KT, ST>;
@@ -524,6 +617,10 @@ void prompt_attention_kernel(RowsArgs A) {
   const int kvh = blockIdx.x;
   const int cap = A.max_blocks << A.bs_log2;
   auto queries = [&](int r, int& s0) {
+    if (Q4 && !A.query_start) {  // row r is sequence r's one token
+      s0 = r;
+      return 1;
+    }
     s0 = min(max(A.query_start[r], 0), A.num_tokens);
     return max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
   };
@@ -579,7 +676,7 @@ void prompt_attention_kernel(RowsArgs A) {
   it.counts = split == 0 && A.splits > 1 ? A.counts : nullptr;
   it.parts = place.parts;
   it.direct = place.parts == 1;
-  attend<HD, WM, WN, KT, ST, BS>(A, it, kvh, smem);
+  attend<HD, WM, WN, KT, ST, BS, Q4>(A, it, kvh, smem);
   stores_done();
 }
 
@@ -905,7 +1002,7 @@ int64_t items_bound(int64_t tiles, int target, int splits) {
   return std::min<int64_t>(tiles * splits, target + tiles + 1);
 }
 
-template <int HD>
+template <int HD, bool Q4>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
   a.zigzag = a.num_seqs == 1 && (int64_t)c.tiles * a.n_kv <= 2 * FILL ? std::max(1, 256 / a.n_kv)
                                                                       : 1 << 30;
@@ -914,11 +1011,11 @@ int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
   a.gain = c.gain;
   const dim3 grid(a.n_kv, (unsigned)items_bound(c.tiles, c.target, c.splits));
   if (c.m == 64)
-    SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2, 32>), grid, dim3(256), 0, stream, a);
+    SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2, 32, Q4>), grid, dim3(256), 0, stream, a);
   else if (a.bs_log2 > 5)
-    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 64>), grid, dim3(256), 0, stream, a);
+    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 64, Q4>), grid, dim3(256), 0, stream, a);
   else
-    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 32>), grid, dim3(256), 0, stream, a);
+    SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 32, Q4>), grid, dim3(256), 0, stream, a);
   const int rc = (int)hipGetLastError();
   return rc || c.splits == 1 ? rc : launch_merge<HD>(stream, a, c.splits, c.splits, true);
 }
@@ -960,6 +1057,41 @@ int merge_rows(hipStream_t stream, int head_dim, const float* part_o, const floa
   a.n_q = n_q;
   return head_dim == 128 ? launch_merge<128>(stream, a, slots, slots, true)
                          : launch_merge<64>(stream, a, slots, slots, true);
+}
+
+int64_t q4_prompt_workspace(const Q4Prompt& p) {
+  const Choice c = choose_prompt(p.num_tokens, p.num_seqs, (int64_t)p.max_blocks << p.bs_log2,
+                                 p.n_q / p.n_kv, p.n_kv);
+  if (items_bound(c.tiles, c.target, c.splits) > 65535) return -1;
+  return partial_bytes((int64_t)p.num_tokens * p.n_q, c.splits, p.head_dim);
+}
+
+int q4_prompt(hipStream_t stream, const Q4Prompt& p) {
+  const Choice c = choose_prompt(p.num_tokens, p.num_seqs, (int64_t)p.max_blocks << p.bs_log2,
+                                 p.n_q / p.n_kv, p.n_kv);
+  RowsArgs a{};
+  a.q = p.q;
+  a.codes = p.codes;
+  a.scales = p.scales;
+  a.table = p.table;
+  a.query_start = p.query_start;
+  a.seq_lens = p.seq_lens;
+  a.out = (uint16_t*)p.out;
+  set_workspace(a, p.workspace, (int64_t)p.num_tokens * p.n_q, c.splits, p.head_dim);
+  a.q_stride = p.q_stride;
+  a.num_tokens = p.num_tokens;
+  a.num_seqs = p.num_seqs;
+  a.max_blocks = p.max_blocks;
+  a.num_blocks = p.num_blocks;
+  a.bs_log2 = p.bs_log2;
+  a.n_q = p.n_q;
+  a.n_kv = p.n_kv;
+  a.group = p.n_q / p.n_kv;
+  a.splits = c.splits;
+  a.tiles = c.tiles;
+  a.scale_log2 = p.scale_log2;
+  return p.head_dim == 128 ? launch_prompt<128, true>(stream, a, c)
+                           : launch_prompt<64, true>(stream, a, c);
 }
 
 }  // namespace smx
@@ -1045,8 +1177,8 @@ extern "C" int smx_prompt_attention(void* stream, const void* q, int64_t q_strid
   a.splits = c.splits;
   a.tiles = c.tiles;
   a.scale_log2 = scale * 1.44269504088896340736f;
-  return head_dim == 128 ? smx::launch_prompt<128>((hipStream_t)stream, a, c)
-                         : smx::launch_prompt<64>((hipStream_t)stream, a, c);
+  return head_dim == 128 ? smx::launch_prompt<128, false>((hipStream_t)stream, a, c)
+                         : smx::launch_prompt<64, false>((hipStream_t)stream, a, c);
 }
 
 extern "C" int64_t smx_shared_prefix_attention_workspace(int32_t num_seqs, int32_t prefix_blocks,

@@ -517,6 +517,12 @@ struct Q4Choice {
   int rt, splits, tiles, target;
 };
 
+// Whether a call's rows are prompts': more than a tile of a sequence on average.
+bool is_prompt(int64_t num_tokens, int64_t num_seqs, int group) {
+  const char* e = tuning_env("SMX_Q4_ROWS");
+  return num_tokens * group > (e ? atoi(e) : 32) * num_seqs;
+}
+
 Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Q4Choice c{};
   const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
@@ -551,6 +557,17 @@ extern "C" int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_se
   if (num_tokens < 1 || num_seqs < 1 || max_blocks < 1 || block_size < 1 || n_kv < 1 ||
       n_q < n_kv || n_q % n_kv || head_dim < 1)
     return -1;
+  if (smx::is_prompt(num_tokens, num_seqs, n_q / n_kv)) {
+    smx::Q4Prompt p{};
+    p.num_tokens = num_tokens;
+    p.num_seqs = num_seqs;
+    p.max_blocks = max_blocks;
+    while ((1 << p.bs_log2) < block_size) ++p.bs_log2;
+    p.n_q = n_q;
+    p.n_kv = n_kv;
+    p.head_dim = head_dim;
+    return smx::q4_prompt_workspace(p);
+  }
   const smx::Q4Choice c = smx::choose_q4(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
                                          n_q / n_kv, n_kv);
   return smx::q4_workspace((int64_t)num_tokens * n_q, c.splits, head_dim);
@@ -585,6 +602,21 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
               "int arrays must be 4-byte aligned");
   SMX_REQUIRE(q_stride >= (int64_t)n_q * head_dim && q_stride % 8 == 0,
               "q_stride must be a multiple of 8 and hold n_q heads");
+  int bs_log2 = 0;
+  while ((1 << bs_log2) < block_size) ++bs_log2;
+  const float scale_log2 = scale * 1.44269504088896340736f;
+  if (smx::is_prompt(num_tokens, num_seqs, n_q / n_kv)) {
+    const smx::Q4Prompt p{(const uint16_t*)q, (const uint8_t*)codes, (const uint16_t*)scales,
+                          block_table, query_start_loc, seq_lens, workspace, out, q_stride,
+                          num_tokens, num_seqs, max_blocks, num_blocks, bs_log2, n_q, n_kv,
+                          head_dim, scale_log2};
+    const int64_t need = smx::q4_prompt_workspace(p);
+    SMX_REQUIRE(need >= 0, "too many row tiles for one launch");
+    SMX_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 &&
+                              workspace_bytes >= need),
+                "workspace must be 16-byte aligned and hold smx_q4_attention_workspace bytes");
+    return smx::q4_prompt((hipStream_t)stream, p);
+  }
   const smx::Q4Choice c = smx::choose_q4(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
                                          n_q / n_kv, n_kv);
   SMX_REQUIRE(smx::q4_items(c) <= 65535, "too many row tiles for one launch");
@@ -608,14 +640,14 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
   a.num_seqs = num_seqs;
   a.max_blocks = max_blocks;
   a.num_blocks = num_blocks;
-  while ((1 << a.bs_log2) < block_size) ++a.bs_log2;
+  a.bs_log2 = bs_log2;
   a.n_q = n_q;
   a.n_kv = n_kv;
   a.group = n_q / n_kv;
   a.splits = c.splits;
   a.target = c.target;
   a.least = 1;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.scale_log2 = scale_log2;
   const dim3 grid(n_kv, (unsigned)smx::q4_items(c));
   const auto kernel = head_dim == 128
       ? (c.rt == 1 ? smx::q4_attention_kernel<128, 1> : smx::q4_attention_kernel<128, 2>)

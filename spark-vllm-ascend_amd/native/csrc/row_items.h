@@ -19,6 +19,24 @@ int merge_rows(hipStream_t stream, int head_dim, const float* part_o, const floa
                const int32_t* counts, void* out, const int32_t* query_start, int num_seqs,
                int num_tokens, int n_q, int slots);
 
+// Packed rows of many tokens a sequence over a cache held in 4 bits, by
+// prompt_attention.hip's kernels.
+struct Q4Prompt {
+  const uint16_t* q;
+  const uint8_t* codes;
+  const uint16_t* scales;
+  const int32_t* table;
+  const int32_t* query_start;
+  const int32_t* seq_lens;
+  void* workspace;  // q4_prompt_workspace bytes
+  void* out;
+  int64_t q_stride;
+  int num_tokens, num_seqs, max_blocks, num_blocks, bs_log2, n_q, n_kv, head_dim;
+  float scale_log2;
+};
+int64_t q4_prompt_workspace(const Q4Prompt& p);  // -1: more row tiles than a launch holds
+int q4_prompt(hipStream_t stream, const Q4Prompt& p);
+
 namespace {
 
 // (lo, hi) as one v_cvt_pk_bf16_f32
