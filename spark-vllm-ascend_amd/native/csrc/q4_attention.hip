@@ -14,14 +14,19 @@
 //
 // Products are transposed, S^T = K Q^T and O^T = V^T P^T: a row (a token's q head; "row =
 // token * group + head in the group") is a column, lane 16 g + n holds row n's scores of
-// tokens 16 t + 4 g + i (i < 4) of a tile's sixteens t, and these registers are the
-// second product's operand as they stand, V's tokens being read in that order: lane j
-// of 16 addresses token 16 (j / 4) + 4 g + j % 4 of a transposing LDS read of half-bytes
-// (ds_read_b64_tr_b4: lane n gets channel n of the 16 lanes' tokens).
+// tokens 16 t + 4 g + i (t < 2, i < 4) of a tile of 32, and these registers are the
+// second product's operand as they stand, V's tokens being read in that order: lane j of
+// 16 addresses token 16 (j / 4 % 2) + 4 g + j % 4, and the lower or the upper half of a
+// block's 32 channels by j / 8, of a transposing LDS read of half-bytes
+// (ds_read_b64_tr_b4: lane n gets channel n of the 16 lanes' tokens and halves).
 //
-// A workgroup is four waves that take the tiles (64 tokens) of its part of the tokens in
-// turn, each with its own softmax and its own buffers in LDS, filled by direct loads:
-// nothing is waited for but a wave's own loads, until the four states are joined.
+// A workgroup is four waves that take the tiles of its part of the tokens in turn, each with
+// its own softmax and its own ring of tiles in LDS, filled by direct loads three tiles
+// ahead: nothing is waited for but a wave's own loads, until the four states are joined.
+//
+// Bound by memory where there are many tokens; by instructions that are not in the
+// instruction cache yet where there are few (about 30 cycles each, in every launch): the
+// code of a tile and of what is done once is kept short for that.
 #include <math.h>
 
 #include <algorithm>
@@ -47,9 +52,11 @@ typedef __attribute__((address_space(4))) int32_t constant_i32;
 
 constexpr float LAG = 8.f;        // log2 units
 constexpr float NO_REF = -3e38f;  // before the first token: below the scores of any use
-constexpr int KT = 64;            // tokens of a tile
+constexpr int KT = 32;            // tokens of a tile
 constexpr int WAVES = 4;
+constexpr int RING = 4;           // tiles of a wave in LDS
 constexpr int ROUND = KT * WAVES;
+constexpr int APART = 16;         // parts shorter than that many rounds are of one tile
 
 struct Q4Args {
   const uint16_t* q;
@@ -64,25 +71,36 @@ struct Q4Args {
   int32_t* counts;  // [rows] parts in use
   int64_t q_stride;
   int num_tokens, num_seqs, max_blocks, num_blocks, bs_log2, n_q, n_kv, group;
-  int splits, target, least;
+  int splits, target;
   float scale_log2;
+  float group_inv, target_inv, splits_inv;  // 1 / group, 1 / target, 1 / (splits - 2)
 };
 
-// Bytes of a wave's buffer: K's codes, V's codes, and their scales.
+// Bytes of a tile in LDS: K's codes, V's codes, K's scales, V's scales.
 template <int HD>
 struct Tile {
   static constexpr int NB = HD / 32;
-  static constexpr int K = KT * HD / 2, V = K, S = KT * NB * 2;
-  static constexpr int BYTES = K + V + 1024;
+  static constexpr int CODES = KT * HD / 2, SCALES = KT * NB * 2;
+  static constexpr int BYTES = 2 * (CODES + SCALES);
 };
 
 // Eight codes (the half-bytes of w) as bf16 numbers 16 + code, pairs of half-bytes j and
-// j + 4: bits 3..6 of a bf16 with exponent 4 are whole units.
-__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w) {
-  constexpr uint32_t M = 0x00780078u, E = 0x41804180u;
-  return __builtin_bit_cast(bf16x8, u32x4{((w << 3) & M) | E, ((w >> 1) & M) | E,
-                                          ((w >> 5) & M) | E, ((w >> 9) & M) | E});
-}
+// j + 4: bits 3..6 of a bf16 with exponent 4 are whole units.  The mask and the exponents
+// come in registers, of which the compiler does not know the value: as literals they
+// would make two instructions of v_and_or_b32 (three a pair of codes, not two).
+struct CodeBits {
+  uint32_t mask = 0x00780078u, one = 0x41804180u;
+  float zero = 0.f;  // likewise, for products that are one instruction with a sum only
+  __device__ __forceinline__ CodeBits() {
+    __asm__("" : "+s"(mask));
+    __asm__("" : "+v"(one));
+    __asm__("" : "+s"(zero));
+  }
+  __device__ __forceinline__ bf16x8 operator()(uint32_t w) const {
+    return __builtin_bit_cast(bf16x8, u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one,
+                                            ((w >> 5) & mask) | one, ((w >> 9) & mask) | one});
+  }
+};
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -92,13 +110,21 @@ __device__ __forceinline__ float half_of(uint32_t w, int i) {
   return (float)__builtin_bit_cast(f16x2, w)[i];
 }
 
-// What one workgroup computes: rows of 16 RT from row0 on, tokens [from, to).
+// One piece of a workgroup's work: 16 rows from row0 on, tokens [from, to), of a tile of
+// rows that `parts` workgroups share, `slot` of them before this one.
 struct Q4Item {
   const int32_t* table;
   int token0, row0, rows, from, to, slot, ahead, parts;
 };
 
-template <int HD, int RT>
+// a / c for 0 <= a < 2^24 and inv = 1 / c to a few units of the last place.
+__device__ __forceinline__ int small_div(int a, int c, float inv) {
+  int q = (int)((float)a * inv);
+  const int r = a - q * c;
+  return q + (r >= c) - (r < 0);
+}
+
+template <int HD>
 __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int kvh,
                                           uint8_t* smem) {
   using T = Tile<HD>;
@@ -106,440 +132,437 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
   constexpr int CHUNKS = RB / 16;                       // 16-byte chunks a row
   constexpr int LOADS = KT * CHUNKS / 64;               // direct loads of a K (V) tile
   constexpr int SPAN = 64 / CHUNKS;                     // tokens of one
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  constexpr int STAGE_LOADS = 1 + 2 * LOADS;
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bs = 1 << A.bs_log2;
 
-  // ---- this lane's rows
-  int lim[RT], tok[RT], head[RT];
-  bool valid[RT];
-  bf16x8 qf[RT][NB];
-  f32x4 c0[RT][NB];
-  int lim_min = it.to;
+  // ---- this lane's row (fewer than 2^24 of a sequence: the host sees to it)
+  const int row = it.row0 + n, row_tok = small_div(row, A.group, A.group_inv);
+  const bool valid = n < it.rows;
+  const int64_t tok = it.token0 + row_tok;
+  const int head = kvh * A.group + row - row_tok * A.group;
+  u32x4 qx[NB];
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = it.row0 + 16 * r + n;
-    valid[r] = 16 * r + n < it.rows;
-    tok[r] = it.token0 + row / A.group;
-    head[r] = kvh * A.group + row % A.group;
-    lim[r] = it.to;
-    if (valid[r]) lim[r] = min(max(it.ahead + row / A.group + 1, 0), it.to);
-    lim_min = min(lim_min, lim[r]);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      u32x4 x = {0u, 0u, 0u, 0u};
-      if (valid[r])
-        x = *reinterpret_cast<const u32x4*>(A.q + (int64_t)tok[r] * A.q_stride + head[r] * HD +
-                                            32 * b + 8 * g);
-      qf[r][b] = __builtin_bit_cast(bf16x8, x);
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) sum += bf16_lo(x[i]) + bf16_hi(x[i]);
-      sum = -24.f * xor_sum<32>(xor_sum<16>(sum));
-      c0[r][b] = f32x4{sum, sum, sum, sum};
-    }
+  for (int b = 0; b < NB; ++b) {
+    qx[b] = u32x4{0u, 0u, 0u, 0u};
+    if (valid)
+      qx[b] = *reinterpret_cast<const u32x4*>(A.q + tok * A.q_stride + head * HD + 32 * b + 8 * g);
   }
-  lim_min = __builtin_amdgcn_readfirstlane(-wave_max_i32(-lim_min));
+  const int lim = valid ? min(max(it.ahead + row_tok + 1, 0), it.to) : it.to;
+  const int lim_min = __builtin_amdgcn_readfirstlane(-wave_max_i32(-lim));
 
   // ---- direct loads of a tile.  LDS is filled in the lanes' order, 16 bytes each; which
   // 16 bytes those are is the lane's choice: chunk c of token t is put in place
   // c ^ swizzle(t) of its row, so that the lanes of one LDS read are on different banks.
   // A table entry outside the cache is read as page 0 (its tokens' scores become NaN),
   // and tokens past the end are the rest of their page.
-  const int ntiles = it.to > it.from ? (it.to - it.from + KT - 1) / KT : 0;
+  const int ntiles = (it.to - it.from + KT - 1) / KT;
   const constant_i32* const table = (const constant_i32*)it.table;
   const int table_end = max(it.to - 1, 0);
   const int64_t plane = (int64_t)A.num_blocks * A.n_kv << A.bs_log2;  // rows of K
   const int ltok = lane / CHUNKS, lchunk = lane % CHUNKS;
-  // (K: the 16 lanes of a read are 16 tokens' chunks of one g; V: see v_addr)
-  const int k_src = HD == 128 ? 16 * (lchunk ^ ((ltok >> 2) & 3)) : 16 * (lchunk ^ ((ltok >> 3) & 1));
-  int page[2];
+  auto k_swz = [](int t) { return HD == 128 ? (t >> 2) & 3 : (t >> 3) & 1; };
+  auto v_swz = [](int t) { return HD == 128 ? (t >> 1 & 2) + (t >> 4 & 1) : t >> 4 & 1; };
   auto look_up = [&](int tile) {
-    const int base = it.from + tile * KT;
-    page[0] = table[min(base, table_end) >> A.bs_log2];
-    page[1] = table[min(base + 32, table_end) >> A.bs_log2];
+    return table[min(it.from + tile * KT, table_end) >> A.bs_log2];
   };
-  auto row_of = [&](int u, int t) -> int64_t {  // of token t, in page[u]
-    const bool known = (unsigned)page[u] < (unsigned)A.num_blocks;
-    return (((int64_t)(known ? page[u] : 0) * A.n_kv + kvh) << A.bs_log2) + (t & (bs - 1));
-  };
-  auto stage = [&](lds_u8* dst, int tile) {
-    const int base = it.from + tile * KT;
-    int64_t row[2];
-    row[0] = row_of(0, base);
-    row[1] = row_of(1, base + 32);
+  auto known = [&](int page) { return (unsigned)page < (unsigned)A.num_blocks; };
+  auto stage = [&](lds_u8* __restrict__ dst, int tile, int page) {
+    const int t0 = it.from + tile * KT;
+    const int64_t row = (((int64_t)(known(page) ? page : 0) * A.n_kv + kvh) << A.bs_log2) +
+                        (t0 & (bs - 1));
     {
       // the scales of two tokens (four of 64 channels) a lane, K's and then V's
       constexpr int PER = 16 / (2 * NB), HALF = KT / PER;
-      const int i = lane % HALF, v = lane / HALF;
-      if (v < 2) {
-        const int t = i * PER;
-        const int64_t at = (t < 32 ? row[0] : row[1]) + (t & 31) + (v ? plane : 0);
+      if (lane < 2 * HALF) {
+        const int64_t at = row + lane % HALF * PER + (lane < HALF ? 0 : plane);
         __builtin_amdgcn_global_load_lds((global_void*)(A.scales + at * NB),
-                                         (lds_void*)(dst + T::K + T::V), 16, 0, 0);
+                                         (lds_void*)(dst + 2 * T::CODES), 16, 0, 0);
       }
     }
 #pragma unroll
     for (int v = 0; v < 2; ++v)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-        const int t0 = i * SPAN;  // the load's first token
-        const int64_t r0 = row[t0 / 32] + (t0 & 31) + (v ? plane : 0);
-        const int v_src = HD == 128 ? 16 * (lchunk ^ (i & 3))
-                                    : 16 * (lchunk ^ (ltok >> 4 & 1));
-        const uint8_t* const src = A.codes + r0 * RB;
-        __builtin_amdgcn_global_load_lds((global_void*)(src + (ltok * RB + (v ? v_src : k_src))),
-                                         (lds_void*)(dst + v * T::K + i * 1024), 16, 0, 0);
+        const int t = i * SPAN + ltok;
+        const int src = t * RB + 16 * (lchunk ^ (v ? v_swz(t) : k_swz(t)));
+        __builtin_amdgcn_global_load_lds((global_void*)(A.codes + (row + (v ? plane : 0)) * RB + src),
+                                         (lds_void*)(dst + v * T::CODES + i * 1024), 16, 0, 0);
       }
   };
-  constexpr int STAGE_LOADS = 1 + 2 * LOADS;
-  auto bad_pages = [&]() {
-    return ((unsigned)page[0] >= (unsigned)A.num_blocks ? 1 : 0) |
-           ((unsigned)page[1] >= (unsigned)A.num_blocks ? 2 : 0);
-  };
 
-  // ---- a row's state: the exponents' reference (log2 units: the running maximum, or up
+  // ---- the row's state: the exponents' reference (log2 units: the running maximum, or up
   // to LAG below it), the sum of 2^(score - ref) over this lane's tokens, the output's
   // products with 16 + code and (register b: block b) the sums of their weights.
-  float ref[RT], l[RT];
-  f32x4 o[RT][DT], w_sum[RT];
+  float ref = NO_REF, l = 0.f;
+  f32x4 o[DT], w_sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    ref[r] = NO_REF;
-    l[r] = 0.f;
-    w_sum[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < DT; ++d) o[r][d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
   // ones in the rows 4 x + b of the weights' product, so that its register b is block b's
-  bf16x8 ones[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const uint32_t x = (lane & 3) == b ? 0x3f803f80u : 0u;
-    ones[b] = __builtin_bit_cast(bf16x8, u32x4{x, x, x, x});
-  }
-  const int k_addr = HD == 128 ? n * RB + 16 * (g ^ (n >> 2))
-                               : n * RB + 16 * ((g >> 1) ^ (n >> 3)) + 8 * (g & 1);
-  // V: lane n of 16 addresses token 16 (n / 4) + 4 g + n % 4
-  const int vt = 16 * (n >> 2) + 4 * g + (n & 3);
-  const int v_swz = HD == 128 ? n >> 2 : (vt >> 4) & 1;
+  bf16x8 qf[NB], ones[NB];
+  f32x4 c0[NB];
+  const CodeBits codes_bf16;
+  const int k_addr = HD == 128 ? n * RB + 16 * (g ^ k_swz(n))
+                               : n * RB + 16 * ((g >> 1) ^ k_swz(n)) + 8 * (g & 1);
+  const int vt = 16 * (n >> 2 & 1) + 4 * g + (n & 3);
+  const int v_addr = T::CODES + vt * RB + 8 * (n >> 3), v_place = v_swz(vt);
+  const int s_addr = 2 * T::CODES + 4 * g * 2 * NB;  // scales of tokens 4 g ..
 
-  auto compute = [&](auto plain, const lds_u8* buf, int tile, int bad) {
-    const int base = it.from + tile * KT;
-    const lds_u8* const sk = buf + T::K + T::V;
-    const lds_u8* const sv = sk + T::S;
-    // scales of tokens 16 t + 4 g + i, block b: fp16 i * NB + b of 8 NB bytes
-    auto scales_of = [&](const lds_u8* s, int t, uint32_t (&w)[2 * NB]) {
+  auto compute = [&](auto plain, const lds_u8* __restrict__ buf, int base, bool bad) {
+    // scales of tokens 16 t + 4 g + i, block b: fp16 i * NB + b
+    auto scales_of = [&](int v, int t, uint32_t (&w)[2 * NB]) {
 #pragma unroll
       for (int j = 0; j < NB / 2; ++j) {
-        const u32x4 x = *(const lds_u32x4*)(s + (16 * t + 4 * g) * 2 * NB + 16 * j);
+        const u32x4 x = *(const lds_u32x4*)(buf + s_addr + v * T::SCALES + 16 * t * 2 * NB + 16 * j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[4 * j + i] = x[i];
       }
     };
-    float p[RT][4][4];  // scores, then weights: [16 tokens][i]
+    float p[2][4];  // scores, then weights
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 2; ++t) {
       uint32_t dk[2 * NB], kw[NB];
-      scales_of(sk, t, dk);
+      scales_of(0, t, dk);
       if constexpr (HD == 128) {
         const u32x4 x = *(const lds_u32x4*)(buf + t * 16 * RB + k_addr);
 #pragma unroll
         for (int b = 0; b < 4; ++b) kw[b] = x[b];
       } else {
-        // (a load's 32 tokens are swizzled by their own bit 3)
         const u32x2 x = *(const lds_u32x2*)(buf + t * 16 * RB + k_addr);
         kw[0] = x[0];
         kw[1] = x[1];
       }
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[r][t][i] = 0.f;
+      for (int i = 0; i < 4; ++i) p[t][i] = 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const bf16x8 a = codes_bf16(kw[b]);
+        const f32x4 s = mfma(codes_bf16(kw[b]), qf[b], c0[b]);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const f32x4 s = mfma(a, qf[r][b], c0[r][b]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            p[r][t][i] = fmaf(half_of(dk[(i * NB + b) / 2], (i * NB + b) & 1), s[i], p[r][t][i]);
-        }
+        for (int i = 0; i < 4; ++i)
+          p[t][i] = fmaf(half_of(dk[(i * NB + b) / 2], (i * NB + b) & 1), s[i], p[t][i]);
       }
     }
+    const int left = lim - base - 4 * g;  // tokens 16 t + i below it are seen
+    if constexpr (!plain) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      if constexpr (!plain) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float x = bad >> (t / 2) & 1 ? __builtin_nanf("") : p[r][t][i];
-            p[r][t][i] = base + 16 * t + 4 * g + i < lim[r] ? x : -INFINITY;
-          }
-      }
-      float mx = p[r][0][0];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, p[r][t][i]);
-      mx = xor_max<32>(xor_max<16>(mx)) * A.scale_log2;
-      if (__builtin_amdgcn_ballot_w64(mx > ref[r] + LAG)) {
-        const float next = fmaxf(ref[r], mx);
-        const float alpha = __builtin_amdgcn_exp2f(ref[r] - next);
-        ref[r] = next;
-        l[r] *= alpha;
-        w_sum[r] *= alpha;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) o[r][d] *= alpha;
-      }
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[r][t][i] = __builtin_amdgcn_exp2f(fmaf(p[r][t][i], A.scale_log2, -ref[r]));
-          part[i] += p[r][t][i];
+          const float x = bad ? __builtin_nanf("") : p[t][i];
+          p[t][i] = 16 * t + i < left ? x : -INFINITY;
         }
-      l[r] += (part[0] + part[1]) + (part[2] + part[3]);
     }
+    float mx = p[0][0];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, p[t][i]);
+    mx = xor_max<32>(xor_max<16>(mx)) * A.scale_log2;
+    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG)) {
+      const float next = fmaxf(ref, mx);
+      const float alpha = __builtin_amdgcn_exp2f(ref - next);
+      ref = next;
+      l *= alpha;
+      w_sum *= alpha;
+#pragma unroll
+      for (int d = 0; d < DT; ++d) o[d] *= alpha;
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        p[t][i] = __builtin_amdgcn_exp2f(fmaf(p[t][i], A.scale_log2, -ref));
+    l += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
     // O^T += V^T P'^T, block by block
+    uint32_t dv[2][2 * NB];
+    scales_of(1, 0, dv[0]);
+    scales_of(1, 1, dv[1]);
+    if constexpr (!plain) {  // (an unseen token's scale may be anything)
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      uint32_t dv0[2 * NB], dv1[2 * NB];  // of sixteens 2 m and 2 m + 1
-      scales_of(sv, 2 * m, dv0);
-      scales_of(sv, 2 * m + 1, dv1);
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        bf16x8 w[RT];
+        for (int i = 0; i < 2 * NB; ++i)
+          dv[t][i] = 16 * t + i * 2 / NB < left ? dv[t][i] : 0u;
+    }
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          u32x4 x;
+    for (int b = 0; b < NB; ++b) {
+      u32x4 x;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int e = i * NB + b;
-            float w0 = p[r][2 * m][i] * half_of(dv0[e / 2], e & 1);
-            float w1 = p[r][2 * m + 1][i] * half_of(dv1[e / 2], e & 1);
-            if constexpr (!plain) {  // (an unseen token's scale may be anything)
-              const int t = base + 32 * m + 4 * g + i;
-              w0 = t < lim[r] ? w0 : 0.f;
-              w1 = t + 16 < lim[r] ? w1 : 0.f;
-            }
-            x[i] = cvt_pk_bf16(w0, w1);
-          }
-          w[r] = __builtin_bit_cast(bf16x8, x);
-          w_sum[r] = mfma(ones[b], w[r], w_sum[r]);
-        }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int d = 2 * b + c;  // 16 dims: chunk d of 8 bytes of every row
-          const i32x2 x = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-              (lds_i32x2*)(buf + T::K + vt * RB + 16 * (b ^ v_swz) + 8 * c));
-          const bf16x8 a = codes_bf16((uint32_t)x[m]);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) o[r][d] = mfma(a, w[r], o[r][d]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int e = i * NB + b;
+        // (one instruction with the conversion, where a product alone would be two)
+        x[i] = cvt_pk_bf16(fmaf(p[0][i], half_of(dv[0][e / 2], e & 1), codes_bf16.zero),
+                           fmaf(p[1][i], half_of(dv[1][e / 2], e & 1), codes_bf16.zero));
       }
+      const bf16x8 w = __builtin_bit_cast(bf16x8, x);
+      w_sum = mfma(ones[b], w, w_sum);
+      const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+          (lds_i32x2*)(buf + v_addr + 16 * (b ^ v_place)));
+      o[2 * b] = mfma(codes_bf16((uint32_t)v[0]), w, o[2 * b]);
+      o[2 * b + 1] = mfma(codes_bf16((uint32_t)v[1]), w, o[2 * b + 1]);
     }
   };
 
-  // ---- this wave's tiles: the next one's loads in flight during the current one
-  lds_u8* const lds = (lds_u8*)smem + wave * 2 * T::BYTES;
-  if (wave < ntiles) {
-    look_up(wave);
-    stage(lds, wave);
-    int bad = bad_pages(), buf = 0;
-    look_up(wave + WAVES);
-    auto round = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ cur, int tile) {
-      int bad_next = 0;
-      if (tile + WAVES < ntiles) {
-        stage(next, tile + WAVES);
-        bad_next = bad_pages();
-        look_up(tile + 2 * WAVES);
-        __builtin_amdgcn_s_waitcnt(0x0f70 | (STAGE_LOADS & 15));  // this tile's have arrived
-      } else {
-        __builtin_amdgcn_s_waitcnt(0x0f70);
-      }
-      __asm__ volatile("" ::: "memory");
-      if (!bad && it.from + tile * KT + KT <= lim_min)
-        compute(std::true_type{}, cur, tile, 0);
-      else
-        compute(std::false_type{}, cur, tile, bad);
-      bad = bad_next;
-    };
-    for (int tile = wave; tile < ntiles; tile += WAVES) {
-      round(lds + (buf ^ 1) * T::BYTES, lds + buf * T::BYTES, tile);
-      buf ^= 1;
+  // ---- this wave's tiles: RING - 1 of them on their way
+  lds_u8* const lds = (lds_u8*)smem + wave * RING * T::BYTES;
+  int page[RING], tile = wave;
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i) {
+    page[i] = look_up(tile + i * WAVES);
+  }
+  page[RING - 1] = look_up(tile + (RING - 1) * WAVES);
+#pragma unroll
+  for (int i = 0; i < RING - 1; ++i)
+    if (tile + i * WAVES < ntiles) stage(lds + i * T::BYTES, tile + i * WAVES, page[i]);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    qf[b] = __builtin_bit_cast(bf16x8, qx[b]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = dot2_bf16(qx[b][i], 0x3f803f80u, sum);
+    sum = -24.f * xor_sum<32>(xor_sum<16>(sum));
+    c0[b] = f32x4{sum, sum, sum, sum};
+    const uint32_t x = (lane & 3) == b ? 0x3f803f80u : 0u;
+    ones[b] = __builtin_bit_cast(bf16x8, u32x4{x, x, x, x});
+  }
+  auto round = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ cur) {
+    // this tile's loads have arrived: at the end all, else all but the two later tiles'
+    if (tile + (RING - 2) * WAVES < ntiles)
+      __builtin_amdgcn_s_waitcnt(0x0f70 | ((RING - 2) * STAGE_LOADS));
+    else
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+    __asm__ volatile("" ::: "memory");
+    const bool bad = !known(page[0]);
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i) page[i] = page[i + 1];
+    if (tile + (RING - 1) * WAVES < ntiles) {
+      stage(next, tile + (RING - 1) * WAVES, page[RING - 2]);
+      page[RING - 1] = look_up(tile + RING * WAVES);
     }
+    const int base = it.from + tile * KT;
+    if (!bad && base + KT <= lim_min)
+      compute(std::true_type{}, cur, base, false);
+    else
+      compute(std::false_type{}, cur, base, bad);
+  };
+  int at = 0;
+  for (; tile < ntiles; tile += WAVES) {
+    round(lds + ((at + RING - 1) & (RING - 1)) * T::BYTES, lds + at * T::BYTES);
+    at = (at + 1) & (RING - 1);
   }
 
-  // ---- what 16 + code added, then the four waves' states
+  // ---- what 16 + code added, then the waves' states: each leaves its own in the place of
+  // its tiles, and joins the four of a quarter of the dims
+  l = xor_sum<32>(xor_sum<16>(l));
+  constexpr int QT = DT / WAVES;            // tiles of dims a wave joins
+  constexpr int STATE = RING * T::BYTES / 4;  // floats between two waves' states
+  static_assert(STATE >= 16 * HD + 32, "a state fits in a ring");
+  float* const jo = reinterpret_cast<float*>(smem);
+  float* const mine = jo + wave * STATE;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    l[r] = xor_sum<32>(xor_sum<16>(l[r]));
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[r][d][i] = fmaf(-24.f, w_sum[r][d / 2], o[r][d][i]);
+  for (int d = 0; d < DT; ++d)
+    *reinterpret_cast<f32x4*>(mine + (d * 64 + lane) * 4) = o[d] + -24.f * w_sum[d / 2];
+  if (g == 0) {
+    mine[16 * HD + n] = ref;
+    mine[16 * HD + 16 + n] = l;
   }
-  constexpr int STATE = RT * (16 * HD + 32);  // floats of a wave's
-  if (ntiles > 1) {
-    float* const jo = reinterpret_cast<float*>(smem);
-    __syncthreads();  // the tiles are read out
-    if (wave > 0) {
-      float* const dst = jo + (wave - 1) * STATE;
+  __syncthreads();
+  float refs[WAVES];
+  ref = NO_REF;
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[((r * DT + d) * 4 + i) * 64 + lane] = o[r][d][i];
-        if (g == 0) {
-          dst[RT * 16 * HD + r * 32 + n] = ref[r];
-          dst[RT * 16 * HD + r * 32 + 16 + n] = l[r];
-        }
-      }
-    }
-    __syncthreads();
+  for (int w = 0; w < WAVES; ++w) {
+    refs[w] = jo[w * STATE + 16 * HD + n];
+    ref = fmaxf(ref, refs[w]);
   }
-  if (wave > 0) return;
+  l = 0.f;
 #pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    if (ntiles > 1) {
-      const float* const jo = reinterpret_cast<const float*>(smem);
+  for (int d = 0; d < QT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) {
-        const float* const src = jo + (w - 1) * STATE;
-        const float ro = src[RT * 16 * HD + r * 32 + n], lo = src[RT * 16 * HD + r * 32 + 16 + n];
-        const float next = fmaxf(ref[r], ro);
-        const float a = __builtin_amdgcn_exp2f(ref[r] - next);
-        const float b = __builtin_amdgcn_exp2f(ro - next);
-        ref[r] = next;
-        l[r] = l[r] * a + lo * b;
+  for (int w = 0; w < WAVES; ++w) {
+    const float a = __builtin_amdgcn_exp2f(refs[w] - ref);
+    l = fmaf(jo[w * STATE + 16 * HD + 16 + n], a, l);
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+    for (int d = 0; d < QT; ++d)
+      o[d] += a * *reinterpret_cast<const f32x4*>(jo + w * STATE +
+                                                  ((wave * QT + d) * 64 + lane) * 4);
+  }
+  if (!valid) return;
+  // l == 0 only where the row sees no token: its output is 0, its weight none
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  // (the row again, from its number: not kept in registers through the tiles)
+  int row_again = it.row0 + n;
+  __asm__ volatile("" : "+v"(row_again));
+  const int again_tok = small_div(row_again, A.group, A.group_inv);
+  const int64_t orow = (int64_t)(it.token0 + again_tok) * A.n_q + kvh * A.group + row_again -
+                       again_tok * A.group;
+  const int dim = wave * QT * 16 + 4 * g;
+  if (it.parts == 1) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            o[r][d][i] = o[r][d][i] * a + src[((r * DT + d) * 4 + i) * 64 + lane] * b;
-      }
-    }
-    if (!valid[r]) continue;
-    const int64_t orow = (int64_t)tok[r] * A.n_q + head[r];
-    // l == 0 only where the row sees no token: its output is 0, its weight none
-    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-    if (it.slot == 0 && A.splits > 1 && g == 0)
-      st_agent(A.counts + orow, it.parts == 1 ? 0 : it.parts);
-    if (it.parts == 1) {
-      uint16_t* const dst = A.out + orow * HD;
+    for (int d = 0; d < QT; ++d)
+      st_agent(reinterpret_cast<u32x2*>(A.out + orow * HD + dim + 16 * d),
+               u32x2{cvt_pk_bf16(o[d][0] * inv, o[d][1] * inv),
+                     cvt_pk_bf16(o[d][2] * inv, o[d][3] * inv)});
+  } else if (l != 0.f) {  // the merge reads no partial whose weight is none
+    float* const dst = A.part_o + (orow * A.splits + it.slot) * HD + dim;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
-        st_agent(reinterpret_cast<u32x2*>(dst + 16 * d + 4 * g),
-                 u32x2{cvt_pk_bf16(o[r][d][0] * inv, o[r][d][1] * inv),
-                       cvt_pk_bf16(o[r][d][2] * inv, o[r][d][3] * inv)});
-    } else {
-      const int64_t prow = orow * A.splits + it.slot;
-      if (g == 0) st_agent(A.part_lse + prow, l[r] == 0.f ? -INFINITY : ref[r] + log2f(l[r]));
-      if (l[r] != 0.f) {  // the merge reads no partial whose weight is none
-        float* const dst = A.part_o + prow * HD;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-          st_agent_b128(dst + 16 * d + 4 * g,
-                        u32x4{__float_as_uint(o[r][d][0] * inv), __float_as_uint(o[r][d][1] * inv),
-                              __float_as_uint(o[r][d][2] * inv),
-                              __float_as_uint(o[r][d][3] * inv)});
-      }
-    }
+    for (int d = 0; d < QT; ++d)
+      st_agent_b128(dst + 16 * d, __builtin_bit_cast(u32x4, o[d] * inv));
+  }
+  if (wave == 0 && g == 0 && A.splits > 1) {
+    if (it.slot == 0) st_agent(A.counts + orow, it.parts == 1 ? 0 : it.parts);
+    if (it.parts > 1)
+      st_agent(A.part_lse + orow * A.splits + it.slot, l == 0.f ? -INFINITY : ref + log2f(l));
   }
 }
 
 // Sequence r's queries are the tokens [query_start[r], query_start[r + 1]), the last n of
-// its L tokens.  Grid: kv heads, items.
-template <int HD, int RT>
+// its L tokens; its work is its tiles of 16 rows times the rounds (ROUND tokens) of L.  The
+// work of all sequences, end to end, is cut into parts of `chunk` rounds, one a workgroup.
+// Long parts are equal whatever the lengths: one can be the end of a tile and the beginning
+// of the next, each with its partial.  Every beginning costs about 4 us (the chain of
+// length, table entry and first tile, and the join), so where parts are short a tile
+// begins a new one.  Grid: kv heads, parts.
+template <int HD>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void q4_attention_kernel(Q4Args A) {
-  constexpr int M = 16 * RT;
-  constexpr int BUF = WAVES * 2 * Tile<HD>::BYTES, JOIN = (WAVES - 1) * RT * (16 * HD + 32) * 4;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[BUF > JOIN ? BUF : JOIN];
-  const int kvh = blockIdx.x;
+  constexpr int M = 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * RING * Tile<HD>::BYTES];
+  const int kvh = blockIdx.x, lane = threadIdx.x & 63;
   const int cap = A.max_blocks << A.bs_log2;
-  auto queries = [&](int r, int& s0) {
-    if (!A.query_start) {
-      s0 = r;
-      return 1;
+  int q0, nq, len, tiles, rounds;  // of sequence b + lane
+  auto load = [&](int b) {
+    const int r = b + lane;
+    q0 = nq = len = tiles = rounds = 0;
+    if (r < A.num_seqs) {
+      len = min(max(A.seq_lens[r], 0), cap);
+      q0 = r;
+      nq = 1;
+      if (A.query_start) {
+        q0 = min(max(A.query_start[r], 0), A.num_tokens);
+        nq = max(min(A.query_start[r + 1], A.num_tokens) - q0, 0);
+      }
+      tiles = (nq * A.group + M - 1) / M;
+      rounds = tiles ? max((len + ROUND - 1) / ROUND, 1) : 0;
     }
-    s0 = min(max(A.query_start[r], 0), A.num_tokens);
-    return max(min(A.query_start[r + 1], A.num_tokens) - s0, 0);
   };
-  auto length = [&](int r) { return min(max(A.seq_lens[r], 0), cap); };
-  int my_q0 = 0, my_nq = 0, my_len = 0;  // of sequence `lane` where there are up to 64
-  auto seg_of = [&](int r, int& tiles, int& rounds) {
-    my_nq = queries(r, my_q0);
-    my_len = length(r);
-    tiles = (int)(((int64_t)my_nq * A.group + M - 1) / M);
-    rounds = tiles ? (int)(((int64_t)my_len + ROUND - 1) / ROUND) : 0;
-  };
-  Place place;
-  if (!find_item<ROUND>(seg_of, A.num_seqs, blockIdx.y, A.target, A.splits, A.least, -INFINITY,
-                        false, place))
-    return;
-  const int seq = place.seg;
-  int q0, nq, L;
-  if (A.num_seqs <= 64) {  // (a second look in memory is a round trip)
-    q0 = __builtin_amdgcn_readlane(my_q0, seq);
-    nq = __builtin_amdgcn_readlane(my_nq, seq);
-    L = __builtin_amdgcn_readlane(my_len, seq);
-  } else {
-    nq = queries(seq, q0);
-    L = length(seq);
+  load(0);
+  float all = (float)tiles * (float)rounds;
+  int top = wave_max_i32(rounds);
+  for (int b = 64; b < A.num_seqs; b += 64) {
+    load(b);
+    all += (float)tiles * (float)rounds;
+    top = max(top, wave_max_i32(rounds));
   }
-  const int tiles = (int)(((int64_t)nq * A.group + M - 1) / M);
-  const int split = place.x / tiles;
-  Q4Item it;
-  it.table = A.table + (int64_t)seq * A.max_blocks;
-  it.token0 = q0;
-  it.row0 = (place.x - split * tiles) * M;
-  it.rows = min(M, nq * A.group - it.row0);
-  it.ahead = L - nq;  // the position of the first query token
-  const int range = max(it.ahead + (it.row0 + it.rows - 1) / A.group + 1, 0);
-  it.from = part_end(0, split * place.chunk, range);
-  it.to = part_end(it.from, place.chunk, range);
-  it.slot = split;
-  it.parts = place.parts;
-  q4_attend<HD, RT>(A, it, kvh, smem);
+  if (A.num_seqs > 64) load(0);
+  all = wave_sum(all);
+  // (the host has bounded the sum for offsets in order; there is no work in others)
+  if (all > 0x1p28f) return;
+  // `chunk` need not be exact (workgroups take a second part where there is one), but a
+  // tile of `top` rounds must lie in at most (top - 2) / chunk + 2 <= splits parts
+  int chunk = (int)(all * A.target_inv + 0.999f);
+  if (A.splits > 2) chunk = max(chunk, (int)((float)top * A.splits_inv) + 1);
+  chunk = max(chunk, 1);
+  float inv;
+  bool apart;
+  auto padded = [&](int r) {
+    if (!apart) return r;
+    const int q = small_div(r, chunk, inv);
+    return q * chunk < r ? (q + 1) * chunk : r;
+  };
+  for (int i = 0;; ++i) {
+    inv = __builtin_amdgcn_rcpf((float)chunk);
+    apart = chunk < APART;
+    if (!apart || A.num_seqs > 64 || i == 3 || chunk >= top) break;
+    // a little longer parts where the tiles' ends make too many
+    const float sum = wave_sum((float)(tiles * padded(rounds)));
+    if (sum <= (float)(chunk * A.target)) break;
+    chunk = min(max(chunk + 1, (int)(sum * A.target_inv + 0.999f)), top);
+  }
+  chunk = __builtin_amdgcn_readfirstlane(chunk);
+  // Part after part (one, unless there are more than workgroups), piece after piece.
+  // What is known of the sequences is loaded again for each: it would be in registers
+  // through the tiles.
+  int part = blockIdx.y, at = part * chunk, b = 0, base = 0;
+  for (;;) {
+    const int work = tiles * padded(rounds);
+    const int incl = wave_scan_i32(work), here = __builtin_amdgcn_readlane(incl, 63);
+    if (at >= base + here) {  // in a later 64 sequences
+      base += here;
+      b += 64;
+      if (b >= A.num_seqs) break;
+      load(b);
+      continue;
+    }
+    const int i = __ffsll((unsigned long long)__ballot(base + incl > at)) - 1;
+    const int r = padded(__builtin_amdgcn_readlane(rounds, i));
+    int tile_at = base + __builtin_amdgcn_readlane(incl, i) - __builtin_amdgcn_readlane(work, i);
+    int tile = 0;
+    if (at - tile_at >= r) {
+      tile = (at - tile_at) / r;
+      tile_at += tile * r;
+    }
+    const int begin = part * chunk, end = begin + chunk;
+    const int from = at - tile_at, to = min(r, end - tile_at);
+    Q4Item it;
+    it.table = A.table + (int64_t)(b + i) * A.max_blocks;
+    it.token0 = __builtin_amdgcn_readlane(q0, i);
+    const int n = __builtin_amdgcn_readlane(nq, i), L = __builtin_amdgcn_readlane(len, i);
+    it.row0 = tile * M;
+    it.rows = min(M, n * A.group - it.row0);
+    it.ahead = L - n;  // the position of the first query token
+    const int range = min(max(it.ahead + (it.row0 + it.rows - 1) / A.group + 1, 0), L);
+    it.from = min(from * ROUND, range);
+    it.to = min(to * ROUND, range);
+    // the parts of this tile that end at or before `begin`, and from `end` on
+    it.slot = from > 0 ? small_div(begin - tile_at + chunk - 1, chunk, inv) : 0;
+    it.parts = it.slot + 1 +
+               (tile_at + r > end ? small_div(tile_at + r - end + chunk - 1, chunk, inv) : 0);
+    q4_attend<HD>(A, it, kvh, smem);
+    at += to - from;
+    if (at >= end) {
+      part += A.target;
+      at = part * chunk;
+    }
+    if (A.num_seqs <= 64 && at >= here) break;
+    load(b);
+    __syncthreads();  // the states are read out
+  }
   stores_done();
 }
 
-// How a call is cut, from its sizes (lengths are on the device).
+// How a call is cut, from its sizes (lengths are on the device).  512 workgroups fill the
+// chip once (73 KB of LDS and 216 registers: two a compute unit).
 constexpr int FILL = 512, MAX_PARTS = 64;
 
+int tune(const char* name, int v) {
+  const char* e = tuning_env(name);
+  return e ? atoi(e) : v;
+}
+
 struct Q4Choice {
-  int rt, splits, tiles, target;
+  int splits, target;
 };
 
-// Whether a call's rows are prompts': more than a tile of a sequence on average.
+// Whether a call's rows are prompts': more than two tiles of a sequence on average.
 bool is_prompt(int64_t num_tokens, int64_t num_seqs, int group) {
-  const char* e = tuning_env("SMX_Q4_ROWS");
-  return num_tokens * group > (e ? atoi(e) : 32) * num_seqs;
+  return num_tokens * group > tune("SMX_Q4_ROWS", 32) * num_seqs;
+}
+
+int64_t q4_tiles(int64_t num_tokens, int64_t num_seqs, int group) {
+  return (num_tokens * group + 15) / 16 + num_seqs - 1;
 }
 
 Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Q4Choice c{};
-  const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
-  c.rt = rows > 16 ? 2 : 1;
-  const int m = 16 * c.rt;
-  c.tiles = (int)((num_tokens * group + m - 1) / m + num_seqs - 1);
-  c.target = std::max(1, FILL / n_kv);
-  const int64_t groups = (rows + m - 1) / m * num_seqs * n_kv;
-  const int64_t even = (FILL + groups - 1) / groups;
-  c.splits = (int)std::clamp<int64_t>(num_seqs == 1 ? even : 4 * even, 1,
-                                      std::min<int64_t>(MAX_PARTS, std::max<int64_t>(1, cap / ROUND)));
-  if (groups >= 2 * FILL) c.splits = 1;
+  const int64_t rounds = (cap + ROUND - 1) / ROUND;  // the most of a tile
+  c.target = std::max(1, tune("SMX_Q4_FILL", FILL) / n_kv);
+  // uneven lengths: the longest may take four times the parts of even ones
+  const int64_t even = (c.target + num_seqs - 1) / num_seqs;
+  c.splits = (int)std::clamp<int64_t>(4 * even + 2, 3, MAX_PARTS);
+  // (a tile of one round is never cut)
+  c.splits = rounds == 1 ? 1 : (int)std::min<int64_t>(c.splits, rounds + 1);
   return c;
-}
-
-int64_t q4_items(const Q4Choice& c) {
-  return std::min<int64_t>((int64_t)c.tiles * c.splits, (int64_t)c.target + c.tiles + 1);
 }
 
 int64_t q4_workspace(int64_t rows, int64_t splits, int hd) {
@@ -619,7 +642,10 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
   }
   const smx::Q4Choice c = smx::choose_q4(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
                                          n_q / n_kv, n_kv);
-  SMX_REQUIRE(smx::q4_items(c) <= 65535, "too many row tiles for one launch");
+  SMX_REQUIRE(smx::q4_tiles(num_tokens, num_seqs, n_q / n_kv) *
+                      (((int64_t)max_blocks * block_size + smx::ROUND - 1) / smx::ROUND) <
+                  (1ll << 28),
+              "row tiles times the sequences' capacity / 256 must be below 2^28");
   const int64_t rows = (int64_t)num_tokens * n_q;
   SMX_REQUIRE(c.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
                                 workspace_bytes >= smx::q4_workspace(rows, c.splits, head_dim)),
@@ -646,12 +672,13 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
   a.group = n_q / n_kv;
   a.splits = c.splits;
   a.target = c.target;
-  a.least = 1;
   a.scale_log2 = scale_log2;
-  const dim3 grid(n_kv, (unsigned)smx::q4_items(c));
-  const auto kernel = head_dim == 128
-      ? (c.rt == 1 ? smx::q4_attention_kernel<128, 1> : smx::q4_attention_kernel<128, 2>)
-      : (c.rt == 1 ? smx::q4_attention_kernel<64, 1> : smx::q4_attention_kernel<64, 2>);
+  a.group_inv = 1.f / a.group;
+  a.target_inv = 1.f / c.target;
+  a.splits_inv = c.splits > 2 ? 1.f / (c.splits - 2) : 0.f;
+  const dim3 grid(n_kv, c.target);
+  const auto kernel = head_dim == 128 ? smx::q4_attention_kernel<128>
+                                      : smx::q4_attention_kernel<64>;
   SMX_LAUNCH(kernel, grid, dim3(64 * smx::WAVES), 0, (hipStream_t)stream, a);
   const int rc = (int)hipGetLastError();
   if (rc || c.splits == 1) return rc;
