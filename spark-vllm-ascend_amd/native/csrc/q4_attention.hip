@@ -21,7 +21,7 @@
 // (ds_read_b64_tr_b4: lane n gets channel n of the 16 lanes' tokens and halves).
 //
 // A workgroup is four waves that take the tiles of its part of the tokens in turn, each with
-// its own softmax and its own ring of tiles in LDS, filled by direct loads three tiles
+// its own softmax and its own two tiles in LDS, filled by direct loads a tile
 // ahead: nothing is waited for but a wave's own loads, until the four states are joined.
 //
 // Bound by memory where there are many tokens; by instructions that are not in the
@@ -54,9 +54,8 @@ constexpr float LAG = 8.f;        // log2 units
 constexpr float NO_REF = -3e38f;  // before the first token: below the scores of any use
 constexpr int KT = 32;            // tokens of a tile
 constexpr int WAVES = 4;
-constexpr int RING = 4;           // tiles of a wave in LDS
 constexpr int ROUND = KT * WAVES;
-constexpr int APART = 16;         // parts shorter than that many rounds are of one tile
+constexpr int BEGIN = 2;          // rounds that the beginning of a tile takes the time of
 
 struct Q4Args {
   const uint16_t* q;
@@ -132,7 +131,6 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
   constexpr int CHUNKS = RB / 16;                       // 16-byte chunks a row
   constexpr int LOADS = KT * CHUNKS / 64;               // direct loads of a K (V) tile
   constexpr int SPAN = 64 / CHUNKS;                     // tokens of one
-  constexpr int STAGE_LOADS = 1 + 2 * LOADS;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int bs = 1 << A.bs_log2;
@@ -304,17 +302,10 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
     }
   };
 
-  // ---- this wave's tiles: RING - 1 of them on their way
-  lds_u8* const lds = (lds_u8*)smem + wave * RING * T::BYTES;
-  int page[RING], tile = wave;
-#pragma unroll
-  for (int i = 0; i < RING - 1; ++i) {
-    page[i] = look_up(tile + i * WAVES);
-  }
-  page[RING - 1] = look_up(tile + (RING - 1) * WAVES);
-#pragma unroll
-  for (int i = 0; i < RING - 1; ++i)
-    if (tile + i * WAVES < ntiles) stage(lds + i * T::BYTES, tile + i * WAVES, page[i]);
+  // ---- this wave's tiles
+  lds_u8* const lds = (lds_u8*)smem + wave * 2 * T::BYTES;
+  int tile = wave, page = look_up(tile), next_page = look_up(tile + WAVES);
+  if (tile < ntiles) stage(lds, tile, page);
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     qf[b] = __builtin_bit_cast(bf16x8, qx[b]);
@@ -327,37 +318,27 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
     ones[b] = __builtin_bit_cast(bf16x8, u32x4{x, x, x, x});
   }
   auto round = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ cur) {
-    // this tile's loads have arrived: at the end all, else all but the two later tiles'
-    if (tile + (RING - 2) * WAVES < ntiles)
-      __builtin_amdgcn_s_waitcnt(0x0f70 | ((RING - 2) * STAGE_LOADS));
-    else
-      __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // this tile's loads have arrived
     __asm__ volatile("" ::: "memory");
-    const bool bad = !known(page[0]);
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i) page[i] = page[i + 1];
-    if (tile + (RING - 1) * WAVES < ntiles) {
-      stage(next, tile + (RING - 1) * WAVES, page[RING - 2]);
-      page[RING - 1] = look_up(tile + RING * WAVES);
-    }
+    const bool bad = !known(page);
+    if (tile + WAVES < ntiles) stage(next, tile + WAVES, next_page);
+    page = next_page;
+    next_page = look_up(tile + 2 * WAVES);
     const int base = it.from + tile * KT;
     if (!bad && base + KT <= lim_min)
       compute(std::true_type{}, cur, base, false);
     else
       compute(std::false_type{}, cur, base, bad);
   };
-  int at = 0;
-  for (; tile < ntiles; tile += WAVES) {
-    round(lds + ((at + RING - 1) & (RING - 1)) * T::BYTES, lds + at * T::BYTES);
-    at = (at + 1) & (RING - 1);
-  }
+  for (int at = 0; tile < ntiles; tile += WAVES, at ^= 1)
+    round(lds + (at ^ 1) * T::BYTES, lds + at * T::BYTES);
 
   // ---- what 16 + code added, then the waves' states: each leaves its own in the place of
   // its tiles, and joins the four of a quarter of the dims
   l = xor_sum<32>(xor_sum<16>(l));
   constexpr int QT = DT / WAVES;            // tiles of dims a wave joins
-  constexpr int STATE = RING * T::BYTES / 4;  // floats between two waves' states
-  static_assert(STATE >= 16 * HD + 32, "a state fits in a ring");
+  constexpr int STATE = 2 * T::BYTES / 4;  // floats between two waves' states
+  static_assert(STATE >= 16 * HD + 32, "a state fits in the place of the tiles");
   float* const jo = reinterpret_cast<float*>(smem);
   float* const mine = jo + wave * STATE;
 #pragma unroll
@@ -419,15 +400,15 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
 // Sequence r's queries are the tokens [query_start[r], query_start[r + 1]), the last n of
 // its L tokens; its work is its tiles of 16 rows times the rounds (ROUND tokens) of L.  The
 // work of all sequences, end to end, is cut into parts of `chunk` rounds, one a workgroup.
-// Long parts are equal whatever the lengths: one can be the end of a tile and the beginning
-// of the next, each with its partial.  Every beginning costs about 4 us (the chain of
-// length, table entry and first tile, and the join), so where parts are short a tile
-// begins a new one.  Grid: kv heads, parts.
+// Equal parts, whatever the lengths, can be the end of a tile and the beginning of the next,
+// each with its partial; every beginning costs about 4 us (the chain of length, table entry
+// and first tile, and the join), as much as BEGIN rounds.  So every tile begins a new part
+// where parts no longer than that allow it.  Grid: kv heads, parts.
 template <int HD>
 __global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
 void q4_attention_kernel(Q4Args A) {
   constexpr int M = 16;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * RING * Tile<HD>::BYTES];
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * 2 * Tile<HD>::BYTES];
   const int kvh = blockIdx.x, lane = threadIdx.x & 63;
   const int cap = A.max_blocks << A.bs_log2;
   int q0, nq, len, tiles, rounds;  // of sequence b + lane
@@ -463,21 +444,22 @@ void q4_attention_kernel(Q4Args A) {
   int chunk = (int)(all * A.target_inv + 0.999f);
   if (A.splits > 2) chunk = max(chunk, (int)((float)top * A.splits_inv) + 1);
   chunk = max(chunk, 1);
-  float inv;
-  bool apart;
+  const int equal = chunk;
+  float inv = __builtin_amdgcn_rcpf((float)chunk);
+  bool apart = A.num_seqs <= 64;
   auto padded = [&](int r) {
     if (!apart) return r;
     const int q = small_div(r, chunk, inv);
     return q * chunk < r ? (q + 1) * chunk : r;
   };
-  for (int i = 0;; ++i) {
-    inv = __builtin_amdgcn_rcpf((float)chunk);
-    apart = chunk < APART;
-    if (!apart || A.num_seqs > 64 || i == 3 || chunk >= top) break;
-    // a little longer parts where the tiles' ends make too many
+  while (apart) {
     const float sum = wave_sum((float)(tiles * padded(rounds)));
-    if (sum <= (float)(chunk * A.target)) break;
+    if (sum <= (float)(chunk * A.target) || chunk >= top) break;
+    // the tiles' ends make too many: somewhat longer parts
     chunk = min(max(chunk + 1, (int)(sum * A.target_inv + 0.999f)), top);
+    apart = chunk <= equal + BEGIN;
+    if (!apart) chunk = equal;
+    inv = __builtin_amdgcn_rcpf((float)chunk);
   }
   chunk = __builtin_amdgcn_readfirstlane(chunk);
   // Part after part (one, unless there are more than workgroups), piece after piece.
