@@ -514,7 +514,8 @@ void q4_attention_kernel(Q4Args A) {
 }
 
 // How a call is cut, from its sizes (lengths are on the device).  512 workgroups fill the
-// chip once (73 KB of LDS and 216 registers: two a compute unit).
+// chip once (two a compute unit, by their registers).  Twice as many parts, 48 sequences
+// behind 2000 to 32000 152 us for 155, but 16 behind 300 to 8000 22 for 19.
 constexpr int FILL = 512, MAX_PARTS = 64;
 
 int tune(const char* name, int v) {
@@ -526,19 +527,30 @@ struct Q4Choice {
   int splits, target;
 };
 
-// Whether a call's rows are prompts': more than two tiles of a sequence on average.
-bool is_prompt(int64_t num_tokens, int64_t num_seqs, int group) {
-  return num_tokens * group > tune("SMX_Q4_ROWS", 32) * num_seqs;
-}
-
+// Tiles of 16 rows, the most there can be.
 int64_t q4_tiles(int64_t num_tokens, int64_t num_seqs, int group) {
   return (num_tokens * group + 15) / 16 + num_seqs - 1;
+}
+
+// Whether a call's rows are prompts': more than two tiles of a sequence on average, and
+// more work altogether than tiles of 16 rows, which widen every code and scale again,
+// are done with first (the tables' capacity stands for the lengths, and a tile's
+// beginning counts as three rounds).  us by tiles / by the prompt kernels, and the work, 32
+// / 8 heads of 128: 100 tokens 8.0 / 9.7 (0.8k), 8 x 20 behind 1000 22 / 31 (3.5k), 300
+// tokens 14.8 / 14.3 (3.6k), 40 behind 8000 27 / 30 (5.3k), 16 x 60 25 / 13 (7.7k), 8 x 60
+// behind 1000 37 / 33 (12k), 60 behind 15000 54 / 47 (15k); heads of 64: 1000 tokens, 14 / 2
+// heads 19 / 23 (9.6k), 8 x 100 behind 500, 16 / 4 18 / 16 (6.4k), 500 behind 4000, 14 / 2
+// 45 / 40 (17k).
+bool is_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv, int hd) {
+  if (num_tokens * group <= 32 * num_seqs) return false;
+  const int64_t work = q4_tiles(num_tokens, num_seqs, group) * ((cap + ROUND - 1) / ROUND + 3) * n_kv;
+  return work > tune("SMX_Q4_WORK", hd == 64 ? 9600 : 5500);
 }
 
 Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
   Q4Choice c{};
   const int64_t rounds = (cap + ROUND - 1) / ROUND;  // the most of a tile
-  c.target = std::max(1, tune("SMX_Q4_FILL", FILL) / n_kv);
+  c.target = std::max(1, FILL / n_kv);
   // uneven lengths: the longest may take four times the parts of even ones
   const int64_t even = (c.target + num_seqs - 1) / num_seqs;
   c.splits = (int)std::clamp<int64_t>(4 * even + 2, 3, MAX_PARTS);
@@ -562,7 +574,8 @@ extern "C" int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_se
   if (num_tokens < 1 || num_seqs < 1 || max_blocks < 1 || block_size < 1 || n_kv < 1 ||
       n_q < n_kv || n_q % n_kv || head_dim < 1)
     return -1;
-  if (smx::is_prompt(num_tokens, num_seqs, n_q / n_kv)) {
+  if (smx::is_prompt(num_tokens, num_seqs, (int64_t)max_blocks * block_size, n_q / n_kv,
+                     n_kv, head_dim)) {
     smx::Q4Prompt p{};
     p.num_tokens = num_tokens;
     p.num_seqs = num_seqs;
@@ -610,7 +623,8 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
   int bs_log2 = 0;
   while ((1 << bs_log2) < block_size) ++bs_log2;
   const float scale_log2 = scale * 1.44269504088896340736f;
-  if (smx::is_prompt(num_tokens, num_seqs, n_q / n_kv)) {
+  if (smx::is_prompt(num_tokens, num_seqs, (int64_t)max_blocks * block_size, n_q / n_kv,
+                     n_kv, head_dim)) {
     const smx::Q4Prompt p{(const uint16_t*)q, (const uint8_t*)codes, (const uint16_t*)scales,
                           block_table, query_start_loc, seq_lens, workspace, out, q_stride,
                           num_tokens, num_seqs, max_blocks, num_blocks, bs_log2, n_q, n_kv,

@@ -46,8 +46,12 @@ class Case:
 
     def prompts(self):
         """Whether the rows go to the kernels that round the cache's values to bf16: more
-        than 32 (token, head in the group) pairs a sequence on average, padding among them."""
-        return self.q.shape[0] * (self.q.shape[1] // self.codes.shape[2]) > 32 * len(self.lens)
+        than 32 (token, head in the group) pairs a sequence on average, padding among them,
+        and more than so many tiles of 16 of them times 128 tokens."""
+        hd, n_kv, bs = self.q.shape[2], self.codes.shape[2], self.codes.shape[3]
+        rows, seqs = self.q.shape[0] * (self.q.shape[1] // n_kv), len(self.lens)
+        work = (-(-rows // 16) + seqs - 1) * (-(-self.table.shape[1] * bs // 128) + 3) * n_kv
+        return rows > 32 * seqs and work > (9600 if hd == 64 else 5500)
 
     def reference(self):
         """(out, sum p |v|, sum p |d|, the largest scale sum |q k| of a seen token, row is of
@@ -118,7 +122,21 @@ CASES = [
     ([257], [0], 64, 1, 64, 32, 0),
     ([9], [500], 100, 1, 64, 64, 0),
     ([2], [300], 34, 2, 128, 4096, 0),
+    # many rows: on both sides of what goes to the prompt kernels
+    ([64, 100, 3], [0, 333, 900], 32, 8, 128, 32, 4),
+    ([300], [0], 32, 8, 128, 64, 0),
+    ([310, 77], [31, 500], 40, 8, 128, 128, 3),
+    ([200, 1, 450], [64, 1000, 0], 16, 4, 64, 32, 0),
+    ([500], [300], 28, 4, 64, 128, 2),
+    ([40, 40, 40, 40, 0, 1], [700, 0, 50, 64, 0, 9], 64, 16, 64, 64, 0),
+    ([1, 600], [0, 40], 16, 1, 128, 256, 0),
 ]
+
+
+def test_cases_reach_both_kernels():
+    kinds = {hd: {Case(1, n, ctx, n_q, n_kv, hd, bs, pad).prompts()
+                  for n, ctx, n_q, n_kv, h, bs, pad in CASES if h == hd} for hd in (64, 128)}
+    assert kinds == {64: {True, False}, 128: {True, False}}
 
 
 @pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
@@ -157,12 +175,12 @@ def test_rows_that_see_nothing_are_zero():
     assert got[2].any() and got[9].any()
 
 
-@pytest.mark.parametrize("n,ctx", [([1], [40]), ([6], [90]), ([40], [30])])
+@pytest.mark.parametrize("n,ctx", [([1], [40]), ([6], [90]), ([40], [30]), ([700], [30])])
 @pytest.mark.parametrize("hd", [64, 128])
 def test_what_is_not_seen_does_not_count(n, ctx, hd):
     """NaN and infinite scales and any codes behind the last token of a page, on pages that no
     sequence lists and at later tokens of other rows' pages."""
-    c = Case(5, n + [2], ctx + [3], 8, 2, hd, 32)
+    c = Case(5, n + [2], ctx + [3], 16, 4, hd, 32)
     clean = c.run()
     bs = 32
     for r in range(2):
@@ -179,28 +197,31 @@ def test_what_is_not_seen_does_not_count(n, ctx, hd):
     assert torch.equal(clean.view(torch.int16), c.run().view(torch.int16))
 
 
-def test_later_tokens_do_not_reach_earlier_rows():
+@pytest.mark.parametrize("n,n_q,n_kv", [(50, 4, 1), (450, 32, 8)])
+def test_later_tokens_do_not_reach_earlier_rows(n, n_q, n_kv):
     """A prompt whose last token's K and V are NaN: only the row that sees it is NaN."""
-    c = Case(6, [50], [0], 4, 1, 128, 32)
-    page, at = int(c.table[0, 49 // 32]), 49 % 32
+    c = Case(6, [n], [0], n_q, n_kv, 128, 32)
+    assert c.prompts() == (n > 400)
+    page, at = int(c.table[0, (n - 1) // 32]), (n - 1) % 32
     for plane in range(2):
         save = c.scales[plane, page, :, at].clone()
         c.scales[plane, page, :, at] = math.nan
         got = c.run().cpu()
-        assert got[49].isnan().all()
-        assert torch.isfinite(got[:49]).all()
+        assert got[n - 1].isnan().all()
+        assert torch.isfinite(got[:n - 1]).all()
         c.scales[plane, page, :, at] = save
 
 
 @pytest.mark.parametrize("bad", [-1, 10 ** 6])
-def test_entries_outside_the_cache(bad):
+@pytest.mark.parametrize("heads,spare", [((8, 2), 1), ((32, 8), 90)])
+def test_entries_outside_the_cache(bad, heads, spare):
     """Rows that see a token whose table entry is outside the cache are NaN, the others are
     what they were."""
-    c = Case(7, [100, 3], [0, 60], 8, 2, 128, 32)
+    c = Case(7, [100, 3], [0, 60], *heads, 128, 32, spare=spare)
+    assert c.prompts() == (spare > 1)
     clean = c.run().cpu()
     c.table[0, 2] = bad  # tokens 64..95
     c.table[1, 2:] = bad  # (entries past the length are not looked at)
-    c.lens[1] = 63
     c.lens[1] = 64
     got = c.run().cpu()
     assert got[64:100].isnan().all()
