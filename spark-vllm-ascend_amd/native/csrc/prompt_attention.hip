@@ -220,10 +220,13 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     stage(A.vc, dst, page, base, [](int r) { return v_swz<HD>(r); });
   };
   // A cache in 4 bits: a lane has a quarter of a token's row, K's dwords of every block's
-  // eight channels 8 (lane & 3) .., and V's NB dwords in channel order, of one block.
+  // eight channels 8 qg .., and V's NB dwords in channel order, of one block.  Sixteen
+  // neighbours have sixteen tokens, which write their values to different banks.
   constexpr int NB = HD / 32, RB = HD / 2;
-  uint32_t kq[NB], vq[NB], kd[NB / 2], vd = 0;
-  const int qtok = (wm * 64 + lane) >> 2, qg = lane & 3;
+  typedef uint32_t Dwords __attribute__((ext_vector_type(NB)));
+  Dwords kq, vq;
+  uint32_t kd[NB / 2], vd = 0;
+  const int qtok = 16 * wm + (lane & 15), qg = lane >> 4;
   auto fetch = [&](const int (&page)[NP], int base) {
     static_assert(!Q4 || (KT == 16 * WM && ST == 2), "a quarter of a row a lane, two buffers");
     const int u = NP > 1 && 16 * wm >= BT ? NP - 1 : 0;
@@ -241,16 +244,12 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
                                                            0x00027000);
       const auto scales = __builtin_amdgcn_make_buffer_rsrc((void*)(A.scales + r * NB), 0,
                                                             rows * 2 * NB, 0x00027000);
-      uint32_t* const w = v ? vq : kq;
-      if constexpr (NB == 4) {
-        const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(codes, at * RB + 16 * qg, 0, 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = x[i];
-      } else {
-        const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(codes, at * RB + 8 * qg, 0, 0);
-        w[0] = x[0];
-        w[1] = x[1];
-      }
+      Dwords w;
+      if constexpr (NB == 4)
+        w = __builtin_amdgcn_raw_buffer_load_b128(codes, at * RB + 16 * qg, 0, 0);
+      else
+        w = __builtin_amdgcn_raw_buffer_load_b64(codes, at * RB + 8 * qg, 0, 0);
+      (v ? vq : kq) = w;
       if (v) {
         vd = __builtin_amdgcn_raw_buffer_load_b16(scales, at * 2 * NB + 2 * (NB * qg / 4), 0, 0);
       } else if constexpr (NB == 4) {
@@ -264,7 +263,9 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   };
   // Eight values of scale d as bf16: bytes of half-bytes 0, 2, 4, 6 (lo) and 1, 3, 5, 7 (hi).
   auto widen = [](uint32_t w, float d, bool key) -> u32x4 {
-    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    // (so that a byte's conversion is one instruction, not a bit field's and one)
+    __asm__("" : "+v"(lo), "+v"(hi));
     const float off = -8.f * d;
     auto val = [&](uint32_t x, int i) { return fmaf((float)((x >> (8 * i)) & 0xffu), d, off); };
     if (key)
@@ -279,10 +280,20 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       const float d = f16_bits_to_f32(kd[b / 2] >> (16 * (b & 1)) & 0xffffu);
       dst[qtok * CH + ((4 * b + qg) ^ k_swz<HD>(qtok))] = widen(kq[b], d, true);
     }
+    // V's swizzle goes by two bits of the token: the others turn the order of the dwords
     const float d = f16_bits_to_f32(vd);
+    const int turn = (qtok >> 2) & (NB - 1);
+    Dwords w = vq;
+    if constexpr (NB == 4) {
+      w = turn & 1 ? w.yzwx : w;
+      w = turn & 2 ? w.zwxy : w;
+    } else {
+      w = turn & 1 ? w.yx : w;
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j)
-      dst[S::TILE + qtok * CH + ((NB * qg + j) ^ v_swz<HD>(qtok))] = widen(vq[j], d, false);
+      dst[S::TILE + qtok * CH + ((NB * qg + ((j + turn) & (NB - 1))) ^ v_swz<HD>(qtok))] =
+          widen(w[j], d, false);
   };
   auto bad_pages = [&](const int (&page)[NP]) {
     int bad = 0;
