@@ -226,10 +226,13 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   typedef uint32_t Dwords __attribute__((ext_vector_type(NB)));
   Dwords kq, vq;
   uint32_t kd[NB / 2], vd = 0;
-  const int qtok = 16 * wm + (lane & 15), qg = lane >> 4;
+  // With eight waves to share a tile, the first four have K and the others V.
+  constexpr int SHARE = WM == 8 ? 4 : WM;
+  const int qwave = wm % SHARE, qtok = 16 * qwave + (lane & 15), qg = lane >> 4;
+  const bool has[2] = {WM <= SHARE || wm < SHARE, WM <= SHARE || wm >= SHARE};
   auto fetch = [&](const int (&page)[NP], int base) {
-    static_assert(!Q4 || (KT == 16 * WM && ST == 2), "a quarter of a row a lane, two buffers");
-    const int u = NP > 1 && 16 * wm >= BT ? NP - 1 : 0;
+    static_assert(!Q4 || (KT == 16 * SHARE && ST == 2), "a quarter of a row a lane, two buffers");
+    const int u = NP > 1 && 16 * qwave >= BT ? NP - 1 : 0;
     const int t = base + BT * u;
     const bool known = (unsigned)page[u] < (unsigned)A.num_blocks;
     const int rows = known ? max(min(it.to - t, BT), 0) : 0;
@@ -239,6 +242,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     const int at = qtok - BT * u;
 #pragma unroll
     for (int v = 0; v < 2; ++v) {
+      if (!has[v]) continue;
       const int64_t r = v ? row + plane : row;
       const auto codes = __builtin_amdgcn_make_buffer_rsrc((void*)(A.codes + r * RB), 0, rows * RB,
                                                            0x00027000);
@@ -274,12 +278,14 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     return u32x4{cvt_pk_bf16(val(lo, 0), val(hi, 0)), cvt_pk_bf16(val(lo, 1), val(hi, 1)),
                  cvt_pk_bf16(val(lo, 2), val(hi, 2)), cvt_pk_bf16(val(lo, 3), val(hi, 3))};
   };
-  auto fill = [&](lds_u32x4* dst) {
+  auto fill_k = [&](lds_u32x4* dst) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const float d = f16_bits_to_f32(kd[b / 2] >> (16 * (b & 1)) & 0xffffu);
       dst[qtok * CH + ((4 * b + qg) ^ k_swz<HD>(qtok))] = widen(kq[b], d, true);
     }
+  };
+  auto fill_v = [&](lds_u32x4* dst) {
     // V's swizzle goes by two bits of the token: the others turn the order of the dwords
     const float d = f16_bits_to_f32(vd);
     const int turn = (qtok >> 2) & (NB - 1);
@@ -468,7 +474,8 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       fetch(page, first + wn * KT);
       bad[0] = bad_pages(page);
       look_up(page, first + (wn + WN) * KT);
-      fill(lds);
+      if (has[0]) fill_k(lds);
+      if (has[1]) fill_v(lds);
       fetch(page, first + (wn + WN) * KT);  // (past the end: of no rows, without an access)
       bad_fetched = bad_pages(page);
       look_up(page, first + (wn + 2 * WN) * KT);
@@ -492,11 +499,14 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     // the branch that would keep the addresses' arithmetic from the products' shadow)
     if (plain || tile + (ST - 1) * WN < ntiles) {
       if constexpr (Q4) {
-        fill(next);
         bad[1] = bad_fetched;
-        fetch(page, ahead + WN * KT);
-        bad_fetched = bad_pages(page);
-        look_up(page, ahead + 2 * WN * KT);
+        if (has[0]) fill_k(next);
+        if (WM <= SHARE) {
+          fill_v(next);
+          fetch(page, ahead + WN * KT);
+          bad_fetched = bad_pages(page);
+          look_up(page, ahead + 2 * WN * KT);
+        }
       } else {
         stage_k(next, page, ahead);
         stage_v(next + S::TILE, page, ahead);
@@ -504,10 +514,20 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
         look_up(page, ahead + WN * KT);
       }
     }
-    if ((!plain && tile >= ntiles) || 32 * wm >= it.rows) return;
-    scores(cur);
-    softmax(plain, base, bad[0]);
-    weigh(plain, cur + S::TILE, base);
+    if (!(!plain && tile >= ntiles) && 32 * wm < it.rows) {
+      scores(cur);
+      softmax(plain, base, bad[0]);
+      weigh(plain, cur + S::TILE, base);
+    }
+    if constexpr (Q4 && WM > SHARE) {
+      // (V after this tile's products: a SIMD's two waves widen and multiply in turn)
+      if (plain || tile + (ST - 1) * WN < ntiles) {
+        if (has[1]) fill_v(next);
+        fetch(page, ahead + WN * KT);
+        bad_fetched = bad_pages(page);
+        look_up(page, ahead + 2 * WN * KT);
+      }
+    }
   };
   int at = 0, rd = 0;  // the buffer of this round's tile
   auto step = [&](auto plain) {
@@ -944,7 +964,17 @@ struct Choice {
 // contexts 128 rows are better: 509 behind 16000 170 / 153, 500 behind 4000 60 / 60.
 // Parts are of at least 256 tokens: 300 behind 1500 31.5 at 512, 32.2 at 256, one
 // token behind 900 14.6 at 512, 12.3 at 256.
-Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
+//
+// Over a cache in 4 bits a tile is widened once for a workgroup's rows, half of a wave's
+// vector instructions with 128 of them, so that 256 (one workgroup a compute unit, eight
+// waves) are the faster where they fill the chip: cut, or behind a context from nine
+// tenths of a filling on, or from twice that on.  us, rows of 64 / 128 / 256: 500 tokens
+// behind 4000 85 / 71 / 64, 300 behind 30000 324 / 225 / 194, 2000 behind 8000 520 / 369 /
+// 335, 16 x 100 behind 1000 78 / 58 / 52, 4000 236 / 182 / 165, 8000 874 / 639 / 588; but
+// 1000 behind 3000 111 / 130 / 139, 2000 82 / 73 / 79, 4000, 16 / 4 heads of 64 82 / 91 /
+// 102.
+Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv,
+                     bool q4 = false) {
   Choice c{};
   const int64_t rows = (num_tokens * group + num_seqs - 1) / num_seqs;  // of a sequence
   auto groups = [&](int m) { return (rows + m - 1) / m * num_seqs * n_kv; };  // of even lengths
@@ -955,9 +985,11 @@ Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int grou
   const bool few = (float)(cap / 64) * (1.f - 1.45f * groups(64) / FILL) >= c.gain &&
                    !(rows <= 64 && cap < 4096 && groups(64) >= 160);
   if (few && rows > 1024 && cap >= 8192) c.m = 128;
-  c.m = tune("SMX_PA_M", c.m) < 128 ? 64 : 128;
+  if (q4 && rows > 128 && (few || groups(256) >= (behind ? 230 : 460))) c.m = 256;
+  c.m = tune("SMX_PA_M", c.m);
+  c.m = c.m < 128 ? 64 : c.m < 256 || !q4 ? 128 : 256;
   c.tiles = (int)((num_tokens * group + c.m - 1) / c.m + num_seqs - 1);
-  c.target = std::max(1, FILL / n_kv);
+  c.target = std::max(1, (c.m == 256 ? FILL / 2 : FILL) / n_kv);
   if (few) {
     const int64_t even = (FILL + groups(c.m) - 1) / groups(c.m);
     const int64_t most = num_seqs == 1 ? even : num_tokens * group <= 1024 ? 4 * even : 2 * even;
@@ -1015,13 +1047,20 @@ int64_t items_bound(int64_t tiles, int target, int splits) {
 
 template <int HD, bool Q4>
 int launch_prompt(hipStream_t stream, RowsArgs& a, const Choice& c) {
-  a.zigzag = a.num_seqs == 1 && (int64_t)c.tiles * a.n_kv <= 2 * FILL ? std::max(1, 256 / a.n_kv)
+  a.zigzag = c.m < 256 && a.num_seqs == 1 && (int64_t)c.tiles * a.n_kv <= 2 * FILL ? std::max(1, 256 / a.n_kv)
                                                                       : 1 << 30;
   a.target = c.target;
   a.least = 256 / 64;
   a.gain = c.gain;
   const dim3 grid(a.n_kv, (unsigned)items_bound(c.tiles, c.target, c.splits));
-  if (c.m == 64)
+  if (Q4 && c.m == 256) {
+    if constexpr (Q4) {  // (no such instance for bf16 caches)
+      if (a.bs_log2 > 5)
+        SMX_LAUNCH((prompt_attention_kernel<HD, 8, 1, 64, 2, 64, Q4>), grid, dim3(512), 0, stream, a);
+      else
+        SMX_LAUNCH((prompt_attention_kernel<HD, 8, 1, 64, 2, 32, Q4>), grid, dim3(512), 0, stream, a);
+    }
+  } else if (c.m == 64)
     SMX_LAUNCH((prompt_attention_kernel<HD, 2, 2, 32, 2, 32, Q4>), grid, dim3(256), 0, stream, a);
   else if (a.bs_log2 > 5)
     SMX_LAUNCH((prompt_attention_kernel<HD, 4, 1, 64, 2, 64, Q4>), grid, dim3(256), 0, stream, a);
@@ -1072,14 +1111,14 @@ int merge_rows(hipStream_t stream, int head_dim, const float* part_o, const floa
 
 int64_t q4_prompt_workspace(const Q4Prompt& p) {
   const Choice c = choose_prompt(p.num_tokens, p.num_seqs, (int64_t)p.max_blocks << p.bs_log2,
-                                 p.n_q / p.n_kv, p.n_kv);
+                                 p.n_q / p.n_kv, p.n_kv, true);
   if (items_bound(c.tiles, c.target, c.splits) > 65535) return -1;
   return partial_bytes((int64_t)p.num_tokens * p.n_q, c.splits, p.head_dim);
 }
 
 int q4_prompt(hipStream_t stream, const Q4Prompt& p) {
   const Choice c = choose_prompt(p.num_tokens, p.num_seqs, (int64_t)p.max_blocks << p.bs_log2,
-                                 p.n_q / p.n_kv, p.n_kv);
+                                 p.n_q / p.n_kv, p.n_kv, true);
   RowsArgs a{};
   a.q = p.q;
   a.codes = p.codes;
