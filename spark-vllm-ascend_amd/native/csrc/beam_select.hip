@@ -6,10 +6,9 @@
 // One pass over the logits.  A beam's best are its largest logits, so a workgroup keeps
 // the `width` largest of its part of a row and the part's maximum and sum of exponentials
 // (beam_parts_kernel); a workgroup a sequence then takes the best of the parts'
-// (beam_merge_kernel).  Beams are compared by their sums, so these are taken in 64 bits,
-// with exponentials good to 4e-11: two beams' candidates whose scores differ by less
-// than that might be taken in the wrong order, where fp32 sums would confuse those within
-// 1e-6.  64-bit fma runs at the rate of the 32-bit one on this chip.
+// (beam_merge_kernel).  Beams are compared by their sums, so these are good to about 1e-9
+// and joined in 64 bits: two beams' candidates whose scores differ by less than that might
+// be taken in the wrong order, where fp32 sums would confuse those within 1e-6.
 //
 // A NaN logit counts as -inf, a token that is never chosen; of several logits of +inf each
 // has an equal share.
@@ -25,7 +24,7 @@ namespace smx {
 namespace {
 
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
-typedef double f64x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
 constexpr int CAP = 128;  // candidates of a wave
@@ -46,66 +45,48 @@ struct BeamArgs {
   int seqs, beams, width, vocab, parts, pad_id;
 };
 
-// exp(a) for a <= 0, relative error 4e-11 (a below -700: something below 1e-304):
-// a = n ln 2 + r with |r| <= ln 2 / 2, a polynomial of degree 7 fitted to exp on that
-// interval by least squares reweighted towards the largest relative error, and n added to
-// the exponent's bits.
-__device__ __forceinline__ double exp_le0(double a) {
-  a = fmax(a, -700.0);
+// exp(a) for |a| <= 700, relative error 8e-13: a = n ln 2 + r with |r| <= ln 2 / 2, a
+// polynomial of degree 8 fitted to exp on that interval by least squares reweighted
+// towards the largest relative error, and n added to the exponent's bits.
+__device__ __forceinline__ double exp_any(double a) {
   const double magic = 0x1.8p52;  // its sum's low bits are the rounded quotient
   const double t = fma(a, 1.4426950408889634, magic);
-  const double n = t - magic;
-  const double r = fma(n, -0.6931471805599453, a);
-  double p = 0x1.9eb71c629715ep-13;
-  p = fma(p, r, 0x1.6da4bf9e8e8dfp-10);
-  p = fma(p, r, 0x1.1112fa548f5cbp-7);
-  p = fma(p, r, 0x1.5554685b28249p-5);
-  p = fma(p, r, 0x1.55555343bd2bcp-3);
-  p = fma(p, r, 0x1.00000059d83e1p-1);
-  p = fma(p, r, 0x1.000000010b76ep+0);
-  p = fma(p, r, 0x1.ffffffffabae7p-1);
+  const double r = fma(t - magic, -0.6931471805599453, a);
+  double p = 0x1.9eda514635a5bp-16;
+  p = fma(p, r, 0x1.a1a83103871fap-13);
+  p = fma(p, r, 0x1.6c18b3a477d5cp-10);
+  p = fma(p, r, 0x1.111082a0498a6p-7);
+  p = fma(p, r, 0x1.55555404b7c02p-5);
+  p = fma(p, r, 0x1.555555a08d61dp-3);
+  p = fma(p, r, 0x1.0000000088227p-1);
+  p = fma(p, r, 0x1.ffffffffd55a3p-1);
+  p = fma(p, r, 0x1.ffffffffff79dp-1);
   const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-  const uint32_t low = (uint32_t)__builtin_bit_cast(uint64_t, t);
-  return __builtin_bit_cast(double, bits + ((uint64_t)(low << 20) << 32));
+  const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
 }
 
-// Values in their order as unsigned integers (no NaN, no -0 among them).
-__device__ __forceinline__ uint32_t order_key(float f) {
-  const uint32_t u = __float_as_uint(f);
-  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+// exp(x - top) for a part's maximum x <= top, either of them infinite (top not -inf, or
+// neither counts: their sums are 0).
+__device__ __forceinline__ double exp_between(float x, float top) {
+  return x == top ? 1.0 : exp_any(fmax((double)x - (double)top, -700.0));
 }
-__device__ __forceinline__ float order_value(uint32_t k) {
-  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
-}
-constexpr uint32_t LEAST = 0x00800000u;  // the order key of the least finite value
 
-// A candidate of a part: bf16 values and the place in the part (below 65536) in 32 bits,
-// fp32 ones in 64; a larger key is a larger value, or the same at a lower place.
-template <typename L>
-struct Keys;
-template <>
-struct Keys<uint16_t> {
-  typedef uint32_t Key;
-  static constexpr Key NONE = LEAST - 1;
-  static __device__ __forceinline__ Key make(float f, uint32_t at) {
-    return (order_key(f) & 0xffff0000u) | (0xffffu - at);
-  }
-  static __device__ __forceinline__ float value(Key k) {
-    // (a negative value's low bits are the complement of its key's)
-    return order_value(k & 0x80000000u ? k & 0xffff0000u : k | 0xffffu);
-  }
-  static __device__ __forceinline__ uint32_t place(Key k) { return 0xffffu - (k & 0xffffu); }
-};
-template <>
-struct Keys<float> {
-  typedef uint64_t Key;
-  static constexpr Key NONE = (uint64_t)LEAST << 32 | 0;
-  static __device__ __forceinline__ Key make(float f, uint32_t at) {
-    return (uint64_t)order_key(f) << 32 | (0xffffffffu - at);
-  }
-  static __device__ __forceinline__ float value(Key k) { return order_value((uint32_t)(k >> 32)); }
-  static __device__ __forceinline__ uint32_t place(Key k) { return 0xffffffffu - (uint32_t)k; }
-};
+// Values in their order as signed integers: the bits of positive ones, minus those of
+// negative ones' magnitudes, so that -0 is 0.
+__device__ __forceinline__ int order_key(uint32_t u) {
+  const int m = (int)u >> 31;
+  return (int)((u & 0x7fffffffu) ^ m) - m;
+}
+__device__ __forceinline__ float order_value(int k) {
+  return __uint_as_float(k < 0 ? (uint32_t)-k | 0x80000000u : (uint32_t)k);
+}
+// The same of two bf16 values in a dword, 16 bits each.
+__device__ __forceinline__ s16x2 order_keys(uint32_t w) {
+  const s16x2 m = __builtin_bit_cast(s16x2, w) >> 15;
+  return __builtin_bit_cast(s16x2, (w & 0x7fff7fffu) ^ __builtin_bit_cast(uint32_t, m)) - m;
+}
+constexpr int INF_KEY = 0x7f800000;
 
 // The value of lane ^ MASK, once the lanes of each group of MASK hold the same value.
 template <int MASK, typename K>
@@ -159,16 +140,20 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return v;
 }
 
-// One part (NT * E logits) of one row.  Each wave reads its share once into registers,
-// finds a bound that `width` of its values reach from its lanes' maxima, and collects
-// those that reach it; the few collected of all waves are ranked by counting.
-template <typename L, int E>
+// One part (NT * LOADS * V logits) of one row, a wave's share of it in registers: its
+// maximum, the values that reach a bound which `width` of its own do (found from its
+// lanes' maxima), and its sum of exponentials; the few collected of all waves are ranked
+// by counting.
+//
+// The sum: exp by the transcendental unit, whose errors are a few 1e-8 of each term, and
+// again in 64 bits for the collected values, which are most of a peaked row's sum; so what
+// is left is 1e-9 of it, and less where many terms' errors average out.
+template <typename L, int LOADS>
 __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
-  typedef Keys<L> Ks;
-  typedef typename Ks::Key Key;
   constexpr int V = 16 / sizeof(L);  // logits of a load
-  constexpr int LOADS = E / V;
-  __shared__ Key list[WAVES * CAP];
+  constexpr int PART = NT * LOADS * V;
+  __shared__ uint64_t list[WAVES * CAP];
+  __shared__ u32x4 tail_s;
   __shared__ int count_s[WAVES];
   __shared__ float max_s[WAVES];
   __shared__ double sum_s[WAVES];
@@ -178,101 +163,213 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   // a beam that is done, or has no score, offers nothing from its logits
   if (A.done && A.done[row]) return;
   if (!(A.scores[row] > -INFINITY)) return;
-  const int first = part * (NT * E), here = min(A.vocab - first, NT * E);
+  const int first = part * PART, here = min(A.vocab - first, PART);
   const L* const src = reinterpret_cast<const L*>(A.logits) + (int64_t)row * A.stride + first;
+  typedef L __attribute__((may_alias)) Value;
+  constexpr uint32_t NONE = sizeof(L) == 2 ? 0xff80ff80u : 0xff800000u;  // -inf
 
-  float x[E];
+  u32x4 x[LOADS];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i) {
     const int at = (i * NT + tid) * V;
-    u32x4 w;
-    if (at + V <= here) {
-      w = *reinterpret_cast<const u32x4_a2*>(src + at);
-    } else {
-      if constexpr (V == 8) {
+    x[i] = u32x4{NONE, NONE, NONE, NONE};
+    if (at + V <= here) x[i] = *reinterpret_cast<const u32x4_a2*>(src + at);
+  }
+  if (here < PART) {
+    // the row's last few logits, by the thread that has their place
+    const int chunk = here / V;
+    if (tid == chunk % NT) {
+      tail_s = u32x4{NONE, NONE, NONE, NONE};
+      for (int j = chunk * V; j < here; ++j)
+        reinterpret_cast<Value*>(&tail_s)[j - chunk * V] = src[j];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t lo = at + 2 * j < here ? (uint32_t)src[at + 2 * j] : 0xff80u;
-          const uint32_t hi = at + 2 * j + 1 < here ? (uint32_t)src[at + 2 * j + 1] : 0xff80u;
-          w[j] = lo | hi << 16;
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          w[j] = at + j < here ? __float_as_uint(src[at + j]) : 0xff800000u;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      float f;
-      if constexpr (V == 8)
-        f = j & 1 ? bf16_hi(w[j / 2]) : bf16_lo(w[j / 2]);
-      else
-        f = __uint_as_float(w[j]);
-      x[i * V + j] = fmaxf(f, -INFINITY) + 0.f;  // NaN as -inf, -0 as 0
+      for (int i = 0; i < LOADS; ++i)
+        if (i == chunk / NT) x[i] = tail_s;
     }
   }
-  float top = -INFINITY;
-#pragma unroll
-  for (int e = 0; e < E; ++e) top = fmaxf(top, x[e]);
-  top = wave_max(top);
 
-  // ---- the sum of exponentials
-  double sum = 0.0;
-  if (top > -INFINITY) {
-    double s0 = 0.0, s1 = 0.0;
-    const double topd = (double)top;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      s0 += exp_le0(x[e] == top ? 0.0 : (double)x[e] - topd);
-      s1 += exp_le0(x[e + 1] == top ? 0.0 : (double)x[e + 1] - topd);
+  // Value j of load i: its key.
+  auto key_of = [&](int i, int j) -> int {
+    if constexpr (V == 8) {
+      const uint32_t w = __builtin_bit_cast(uint32_t, order_keys(x[i][j / 2]));
+      return j & 1 ? (int)w : (int)(w << 16);  // (an odd one's lower half is below every step)
+    } else {
+      return order_key(x[i][j]);
     }
-    sum = wave_sum64(s0 + s1);
+  };
+  constexpr int STEP = V == 8 ? 0x10000 : 1;  // between two keys
+  auto exact = [&](int key) { return V == 8 ? key & ~0xffff : key; };
+  // ---- the lanes' maxima
+  int best;
+  auto maxima = [&]() {
+    if constexpr (V == 8) {
+      s16x2 m = {-32768, -32768};
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, order_keys(x[i][j]));
+      best = max((int)m[0], (int)m[1]) << 16;
+    } else {
+      best = INT_MIN;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) best = max(best, key_of(i, j));
+    }
+  };
+  maxima();
+  if (__builtin_amdgcn_ballot_w64(best > INF_KEY)) {
+    // a NaN (one with its sign set is below -inf): -inf in its place
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w = x[i][j];
+        if constexpr (V == 8) {
+          if ((w & 0x7fffu) > 0x7f80u) w = (w & 0xffff0000u) | 0xff80u;
+          if ((w & 0x7fff0000u) > 0x7f800000u) w = (w & 0xffffu) | 0xff800000u;
+        } else {
+          if ((w & 0x7fffffffu) > 0x7f800000u) w = NONE;
+        }
+        x[i][j] = w;
+      }
+    maxima();
   }
+  int top_key = best;
+  top_key = max(top_key, other<1>(top_key));
+  top_key = max(top_key, other<2>(top_key));
+  top_key = max(top_key, other<4>(top_key));
+  top_key = max(top_key, other<8>(top_key));
+  top_key = max(top_key, other<16>(top_key));
+  top_key = max(top_key, other<32>(top_key));
+  const float top = order_value(max(top_key, -INF_KEY));
 
   // ---- the largest
-  Key key[E], best = 0;
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int e = i * V + j;
-      key[e] = Ks::make(x[e], (uint32_t)((i * NT + tid) * V + j));
-      best = max(best, key[e]);
-    }
   int groups = 1;
   while (groups < A.width) groups <<= 1;
-  Key bound = max(least_of_maxima(best, groups), (Key)(Ks::NONE + 1));
-  auto reach = [&](Key b) {
-    int c = 0;
+  constexpr int LOWEST = -INF_KEY + STEP;  // the lowest finite value's
+  int bound = max(least_of_maxima(best, groups), LOWEST);
+  uint64_t* const mine = list + wave * CAP;
+  int n = 0;
+  // Puts the values that `in(i, j)` says into the list, in no particular order: a bit a
+  // value, the set ones of a load lane by lane.
+  auto collect = [&](int i, auto in) {
+    uint32_t bits = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) c += __popcll(__builtin_amdgcn_ballot_w64(key[e] >= b));
-    return c;
+    for (int j = 0; j < V; ++j) bits = bits + bits + (in(j) ? 1u : 0u);
+    while (const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0)) {
+      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      if (bits && at < CAP) {
+        const int low = __ffs(bits) - 1, j = V - 1 - low;
+        uint32_t w;
+        if constexpr (V == 8) {
+          const uint32_t lo = j & 2 ? x[i][1] : x[i][0], hi = j & 2 ? x[i][3] : x[i][2];
+          w = j & 4 ? hi : lo;
+          w = j & 1 ? w & 0xffff0000u : w << 16;
+        } else {
+          const uint32_t lo = j & 1 ? x[i][1] : x[i][0], hi = j & 1 ? x[i][3] : x[i][2];
+          w = j & 2 ? hi : lo;
+        }
+        mine[at] = (uint64_t)((uint32_t)order_key(w) ^ 0x80000000u) << 32 |
+                   (0xffffffffu - (uint32_t)((i * NT + tid) * V + j));
+      }
+      bits &= bits - 1;
+      n += __popcll(m);
+    }
   };
-  int n = reach(bound);
-  if (n > CAP) {
-    // (sorted or equal logits: the bound is loose)  The largest bound that `width` keys
-    // reach, bit by bit from above; all keys are different, so it ends at `width`.
-    Key b = 0;
-    for (int bit = 8 * (int)sizeof(Key) - 1; bit >= 0; --bit) {
-      const Key c = b | (Key)1 << bit;
-      const int m = reach(c);
-      if (m < A.width) continue;
-      b = c;
-      if (m <= CAP) break;
-    }
-    bound = max(b, (Key)(Ks::NONE + 1));
-    n = reach(bound);
-  }
-  int at = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const bool in = key[e] >= bound;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
-    if (m) {
-      if (in) list[wave * CAP + at + __popcll(m & ((1ull << lane) - 1))] = key[e];
-      at += __popcll(m);
+  for (int i = 0; i < LOADS; ++i)
+    collect(i, [&](int j) { return key_of(i, j) >= bound; });
+  if (n > CAP) {
+    // (sorted or equal logits: the bound is loose)  The width-th largest value, bit by bit
+    // from above; then those above it, and as many of its equals as are missing, the
+    // lowest places first: load by load, lane by lane.
+    auto reach = [&](int b) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          c += __popcll(__builtin_amdgcn_ballot_w64(key_of(i, j) >= b));
+      return c;
+    };
+    // (more than CAP reach `bound`, so the value is not below it)
+    int64_t least = bound;
+    for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
+      if (least + bit <= INF_KEY && reach((int)(least + bit)) >= A.width) least += bit;
+    n = 0;
+    int missing = A.width - reach((int)least + STEP);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      int equal = 0;
+#pragma unroll
+      for (int j = 0; j < V; ++j) equal += exact(key_of(i, j)) == (int)least;
+      const int incl = wave_scan_i32(equal);
+      int before = incl - equal;
+      collect(i, [&](int j) {
+        const int k = exact(key_of(i, j));
+        const bool same = k == (int)least;
+        const bool in = k > (int)least || (same && before < missing);
+        before += same;
+        return in;
+      });
+      missing = max(missing - __builtin_amdgcn_readlane(incl, 63), 0);
     }
+  }
+
+  // ---- the sum of exponentials, relative to the maximum
+  double sum = 0.0;
+  if (top_key > -INF_KEY && top_key < INF_KEY) {
+    // exp of a value as it is, where the type's range allows it: 2^(x log2 e) with the
+    // product's rounding made good
+    const bool near = top > -40.f && top < 80.f;
+    constexpr float LOG2E = 0x1.715476p+0f, REST = 0x1.4ae0c0p-26f, LN2 = 0x1.62e430p-1f;
+    auto quick = [&](float f) -> float {
+      const float t = f * LOG2E;
+      const float e = fmaf(f, REST, fmaf(f, LOG2E, -t));
+      const float p = __builtin_amdgcn_exp2f(t);
+      return fmaf(p * LN2, e, p);
+    };
+    double s[2] = {0.0, 0.0};
+    if (near) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float f;
+          if constexpr (V == 8)
+            f = j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
+          else
+            f = __uint_as_float(x[i][j]);
+          s[j & 1] += (double)quick(fmaxf(f, -200.f));  // (-inf, and a NaN with its sign set)
+        }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
+      for (int i = lane; i < n; i += 64) {
+        const float f = order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u));
+        s[0] += exp_any((double)f) - (double)quick(f);
+      }
+      sum = wave_sum64(s[0] + s[1]) / exp_any((double)top);
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float f;
+          if constexpr (V == 8)
+            f = j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
+          else
+            f = __uint_as_float(x[i][j]);
+          s[j & 1] += exp_any(fmax((double)fmaxf(f, -INFINITY) - (double)top, -700.0));
+        }
+      sum = wave_sum64(s[0] + s[1]);
+    }
+  } else if (top_key == INF_KEY) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += exact(key_of(i, j)) == INF_KEY;
+    sum = wave_sum64(sum);
   }
   if (lane == 0) {
     count_s[wave] = n;
@@ -288,13 +385,15 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   for (int w = 0; w < WAVES; ++w) total += count_s[w];
   for (int i = tid; i < WAVES * CAP; i += NT) {
     if ((i & (CAP - 1)) >= count_s[i / CAP]) continue;
-    const Key mine = list[i];
+    const uint64_t key = list[i];
     int rank = 0;
     for (int w = 0; w < WAVES; ++w)
-      for (int j = 0; j < count_s[w]; ++j) rank += list[w * CAP + j] > mine;
+      for (int j = 0; j < count_s[w]; ++j) rank += list[w * CAP + j] > key;
     if (rank < A.width) {
-      st_agent(A.cand_value + out + (int64_t)rank * lists, Ks::value(mine));
-      st_agent(A.cand_token + out + (int64_t)rank * lists, first + (int)Ks::place(mine));
+      st_agent(A.cand_value + out + (int64_t)rank * lists,
+               order_value((int)((uint32_t)(key >> 32) ^ 0x80000000u)));
+      st_agent(A.cand_token + out + (int64_t)rank * lists,
+               first + (int)(0xffffffffu - (uint32_t)key));
     }
   }
   for (int i = total + tid; i < A.width; i += NT)
@@ -304,10 +403,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) m = fmaxf(m, max_s[w]);
     double s = 0.0;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      if (max_s[w] > -INFINITY)
-        s += sum_s[w] * exp_le0(max_s[w] == m ? 0.0 : (double)max_s[w] - (double)m);
+    for (int w = 0; w < WAVES; ++w) s += sum_s[w] * exp_between(max_s[w], m);
     st_agent(A.part_max + (int64_t)row * A.parts + part, m);
     st_agent(reinterpret_cast<uint64_t*>(A.part_sum) + (int64_t)row * A.parts + part,
              __builtin_bit_cast(uint64_t, s));
@@ -324,39 +420,63 @@ __device__ __forceinline__ bool before(double s, int64_t p, double t, int64_t r)
   return s > t || (s == t && p < r);
 }
 
+// a / c for 0 <= a < 2^24 and inv = 1 / c to a few units of the last place.
+__device__ __forceinline__ int small_div(int a, int c, float inv) {
+  const int q = (int)((float)a * inv);
+  const int r = a - q * c;
+  return q + (r >= c) - (r < 0);
+}
+
 // One workgroup a sequence.  A beam's parts are joined to its log sum; the candidates that
 // reach a bound found as above are collected and ranked.  Where too many do (equal
-// scores), they are found one after another instead.
-constexpr int MERGE_CAP = 1024;
+// scores), they are found one after another instead.  Bound by the chain of its loads.
+constexpr int MERGE_NT = 1024, MERGE_WAVES = MERGE_NT / 64;
+constexpr int MERGE_CAP = 1024, HELD = 4;  // candidates a thread keeps in registers
 
-__global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
+__global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   __shared__ float top_s[MAX_BEAMS];
   __shared__ double log_s[MAX_BEAMS];  // the log of the sum relative to the maximum
   __shared__ float score_s[MAX_BEAMS];
   __shared__ double cs[MERGE_CAP];
   __shared__ int64_t cp[MERGE_CAP];
-  __shared__ double bound_s[WAVES];
-  __shared__ int64_t best_s[WAVES];
+  __shared__ double bound_s[MERGE_WAVES];
+  __shared__ int64_t best_s[MERGE_WAVES];
   __shared__ int count_s;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lists = A.beams * A.parts;
+  const float lists_inv = 1.f / (float)lists, parts_inv = 1.f / (float)A.parts;
+  // Candidate e of `n`: rank, beam, part; the done beams' own ones come last.  The first
+  // of a thread are loaded before anything else.
+  const int n = A.width * lists, all = n + A.beams;
+  const int32_t* const token_of = A.cand_token + (int64_t)seq * n;
+  const float* const value_of = A.cand_value + (int64_t)seq * n;
+  int token[HELD];
+  float value[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; ++i) {
+    const int e = min(tid + i * MERGE_NT, n - 1);
+    token[i] = token_of[e];
+    value[i] = value_of[e];
+  }
   // score_s: NaN marks a beam that offers nothing, log_s NaN one that is done
-  for (int b = wave; b < A.beams; b += WAVES) {
+  for (int b = wave; b < A.beams; b += MERGE_WAVES) {
     const int row = seq * A.beams + b;
+    const float* const pm = A.part_max + (int64_t)row * A.parts;
+    const double* const ps = A.part_sum + (int64_t)row * A.parts;
     const float c = A.scores[row];
-    const bool dead = !(c > -INFINITY), done = A.done && A.done[row];
+    const bool done = A.done && A.done[row], dead = !(c > -INFINITY);
+    const int at = min(lane, A.parts - 1);
+    const float m0 = pm[at];
+    const double s0 = ps[at];
     float m = -INFINITY;
     double s = 0.0;
     if (!dead && !done) {
-      for (int p = lane; p < A.parts; p += 64) m = fmaxf(m, A.part_max[(int64_t)row * A.parts + p]);
+      m = lane < A.parts ? m0 : -INFINITY;
+      for (int p = lane + 64; p < A.parts; p += 64) m = fmaxf(m, pm[p]);
       m = wave_max(m);
-      for (int p = lane; p < A.parts; p += 64) {
-        const float pm = A.part_max[(int64_t)row * A.parts + p];
-        if (pm > -INFINITY)
-          s += A.part_sum[(int64_t)row * A.parts + p] *
-               exp_le0(pm == m ? 0.0 : (double)pm - (double)m);
-      }
+      if (lane < A.parts) s = s0 * exp_between(m0, m);
+      for (int p = lane + 64; p < A.parts; p += 64) s += ps[p] * exp_between(pm[p], m);
       s = wave_sum64(s);
     }
     if (lane == 0) {
@@ -368,10 +488,9 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
   if (tid == 0) count_s = 0;
   __syncthreads();
 
-  // Candidate e of `n`: rank, beam, part; the done beams' own ones come last.
-  const int n = A.width * lists, all = n + A.beams;
-  auto candidate = [&](int e, double& s, int64_t& place) {
+  auto candidate = [&](int e, int tok, float v, double& s, int64_t& place) {
     s = -INFINITY;
+    if (e >= all) return;
     if (e >= n) {
       const int b = e - n;
       if (log_s[b] != log_s[b] && score_s[b] == score_s[b]) {
@@ -380,35 +499,58 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
       }
       return;
     }
-    const int list = e % lists, b = list / A.parts;
-    if (log_s[b] != log_s[b] || score_s[b] != score_s[b]) return;
-    const int64_t at = (int64_t)seq * A.width * lists + e;
-    const int token = A.cand_token[at];
-    if (token < 0) return;
-    const float v = A.cand_value[at];
+    const int list = e - small_div(e, lists, lists_inv) * lists;
+    const int b = small_div(list, A.parts, parts_inv);
+    if (log_s[b] != log_s[b] || score_s[b] != score_s[b] || tok < 0) return;
     s = (double)score_s[b] + ((v == top_s[b] ? 0.0 : (double)v - (double)top_s[b]) - log_s[b]);
-    place = (int64_t)b * A.vocab + token;
+    place = (int64_t)b * A.vocab + tok;
   };
+  // Every candidate of this thread, those in registers and those beyond them.
+  auto each = [&](auto use) {
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+      const int e = tid + i * MERGE_NT;
+      double s;
+      int64_t p = 0;
+      if (e >= n + MERGE_NT) break;
+      candidate(e < n ? e : all, token[i], value[i], s, p);
+      use(s, p);
+    }
+    for (int e = tid + HELD * MERGE_NT; e < n; e += MERGE_NT) {
+      double s;
+      int64_t p = 0;
+      candidate(e, token_of[e], value_of[e], s, p);
+      use(s, p);
+    }
+    double s;
+    int64_t p = 0;
+    candidate(n + tid, 0, 0.f, s, p);
+    use(s, p);
+  };
+  // The bound: the width-th largest of the lanes' best list heads (ranks of 0), lane l of
+  // every wave with the lists l, l + 64, ..; -inf where there are fewer.
   double best = -INFINITY;
-  for (int e = tid; e < all; e += NT) {
+  for (int e = lane; e < lists; e += 64) {
     double s;
     int64_t p;
-    candidate(e, s, p);
+    candidate(e, token_of[e], value_of[e], s, p);
     best = fmax(best, s);
   }
-  // (a group of lanes sees every rank of its lists)
-  int groups = WAVES;
-  while (groups < A.width) groups <<= 1;
-  const double bound_w = least_of_maxima(best, groups / WAVES);
-  if (lane == 0) bound_s[wave] = bound_w;
-  __syncthreads();
-  double bound = bound_s[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) bound = fmin(bound, bound_s[w]);
-  for (int e = tid; e < all; e += NT) {
-    double s;
-    int64_t p;
-    candidate(e, s, p);
+  int above = 0;
+#pragma unroll 8
+  for (int l = 0; l < 64; ++l) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, best);
+    const double o = __builtin_bit_cast(
+        double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), l) << 32 |
+                    (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, l));
+    above += o > best || (o == best && l < lane);
+  }
+  const int at = __ffsll((unsigned long long)__ballot(above == A.width - 1)) - 1;
+  const uint64_t u = __builtin_bit_cast(uint64_t, best);
+  const double bound = __builtin_bit_cast(
+      double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), at) << 32 |
+                  (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, at));
+  each([&](double s, int64_t p) {
     if (s >= bound && s > -INFINITY) {
       const int i = atomicAdd(&count_s, 1);  // (any order: they are ranked)
       if (i < MERGE_CAP) {
@@ -416,7 +558,7 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
         cp[i] = p;
       }
     }
-  }
+  });
   __syncthreads();
   const int64_t out = (int64_t)seq * A.width;
   auto put = [&](int rank, double s, int64_t p) {
@@ -428,7 +570,7 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
   };
   int found = count_s;
   if (found <= MERGE_CAP) {
-    for (int i = tid; i < found; i += NT) {
+    for (int i = tid; i < found; i += MERGE_NT) {
       const double s = cs[i];
       const int64_t p = cp[i];
       int rank = 0;
@@ -441,15 +583,12 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
     for (found = 0; found < A.width; ++found) {
       double bs = -INFINITY;
       int64_t bp = INT64_MAX;
-      for (int e = tid; e < all; e += NT) {
-        double s;
-        int64_t p;
-        candidate(e, s, p);
+      each([&](double s, int64_t p) {
         if (s > -INFINITY && before(last_s, last_p, s, p) && before(s, p, bs, bp)) {
           bs = s;
           bp = p;
         }
-      }
+      });
 #pragma unroll
       for (int mask = 1; mask < 64; mask <<= 1) {
         const double s = __shfl_xor(bs, mask);
@@ -465,7 +604,7 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
         best_s[wave] = bp;
       }
       __syncthreads();
-      for (int w = 0; w < WAVES; ++w)
+      for (int w = 0; w < MERGE_WAVES; ++w)
         if (before(bound_s[w], best_s[w], bs, bp)) {
           bs = bound_s[w];
           bp = best_s[w];
@@ -476,7 +615,7 @@ __global__ __launch_bounds__(NT) void beam_merge_kernel(BeamArgs A) {
       last_p = bp;
     }
   }
-  for (int i = found + tid; i < A.width; i += NT) {
+  for (int i = found + tid; i < A.width; i += MERGE_NT) {
     st_agent(A.parents + out + i, -1);
     st_agent(reinterpret_cast<uint64_t*>(A.tokens) + out + i, (uint64_t)-1);
     st_agent(A.out_scores + out + i, -INFINITY);
@@ -549,11 +688,11 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   a.parts = parts;
   a.pad_id = pad_id;
   const auto kernel = element_size == 2
-      ? (size == 16384 ? smx::beam_parts_kernel<uint16_t, 64> : smx::beam_parts_kernel<uint16_t, 16>)
-      : (size == 8192 ? smx::beam_parts_kernel<float, 32> : smx::beam_parts_kernel<float, 8>);
+      ? (size == 16384 ? smx::beam_parts_kernel<uint16_t, 8> : smx::beam_parts_kernel<uint16_t, 2>)
+      : (size == 8192 ? smx::beam_parts_kernel<float, 8> : smx::beam_parts_kernel<float, 2>);
   SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(smx::NT), 0, (hipStream_t)stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
-  SMX_LAUNCH(smx::beam_merge_kernel, dim3(seqs), dim3(smx::NT), 0, (hipStream_t)stream, a);
+  SMX_LAUNCH(smx::beam_merge_kernel, dim3(seqs), dim3(smx::MERGE_NT), 0, (hipStream_t)stream, a);
   return (int)hipGetLastError();
 }
