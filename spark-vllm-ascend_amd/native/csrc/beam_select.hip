@@ -110,25 +110,6 @@ __device__ __forceinline__ K other(K v) {
   }
 }
 
-// The least of the maxima of `groups` (a power of two up to 64) equal groups of a wave's
-// neighbouring lanes: `groups` values or more are at least that.
-template <typename K>
-__device__ __forceinline__ K least_of_maxima(K v, int groups) {
-  auto step = [&](auto mask) {
-    constexpr int MASK = decltype(mask)::value;
-    const K o = other<MASK>(v);
-    const bool up = groups * MASK < 64;  // still within a group: the maximum
-    v = (o > v) == up ? o : v;
-  };
-  step(std::integral_constant<int, 1>{});
-  step(std::integral_constant<int, 2>{});
-  step(std::integral_constant<int, 4>{});
-  step(std::integral_constant<int, 8>{});
-  step(std::integral_constant<int, 16>{});
-  step(std::integral_constant<int, 32>{});
-  return v;
-}
-
 // The sum over a wave, in an order that does not depend on the lane.
 __device__ __forceinline__ double wave_sum64(double v) {
   v += other<1>(v);
@@ -141,7 +122,7 @@ __device__ __forceinline__ double wave_sum64(double v) {
 }
 
 // One part (NT * LOADS * V logits) of one row, a wave's share of it in registers: its
-// maximum, the values that reach a bound which `width` of its own do (found from its
+// maximum, the values that reach a bound which `width` of the part do (found from the
 // lanes' maxima), and its sum of exponentials; the few collected of all waves are ranked
 // by counting.
 //
@@ -154,7 +135,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   constexpr int PART = NT * LOADS * V;
   __shared__ uint64_t list[WAVES * CAP];
   __shared__ u32x4 tail_s;
-  __shared__ int count_s[WAVES];
+  __shared__ int count_s[WAVES], bound_s[WAVES];
   __shared__ float max_s[WAVES];
   __shared__ double sum_s[WAVES];
   const int part = blockIdx.x, row = blockIdx.y;
@@ -245,10 +226,17 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   const float top = order_value(max(top_key, -INF_KEY));
 
   // ---- the largest
-  int groups = 1;
-  while (groups < A.width) groups <<= 1;
+  // The bound: the width-th largest of a wave's lanes' maxima, bit by bit from above, and
+  // the highest of the four waves' (each is one for the whole part).
   constexpr int LOWEST = -INF_KEY + STEP;  // the lowest finite value's
-  int bound = max(least_of_maxima(best, groups), LOWEST);
+  int64_t bound_w = LOWEST;
+  for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
+    if (bound_w + bit <= INF_KEY &&
+        __popcll(__builtin_amdgcn_ballot_w64(best >= (int)(bound_w + bit))) >= A.width)
+      bound_w += bit;
+  if (lane == 0) bound_s[wave] = (int)bound_w;
+  __syncthreads();
+  const int bound = max(max(bound_s[0], bound_s[1]), max(bound_s[2], bound_s[3]));
   uint64_t* const mine = list + wave * CAP;
   int n = 0;
   // Puts the values that `in(i, j)` says into the list, in no particular order: a bit a
@@ -321,17 +309,21 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   // ---- the sum of exponentials, relative to the maximum
   double sum = 0.0;
   if (top_key > -INF_KEY && top_key < INF_KEY) {
-    // exp of a value as it is, where the type's range allows it: 2^(x log2 e) with the
-    // product's rounding made good
-    const bool near = top > -40.f && top < 80.f;
-    constexpr float LOG2E = 0x1.715476p+0f, REST = 0x1.4ae0c0p-26f, LN2 = 0x1.62e430p-1f;
-    auto quick = [&](float f) -> float {
-      const float t = f * LOG2E;
-      const float e = fmaf(f, REST, fmaf(f, LOG2E, -t));
+    // exp of a value as it is: p = 2^(x HI) times 1 + x REST, HI log2(e) to 16 bits, so that
+    // a bf16 value's product with it is exact (an fp32 one's rounding is made good), and
+    // REST what is missing, times log 2; the sum of p x REST by itself.  The next term, half
+    // of (x REST)^2, is below 7e-9 up to 24; larger logits are taken in 64 bits.
+    const bool near = top > -24.f && top < 24.f;
+    constexpr float HI = 0x1.7154p+0f, REST = 0x1.480fb6p-18f;
+    auto quick = [&](float f, float& rest) -> float {
+      const float t = f * HI;
       const float p = __builtin_amdgcn_exp2f(t);
-      return fmaf(p * LN2, e, p);
+      rest = f * REST;
+      if constexpr (V == 4) rest = fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f, rest);
+      return p;
     };
     double s[2] = {0.0, 0.0};
+    float small = 0.f;
     if (near) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i)
@@ -342,12 +334,20 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
             f = j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
           else
             f = __uint_as_float(x[i][j]);
-          s[j & 1] += (double)quick(fmaxf(f, -200.f));  // (-inf, and a NaN with its sign set)
+          // (-inf, and a NaN with its sign set, at -200)
+          float rest;
+          const float p = quick(__builtin_amdgcn_fmed3f(f, -200.f, INFINITY), rest);
+          s[j & 1] += (double)p;
+          small = fmaf(p, rest, small);
         }
+      s[0] += (double)small;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
       for (int i = lane; i < n; i += 64) {
-        const float f = order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u));
-        s[0] += exp_any((double)f) - (double)quick(f);
+        const float f =
+            fmaxf(order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u)), -200.f);
+        float rest;
+        const double p = (double)quick(f, rest);
+        s[0] += (exp_any((double)f) - p) - p * (double)rest;
       }
       sum = wave_sum64(s[0] + s[1]) / exp_any((double)top);
     } else {
@@ -429,14 +429,14 @@ __device__ __forceinline__ int small_div(int a, int c, float inv) {
 
 // One workgroup a sequence.  A beam's parts are joined to its log sum; the candidates that
 // reach a bound found as above are collected and ranked.  Where too many do (equal
-// scores), they are found one after another instead.  Bound by the chain of its loads.
-constexpr int MERGE_NT = 1024, MERGE_WAVES = MERGE_NT / 64;
-constexpr int MERGE_CAP = 1024, HELD = 4;  // candidates a thread keeps in registers
+// scores), they are found one after another instead.  Bound by instructions that are not
+// in the cache yet: one loop does for the bound and for the candidates.
+constexpr int MERGE_NT = 512, MERGE_WAVES = MERGE_NT / 64;
+constexpr int MERGE_CAP = 1024, HELD = 4;
 
 __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   __shared__ float top_s[MAX_BEAMS];
-  __shared__ double log_s[MAX_BEAMS];  // the log of the sum relative to the maximum
-  __shared__ float score_s[MAX_BEAMS];
+  __shared__ double log_s[MAX_BEAMS];  // score - the log of the sum relative to the maximum
   __shared__ double cs[MERGE_CAP];
   __shared__ int64_t cp[MERGE_CAP];
   __shared__ double bound_s[MERGE_WAVES];
@@ -445,120 +445,127 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lists = A.beams * A.parts;
-  const float lists_inv = 1.f / (float)lists, parts_inv = 1.f / (float)A.parts;
-  // Candidate e of `n`: rank, beam, part; the done beams' own ones come last.  The first
-  // of a thread are loaded before anything else.
-  const int n = A.width * lists, all = n + A.beams;
+  const float lists_inv = __builtin_amdgcn_rcpf((float)lists);
+  const float parts_inv = __builtin_amdgcn_rcpf((float)A.parts);
+  if (tid == 0) count_s = 0;
+  // Candidate e of `n`: rank, beam, part.  The first list head of a lane and the first
+  // candidates of a thread are on their way before anything else.
+  const int n = A.width * lists;
   const int32_t* const token_of = A.cand_token + (int64_t)seq * n;
   const float* const value_of = A.cand_value + (int64_t)seq * n;
   int token[HELD];
   float value[HELD];
 #pragma unroll
   for (int i = 0; i < HELD; ++i) {
-    const int e = min(tid + i * MERGE_NT, n - 1);
+    const int e = min(i == 0 ? lane : tid + (i - 1) * MERGE_NT, n - 1);
     token[i] = token_of[e];
     value[i] = value_of[e];
   }
-  // score_s: NaN marks a beam that offers nothing, log_s NaN one that is done
+  // a beam that offers nothing from its logits has the score -inf
   for (int b = wave; b < A.beams; b += MERGE_WAVES) {
     const int row = seq * A.beams + b;
     const float* const pm = A.part_max + (int64_t)row * A.parts;
     const double* const ps = A.part_sum + (int64_t)row * A.parts;
     const float c = A.scores[row];
-    const bool done = A.done && A.done[row], dead = !(c > -INFINITY);
-    const int at = min(lane, A.parts - 1);
-    const float m0 = pm[at];
-    const double s0 = ps[at];
     float m = -INFINITY;
+    for (int p = lane; p < A.parts; p += 64) m = fmaxf(m, pm[p]);
+    m = wave_max(m);
     double s = 0.0;
-    if (!dead && !done) {
-      m = lane < A.parts ? m0 : -INFINITY;
-      for (int p = lane + 64; p < A.parts; p += 64) m = fmaxf(m, pm[p]);
-      m = wave_max(m);
-      if (lane < A.parts) s = s0 * exp_between(m0, m);
-      for (int p = lane + 64; p < A.parts; p += 64) s += ps[p] * exp_between(pm[p], m);
-      s = wave_sum64(s);
-    }
+    for (int p = lane; p < A.parts; p += 64) s += ps[p] * exp_between(pm[p], m);
+    s = wave_sum64(s);
+    // log s: fp32's, and what is missing from s exp(-log s) = 1
+    const double y = (double)(__builtin_amdgcn_logf((float)s) * 0x1.62e430p-1f);
+    const double d = s * exp_any(-y) - 1.0;
     if (lane == 0) {
+      const bool out = (A.done && A.done[row]) || !(c > -INFINITY) || !(s > 0.0);
       top_s[b] = m;
-      log_s[b] = done ? __builtin_nan("") : log(s);
-      score_s[b] = dead ? __builtin_nanf("") : c;
+      log_s[b] = out ? -INFINITY : (double)c - (y + (d - 0.5 * d * d));
     }
   }
-  if (tid == 0) count_s = 0;
   __syncthreads();
 
   auto candidate = [&](int e, int tok, float v, double& s, int64_t& place) {
-    s = -INFINITY;
-    if (e >= all) return;
-    if (e >= n) {
-      const int b = e - n;
-      if (log_s[b] != log_s[b] && score_s[b] == score_s[b]) {
-        s = (double)score_s[b];
-        place = (int64_t)b * A.vocab + A.pad_id;
-      }
-      return;
-    }
     const int list = e - small_div(e, lists, lists_inv) * lists;
     const int b = small_div(list, A.parts, parts_inv);
-    if (log_s[b] != log_s[b] || score_s[b] != score_s[b] || tok < 0) return;
-    s = (double)score_s[b] + ((v == top_s[b] ? 0.0 : (double)v - (double)top_s[b]) - log_s[b]);
+    s = log_s[b];
+    if (s == -INFINITY || tok < 0) {
+      s = -INFINITY;
+      return;
+    }
+    s += v == top_s[b] ? 0.0 : (double)v - (double)top_s[b];
     place = (int64_t)b * A.vocab + tok;
   };
-  // Every candidate of this thread, those in registers and those beyond them.
-  auto each = [&](auto use) {
-#pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-      const int e = tid + i * MERGE_NT;
-      double s;
-      int64_t p = 0;
-      if (e >= n + MERGE_NT) break;
-      candidate(e < n ? e : all, token[i], value[i], s, p);
-      use(s, p);
-    }
-    for (int e = tid + HELD * MERGE_NT; e < n; e += MERGE_NT) {
-      double s;
-      int64_t p = 0;
-      candidate(e, token_of[e], value_of[e], s, p);
-      use(s, p);
-    }
-    double s;
-    int64_t p = 0;
-    candidate(n + tid, 0, 0.f, s, p);
-    use(s, p);
-  };
   // The bound: the width-th largest of the lanes' best list heads (ranks of 0), lane l of
-  // every wave with the lists l, l + 64, ..; -inf where there are fewer.
-  double best = -INFINITY;
-  for (int e = lane; e < lists; e += 64) {
+  // every wave with the lists l, l + 64, ..; -inf where there are fewer.  Then all of them.
+  double bound = -INFINITY;
+  for (int pass = 0; pass < 2; ++pass) {
+    double best = -INFINITY;
+    const int step = pass ? MERGE_NT : 64, end = pass ? n : lists;
+    int i = pass;
+#pragma unroll 1
+    for (int e = pass ? tid : lane; e < end; e += step, ++i) {
+      double s;
+      int64_t p;
+      int tok;
+      float v;
+      if (pass ? i < HELD : i == 0) {
+        tok = i == 0 ? token[0] : token[1];
+        v = i == 0 ? value[0] : value[1];
+#pragma unroll
+        for (int h = 2; h < HELD; ++h) {
+          tok = i == h ? token[h] : tok;
+          v = i == h ? value[h] : v;
+        }
+      } else {
+        tok = token_of[e];
+        v = value_of[e];
+      }
+      candidate(e, tok, v, s, p);
+      best = fmax(best, s);
+      if (pass && s >= bound && s > -INFINITY) {
+        const int i = atomicAdd(&count_s, 1);  // (any order: they are ranked)
+        if (i < MERGE_CAP) {
+          cs[i] = s;
+          cp[i] = p;
+        }
+      }
+    }
+    if (pass) break;
+    const uint64_t u = __builtin_bit_cast(uint64_t, best);
+    auto of_lane = [&](int l) {
+      return __builtin_bit_cast(
+          double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), l) << 32 |
+                      (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, l));
+    };
+    int above = 0;
+#pragma unroll 4
+    for (int l = 0; l < 64; ++l) {
+      const double o = of_lane(l);
+      above += o > best || (o == best && l < lane);
+    }
+    bound = of_lane(__ffsll((unsigned long long)__ballot(above == A.width - 1)) - 1);
+  }
+  // a beam that is done: itself
+  auto own = [&](int b, double& s, int64_t& place) {
+    s = -INFINITY;
+    const int row = seq * A.beams + b;
+    if (b < A.beams && A.done && A.done[row] && A.scores[row] > -INFINITY) {
+      s = (double)A.scores[row];
+      place = (int64_t)b * A.vocab + A.pad_id;
+    }
+  };
+  if (A.done && tid < A.beams) {
     double s;
     int64_t p;
-    candidate(e, token_of[e], value_of[e], s, p);
-    best = fmax(best, s);
-  }
-  int above = 0;
-#pragma unroll 8
-  for (int l = 0; l < 64; ++l) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, best);
-    const double o = __builtin_bit_cast(
-        double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), l) << 32 |
-                    (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, l));
-    above += o > best || (o == best && l < lane);
-  }
-  const int at = __ffsll((unsigned long long)__ballot(above == A.width - 1)) - 1;
-  const uint64_t u = __builtin_bit_cast(uint64_t, best);
-  const double bound = __builtin_bit_cast(
-      double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), at) << 32 |
-                  (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, at));
-  each([&](double s, int64_t p) {
-    if (s >= bound && s > -INFINITY) {
-      const int i = atomicAdd(&count_s, 1);  // (any order: they are ranked)
+    own(tid, s, p);
+    if (s > -INFINITY) {
+      const int i = atomicAdd(&count_s, 1);
       if (i < MERGE_CAP) {
         cs[i] = s;
         cp[i] = p;
       }
     }
-  });
+  }
   __syncthreads();
   const int64_t out = (int64_t)seq * A.width;
   auto put = [&](int rank, double s, int64_t p) {
@@ -583,12 +590,18 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
     for (found = 0; found < A.width; ++found) {
       double bs = -INFINITY;
       int64_t bp = INT64_MAX;
-      each([&](double s, int64_t p) {
+      for (int e = tid; e < n + MERGE_NT; e += MERGE_NT) {
+        double s = -INFINITY;
+        int64_t p = 0;
+        if (e < n)
+          candidate(e, token_of[e], value_of[e], s, p);
+        else
+          own(tid, s, p);
         if (s > -INFINITY && before(last_s, last_p, s, p) && before(s, p, bs, bp)) {
           bs = s;
           bp = p;
         }
-      });
+      }
 #pragma unroll
       for (int mask = 1; mask < 64; mask <<= 1) {
         const double s = __shfl_xor(bs, mask);
@@ -625,7 +638,7 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
 
 // Logits of a part: many rows take long ones, few rows short ones that fill the chip.
 int part_size(int64_t rows, int64_t vocab, int elem) {
-  const int large = elem == 2 ? 16384 : 8192, small = large / 4;
+  const int large = elem == 2 ? 16384 : 8192, small = large / 8;
   return rows * ((vocab + large - 1) / large) >= 512 ? large : small;
 }
 
@@ -688,8 +701,8 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   a.parts = parts;
   a.pad_id = pad_id;
   const auto kernel = element_size == 2
-      ? (size == 16384 ? smx::beam_parts_kernel<uint16_t, 8> : smx::beam_parts_kernel<uint16_t, 2>)
-      : (size == 8192 ? smx::beam_parts_kernel<float, 8> : smx::beam_parts_kernel<float, 2>);
+      ? (size == 16384 ? smx::beam_parts_kernel<uint16_t, 8> : smx::beam_parts_kernel<uint16_t, 1>)
+      : (size == 8192 ? smx::beam_parts_kernel<float, 8> : smx::beam_parts_kernel<float, 1>);
   SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(smx::NT), 0, (hipStream_t)stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
