@@ -28,7 +28,6 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
 constexpr int CAP = 128;  // candidates of a wave
-constexpr int NT = 256, WAVES = NT / 64;
 
 struct BeamArgs {
   const void* logits;
@@ -81,10 +80,15 @@ __device__ __forceinline__ int order_key(uint32_t u) {
 __device__ __forceinline__ float order_value(int k) {
   return __uint_as_float(k < 0 ? (uint32_t)-k | 0x80000000u : (uint32_t)k);
 }
-// The same of two bf16 values in a dword, 16 bits each.
-__device__ __forceinline__ s16x2 order_keys(uint32_t w) {
-  const s16x2 m = __builtin_bit_cast(s16x2, w) >> 15;
-  return __builtin_bit_cast(s16x2, (w & 0x7fff7fffu) ^ __builtin_bit_cast(uint32_t, m)) - m;
+// Where -0 may be below 0: negative values' bits but the sign's flipped, and back.  (Of
+// bf16 values 16 bits, the upper ones of a key.)
+__device__ __forceinline__ int quick_key(float f) {
+  const int u = (int)__float_as_uint(f);
+  return u ^ ((u >> 31) & 0x7fffffff);
+}
+template <int BITS>
+__device__ __forceinline__ float key_value(int k) {
+  return __uint_as_float((uint32_t)(k ^ ((k >> 31) & 0x7fffffff)) & (~0u << (32 - BITS)));
 }
 constexpr int INF_KEY = 0x7f800000;
 
@@ -126,17 +130,18 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // lanes' maxima), and its sum of exponentials; the few collected of all waves are ranked
 // by counting.
 //
-// The sum: exp by the transcendental unit, whose errors are a few 1e-8 of each term, and
-// again in 64 bits for the collected values, which are most of a peaked row's sum; so what
-// is left is 1e-9 of it, and less where many terms' errors average out.
-template <typename L, int LOADS>
+// The sum, in 64 bits: exp by the transcendental unit, whose errors are a few 1e-8 of each
+// term; the collected values, which are most of a peaked row's sum, are left out of it and
+// taken in 64 bits.  So what is left is 1e-9 of it, and less where many terms' errors
+// average out; equal logits of two beams have equal errors.
+template <typename L, int NT, int LOADS>
 __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
+  constexpr int WAVES = NT / 64;
   constexpr int V = 16 / sizeof(L);  // logits of a load
   constexpr int PART = NT * LOADS * V;
-  __shared__ uint64_t list[WAVES * CAP];
+  __shared__ uint64_t list[WAVES][CAP + 4];
   __shared__ u32x4 tail_s;
-  __shared__ int count_s[WAVES], bound_s[WAVES];
-  __shared__ float max_s[WAVES];
+  __shared__ int count_s[WAVES], bound_s[WAVES], top_s[WAVES];
   __shared__ double sum_s[WAVES];
   const int part = blockIdx.x, row = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -168,53 +173,51 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
         if (i == chunk / NT) x[i] = tail_s;
     }
   }
-
-  // Value j of load i: its key.
-  auto key_of = [&](int i, int j) -> int {
-    if constexpr (V == 8) {
-      const uint32_t w = __builtin_bit_cast(uint32_t, order_keys(x[i][j / 2]));
-      return j & 1 ? (int)w : (int)(w << 16);  // (an odd one's lower half is below every step)
-    } else {
-      return order_key(x[i][j]);
-    }
-  };
+  // ---- the loads' and the lanes' maxima, as keys
   constexpr int STEP = V == 8 ? 0x10000 : 1;  // between two keys
-  auto exact = [&](int key) { return V == 8 ? key & ~0xffff : key; };
-  // ---- the lanes' maxima
-  int best;
-  auto maxima = [&]() {
-    if constexpr (V == 8) {
-      s16x2 m = {-32768, -32768};
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) m = __builtin_elementwise_max(m, order_keys(x[i][j]));
-      best = max((int)m[0], (int)m[1]) << 16;
-    } else {
-      best = INT_MIN;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) best = max(best, key_of(i, j));
-    }
+  constexpr int NO_KEY = (int)0x807fffff & -STEP;  // of -inf
+  constexpr int BITS = V == 8 ? 16 : 32;
+  typedef typename std::conditional<V == 8, s16x2, int>::type Key;
+  Key most[LOADS];  // V == 8: of the even values and of the odd ones
+  auto key = [](Key k) -> int {
+    if constexpr (V == 8)
+      return max((int)k[0], (int)k[1]) << 16;
+    else
+      return k;
   };
-  maxima();
+  auto maxima = [&]() {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t u = x[i][j];  // (an element itself is no operand for a bit_cast)
+        const Key w = __builtin_bit_cast(Key, u);
+        const Key k = w ^ ((w >> (V == 8 ? 15 : 31)) & (Key)(V == 8 ? 0x7fff : 0x7fffffff));
+        most[i] = j == 0 ? k : __builtin_elementwise_max(most[i], k);
+      }
+    }
+    Key best = most[0];
+#pragma unroll
+    for (int i = 1; i < LOADS; ++i) best = __builtin_elementwise_max(best, most[i]);
+    return key(best);
+  };
+  int best = maxima();
   if (__builtin_amdgcn_ballot_w64(best > INF_KEY)) {
-    // a NaN (one with its sign set is below -inf): -inf in its place
+    // -inf in the place of a NaN without a sign (one with it is below -inf in this order)
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint32_t w = x[i][j];
         if constexpr (V == 8) {
-          if ((w & 0x7fffu) > 0x7f80u) w = (w & 0xffff0000u) | 0xff80u;
-          if ((w & 0x7fff0000u) > 0x7f800000u) w = (w & 0xffffu) | 0xff800000u;
+          if ((w & 0xffffu) - 0x7f81u < 0x7fu) w = (w & 0xffff0000u) | 0xff80u;
+          if ((w >> 16) - 0x7f81u < 0x7fu) w = (w & 0xffffu) | 0xff800000u;
         } else {
-          if ((w & 0x7fffffffu) > 0x7f800000u) w = NONE;
+          if (w - 0x7f800001u < 0x7fffffu) w = NONE;
         }
         x[i][j] = w;
       }
-    maxima();
+    best = maxima();
   }
   int top_key = best;
   top_key = max(top_key, other<1>(top_key));
@@ -223,28 +226,54 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   top_key = max(top_key, other<8>(top_key));
   top_key = max(top_key, other<16>(top_key));
   top_key = max(top_key, other<32>(top_key));
-  const float top = order_value(max(top_key, -INF_KEY));
 
   // ---- the largest
   // The bound: the width-th largest of a wave's lanes' maxima, bit by bit from above, and
-  // the highest of the four waves' (each is one for the whole part).
-  constexpr int LOWEST = -INF_KEY + STEP;  // the lowest finite value's
-  int64_t bound_w = LOWEST;
+  // the highest of the waves' (each is one for the whole part).
+  int64_t bound_w = NO_KEY + STEP;
   for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
     if (bound_w + bit <= INF_KEY &&
         __popcll(__builtin_amdgcn_ballot_w64(best >= (int)(bound_w + bit))) >= A.width)
       bound_w += bit;
-  if (lane == 0) bound_s[wave] = (int)bound_w;
+  if (lane == 0) {
+    bound_s[wave] = (int)bound_w;
+    top_s[wave] = top_key;
+  }
   __syncthreads();
-  const int bound = max(max(bound_s[0], bound_s[1]), max(bound_s[2], bound_s[3]));
-  uint64_t* const mine = list + wave * CAP;
+  int bound_key = bound_s[0];
+  top_key = top_s[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) {
+    bound_key = max(bound_key, bound_s[w]);
+    top_key = max(top_key, top_s[w]);
+  }
+  const float bound = key_value<BITS>(bound_key);
+  const float top = key_value<BITS>(max(top_key, NO_KEY));
+  uint64_t* const mine = list[wave];
   int n = 0;
-  // Puts the values that `in(i, j)` says into the list, in no particular order: a bit a
-  // value, the set ones of a load lane by lane.
+  // (what is computed of a load's values is not kept over this)
+  auto opaque = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t w = x[i][j];
+      asm volatile("" : "+v"(w));
+      x[i][j] = w;
+    }
+  };
+  auto value = [&](int i, int j) -> float {
+    if constexpr (V == 8)
+      return j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
+    else
+      return __uint_as_float(x[i][j]);
+  };
+  // Puts the values of load i that `in(j)` says into the list, in no particular order: a
+  // bit a value, the set ones lane by lane.
+  uint32_t taken[(LOADS * V + 31) / 32] = {};
   auto collect = [&](int i, auto in) {
     uint32_t bits = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) bits = bits + bits + (in(j) ? 1u : 0u);
+    taken[i * V / 32] |= bits << (i * V % 32);
     while (const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0)) {
       const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
@@ -268,35 +297,42 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   };
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
-    collect(i, [&](int j) { return key_of(i, j) >= bound; });
+    if (__builtin_amdgcn_ballot_w64(key(most[i]) >= bound_key))
+      collect(i, [&](int j) { return value(i, j) >= bound; });
   if (n > CAP) {
     // (sorted or equal logits: the bound is loose)  The width-th largest value, bit by bit
     // from above; then those above it, and as many of its equals as are missing, the
     // lowest places first: load by load, lane by lane.
+    auto key_of = [&](int i, int j) { return order_key(__float_as_uint(value(i, j))); };
     auto reach = [&](int b) {
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i)
+      for (int i = 0; i < LOADS; ++i) {
+        opaque(i);
 #pragma unroll
         for (int j = 0; j < V; ++j)
           c += __popcll(__builtin_amdgcn_ballot_w64(key_of(i, j) >= b));
+      }
       return c;
     };
     // (more than CAP reach `bound`, so the value is not below it)
-    int64_t least = bound;
+    int64_t least = order_key(__float_as_uint(bound));
+#pragma unroll 1
     for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
       if (least + bit <= INF_KEY && reach((int)(least + bit)) >= A.width) least += bit;
     n = 0;
+    for (uint32_t& bits : taken) bits = 0;
     int missing = A.width - reach((int)least + STEP);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       int equal = 0;
+      opaque(i);
 #pragma unroll
-      for (int j = 0; j < V; ++j) equal += exact(key_of(i, j)) == (int)least;
+      for (int j = 0; j < V; ++j) equal += key_of(i, j) == (int)least;
       const int incl = wave_scan_i32(equal);
       int before = incl - equal;
       collect(i, [&](int j) {
-        const int k = exact(key_of(i, j));
+        const int k = key_of(i, j);
         const bool same = k == (int)least;
         const bool in = k > (int)least || (same && before < missing);
         before += same;
@@ -306,74 +342,87 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     }
   }
 
-  // ---- the sum of exponentials, relative to the maximum
+  // ---- the sum of exponentials: as they are, relative to `top` where that is large
+  const bool near = top > -16.f && top < 16.f;
   double sum = 0.0;
-  if (top_key > -INF_KEY && top_key < INF_KEY) {
-    // exp of a value as it is: p = 2^(x HI) times 1 + x REST, HI log2(e) to 16 bits, so that
-    // a bf16 value's product with it is exact (an fp32 one's rounding is made good), and
-    // REST what is missing, times log 2; the sum of p x REST by itself.  The next term, half
-    // of (x REST)^2, is below 7e-9 up to 24; larger logits are taken in 64 bits.
-    const bool near = top > -24.f && top < 24.f;
+  // a term in 64 bits (+inf: as many equal ones; -inf and NaN: 0)
+  auto exact = [&](float f) -> double {
+    if (!(f > -INFINITY)) return 0.0;
+    if (near) return exp_any(fmax((double)f, -700.0));
+    return exp_between(f, top);
+  };
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
+  for (int i = lane; i < n; i += 64)
+    sum += exact(order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u)));
+  // the collected values of load i: -inf from here on
+  auto remove = [&](int i) {
+    const uint32_t bits = taken[i * V / 32] >> (i * V % 32);
+    if (!__builtin_amdgcn_ballot_w64((bits & ((1u << V) - 1)) != 0)) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!(bits >> (V - 1 - j) & 1)) continue;
+      uint32_t w = x[i][j / (V / 4)];
+      if constexpr (V == 8)
+        w = j & 1 ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
+      else
+        w = NONE;
+      x[i][j / (V / 4)] = w;
+    }
+  };
+  // The others': exp f = 2^(f HI) (1 + f REST), HI log2(e) to 16 bits, so that a bf16 value's
+  // product with it is exact, and REST what is missing, times log 2; the next term, half of
+  // (f REST)^2, is below 4e-9 at 16 and less below.  Other products' rounding is made good.
+  auto add = [&](auto relative) {
     constexpr float HI = 0x1.7154p+0f, REST = 0x1.480fb6p-18f;
-    auto quick = [&](float f, float& rest) -> float {
-      const float t = f * HI;
-      const float p = __builtin_amdgcn_exp2f(t);
-      rest = f * REST;
-      if constexpr (V == 4) rest = fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f, rest);
-      return p;
-    };
+    // (values below -200, -inf and NaN with a sign are larger as unsigned numbers)
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    typedef typename std::conditional<V == 8, u16x2, uint32_t>::type Bits;
     double s[2] = {0.0, 0.0};
     float small = 0.f;
-    if (near) {
 #pragma unroll
-      for (int i = 0; i < LOADS; ++i)
+    for (int i = 0; i < LOADS; ++i) {
+      remove(i);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float f;
-          if constexpr (V == 8)
-            f = j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
-          else
-            f = __uint_as_float(x[i][j]);
-          // (-inf, and a NaN with its sign set, at -200)
-          float rest;
-          const float p = quick(__builtin_amdgcn_fmed3f(f, -200.f, INFINITY), rest);
-          s[j & 1] += (double)p;
-          small = fmaf(p, rest, small);
+      for (int j = 0; j < V; ++j) {
+        float f;
+        if constexpr (relative) {
+          // exact where it is small: f is half of `top` at least, or exp(f - top) below e^-8
+          f = value(i, j) - top;
+          f = f > -200.f ? f : -200.f;
+        } else {
+          if (j % (V / 4) == 0) {
+            const uint32_t u = x[i][j / (V / 4)];
+            x[i][j / (V / 4)] = __builtin_bit_cast(
+                uint32_t, __builtin_elementwise_min(__builtin_bit_cast(Bits, u),
+                                                    (Bits)(V == 8 ? 0xc348u : 0xc3480000u)));
+          }
+          f = value(i, j);
         }
-      s[0] += (double)small;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
-      for (int i = lane; i < n; i += 64) {
-        const float f =
-            fmaxf(order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u)), -200.f);
-        float rest;
-        const double p = (double)quick(f, rest);
-        s[0] += (exp_any((double)f) - p) - p * (double)rest;
+        const float t = f * HI, p = __builtin_amdgcn_exp2f(t);
+        const float more = V == 8 && !relative ? f : fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f / REST, f);
+        small = fmaf(p, more, small);
+        s[j & 1] += (double)p;
       }
-      sum = wave_sum64(s[0] + s[1]) / exp_any((double)top);
-    } else {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          float f;
-          if constexpr (V == 8)
-            f = j & 1 ? bf16_hi(x[i][j / 2]) : bf16_lo(x[i][j / 2]);
-          else
-            f = __uint_as_float(x[i][j]);
-          s[j & 1] += exp_any(fmax((double)fmaxf(f, -INFINITY) - (double)top, -700.0));
-        }
-      sum = wave_sum64(s[0] + s[1]);
+      asm volatile("" : "+v"(small));  // (its products here, not all of them at the end)
     }
+    sum += s[0] + s[1] + (double)(small * REST);
+  };
+  if (near) {
+    add(std::false_type());
+  } else if (top_key < INF_KEY && top_key > NO_KEY) {
+    add(std::true_type());
   } else if (top_key == INF_KEY) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i)
+    for (int i = 0; i < LOADS; ++i) {
+      remove(i);
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += exact(key_of(i, j)) == INF_KEY;
-    sum = wave_sum64(sum);
+      for (int j = 0; j < V; ++j) sum += value(i, j) == INFINITY;
+    }
   }
+  sum = wave_sum64(sum);
+  if (lane < 4) mine[n + lane] = 0;  // four of them are compared at a time
   if (lane == 0) {
     count_s[wave] = n;
-    max_s[wave] = top;
     sum_s[wave] = sum;
   }
   __syncthreads();
@@ -383,12 +432,13 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   int total = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) total += count_s[w];
-  for (int i = tid; i < WAVES * CAP; i += NT) {
-    if ((i & (CAP - 1)) >= count_s[i / CAP]) continue;
-    const uint64_t key = list[i];
+  for (int i = lane; i < n; i += 64) {
+    const uint64_t key = mine[i];
     int rank = 0;
     for (int w = 0; w < WAVES; ++w)
-      for (int j = 0; j < count_s[w]; ++j) rank += list[w * CAP + j] > key;
+      for (int j = 0; j < count_s[w]; j += 4)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rank += list[w][j + k] > key;
     if (rank < A.width) {
       st_agent(A.cand_value + out + (int64_t)rank * lists,
                order_value((int)((uint32_t)(key >> 32) ^ 0x80000000u)));
@@ -399,24 +449,18 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   for (int i = total + tid; i < A.width; i += NT)
     st_agent(A.cand_token + out + (int64_t)i * lists, -1);
   if (tid == 0) {
-    float m = max_s[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; ++w) m = fmaxf(m, max_s[w]);
     double s = 0.0;
-    for (int w = 0; w < WAVES; ++w) s += sum_s[w] * exp_between(max_s[w], m);
-    st_agent(A.part_max + (int64_t)row * A.parts + part, m);
+    for (int w = 0; w < WAVES; ++w) s += sum_s[w];
+    if (near) s /= exp_any((double)top);
+    st_agent(A.part_max + (int64_t)row * A.parts + part, top);
     st_agent(reinterpret_cast<uint64_t*>(A.part_sum) + (int64_t)row * A.parts + part,
              __builtin_bit_cast(uint64_t, s));
   }
   stores_done();
 }
 
-// A continuation in order: the larger score first, then the lower place.
-struct Cand {
-  double score;
-  int64_t place;  // beam * vocab + token
-};
-__device__ __forceinline__ bool before(double s, int64_t p, double t, int64_t r) {
+// In order: the larger score first, then the lower place, beam << 24 | token.
+__device__ __forceinline__ bool before(double s, int p, double t, int r) {
   return s > t || (s == t && p < r);
 }
 
@@ -437,10 +481,11 @@ constexpr int MERGE_CAP = 1024, HELD = 4;
 __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   __shared__ float top_s[MAX_BEAMS];
   __shared__ double log_s[MAX_BEAMS];  // score - the log of the sum relative to the maximum
+  __shared__ float own_s[MAX_BEAMS];   // the score of a beam that is done
   __shared__ double cs[MERGE_CAP];
-  __shared__ int64_t cp[MERGE_CAP];
-  __shared__ double bound_s[MERGE_WAVES];
-  __shared__ int64_t best_s[MERGE_WAVES];
+  __shared__ int cp[MERGE_CAP];
+  __shared__ double best_s[MERGE_WAVES];
+  __shared__ int place_s[MERGE_WAVES];
   __shared__ int count_s;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -467,24 +512,33 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
     const float* const pm = A.part_max + (int64_t)row * A.parts;
     const double* const ps = A.part_sum + (int64_t)row * A.parts;
     const float c = A.scores[row];
-    float m = -INFINITY;
-    for (int p = lane; p < A.parts; p += 64) m = fmaxf(m, pm[p]);
+    const uint8_t flag = *(A.done ? A.done + row : reinterpret_cast<const uint8_t*>(A.scores));
+    const int at = min(lane, A.parts - 1);
+    const float m0 = pm[at];
+    const double s0 = ps[at];
+    float m = m0;
+    for (int p = lane + 64; p < A.parts; p += 64) m = fmaxf(m, pm[p]);
     m = wave_max(m);
     double s = 0.0;
-    for (int p = lane; p < A.parts; p += 64) s += ps[p] * exp_between(pm[p], m);
+    for (int p = lane; p < A.parts; p += 64) {
+      const bool held = p == lane;
+      s += (held ? s0 : ps[p]) * exp_between(held ? m0 : pm[p], m);
+    }
     s = wave_sum64(s);
     // log s: fp32's, and what is missing from s exp(-log s) = 1
     const double y = (double)(__builtin_amdgcn_logf((float)s) * 0x1.62e430p-1f);
     const double d = s * exp_any(-y) - 1.0;
     if (lane == 0) {
-      const bool out = (A.done && A.done[row]) || !(c > -INFINITY) || !(s > 0.0);
       top_s[b] = m;
-      log_s[b] = out ? -INFINITY : (double)c - (y + (d - 0.5 * d * d));
+      const bool done = A.done && flag;
+      log_s[b] = done || !(c > -INFINITY) || !(s > 0.0) ? -INFINITY
+                                                        : (double)c - (y + (d - 0.5 * d * d));
+      own_s[b] = done ? c : -INFINITY;
     }
   }
   __syncthreads();
 
-  auto candidate = [&](int e, int tok, float v, double& s, int64_t& place) {
+  auto candidate = [&](int e, int tok, float v, double& s, int& place) {
     const int list = e - small_div(e, lists, lists_inv) * lists;
     const int b = small_div(list, A.parts, parts_inv);
     s = log_s[b];
@@ -493,11 +547,12 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
       return;
     }
     s += v == top_s[b] ? 0.0 : (double)v - (double)top_s[b];
-    place = (int64_t)b * A.vocab + tok;
+    place = b << 24 | tok;
   };
   // The bound: the width-th largest of the lanes' best list heads (ranks of 0), lane l of
-  // every wave with the lists l, l + 64, ..; -inf where there are fewer.  Then all of them.
-  double bound = -INFINITY;
+  // every wave with the lists l, l + 64, .., rounded downwards and found bit by bit (of 16);
+  // -inf where there are fewer.  Then all of them.
+  float bound = -INFINITY;
   for (int pass = 0; pass < 2; ++pass) {
     double best = -INFINITY;
     const int step = pass ? MERGE_NT : 64, end = pass ? n : lists;
@@ -505,8 +560,7 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
 #pragma unroll 1
     for (int e = pass ? tid : lane; e < end; e += step, ++i) {
       double s;
-      int64_t p;
-      int tok;
+      int p, tok;
       float v;
       if (pass ? i < HELD : i == 0) {
         tok = i == 0 ? token[0] : token[1];
@@ -522,7 +576,7 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
       }
       candidate(e, tok, v, s, p);
       best = fmax(best, s);
-      if (pass && s >= bound && s > -INFINITY) {
+      if (pass && s >= (double)bound && s > -INFINITY) {
         const int i = atomicAdd(&count_s, 1);  // (any order: they are ranked)
         if (i < MERGE_CAP) {
           cs[i] = s;
@@ -531,72 +585,60 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
       }
     }
     if (pass) break;
-    const uint64_t u = __builtin_bit_cast(uint64_t, best);
-    auto of_lane = [&](int l) {
-      return __builtin_bit_cast(
-          double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(u >> 32), l) << 32 |
-                      (uint32_t)__builtin_amdgcn_readlane((uint32_t)u, l));
-    };
-    int above = 0;
-#pragma unroll 4
-    for (int l = 0; l < 64; ++l) {
-      const double o = of_lane(l);
-      above += o > best || (o == best && l < lane);
-    }
-    bound = of_lane(__ffsll((unsigned long long)__ballot(above == A.width - 1)) - 1);
+    int least = quick_key((float)best);
+    least -= (double)(float)best > best;
+    int64_t key = quick_key(-INFINITY);
+#pragma unroll 1
+    for (int64_t bit = 1ll << 31; bit >= 1 << 16; bit >>= 1)
+      if (key + bit <= INF_KEY &&
+          __popcll(__builtin_amdgcn_ballot_w64(least >= (int)(key + bit))) >= A.width)
+        key += bit;
+    bound = key_value<32>((int)key);
   }
   // a beam that is done: itself
-  auto own = [&](int b, double& s, int64_t& place) {
-    s = -INFINITY;
-    const int row = seq * A.beams + b;
-    if (b < A.beams && A.done && A.done[row] && A.scores[row] > -INFINITY) {
-      s = (double)A.scores[row];
-      place = (int64_t)b * A.vocab + A.pad_id;
-    }
-  };
-  if (A.done && tid < A.beams) {
-    double s;
-    int64_t p;
-    own(tid, s, p);
-    if (s > -INFINITY) {
-      const int i = atomicAdd(&count_s, 1);
-      if (i < MERGE_CAP) {
-        cs[i] = s;
-        cp[i] = p;
-      }
+  if (tid < A.beams && own_s[tid] > -INFINITY) {
+    const int i = atomicAdd(&count_s, 1);
+    if (i < MERGE_CAP) {
+      cs[i] = (double)own_s[tid];
+      cp[i] = tid << 24 | A.pad_id;
     }
   }
   __syncthreads();
   const int64_t out = (int64_t)seq * A.width;
-  auto put = [&](int rank, double s, int64_t p) {
-    const int b = (int)(p / A.vocab);
-    st_agent(A.parents + out + rank, seq * A.beams + b);
-    st_agent(reinterpret_cast<uint64_t*>(A.tokens) + out + rank,
-             (uint64_t)(p - (int64_t)b * A.vocab));
+  auto put = [&](int rank, double s, int p) {
+    st_agent(A.parents + out + rank, seq * A.beams + (p >> 24));
+    st_agent(reinterpret_cast<uint64_t*>(A.tokens) + out + rank, (uint64_t)(p & 0xffffff));
     st_agent(A.out_scores + out + rank, (float)s);
   };
   int found = count_s;
   if (found <= MERGE_CAP) {
-    for (int i = tid; i < found; i += MERGE_NT) {
-      const double s = cs[i];
-      const int64_t p = cp[i];
+    // eight lanes a candidate
+    for (int i0 = 0; i0 < found; i0 += MERGE_NT / 8) {
+      const int i = i0 + tid / 8, at = min(i, found - 1);
+      const double s = cs[at];
+      const int p = cp[at];
       int rank = 0;
-      for (int j = 0; j < found; ++j) rank += before(cs[j], cp[j], s, p);
-      if (rank < A.width) put(rank, s, p);
+#pragma unroll 4
+      for (int j = tid & 7; j < found; j += 8)
+        rank += (int)(cs[j] > s) | ((int)(cs[j] == s) & (int)(cp[j] < p));
+      rank += other<1>(rank);
+      rank += other<2>(rank);
+      rank += other<4>(rank);
+      if ((tid & 7) == 0 && i < found && rank < A.width) put(rank, s, p);
     }
   } else {
     double last_s = INFINITY;
-    int64_t last_p = -1;
+    int last_p = -1;
     for (found = 0; found < A.width; ++found) {
       double bs = -INFINITY;
-      int64_t bp = INT64_MAX;
-      for (int e = tid; e < n + MERGE_NT; e += MERGE_NT) {
+      int bp = INT_MAX;
+      for (int e = tid; e < n + A.beams; e += MERGE_NT) {
         double s = -INFINITY;
-        int64_t p = 0;
+        int p = 0;
         if (e < n)
           candidate(e, token_of[e], value_of[e], s, p);
-        else
-          own(tid, s, p);
+        else if (e - n < A.beams)
+          s = (double)own_s[e - n], p = (e - n) << 24 | A.pad_id;
         if (s > -INFINITY && before(last_s, last_p, s, p) && before(s, p, bs, bp)) {
           bs = s;
           bp = p;
@@ -605,7 +647,7 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
 #pragma unroll
       for (int mask = 1; mask < 64; mask <<= 1) {
         const double s = __shfl_xor(bs, mask);
-        const int64_t p = __shfl_xor(bp, mask);
+        const int p = __shfl_xor(bp, mask);
         if (before(s, p, bs, bp)) {
           bs = s;
           bp = p;
@@ -613,14 +655,14 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
       }
       __syncthreads();  // the last round's have been read
       if (lane == 0) {
-        bound_s[wave] = bs;
-        best_s[wave] = bp;
+        best_s[wave] = bs;
+        place_s[wave] = bp;
       }
       __syncthreads();
       for (int w = 0; w < MERGE_WAVES; ++w)
-        if (before(bound_s[w], best_s[w], bs, bp)) {
-          bs = bound_s[w];
-          bp = best_s[w];
+        if (before(best_s[w], place_s[w], bs, bp)) {
+          bs = best_s[w];
+          bp = place_s[w];
         }
       if (!(bs > -INFINITY)) break;
       if (tid == 0) put(found, bs, bp);
@@ -636,6 +678,7 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   stores_done();
 }
 
+constexpr int LARGE_NT = 256;
 // Logits of a part: many rows take long ones, few rows short ones that fill the chip.
 int part_size(int64_t rows, int64_t vocab, int elem) {
   const int large = elem == 2 ? 16384 : 8192, small = large / 8;
@@ -682,6 +725,7 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   const int64_t rows = (int64_t)seqs * beams;
   const int size = smx::part_size(rows, vocab, element_size);
   const int parts = (vocab + size - 1) / size;
+  const bool large = size * element_size == 32768;
   smx::BeamArgs a{};
   a.logits = logits;
   a.scores = scores;
@@ -701,9 +745,12 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   a.parts = parts;
   a.pad_id = pad_id;
   const auto kernel = element_size == 2
-      ? (size == 16384 ? smx::beam_parts_kernel<uint16_t, 8> : smx::beam_parts_kernel<uint16_t, 1>)
-      : (size == 8192 ? smx::beam_parts_kernel<float, 8> : smx::beam_parts_kernel<float, 1>);
-  SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(smx::NT), 0, (hipStream_t)stream, a);
+      ? (large ? smx::beam_parts_kernel<uint16_t, smx::LARGE_NT, 2048 / smx::LARGE_NT>
+               : smx::beam_parts_kernel<uint16_t, 256, 1>)
+      : (large ? smx::beam_parts_kernel<float, smx::LARGE_NT, 2048 / smx::LARGE_NT>
+               : smx::beam_parts_kernel<float, 256, 1>);
+  SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(large ? smx::LARGE_NT : 256), 0,
+             (hipStream_t)stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
   SMX_LAUNCH(smx::beam_merge_kernel, dim3(seqs), dim3(smx::MERGE_NT), 0, (hipStream_t)stream, a);
