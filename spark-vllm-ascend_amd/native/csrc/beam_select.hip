@@ -126,8 +126,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 }
 
 // One part (NT * LOADS * V logits) of one row, a wave's share of it in registers: its
-// maximum, the values that reach a bound which `width` of the part do (found from the
-// lanes' maxima), and its sum of exponentials; the few collected of all waves are ranked
+// maximum, the values that reach a bound which `width` of the part do (found from maxima
+// over a lane of each wave), and its sum of exponentials; the few collected of all waves are ranked
 // by counting.
 //
 // The sum, in 64 bits: exp by the transcendental unit, whose errors are a few 1e-8 of each
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   constexpr int PART = NT * LOADS * V;
   __shared__ uint64_t list[WAVES][CAP + 4];
   __shared__ u32x4 tail_s;
-  __shared__ int count_s[WAVES], bound_s[WAVES], top_s[WAVES];
+  __shared__ int count_s[WAVES], best_s[WAVES][64];
   __shared__ double sum_s[WAVES];
   const int part = blockIdx.x, row = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -219,6 +219,12 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
       }
     best = maxima();
   }
+  // Of the lanes l of all waves.
+  best_s[wave][lane] = best;
+  __syncthreads();
+  best = best_s[0][lane];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) best = max(best, best_s[w][lane]);
   int top_key = best;
   top_key = max(top_key, other<1>(top_key));
   top_key = max(top_key, other<2>(top_key));
@@ -228,25 +234,14 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   top_key = max(top_key, other<32>(top_key));
 
   // ---- the largest
-  // The bound: the width-th largest of a wave's lanes' maxima, bit by bit from above, and
-  // the highest of the waves' (each is one for the whole part).
-  int64_t bound_w = NO_KEY + STEP;
-  for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
-    if (bound_w + bit <= INF_KEY &&
-        __popcll(__builtin_amdgcn_ballot_w64(best >= (int)(bound_w + bit))) >= A.width)
-      bound_w += bit;
-  if (lane == 0) {
-    bound_s[wave] = (int)bound_w;
-    top_s[wave] = top_key;
-  }
-  __syncthreads();
-  int bound_key = bound_s[0];
-  top_key = top_s[0];
-#pragma unroll
-  for (int w = 1; w < WAVES; ++w) {
-    bound_key = max(bound_key, bound_s[w]);
-    top_key = max(top_key, top_s[w]);
-  }
+  // The bound: the width-th largest of these 64 maxima, which 1.15 times `width` of a part's
+  // values are expected to reach at a width of 16; bit by bit from above, of 16.
+  int64_t least_key = NO_KEY + STEP;
+  for (int64_t bit = 1ll << 31; bit >= 1 << 16; bit >>= 1)
+    if (least_key + bit <= INF_KEY &&
+        __popcll(__builtin_amdgcn_ballot_w64(best >= (int)(least_key + bit))) >= A.width)
+      least_key += bit;
+  const int bound_key = (int)least_key;
   const float bound = key_value<BITS>(bound_key);
   const float top = key_value<BITS>(max(top_key, NO_KEY));
   uint64_t* const mine = list[wave];
