@@ -61,6 +61,49 @@ __device__ __forceinline__ int scan(int v, int* total, int* waves) {
   return v;
 }
 
+// Calls f(row, aux of the row, place, entry) for the first `pages` entries of each row: a
+// wave two rows at a time with eight loads a lane on their way, the rows' sizes by one load
+// for 64 of them.
+template <typename Pages, typename Aux, typename F>
+__device__ __forceinline__ void each_entry(const int32_t* table, int rows, int max_blocks,
+                                           Pages pages_of, Aux aux_of, F f) {
+  constexpr int WAVES = NT / 64, HELD = 4;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int base = wave; base < rows; base += NT) {
+    const int own = base + WAVES * lane;
+    const int pages = own < rows ? pages_of(own) : 0, aux = own < rows ? aux_of(own) : 0;
+    const int n = min(64, (rows - base + WAVES - 1) / WAVES);
+    for (int l = 0; l < n; l += 2) {
+      int count[2], extra[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // (a lane past the rows has no pages)
+        count[h] = __builtin_amdgcn_readlane(pages, l + h);
+        extra[h] = __builtin_amdgcn_readlane(aux, l + h);
+      }
+      const int most = max(count[0], count[1]);
+      for (int b0 = 0; b0 < most; b0 += 64 * HELD) {
+        int v[2][HELD];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < HELD; ++k) {
+            const int b = b0 + 64 * k + lane;
+            if (b < count[h])
+              v[h][k] = table[(int64_t)(base + WAVES * (l + h)) * max_blocks + b];
+          }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < HELD; ++k) {
+            const int b = b0 + 64 * k + lane;
+            if (b < count[h]) f(base + WAVES * (l + h), extra[h], b, v[h][k]);
+          }
+      }
+    }
+  }
+}
+
 // A row's pages, tokens and pages kept.
 __device__ __forceinline__ void row_sizes(const ForkArgs& A, int r, int& pages, int& len,
                                           int& kept) {
@@ -73,9 +116,9 @@ __device__ __forceinline__ void row_sizes(const ForkArgs& A, int r, int& pages, 
 // a wave a row.
 template <int PAGES, int ROWS>
 __global__ __launch_bounds__(NT) void fork_pages_kernel(ForkArgs A) {
-  __shared__ uint32_t listed[PAGES / 32];  // by an old row, and by no new one in the end
-  __shared__ uint32_t live[PAGES / 32];    // among the kept pages of a row with children
-  __shared__ uint32_t twice[PAGES / 32];   // the same by two rows
+  __shared__ uint32_t listed[PAGES / 32];  // by an old row, other than as a page that stays
+  __shared__ uint32_t live[PAGES / 32];    // whole in a row with children; then all that stay
+  __shared__ uint32_t twice[PAGES / 32];   // listed twice among the kept pages of such rows
   __shared__ int first_s[ROWS];            // a row's first child, INT_MAX: none
   __shared__ int waves[NT / 64];
   const int tid = threadIdx.x;
@@ -98,51 +141,81 @@ __global__ __launch_bounds__(NT) void fork_pages_kernel(ForkArgs A) {
     stores_done();
     return;
   }
+  // What the threads' old rows end with, and their new rows: asked for before all else.
+  constexpr int OWN = ROWS / NT;
+  const int count = min(max(A.free_count[0], 0), A.num_free);
+  int parent[OWN], kept[OWN], len[OWN], page[OWN], tail[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const int j = tid + i * NT;
+    parent[i] = page[i] = tail[i] = -1;
+    kept[i] = len[i] = 0;
+    if (j < A.rows) {
+      int pages, n, k;
+      row_sizes(A, j, pages, n, k);
+      if (n & (bs - 1)) tail[i] = A.table[(int64_t)j * A.max_blocks + k - 1];
+      const int r = A.parents[j];
+      if (r >= 0 && r < A.rows) {
+        parent[i] = r;
+        row_sizes(A, r, pages, len[i], kept[i]);
+        if (len[i] & (bs - 1)) page[i] = A.table[(int64_t)r * A.max_blocks + kept[i] - 1];
+      }
+    }
+  }
   for (int i = tid; i < PAGES / 32; i += NT) listed[i] = live[i] = twice[i] = 0;
   for (int i = tid; i < A.rows; i += NT) first_s[i] = INT_MAX;
   __syncthreads();
-  for (int j = tid; j < A.rows; j += NT) {
-    const int r = A.parents[j];
-    if (r >= 0 && r < A.rows) atomicMin(first_s + r, j);
+#pragma unroll
+  for (int i = 0; i < OWN; ++i)
+    if (parent[i] >= 0) atomicMin(first_s + parent[i], tid + i * NT);
+  __syncthreads();
+  const auto pages_of = [&](int r) { return min(max(A.num_pages[r], 0), A.max_blocks); };
+  const auto whole_of = [&](int r) {
+    int pages, n, k;
+    row_sizes(A, r, pages, n, k);
+    return first_s[r] == INT_MAX ? 0 : n >> A.bs_log2;
+  };
+  each_entry(A.table, A.rows, A.max_blocks, pages_of, whole_of,
+             [&](int, int whole, int b, int p) {
+               if ((unsigned)p >= (unsigned)A.num_blocks) return;
+               if (b >= whole) {
+                 set_bit(listed, p);
+                 return;
+               }
+               const uint32_t bit = 1u << (p & 31);
+               if (atomicOr(live + (p >> 5), bit) & bit) set_bit(twice, p);
+             });
+  __syncthreads();
+  // ---- tails: which of their pages are whole ones elsewhere, then which are listed twice
+  // (each new row takes a copy of such a page, so that it stays only as a whole one)
+  bool only[OWN];
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    const int r = tid + i * NT;
+    if ((unsigned)tail[i] >= (unsigned)A.num_blocks || first_s[r] == INT_MAX) tail[i] = -1;
+    only[i] = tail[i] >= 0 && !get_bit(live, tail[i]);
   }
   __syncthreads();
-  // a wave a row
-  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
-    int pages, len, kept;
-    row_sizes(A, r, pages, len, kept);
-    const bool parent = first_s[r] != INT_MAX;
-    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
-    for (int b = tid & 63; b < pages; b += 64) {
-      const int p = src[b];
-      if ((unsigned)p >= (unsigned)A.num_blocks) continue;
-      set_bit(listed, p);
-      if (parent && b < kept) {
-        const uint32_t bit = 1u << (p & 31);
-        if (atomicOr(live + (p >> 5), bit) & bit) set_bit(twice, p);
-      }
+#pragma unroll
+  for (int i = 0; i < OWN; ++i)
+    if (tail[i] >= 0) {
+      const uint32_t bit = 1u << (tail[i] & 31);
+      if (atomicOr(live + (tail[i] >> 5), bit) & bit) set_bit(twice, tail[i]);
     }
-  }
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < OWN; ++i)
+    if (only[i] && get_bit(twice, tail[i]))
+      atomicAnd(live + (tail[i] >> 5), ~(1u << (tail[i] & 31)));
   // ---- copies, in the order of the new rows, from the end of the free list
-  const int count = min(max(A.free_count[0], 0), A.num_free);
   int taken = 0;
-  for (int j0 = 0; j0 < A.rows; j0 += NT) {
-    const int j = j0 + tid;
-    int kept = 0, len = 0, page = -1;
-    bool tail = false, copy = false;
-    if (j < A.rows) {
-      const int r = A.parents[j];
-      if (r >= 0 && r < A.rows) {
-        int pages;
-        row_sizes(A, r, pages, len, kept);
-        tail = len & (bs - 1);
-        if (tail) {
-          page = A.table[(int64_t)r * A.max_blocks + kept - 1];
-          copy = (unsigned)page < (unsigned)A.num_blocks &&
-                 (first_s[r] != j || get_bit(twice, page));
-        }
-      }
-    }
+#pragma unroll
+  for (int i = 0; i < OWN; ++i) {
+    if (i * NT >= A.rows) break;
+    const int j = tid + i * NT;
+    const bool ends = len[i] & (bs - 1);
+    const bool copy = ends && (unsigned)page[i] < (unsigned)A.num_blocks &&
+                      (first_s[parent[i]] != j || get_bit(twice, page[i]));
     int all;
     const int at = count - taken - scan(copy, &all, waves);
     if (j < A.rows) {
@@ -151,40 +224,23 @@ __global__ __launch_bounds__(NT) void fork_pages_kernel(ForkArgs A) {
         // (an entry of the free list outside the pool is no page)
         dst = at >= 0 ? A.free_pages[at] : -1;
         if ((unsigned)dst >= (unsigned)A.num_blocks) dst = -1;
-        if (dst >= 0) src = page;
+        if (dst >= 0) src = page[i];
       }
-      if (tail)
-        st_agent(A.table_out + (int64_t)j * A.max_blocks + kept - 1, copy ? dst : page);
+      if (ends)
+        st_agent(A.table_out + (int64_t)j * A.max_blocks + kept[i] - 1, copy ? dst : page[i]);
       if (copy && dst < 0) {  // no room: the row ends with its whole pages
-        --kept;
-        len = kept << A.bs_log2;
+        --kept[i];
+        len[i] = kept[i] << A.bs_log2;
       }
-      st_agent(A.num_pages_out + j, kept);
-      st_agent(A.lens_out + j, len);
+      st_agent(A.num_pages_out + j, kept[i]);
+      st_agent(A.lens_out + j, len[i]);
       st_agent(A.copies + 2 * j, src);
       st_agent(A.copies + 2 * j + 1, dst);
     }
     taken += all;
   }
-  // ---- pages that no new row lists: `live` is now what the new rows list, which their
-  // first child lists (the pages of the free list apart): whole pages, and a tail that it
-  // has no copy of.
   __syncthreads();
-  for (int i = tid; i < PAGES / 32; i += NT) live[i] = 0;
-  __syncthreads();
-  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
-    if (first_s[r] == INT_MAX) continue;
-    int pages, len, kept;
-    row_sizes(A, r, pages, len, kept);
-    const int whole = len >> A.bs_log2;
-    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
-    for (int b = tid & 63; b < kept; b += 64) {
-      const int p = src[b];
-      if ((unsigned)p < (unsigned)A.num_blocks && (b < whole || !get_bit(twice, p)))
-        set_bit(live, p);
-    }
-  }
-  __syncthreads();
+  // ---- pages that no new row lists: free again
   const int left = max(count - taken, 0);
   for (int i = tid; i < left; i += NT)
     if (A.free_pages_out != A.free_pages) st_agent(A.free_pages_out + i, A.free_pages[i]);
@@ -218,7 +274,8 @@ struct CompactArgs {
 };
 
 // With U pages in use, those from U on move to the unused ones below it, in order: the
-// k-th such page to the k-th such place.  Both ranks come from the sums of the set's words.
+// k-th such page to the k-th such place.  Both ranks come from the sums of the set's words;
+// the tables' new entries are read off the list of moves.
 template <int PAGES>
 __global__ __launch_bounds__(NT) void compact_pages_kernel(CompactArgs A) {
   __shared__ uint32_t used[PAGES / 32];
@@ -228,14 +285,11 @@ __global__ __launch_bounds__(NT) void compact_pages_kernel(CompactArgs A) {
   const int words = (A.num_blocks + 31) / 32;
   for (int i = tid; i < words; i += NT) used[i] = 0;
   __syncthreads();
-  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
-    const int pages = min(max(A.num_pages[r], 0), A.max_blocks);
-    const int32_t* const src = A.table + (int64_t)r * A.max_blocks;
-    for (int b = tid & 63; b < pages; b += 64) {
-      const int p = src[b];
-      if ((unsigned)p < (unsigned)A.num_blocks) set_bit(used, p);
-    }
-  }
+  const auto pages_of = [&](int r) { return min(max(A.num_pages[r], 0), A.max_blocks); };
+  each_entry(A.table, A.rows, A.max_blocks, pages_of, [](int) { return 0; },
+             [&](int, int, int, int p) {
+               if ((unsigned)p < (unsigned)A.num_blocks) set_bit(used, p);
+             });
   __syncthreads();
   int total = 0;
   for (int w0 = 0; w0 < words; w0 += NT) {
@@ -251,42 +305,30 @@ __global__ __launch_bounds__(NT) void compact_pages_kernel(CompactArgs A) {
     return before[p >> 5] + __popc(used[p >> 5] & ((1u << (p & 31)) - 1));
   };
   const int kept = total > 0 ? rank_of(total - 1) + get_bit(used, total - 1) : 0;  // below `total`
-  auto hole = [&](int k) {  // the k-th unused page
-    int lo = 0, hi = words;  // the last word with at most k unused pages before it
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (32 * mid - before[mid] <= k)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    uint32_t free_bits = ~used[lo];
-    for (int i = k - (32 * lo - before[lo]); i > 0; --i) free_bits &= free_bits - 1;
-    return 32 * lo + __ffs(free_bits) - 1;
-  };
-  const int moved = total - kept;  // pages in use from `total` on
-  for (int w = (total >> 5) + tid; w < words; w += NT) {
-    uint32_t bits = used[w];
-    if (w == total >> 5) bits &= ~0u << (total & 31);
-    for (; bits; bits &= bits - 1) {
-      const int p = 32 * w + __ffs(bits) - 1, k = rank_of(p) - kept;
-      st_agent(A.moves + 2 * k, p);
-      st_agent(A.moves + 2 * k + 1, hole(k));
-    }
+  // Moves: a thread a word, its pages in use from `total` on and its unused ones below it.
+  const int moved = total - kept;
+  for (int w = tid; w < words; w += NT) {
+    const int rest = total - 32 * w;  // the word's pages below `total`
+    const uint32_t low = rest >= 32 ? ~0u : rest <= 0 ? 0u : (1u << rest) - 1;
+    int k = before[w] + __popc(used[w] & low) - kept;
+    for (uint32_t bits = used[w] & ~low; bits; bits &= bits - 1)
+      st_agent(A.moves + 2 * k++, 32 * w + __ffs(bits) - 1);
+    k = 32 * w - before[w];
+    for (uint32_t bits = ~used[w] & low; bits; bits &= bits - 1)
+      st_agent(A.moves + 2 * k++ + 1, 32 * w + __ffs(bits) - 1);
   }
   for (int i = 2 * moved + tid; i < 2 * (A.num_blocks / 2); i += NT) st_agent(A.moves + i, -1);
-  for (int r = tid >> 6; r < A.rows; r += NT / 64) {
-    const int pages = min(max(A.num_pages[r], 0), A.max_blocks);
-    for (int b = tid & 63; b < A.max_blocks; b += 64) {
-      const int64_t at = (int64_t)r * A.max_blocks + b;
-      int p = b < pages ? A.table[at] : -1;
-      if ((unsigned)p >= (unsigned)A.num_blocks)
-        p = -1;
-      else if (p >= total)
-        p = hole(rank_of(p) - kept);
-      st_agent(A.table_out + at, p);
-    }
-  }
+  stores_done();
+  __syncthreads();
+  each_entry(A.table, A.rows, A.max_blocks, [&](int) { return A.max_blocks; }, pages_of,
+             [&](int r, int pages, int b, int p) {
+               if (b >= pages || (unsigned)p >= (unsigned)A.num_blocks)
+                 p = -1;
+               else if (p >= total)
+                 p = __hip_atomic_load(A.moves + 2 * (rank_of(p) - kept) + 1, __ATOMIC_RELAXED,
+                                       __HIP_MEMORY_SCOPE_AGENT);
+               st_agent(A.table_out + (int64_t)r * A.max_blocks + b, p);
+             });
   for (int i = tid; i < A.num_blocks; i += NT)
     st_agent(A.free_pages + i, i < A.num_blocks - total ? A.num_blocks - 1 - i : -1);
   if (tid == 0) st_agent(A.free_count, A.num_blocks - total);
