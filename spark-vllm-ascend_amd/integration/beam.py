@@ -1,0 +1,77 @@
+"""Beam search over paged caches, on the device.
+
+The reference samples one sequence greedily (src/spark_vllm_ascend/integration/
+head.py:12-31).  Here a step of logits becomes the next step's rows without the host:
+``torch_ops.beam_select`` takes each sequence's best continuations, ``DeviceBlockTables.fork``
+the pages that they share and ``torch_ops.copy_pages`` the last pages that they write to.
+
+    search = BeamSearch(tables, torch_ops.PageSet(cache.planes()), beams, eos_id)
+    tables.step(lens)               # the prompts, in each sequence's first row
+    ... logits of the prompts' last tokens ...
+    for _ in range(n):
+        tokens = search.step(logits)
+        step = tables.step(search.query_lens())
+        ... logits of the rows' new tokens ...
+    search.sequences()
+"""
+from __future__ import annotations
+
+import torch
+
+from ..native import torch_ops
+from .block_table import DeviceBlockTables
+
+
+class BeamSearch:
+    """The beams of several sequences: row s * beams + b of `tables` is sequence s's beam b,
+    the best first; `pages` are the caches that the tables' pages are of.  A sequence
+    starts with one beam, its prompt in row s * beams.  A beam ends with eos_id (-1: none
+    does) and keeps its score and place among the others; it takes no more tokens."""
+
+    def __init__(self, tables: DeviceBlockTables, pages: torch_ops.PageSet, beams: int,
+                 eos_id: int = -1, pad_id: int = 0):
+        rows = tables.lens.numel()
+        if not 1 <= beams <= 64 or rows % beams:
+            raise ValueError("the tables must have `beams` rows, 1 to 64, for each sequence")
+        if not isinstance(pages, torch_ops.PageSet):
+            raise ValueError("pages must be a PageSet")
+        if pages.num_blocks != tables.free_pages.numel():
+            raise ValueError("the caches must have as many pages as the tables")
+        self.tables, self.pages, self.beams = tables, pages, beams
+        self.eos_id, self.pad_id = eos_id, pad_id
+        dev = tables.lens.device
+        self.scores = torch.zeros((rows // beams, beams), dtype=torch.float32, device=dev)
+        self.scores[:, 1:] = float("-inf")
+        self.done = torch.zeros(rows, dtype=torch.bool, device=dev)
+        self._history: list = []
+
+    def step(self, logits: torch.Tensor) -> torch.Tensor:
+        """Goes on from the rows' logits [rows, vocab] (those of a row without a score, or
+        done, are not looked at): the rows' next tokens, int64 [rows], pad_id where a beam is
+        done or there is none.  The tables' rows are those of the new beams."""
+        best = torch_ops.beam_select(logits, self.scores.view(-1), self.beams, self.beams,
+                                     done=self.done, pad_id=self.pad_id)
+        parents, tokens = best.parents.view(-1), best.tokens.view(-1)
+        was_done = self.done[parents.clamp(min=0).long()]
+        self.scores = best.scores
+        self.done = (tokens == self.eos_id) | was_done | (parents < 0)
+        torch_ops.copy_pages(self.pages, self.tables.fork(parents))
+        self._history.append((parents, torch.where(parents < 0, self.pad_id, tokens)))
+        return self._history[-1][1]
+
+    def query_lens(self) -> torch.Tensor:
+        """The tokens a row takes in the next step, 1 or 0: tables.step's argument."""
+        return (~self.done).to(torch.int32)
+
+    def sequences(self) -> torch.Tensor:
+        """The beams' tokens so far, int64 [seqs, beams, steps], the best first (`scores`;
+        rows of -inf are no beams), pad_id behind the end of one that is done."""
+        rows = self.done.numel()
+        at = torch.arange(rows, device=self.done.device)
+        out = []
+        for parents, tokens in reversed(self._history):
+            out.append(tokens[at])
+            at = parents[at].clamp(min=0).long()
+        if not out:
+            return at.new_zeros((rows // self.beams, self.beams, 0))
+        return torch.stack(out[::-1], 1).view(rows // self.beams, self.beams, -1)

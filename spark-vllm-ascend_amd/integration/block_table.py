@@ -12,7 +12,9 @@ are -1).  Slots for a step come from ``torch_ops.compute_slot_mapping``.
 DeviceBlockTables keeps all of that on the device instead, where the lengths
 may be known there alone (drafted tokens accepted by a kernel, steps in a
 captured graph): a step is one or two launches of ``torch_ops.request_tables``
-and five small ones that count what it kept, ``keep`` is three.
+and five small ones that count what it kept, ``keep`` is three.  ``fork`` makes rows
+that share pages (beams, several samples of a prompt) and ``compact`` moves the pages
+in use to the front of the pool.
 """
 from __future__ import annotations
 
@@ -117,7 +119,8 @@ class BlockManager:
 
 class DeviceBlockTables:
     """Pages, block tables and lengths of up to `max_seqs` requests, on the device:
-    request r is row r, a page is one request's.  Steps follow one another on a stream.
+    request r is row r, a page is one request's until fork() makes several share it.
+    Steps follow one another on a stream.
 
     Nothing is read back, so a step is not refused where there is no room: a token
     without a page (the free list is used up, or the row's max_blocks_per_seq pages
@@ -146,6 +149,7 @@ class DeviceBlockTables:
             num_pages=self.num_pages, free_count=self.free_count)
         self._ends = torch.zeros(max_seqs + 1, **i32)
         self._room = torch.zeros(max_seqs, **i32)
+        self._forked = self._moves = None
 
     def step(self, query_lens: torch.Tensor) -> torch_ops.RequestTables:
         """query_lens (int32 [max_seqs], on the device) more tokens a request: takes
@@ -167,7 +171,44 @@ class DeviceBlockTables:
 
     def keep(self, lens: torch.Tensor) -> None:
         """Takes every request back to its first lens[r] tokens (int32 [max_seqs]; one
-        past its length keeps it, 0 ends it): pages no longer needed are free again."""
+        past its length keeps it, 0 ends it): pages no longer needed are free again.
+        Not after a fork, since it takes a row's pages for its own: fork() ends requests
+        then, by not continuing them."""
+        if self._forked is not None:
+            raise RuntimeError("keep() frees a row's pages, which rows share after a fork()")
         torch_ops.release_pages(lens, self.num_pages, self.free_pages, self.free_count,
                                 self.block_table, self.block_size)
         torch.minimum(self.lens, lens.clamp(min=0), out=self.lens)
+
+    def fork(self, parents: torch.Tensor) -> torch.Tensor:
+        """Row r goes on with what row parents[r] holds (int32 [max_seqs]; -1: with
+        nothing).  Full pages are shared, a last page that is not full is one row's: the
+        copies that this takes are returned, int32 [max_seqs, 2], to be done by
+        torch_ops.copy_pages before the next tokens are written (a buffer of this object,
+        valid until the next fork).  A row for whose copy there is no page is cut to its
+        whole pages."""
+        if self._forked is None:
+            self._forked = torch_ops.ForkedPages(
+                torch.empty_like(self.block_table), torch.empty_like(self.num_pages),
+                torch.empty_like(self.lens), self.free_pages, self.free_count,
+                self.num_pages.new_empty((self.num_pages.numel(), 2)))
+        out = torch_ops.fork_pages(parents, self.lens, self.num_pages, self.free_pages,
+                                   self.free_count, self.block_table, self.free_pages.numel(),
+                                   self.block_size, out=self._forked)
+        # (in place: graphs hold the tables' addresses)
+        self.block_table.copy_(out.block_table)
+        self.num_pages.copy_(out.num_pages)
+        self.lens.copy_(out.lens)
+        return out.copies
+
+    def compact(self) -> torch.Tensor:
+        """Moves the pages in use to the front of the pool: the moves are returned, int32
+        [num_blocks // 2, 2], to be done by torch_ops.copy_pages before the cache is used
+        again (a buffer of this object, valid until the next compact)."""
+        if self._moves is None:
+            self._moves = self.num_pages.new_empty((self.free_pages.numel() // 2, 2))
+        torch_ops.compact_pages(
+            self.num_pages, self.block_table, self.free_pages.numel(),
+            out=torch_ops.CompactedPages(self.block_table, self.free_pages, self.free_count,
+                                         self._moves))
+        return self._moves
