@@ -131,9 +131,9 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // by counting.
 //
 // The sum, in 64 bits: exp by the transcendental unit, whose errors are a few 1e-8 of each
-// term; the collected values, which are most of a peaked row's sum, are left out of it and
-// taken in 64 bits.  So what is left is 1e-9 of it, and less where many terms' errors
-// average out; equal logits of two beams have equal errors.
+// term, and again in 64 bits for the collected values, which are most of a peaked row's
+// sum.  So what is left is 1e-9 of it, and less where many terms' errors average out; equal
+// logits of two beams have equal errors.
 template <typename L, int NT, int LOADS>
 __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   constexpr int WAVES = NT / 64;
@@ -263,12 +263,10 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   };
   // Puts the values of load i that `in(j)` says into the list, in no particular order: a
   // bit a value, the set ones lane by lane.
-  uint32_t taken[(LOADS * V + 31) / 32] = {};
   auto collect = [&](int i, auto in) {
     uint32_t bits = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) bits = bits + bits + (in(j) ? 1u : 0u);
-    taken[i * V / 32] |= bits << (i * V % 32);
     while (const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0)) {
       const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
@@ -316,7 +314,6 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
       if (least + bit <= INF_KEY && reach((int)(least + bit)) >= A.width) least += bit;
     n = 0;
-    for (uint32_t& bits : taken) bits = 0;
     int missing = A.width - reach((int)least + STEP);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -340,35 +337,22 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   // ---- the sum of exponentials: as they are, relative to `top` where that is large
   const bool near = top > -16.f && top < 16.f;
   double sum = 0.0;
-  // a term in 64 bits (+inf: as many equal ones; -inf and NaN: 0)
-  auto exact = [&](float f) -> double {
-    if (!(f > -INFINITY)) return 0.0;
-    if (near) return exp_any(fmax((double)f, -700.0));
-    return exp_between(f, top);
+  // exp f = 2^(f HI) (1 + f REST), HI log2(e) to 16 bits, so that a bf16 value's product with
+  // it is exact, and REST what is missing, times log 2; the next term, half of (f REST)^2, is
+  // below 4e-9 at 16 and less below.  Other products' rounding is made good.  The first
+  // factor is `p`, the second 1 + `more` REST.
+  constexpr float HI = 0x1.7154p+0f, REST = 0x1.480fb6p-18f;
+  auto quick = [&](auto relative, float f, float& more) -> float {
+    const float t = f * HI;
+    more = V == 8 && !relative ? f : fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f / REST, f);
+    return __builtin_amdgcn_exp2f(t);
   };
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
-  for (int i = lane; i < n; i += 64)
-    sum += exact(order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u)));
-  // the collected values of load i: -inf from here on
-  auto remove = [&](int i) {
-    const uint32_t bits = taken[i * V / 32] >> (i * V % 32);
-    if (!__builtin_amdgcn_ballot_w64((bits & ((1u << V) - 1)) != 0)) return;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      if (!(bits >> (V - 1 - j) & 1)) continue;
-      uint32_t w = x[i][j / (V / 4)];
-      if constexpr (V == 8)
-        w = j & 1 ? (w & 0xffffu) | 0xff800000u : (w & 0xffff0000u) | 0xff80u;
-      else
-        w = NONE;
-      x[i][j / (V / 4)] = w;
-    }
+  // (exact where it is small: v is half of `top` at least, or exp(v - top) below e^-8)
+  auto from_top = [&](float v) {
+    const float f = v - top;
+    return f > -200.f ? f : -200.f;
   };
-  // The others': exp f = 2^(f HI) (1 + f REST), HI log2(e) to 16 bits, so that a bf16 value's
-  // product with it is exact, and REST what is missing, times log 2; the next term, half of
-  // (f REST)^2, is below 4e-9 at 16 and less below.  Other products' rounding is made good.
   auto add = [&](auto relative) {
-    constexpr float HI = 0x1.7154p+0f, REST = 0x1.480fb6p-18f;
     // (values below -200, -inf and NaN with a sign are larger as unsigned numbers)
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     typedef typename std::conditional<V == 8, u16x2, uint32_t>::type Bits;
@@ -376,14 +360,11 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     float small = 0.f;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      remove(i);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         float f;
         if constexpr (relative) {
-          // exact where it is small: f is half of `top` at least, or exp(f - top) below e^-8
-          f = value(i, j) - top;
-          f = f > -200.f ? f : -200.f;
+          f = from_top(value(i, j));
         } else {
           if (j % (V / 4) == 0) {
             const uint32_t u = x[i][j / (V / 4)];
@@ -393,14 +374,24 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
           }
           f = value(i, j);
         }
-        const float t = f * HI, p = __builtin_amdgcn_exp2f(t);
-        const float more = V == 8 && !relative ? f : fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f / REST, f);
+        float more;
+        const float p = quick(relative, f, more);
         small = fmaf(p, more, small);
         s[j & 1] += (double)p;
       }
       asm volatile("" : "+v"(small));  // (its products here, not all of them at the end)
     }
-    sum += s[0] + s[1] + (double)(small * REST);
+    sum = s[0] + s[1] + (double)(small * REST);
+    // the collected ones' in 64 bits
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
+    for (int i = lane; i < n; i += 64) {
+      const float v = order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u));
+      const float f = relative ? from_top(v) : fmaxf(v, -200.f);
+      float more;
+      const double p = (double)quick(relative, f, more);
+      sum += (exp_any(relative ? fmax((double)v - (double)top, -700.0) : (double)f) - p) -
+             p * (double)(more * REST);
+    }
   };
   if (near) {
     add(std::false_type());
@@ -408,11 +399,9 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     add(std::true_type());
   } else if (top_key == INF_KEY) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      remove(i);
+    for (int i = 0; i < LOADS; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) sum += value(i, j) == INFINITY;
-    }
   }
   sum = wave_sum64(sum);
   if (lane < 4) mine[n + lane] = 0;  // four of them are compared at a time
