@@ -112,7 +112,7 @@ __device__ __forceinline__ void row_sizes(const ForkArgs& A, int r, int& pages, 
   kept = (int)(((int64_t)len + (1 << A.bs_log2) - 1) >> A.bs_log2);
 }
 
-// Workgroup 0 does all but the tables' whole columns, which the others copy: 4 rows each,
+// Workgroup 0 does all but the tables' whole columns, which the others copy: 16 rows each,
 // a wave a row.
 template <int PAGES, int ROWS>
 __global__ __launch_bounds__(NT) void fork_pages_kernel(ForkArgs A) {
