@@ -6,9 +6,14 @@
 // One pass over the logits.  A beam's best are its largest logits, so a workgroup keeps
 // the `width` largest of its part of a row and the part's maximum and sum of exponentials
 // (beam_parts_kernel); a workgroup a sequence then takes the best of the parts'
-// (beam_merge_kernel).  Beams are compared by their sums, so these are good to about 1e-9
+// (beam_merge_kernel).  Beams are compared by their sums, so these are good to about 2e-9
 // and joined in 64 bits: two beams' candidates whose scores differ by less than that might
 // be taken in the wrong order, where fp32 sums would confuse those within 1e-6.
+//
+// Bound by vector instructions where there are many rows: 512 rows of 151936 bf16 values,
+// a tenth of them done, 16 best of 8 beams: 56 us, the parts 45 (3.1 TB/s; about 17
+// instructions a value, an exponential and a 64-bit sum among them), the merge 9.  4 rows
+// 10.9 us: two launches of short latencies one after another.
 //
 // A NaN logit counts as -inf, a token that is never chosen; of several logits of +inf each
 // has an equal share.
@@ -28,6 +33,12 @@ typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
 constexpr int CAP = 128;  // candidates of a wave
+constexpr int NT = 256, WAVES = NT / 64;
+// Of 16 bytes, a lane: a part is 32 KB of a row.  us with 2 / 4 / 8 of them, rows of 151936
+// bf16 values: 1 row 9.2 / 9.3 / 10.0, 16 rows 11.2 / 10.9 / 10.8, 128 rows 25 / 21 / 20,
+// 512 rows (an eighth done) 77 / 58 / 56; 64 rows of 32000 10.0 / 10.1 / 10.9, 512 rows 22 /
+// 19 / 19.
+constexpr int LOADS = 8;
 
 struct BeamArgs {
   const void* logits;
@@ -134,9 +145,8 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // term, and again in 64 bits for the collected values, which are most of a peaked row's
 // sum.  So what is left is 1e-9 of it, and less where many terms' errors average out; equal
 // logits of two beams have equal errors.
-template <typename L, int NT, int LOADS>
+template <typename L>
 __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
-  constexpr int WAVES = NT / 64;
   constexpr int V = 16 / sizeof(L);  // logits of a load
   constexpr int PART = NT * LOADS * V;
   __shared__ uint64_t list[WAVES][CAP + 4];
@@ -662,11 +672,10 @@ __global__ __launch_bounds__(MERGE_NT) void beam_merge_kernel(BeamArgs A) {
   stores_done();
 }
 
-constexpr int LARGE_NT = 256;
-// Logits of a part: many rows take long ones, few rows short ones that fill the chip.
-int part_size(int64_t rows, int64_t vocab, int elem) {
-  const int large = elem == 2 ? 16384 : 8192, small = large / 8;
-  return rows * ((vocab + large - 1) / large) >= 512 ? large : small;
+// Parts of a row of `vocab` logits of `elem` bytes.
+int num_parts(int64_t vocab, int elem) {
+  const int64_t size = NT * LOADS * 16 / elem;
+  return (int)((vocab + size - 1) / size);
 }
 
 }  // namespace
@@ -679,9 +688,7 @@ extern "C" int64_t smx_beam_select_workspace(int32_t seqs, int32_t beams, int32_
   if (seqs < 1 || beams < 1 || width < 1 || vocab < 1 || (element_size != 2 && element_size != 4))
     return -1;
   const int64_t rows = (int64_t)seqs * beams;
-  const int64_t size = smx::part_size(rows, vocab, element_size);
-  const int64_t parts = (vocab + size - 1) / size;
-  return rows * parts * (8 + 4 + 8 * (int64_t)width);
+  return rows * smx::num_parts(vocab, element_size) * (8 + 4 + 8 * (int64_t)width);
 }
 
 extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
@@ -707,9 +714,7 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   SMX_REQUIRE(workspace_bytes >= smx_beam_select_workspace(seqs, beams, width, vocab, element_size),
               "workspace must hold smx_beam_select_workspace bytes");
   const int64_t rows = (int64_t)seqs * beams;
-  const int size = smx::part_size(rows, vocab, element_size);
-  const int parts = (vocab + size - 1) / size;
-  const bool large = size * element_size == 32768;
+  const int parts = smx::num_parts(vocab, element_size);
   smx::BeamArgs a{};
   a.logits = logits;
   a.scores = scores;
@@ -728,13 +733,9 @@ extern "C" int smx_beam_select(void* stream, const void* logits, int64_t stride,
   a.vocab = vocab;
   a.parts = parts;
   a.pad_id = pad_id;
-  const auto kernel = element_size == 2
-      ? (large ? smx::beam_parts_kernel<uint16_t, smx::LARGE_NT, 2048 / smx::LARGE_NT>
-               : smx::beam_parts_kernel<uint16_t, 256, 1>)
-      : (large ? smx::beam_parts_kernel<float, smx::LARGE_NT, 2048 / smx::LARGE_NT>
-               : smx::beam_parts_kernel<float, 256, 1>);
-  SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(large ? smx::LARGE_NT : 256), 0,
-             (hipStream_t)stream, a);
+  const auto kernel = element_size == 2 ? smx::beam_parts_kernel<uint16_t>
+                                        : smx::beam_parts_kernel<float>;
+  SMX_LAUNCH(kernel, dim3(parts, (unsigned)rows), dim3(smx::NT), 0, (hipStream_t)stream, a);
   const int rc = (int)hipGetLastError();
   if (rc) return rc;
   SMX_LAUNCH(smx::beam_merge_kernel, dim3(seqs), dim3(smx::MERGE_NT), 0, (hipStream_t)stream, a);
