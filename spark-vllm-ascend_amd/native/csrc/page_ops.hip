@@ -61,44 +61,43 @@ __device__ __forceinline__ int scan(int v, int* total, int* waves) {
   return v;
 }
 
-// Calls f(row, aux of the row, place, entry) for the first `pages` entries of each row: a
-// wave two rows at a time with eight loads a lane on their way, the rows' sizes by one load
-// for 64 of them.
+// Calls f(row, aux of the row, place, entry) for the first `pages` entries of each row: 16
+// lanes a row, a wave eight rows at a time with eight loads a lane on their way (rows of
+// some tens of pages are the common ones), the rows' sizes by one load for 64 of them.
 template <typename Pages, typename Aux, typename F>
 __device__ __forceinline__ void each_entry(const int32_t* table, int rows, int max_blocks,
                                            Pages pages_of, Aux aux_of, F f) {
-  constexpr int WAVES = NT / 64, HELD = 4;
+  constexpr int WAVES = NT / 64, HELD = 4, SIDE = 2, LANES = 16, AT_ONCE = 64 / LANES;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   for (int base = wave; base < rows; base += NT) {
     const int own = base + WAVES * lane;
     const int pages = own < rows ? pages_of(own) : 0, aux = own < rows ? aux_of(own) : 0;
     const int n = min(64, (rows - base + WAVES - 1) / WAVES);
-    for (int l = 0; l < n; l += 2) {
-      int count[2], extra[2];
+    for (int l = lane / LANES; l - lane / LANES < n; l += AT_ONCE * SIDE) {
+      int count[SIDE], extra[SIDE];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // (a lane past the rows has no pages)
-        count[h] = __builtin_amdgcn_readlane(pages, l + h);
-        extra[h] = __builtin_amdgcn_readlane(aux, l + h);
+      for (int h = 0; h < SIDE; ++h) {  // (a lane past the rows has no pages)
+        count[h] = __shfl(pages, l + AT_ONCE * h);
+        extra[h] = __shfl(aux, l + AT_ONCE * h);
       }
-      const int most = max(count[0], count[1]);
-      for (int b0 = 0; b0 < most; b0 += 64 * HELD) {
-        int v[2][HELD];
+      int b0 = lane % LANES;
+      while (__builtin_amdgcn_ballot_w64(b0 < max(count[0], count[1]))) {
+        int v[SIDE][HELD];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < SIDE; ++h)
 #pragma unroll
-          for (int k = 0; k < HELD; ++k) {
-            const int b = b0 + 64 * k + lane;
-            if (b < count[h])
-              v[h][k] = table[(int64_t)(base + WAVES * (l + h)) * max_blocks + b];
-          }
+          for (int k = 0; k < HELD; ++k)
+            if (b0 + LANES * k < count[h])
+              v[h][k] = table[(int64_t)(base + WAVES * (l + AT_ONCE * h)) * max_blocks + b0 +
+                              LANES * k];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < SIDE; ++h)
 #pragma unroll
-          for (int k = 0; k < HELD; ++k) {
-            const int b = b0 + 64 * k + lane;
-            if (b < count[h]) f(base + WAVES * (l + h), extra[h], b, v[h][k]);
-          }
+          for (int k = 0; k < HELD; ++k)
+            if (b0 + LANES * k < count[h])
+              f(base + WAVES * (l + AT_ONCE * h), extra[h], b0 + LANES * k, v[h][k]);
+        b0 += LANES * HELD;
       }
     }
   }
