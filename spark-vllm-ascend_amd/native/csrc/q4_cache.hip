@@ -10,8 +10,8 @@
 namespace smx {
 namespace {
 
-// HD / 8 lanes a (token, head) pair, K's pairs and then V's.  Lanes past the end work on
-// the last pair (a block's four lanes trade values) and store nothing.
+// HD / 8 lanes a (token, head) pair, its K and its V: two loads a lane on their way.  Lanes
+// past the end work on the last pair (a block's four lanes trade values) and store nothing.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_write_kernel(const uint16_t* __restrict__ key,
                                                        const uint16_t* __restrict__ value,
@@ -21,16 +21,16 @@ __global__ __launch_bounds__(256) void q4_write_kernel(const uint16_t* __restric
   constexpr int LANES = HD / 8, PER = 256 / LANES;
   const int j = threadIdx.x % LANES;
   const int64_t raw = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-  const int64_t at = min(raw, 2 * pairs - 1);
-  const int plane = at >= pairs;
-  const int64_t pair = plane ? at - pairs : at;
+  const int64_t pair = min(raw, pairs - 1);
   const int64_t t = (uint32_t)pair / (uint32_t)c.n_kv;
   const int head = (int)(pair - t * c.n_kv);
-  const uint16_t* const src = plane ? value + t * value_stride : key + t * key_stride;
-  const u32x4 x = *reinterpret_cast<const u32x4*>(src + head * HD + 8 * j);
   const int64_t slot = slots[t];
-  const bool store = raw < 2 * pairs && slot >= 0 && slot < cache_slots;
-  q4_store_chunk<HD>(c, plane, store ? slot : 0, head, j, x, store);
+  const u32x4 k = *reinterpret_cast<const u32x4*>(key + t * key_stride + head * HD + 8 * j);
+  const u32x4 v = *reinterpret_cast<const u32x4*>(value + t * value_stride + head * HD + 8 * j);
+  const bool store = raw < pairs && slot >= 0 && slot < cache_slots;
+#pragma unroll 1
+  for (int plane = 0; plane < 2; ++plane)  // (one time the code: it is not in the cache)
+    q4_store_chunk<HD>(c, plane, store ? slot : 0, head, j, plane ? v : k, store);
   stores_done();
 }
 
@@ -137,7 +137,7 @@ extern "C" int smx_q4_reshape_and_cache(void* stream, const void* key, int64_t k
               "a token's stride must hold its heads");
   const smx::Q4Cache c = q4_cache(codes, scales, num_blocks, block_size, n_kv);
   const int64_t pairs = (int64_t)num_tokens * n_kv, per = 256 * 8 / head_dim;
-  const dim3 grid((unsigned)((2 * pairs + per - 1) / per));
+  const dim3 grid((unsigned)((pairs + per - 1) / per));
   SMX_LAUNCH((head_dim == 128 ? smx::q4_write_kernel<128> : smx::q4_write_kernel<64>), grid,
              dim3(256), 0, (hipStream_t)stream, (const uint16_t*)key, (const uint16_t*)value,
              slot_mapping, c, pairs, key_stride, value_stride, (int64_t)num_blocks * block_size);
