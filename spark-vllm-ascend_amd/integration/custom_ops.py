@@ -20,6 +20,10 @@ under the namespace ``smx``:
   smx::shared_prefix_attention(q, k_cache, v_cache, prefix_table, prefix_len,
                                block_table, seq_lens, scale) -> out
                                                        bf16 [seqs, n_q, hd]
+  smx::q4_attention(q, codes, scales, block_table, seq_lens, scale,
+                    query_start_loc=None) -> out       bf16 [tokens, n_q, hd]
+  smx::beam_select(logits, scores, beams, width, done=None, pad_id=0)
+      -> (parents int32, tokens int64, scores fp32)    [seqs, width]
   smx::argmax(logits) -> ids                           int64 [rows]
   smx::layer_run(x, residual, positions, layer_name) -> (y, residual_out)
       one decoder layer's decode step over the layers layer_run.install()
@@ -112,6 +116,32 @@ def register() -> None:
     @shared_prefix_attention.register_fake
     def _(q, k_cache, v_cache, prefix_table, prefix_len, block_table, seq_lens, scale):
         return q.new_empty(q.shape)
+
+    @torch.library.custom_op(f"{_NS}::q4_attention", mutates_args=())
+    def q4_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                     query_start_loc: torch.Tensor | None = None) -> torch.Tensor:
+        q = q.contiguous()
+        return torch_ops.q4_attention(q, torch_ops.Q4KVCache(codes, scales), block_table, seq_lens,
+                                      scale, query_start_loc=query_start_loc,
+                                      out=torch.zeros_like(q))
+
+    @q4_attention.register_fake
+    def _(q, codes, scales, block_table, seq_lens, scale, query_start_loc=None):
+        return q.new_empty(q.shape)
+
+    @torch.library.custom_op(f"{_NS}::beam_select", mutates_args=())
+    def beam_select(logits: torch.Tensor, scores: torch.Tensor, beams: int, width: int,
+                    done: torch.Tensor | None = None,
+                    pad_id: int = 0) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        best = torch_ops.beam_select(logits, scores, beams, width, done=done, pad_id=pad_id)
+        return best.parents, best.tokens, best.scores
+
+    @beam_select.register_fake
+    def _(logits, scores, beams, width, done=None, pad_id=0):
+        shape = (logits.shape[0] // beams, width)
+        return (logits.new_empty(shape, dtype=torch.int32), logits.new_empty(shape, dtype=torch.int64),
+                logits.new_empty(shape, dtype=torch.float32))
 
     @torch.library.custom_op(f"{_NS}::argmax", mutates_args=())
     def argmax(logits: torch.Tensor) -> torch.Tensor:

@@ -37,6 +37,8 @@ typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) uint16_t lds_u16;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(4))) int32_t constant_i32;
 
 // A dword of two bf16 values with those that are infinite or NaN replaced by 0.
@@ -92,12 +94,13 @@ struct Item {
 // HD: head_dim.  WM waves take 32 rows each, WN groups of them take every WN-th
 // tile of KT tokens; ST tiles of K and V a group are in LDS, one that is read and
 // ST - 1 that are on their way.
-template <int HD, int WM, int WN, int KT, int ST>
+template <int HD, int WM, int WN, int KT, int ST, bool Q4 = false>
 struct Shape {
   static constexpr int M = 32 * WM, NT = 64 * WM * WN;
   static constexpr int CH = HD / 8;                  // 16-byte chunks of a row
   static constexpr int TILE = KT * CH;               // chunks of a K or V tile
-  static constexpr int GROUP = ST * 2 * TILE;        // the buffers of K and V
+  static constexpr int BUFFER = 2 * TILE + (Q4 ? KT / 4 : 0);  // K, V (Q4: and its flags)
+  static constexpr int GROUP = ST * BUFFER;
   static constexpr int JOIN = WN > 1 ? (WN - 1) * WM * (32 * HD + 64) / 4 : 0;
   static constexpr int LDS = WN * GROUP > JOIN ? WN * GROUP : JOIN;
   static constexpr int LOADS = TILE / 64 / WM;       // a wave's loads of a K (V) tile
@@ -136,7 +139,7 @@ __device__ __forceinline__ void meet() {
 // a prompt's time.)
 template <int HD, int WM, int WN, int KT, int ST, int BS, bool Q4 = false>
 __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
-  using S = Shape<HD, WM, WN, KT, ST>;
+  using S = Shape<HD, WM, WN, KT, ST, Q4>;
   constexpr int KS = HD / 16, DT = HD / 32, NU = KT / 32, CH = S::CH;
   constexpr int BT = KT < BS ? KT : BS, NP = KT / BT;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
@@ -286,8 +289,12 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     }
   };
   auto fill_v = [&](lds_u32x4* dst) {
+    // A token's block without a value (its scale is not finite) is 0 here, so that it does
+    // not reach the rows that do not see the token, and a flag for those that do.
+    const bool none = (vd & 0x7fffu) >= 0x7c00u;
+    const float d = none ? 0.f : f16_bits_to_f32(vd);
+    ((lds_u8*)(dst + 2 * S::TILE))[4 * qtok + qg] = none;
     // V's swizzle goes by two bits of the token: the others turn the order of the dwords
-    const float d = f16_bits_to_f32(vd);
     const int turn = (qtok >> 2) & (NB - 1);
     Dwords w = vq;
     if constexpr (NB == 4) {
@@ -425,7 +432,9 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   auto weigh = [&](auto plain, const lds_u32x4* vtile, int base) {
     const lds_u16* const vt = (const lds_u16*)vtile;
     bool odd = false;
-    if constexpr (!plain) odd = odd_values(vt);
+    if constexpr (!plain && !Q4) odd = odd_values(vt);
+    uint32_t flags = 0;  // Q4: of token lane % KT
+    if constexpr (Q4) flags = ((const lds_u32*)(vtile + S::TILE))[lane % KT];
     if (!odd) {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
@@ -434,6 +443,19 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8, v_operand(vt, kk, d)),
               __builtin_bit_cast(bf16x8, p_operand(kk)), o[d], 0, 0, 0);
+      if (Q4 && __builtin_amdgcn_ballot_w64(flags != 0)) {
+#pragma unroll 1
+        for (int r = 0; r < KT; ++r) {
+          const uint32_t w = __builtin_amdgcn_readlane(flags, r);
+          const bool seen = base + r >= it.from && base + r < lim;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const float x = seen && (w >> (8 * 4 / DT * d) & 1u) ? __builtin_nanf("") : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] += x;
+          }
+        }
+      }
     } else {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
@@ -485,7 +507,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   for (int i = 0; i < (Q4 ? 0 : ST - 1); ++i) {
     const int tile = i * WN + wn, base = first + tile * KT;
     if (tile < ntiles) {
-      lds_u32x4* const dst = lds + i * 2 * S::TILE;
+      lds_u32x4* const dst = lds + i * S::BUFFER;
       stage_k(dst, page, base);
       stage_v(dst + S::TILE, page, base);
       bad[i] = bad_pages(page);
@@ -541,7 +563,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       __builtin_amdgcn_s_waitcnt(wait_vm(0));
     meet();
     const int before = at == 0 ? ST - 1 : at - 1;
-    round(plain, lds + before * 2 * S::TILE, lds + at * 2 * S::TILE, rd * WN + wn);
+    round(plain, lds + before * S::BUFFER, lds + at * S::BUFFER, rd * WN + wn);
     at = at == ST - 1 ? 0 : at + 1;
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) bad[i] = bad[i + 1];
@@ -642,7 +664,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 template <int HD, int WM, int WN, int KT, int ST, int BS, bool Q4>
 __global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(2)))
 void prompt_attention_kernel(RowsArgs A) {
-  using S = Shape<HD, WM, WN, KT, ST>;
+  using S = Shape<HD, WM, WN, KT, ST, Q4>;
   __shared__ __attribute__((aligned(16))) u32x4 smem[S::LDS];
   constexpr int ROUND = WN * KT;
   const int kvh = blockIdx.x;
