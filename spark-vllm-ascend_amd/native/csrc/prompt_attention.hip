@@ -348,7 +348,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   auto is_plain = [&](int base, int bad) {
     return base >= it.from && base + KT <= lim_min && !bad;
   };
-  auto softmax = [&](auto plain, int base, int bad) {
+  auto softmax = [&](auto plain, int base, int bad, uint32_t flags) {
     // the scores of tokens without a page are NaN, and so is every row that sees one
     if constexpr (!plain) {
 #pragma unroll
@@ -369,7 +369,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     // The reference follows the maximum only once that has grown by LAG: p is then
     // at most 2^LAG, which neither fp32 nor bf16 minds, and most tiles leave o and
     // l as they are.
-    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG)) {
+    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG || (Q4 && flags != 0))) {
       const float next = fmaxf(ref, mx);
       const float alpha = __builtin_amdgcn_exp2f(ref - next);
       ref = next;
@@ -378,6 +378,20 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+      if (Q4 && __builtin_amdgcn_ballot_w64(flags != 0)) {
+        // blocks without a value: NaN for the rows that see their tokens
+#pragma unroll 1
+        for (int r = 0; r < KT; ++r) {
+          const uint32_t w = __builtin_amdgcn_readlane(flags, r);
+          const bool seen = base + r >= it.from && base + r < lim;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const float x = seen && (w >> (8 * 4 / DT * d) & 1u) ? __builtin_nanf("") : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] += x;
+          }
+        }
+      }
     }
     float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -433,8 +447,6 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     const lds_u16* const vt = (const lds_u16*)vtile;
     bool odd = false;
     if constexpr (!plain && !Q4) odd = odd_values(vt);
-    uint32_t flags = 0;  // Q4: of token lane % KT
-    if constexpr (Q4) flags = ((const lds_u32*)(vtile + S::TILE))[lane % KT];
     if (!odd) {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
@@ -443,19 +455,6 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
           o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8, v_operand(vt, kk, d)),
               __builtin_bit_cast(bf16x8, p_operand(kk)), o[d], 0, 0, 0);
-      if (Q4 && __builtin_amdgcn_ballot_w64(flags != 0)) {
-#pragma unroll 1
-        for (int r = 0; r < KT; ++r) {
-          const uint32_t w = __builtin_amdgcn_readlane(flags, r);
-          const bool seen = base + r >= it.from && base + r < lim;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const float x = seen && (w >> (8 * 4 / DT * d) & 1u) ? __builtin_nanf("") : 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[d][i] += x;
-          }
-        }
-      }
     } else {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
@@ -537,8 +536,10 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       }
     }
     if (!(!plain && tile >= ntiles) && 32 * wm < it.rows) {
+      uint32_t flags = 0;  // Q4: of token lane % KT
+      if constexpr (Q4) flags = ((const lds_u32*)(cur + 2 * S::TILE))[lane % KT];
       scores(cur);
-      softmax(plain, base, bad[0]);
+      softmax(plain, base, bad[0], flags);
       weigh(plain, cur + S::TILE, base);
     }
     if constexpr (Q4 && WM > SHARE) {
