@@ -192,13 +192,17 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
 
   // ---- the row's state: the exponents' reference (log2 units: the running maximum, or up
   // to LAG below it), the sum of 2^(score - ref) over this lane's tokens, the output's
-  // products with 16 + code and (register b: block b) the sums of their weights.
+  // products with 16 + code and, block by block, the sums of their weights (in every register
+  // the same; of its own for each block, so that one that is NaN stays among its dims).
   float ref = NO_REF, l = 0.f;
-  f32x4 o[DT], w_sum = {0.f, 0.f, 0.f, 0.f};
+  f32x4 o[DT], w_sum[NB];
 #pragma unroll
   for (int d = 0; d < DT; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-  // ones in the rows 4 x + b of the weights' product, so that its register b is block b's
-  bf16x8 qf[NB], ones[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) w_sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bf16x8 qf[NB];
+  const uint32_t one2 = 0x3f803f80u;
+  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one2, one2, one2, one2});
   f32x4 c0[NB];
   const CodeBits codes_bf16;
   const int k_addr = HD == 128 ? n * RB + 16 * (g ^ k_swz(n))
@@ -262,7 +266,8 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
       const float alpha = __builtin_amdgcn_exp2f(ref - next);
       ref = next;
       l *= alpha;
-      w_sum *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) w_sum[b] *= alpha;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= alpha;
     }
@@ -294,7 +299,7 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
                            fmaf(p[1][i], half_of(dv[1][e / 2], e & 1), codes_bf16.zero));
       }
       const bf16x8 w = __builtin_bit_cast(bf16x8, x);
-      w_sum = mfma(ones[b], w, w_sum);
+      w_sum[b] = mfma(ones, w, w_sum[b]);
       const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
           (lds_i32x2*)(buf + v_addr + 16 * (b ^ v_place)));
       o[2 * b] = mfma(codes_bf16((uint32_t)v[0]), w, o[2 * b]);
@@ -314,8 +319,6 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
     for (int i = 0; i < 4; ++i) sum = dot2_bf16(qx[b][i], 0x3f803f80u, sum);
     sum = -24.f * xor_sum<32>(xor_sum<16>(sum));
     c0[b] = f32x4{sum, sum, sum, sum};
-    const uint32_t x = (lane & 3) == b ? 0x3f803f80u : 0u;
-    ones[b] = __builtin_bit_cast(bf16x8, u32x4{x, x, x, x});
   }
   auto round = [&](lds_u8* __restrict__ next, const lds_u8* __restrict__ cur) {
     __builtin_amdgcn_s_waitcnt(0x0f70);  // this tile's loads have arrived
@@ -343,7 +346,7 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
   float* const mine = jo + wave * STATE;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
-    *reinterpret_cast<f32x4*>(mine + (d * 64 + lane) * 4) = o[d] + -24.f * w_sum[d / 2];
+    *reinterpret_cast<f32x4*>(mine + (d * 64 + lane) * 4) = o[d] + -24.f * w_sum[d / 2][0];
   if (g == 0) {
     mine[16 * HD + n] = ref;
     mine[16 * HD + 16 + n] = l;

@@ -326,3 +326,26 @@ def test_refusals():
     for change in (dict(scale=0.0), dict(scale=math.nan), dict(q=q[:, :7].contiguous())):
         with pytest.raises(pkg("native").SmxError):
             f(**change)
+
+
+@pytest.mark.parametrize("n,ctx,n_q,n_kv,hd,bs", [
+    (50, 0, 4, 1, 128, 32), (450, 0, 32, 8, 128, 32), (1500, 0, 16, 4, 64, 64),
+    (300, 3000, 32, 8, 128, 64), (2100, 0, 32, 8, 128, 128), (2100, 0, 32, 8, 64, 32)])
+def test_blocks_of_v_without_a_value(n, ctx, n_q, n_kv, hd, bs):
+    """A NaN scale of V is one block's of 32 dims: the rows that see its token are NaN there,
+    and everything else is what it was."""
+    c = Case(8, [n], [ctx], n_q, n_kv, hd, bs)
+    assert c.prompts() == (n > 50)
+    clean = c.run().cpu()
+    for t, block in ((n + ctx - 2, 0), (ctx + n // 2, hd // 32 - 1), (ctx + 5, 1)):
+        where = (1, int(c.table[0, t // bs]), n_kv - 1, t % bs, block)
+        save = c.scales[where].clone()
+        c.scales[where] = math.nan
+        got = c.run().cpu()
+        c.scales[where] = save
+        heads, dims = slice(n_q - n_q // n_kv, n_q), slice(32 * block, 32 * block + 32)
+        assert got[t - ctx:, heads, dims].isnan().all()
+        got[t - ctx:, heads, dims] = clean[t - ctx:, heads, dims]
+        assert torch.isfinite(got).all()
+        # (the weights of a tile are rescaled or not by rows that are NaN now: one rounding)
+        torch.testing.assert_close(got, clean, rtol=2.0 ** -7, atol=2.0 ** -9)
