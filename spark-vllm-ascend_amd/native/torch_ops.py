@@ -980,12 +980,13 @@ def q4_kv_read(cache: Q4KVCache, slot_mapping: torch.Tensor,
     _check(slot_mapping, "slot_mapping", torch.int64)
     c = _q4_cache(cache, slot_mapping.get_device())
     shape = (slot_mapping.numel(), c.n_kv, c.head_dim)
-    if out is None:
-        out = tuple(torch.empty(shape, dtype=torch.float32, device=slot_mapping.device)
-                    for _ in range(2))
     n = shape[0] * shape[1] * shape[2]
-    for t, name in zip(out, ("out[0]", "out[1]")):
-        _check(t, name, torch.float32, n, slot_mapping.device)
+    if out is None:
+        first = torch.empty(shape, dtype=torch.float32, device=slot_mapping.device)
+        out = first, first.new_empty(shape)
+    else:
+        for t, name in zip(out, ("out[0]", "out[1]")):
+            _check(t, name, torch.float32, n, slot_mapping.device)
     if n:
         call("smx_q4_kv_read", _stream(slot_mapping), c.codes.data_ptr(), c.scales.data_ptr(),
              slot_mapping.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), *shape, c.num_blocks,
@@ -1085,6 +1086,15 @@ def q4_attention(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
     return out
 
 
+def _made(cls, *tensors):
+    """A `cls` of tensors that this module has allocated, without the checks of its
+    constructor (a microsecond or two of calls of four)."""
+    x = object.__new__(cls)
+    for name, t in zip(cls.__slots__, tensors):
+        setattr(x, name, t)
+    return x
+
+
 class BeamSelection:
     """What beam_select() writes, [seqs, width], the best first:
       parents  int32: the row of logits it continues, -1 where there is none
@@ -1105,9 +1115,9 @@ class BeamSelection:
 
 def beam_select_out(seqs: int, width: int, device) -> BeamSelection:
     """Buffers for beam_select(out=...)."""
-    return BeamSelection(torch.empty((seqs, width), dtype=torch.int32, device=device),
-                         torch.empty((seqs, width), dtype=torch.int64, device=device),
-                         torch.empty((seqs, width), dtype=torch.float32, device=device))
+    return _made(BeamSelection, torch.empty((seqs, width), dtype=torch.int32, device=device),
+                 torch.empty((seqs, width), dtype=torch.int64, device=device),
+                 torch.empty((seqs, width), dtype=torch.float32, device=device))
 
 
 def beam_select_workspace(logits: torch.Tensor, beams: int, width: int) -> torch.Tensor | None:
@@ -1193,11 +1203,16 @@ class ForkedPages:
 
 def fork_pages_out(block_table: torch.Tensor, free_pages: torch.Tensor) -> ForkedPages:
     """Buffers for fork_pages(out=...) of a table and free list of these sizes."""
-    rows, dev = block_table.shape[0], block_table.device
-    i32 = dict(dtype=torch.int32, device=dev)
-    return ForkedPages(torch.empty_like(block_table), torch.empty(rows, **i32),
-                       torch.empty(rows, **i32), torch.empty_like(free_pages),
-                       torch.empty(1, **i32), torch.empty((rows, 2), **i32))
+    _check(block_table, "block_table", torch.int32)
+    _check(free_pages, "free_pages", torch.int32, device=block_table.device)
+    _need(block_table.dim() == 2, "block_table must be [rows, max_blocks]")
+    return _forked_pages(block_table, free_pages)
+
+
+def _forked_pages(block_table, free_pages):
+    new, rows = block_table.new_empty, block_table.shape[0]
+    return _made(ForkedPages, new(block_table.shape), new(rows), new(rows),
+                 new(free_pages.shape), new(1), new((rows, 2)))
 
 
 def fork_pages(parents: torch.Tensor, lens: torch.Tensor, num_pages: torch.Tensor,
@@ -1216,7 +1231,7 @@ def fork_pages(parents: torch.Tensor, lens: torch.Tensor, num_pages: torch.Tenso
     if parents.numel() != reqs:
         raise ValueError("parents must have an entry for each row of block_table")
     if out is None:
-        out = fork_pages_out(block_table, free_pages)
+        out = _forked_pages(block_table, free_pages)
     elif not (isinstance(out, ForkedPages) and out.block_table.shape == block_table.shape
               and out.free_pages.numel() == free_pages.numel()
               and out.block_table.get_device() == i):
@@ -1264,9 +1279,9 @@ def compact_pages(num_pages: torch.Tensor, block_table: torch.Tensor, num_blocks
         raise ValueError("block_table must be [rows, max_blocks]")
     _need(num_blocks >= 2, "num_blocks must be >= 2")
     if out is None:
-        i32 = dict(dtype=torch.int32, device=num_pages.device)
-        out = CompactedPages(torch.empty_like(block_table), torch.empty(num_blocks, **i32),
-                             torch.empty(1, **i32), torch.empty((num_blocks // 2, 2), **i32))
+        new = num_pages.new_empty
+        out = _made(CompactedPages, new(block_table.shape), new(num_blocks), new(1),
+                    new((num_blocks // 2, 2)))
     elif not (isinstance(out, CompactedPages) and out.block_table.shape == block_table.shape
               and out.free_pages.numel() == num_blocks and out.block_table.get_device() == i):
         raise ValueError("out must be CompactedPages of this table and num_blocks")
