@@ -677,7 +677,8 @@ int smx_decode_advance(void* stream, int64_t* next_ids,
  * (kernels/qkv.py:192-198,226-236) and so are smx_reshape_and_cache's.
  *
  * smx_q4_reshape_and_cache: smx_reshape_and_cache into it; a token's heads are contiguous,
- * tokens key_stride (value_stride) elements apart, a multiple of 8.
+ * tokens key_stride (value_stride) elements apart, a multiple of 8.  A slot is given once
+ * in a call: of two tokens' codes and scales in one slot some of each may stay.
  * smx_q4_qknorm_rope_kv_write: smx_qknorm_rope_kv_write into it (head_dim 128).
  * smx_q4_kv_read: the values of the tokens at slot_mapping as fp32 [num_tokens, n_kv,
  * head_dim], exactly; 0 for slots outside the cache.
@@ -700,9 +701,11 @@ int smx_q4_kv_read(void* stream, const void* codes, const void* scales,
  * smx_prompt_attention over a cache held in 4 bits: the same rows, masks and table rules
  * (rows that see a token whose table entry is outside the cache are NaN, rows that see
  * none 0, rows of no sequence stay as they are).  query_start_loc may be NULL where
- * num_tokens is num_seqs: row r is sequence r's newest token, a decode step.  The cache's
- * values are not rounded; scores, sums and outputs are fp32, the weights of the second
- * product (softmax weight times V's scale) bf16.
+ * num_tokens is num_seqs: row r is sequence r's newest token, a decode step.  Scores,
+ * sums and outputs are fp32.  Of few rows the cache's values are not rounded, and the
+ * weights of the second product (softmax weight times V's scale) are bf16; of prompts
+ * (more than 32 pairs of a token and a head of a group a sequence, and enough of them
+ * times the tables' capacity) the values are rounded to bf16, as are the weights.
  */
 int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_seqs, int32_t max_blocks,
                                    int32_t block_size, int32_t n_q, int32_t n_kv,

@@ -6,6 +6,12 @@
 // num_pages first, and free again once no row does.  No counts are kept, so that there
 // are none to go wrong.  A workgroup collects the pages in bit sets in LDS (32768 pages
 // a 4 KB set); nothing of a call is left for the next.
+//
+// One workgroup has all of what the tables say (the others copy): bound by its chains of
+// loads and LDS operations.  us: 512 rows of up to 34 pages 12.9, 4 rows 5.3 (a wave a row 57);
+// the moves of 256 rows of up to 17 pages in a pool of 2198 14.5, of 16 rows 5.6 (with a
+// search for every moved entry 57).  Copies go at memory's rate: 433 MB read and written in 74
+// us (5.9 TB/s, some of it from the caches), 1 GB in 195.
 #include <limits.h>
 
 #include <algorithm>

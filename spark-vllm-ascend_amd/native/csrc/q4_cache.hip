@@ -1,6 +1,8 @@
 // Writes to and reads from the paged KV cache held in 4 bits (q4_cache.h), for gfx950:
 // a step's keys and values, the same behind q/k RMSNorm and RoPE, and tokens' values.
-// Bound by memory: 2 bytes a value in, 4.5 bits out (read: 4.5 bits in, 4 bytes out).
+// Bound by memory: 2 bytes a value in, 4.5 bits out (read: 4.5 bits in, 4 bytes out).  8000
+// tokens of 8 heads of 128: written in 10.8 us (3.9 TB/s; 12.0 with one load a lane), read in
+// 18.1 (4.1 TB/s, most of it stores); 16 tokens 2.8 and 2.7.
 #include <math.h>
 
 #include "q4_cache.h"

@@ -946,7 +946,8 @@ def _q4_cache(cache, index: int) -> Q4KVCache:
 def reshape_and_cache_q4(key: torch.Tensor, value: torch.Tensor, cache: Q4KVCache,
                          slot_mapping: torch.Tensor) -> None:
     """reshape_and_cache into a cache in 4 bits.  key, value [tokens, n_kv, hd]: a token's
-    heads are contiguous, tokens may be strided (a slice of the QKV rows)."""
+    heads are contiguous, tokens may be strided (a slice of the QKV rows).  A slot is given
+    once in a call."""
     _need(isinstance(slot_mapping, torch.Tensor), "slot_mapping must be a tensor")
     i = slot_mapping.get_device()
     c = _q4_cache(cache, i)
@@ -1037,8 +1038,8 @@ def q4_attention(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
     """prompt_attention over a cache in 4 bits: sequence r's queries are the rows
     query_start_loc[r]..query_start_loc[r + 1] of q [tokens, n_q, hd] (tokens may be
     strided), the last of its seq_lens[r] tokens.  Without query_start_loc row r is
-    sequence r's newest token: a decode step.  Rows of no sequence are left as they are
-    in `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
+    sequence r's newest token: a decode step.  Of few rows the cache's values are not
+    rounded; prompts round them to bf16.  Rows of no sequence are left as they are in `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
     needs it."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is BF16 and q.dim() == 3):
         raise ValueError("q must be a bf16 GPU tensor [tokens, n_q, hd]")
