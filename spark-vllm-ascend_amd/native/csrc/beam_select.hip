@@ -11,9 +11,9 @@
 // be taken in the wrong order, where fp32 sums would confuse those within 1e-6.
 //
 // Bound by vector instructions where there are many rows: 512 rows of 151936 bf16 values,
-// a tenth of them done, 16 best of 8 beams: 56 us, the parts 45 (3.1 TB/s; about 17
+// a tenth of them done, 16 best of 8 beams: 52 us, the parts 41 (3.4 TB/s; about 14
 // instructions a value, an exponential and a 64-bit sum among them), the merge 9.  4 rows
-// 10.9 us: two launches of short latencies one after another.
+// 10.7 us: two launches of short latencies one after another.
 //
 // A NaN logit counts as -inf, a token that is never chosen; of several logits of +inf each
 // has an equal share.
@@ -32,7 +32,8 @@ typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
-constexpr int CAP = 128;  // candidates of a wave
+constexpr int CAP = 128;     // candidates of a wave
+constexpr int CHUNKS = 128;  // loads of a wave that hold candidates
 constexpr int NT = 256, WAVES = NT / 64;
 // Of 16 bytes, a lane: a part is 32 KB of a row.  us with 2 / 4 / 8 of them, rows of 151936
 // bf16 values: 1 row 9.2 / 9.3 / 10.0, 16 rows 11.2 / 10.9 / 10.8, 128 rows 25 / 21 / 20,
@@ -150,7 +151,8 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   constexpr int V = 16 / sizeof(L);  // logits of a load
   constexpr int PART = NT * LOADS * V;
   __shared__ uint64_t list[WAVES][CAP + 4];
-  __shared__ u32x4 tail_s;
+  __shared__ u32x4 tail_s, chunk_s[WAVES][CHUNKS];
+  __shared__ int where_s[WAVES][CHUNKS];
   __shared__ int count_s[WAVES], best_s[WAVES][64];
   __shared__ double sum_s[WAVES];
   const int part = blockIdx.x, row = blockIdx.y;
@@ -271,6 +273,37 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     else
       return __uint_as_float(x[i][j]);
   };
+  // The few lanes' loads that hold a value which reaches it go to LDS, and their values are
+  // looked at there, a lane each.
+  auto below = [](uint64_t m) {  // its bits below this lane's
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  };
+  int chunks = 0;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const bool hit = key(most[i]) >= bound_key;
+    if (const uint64_t m = __builtin_amdgcn_ballot_w64(hit)) {
+      const int at = chunks + below(m);
+      if (hit && at < CHUNKS) {
+        chunk_s[wave][at] = x[i];
+        where_s[wave][at] = i * NT + tid;
+      }
+      chunks += __popcll(m);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  typedef typename std::conditional<V == 8, uint16_t, uint32_t>::type __attribute__((may_alias)) Raw;
+  const Raw* const chunk = reinterpret_cast<const Raw*>(chunk_s[wave]);
+  for (int e = lane; e - lane < min(chunks, CHUNKS) * V; e += 64) {
+    const uint32_t w = e < chunks * V ? (uint32_t)chunk[e] << (V == 8 ? 16 : 0) : 0xff800000u;
+    const bool in = __uint_as_float(w) >= bound;
+    const uint64_t m = __builtin_amdgcn_ballot_w64(in);
+    const int at = n + below(m);
+    if (in && at < CAP)
+      mine[at] = (uint64_t)((uint32_t)order_key(w) ^ 0x80000000u) << 32 |
+                 (0xffffffffu - (uint32_t)(where_s[wave][e / V] * V + e % V));
+    n += __popcll(m);
+  }
   // Puts the values of load i that `in(j)` says into the list, in no particular order: a
   // bit a value, the set ones lane by lane.
   auto collect = [&](int i, auto in) {
@@ -278,8 +311,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
 #pragma unroll
     for (int j = 0; j < V; ++j) bits = bits + bits + (in(j) ? 1u : 0u);
     while (const uint64_t m = __builtin_amdgcn_ballot_w64(bits != 0)) {
-      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32),
-                                                   __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+      const int at = n + below(m);
       if (bits && at < CAP) {
         const int low = __ffs(bits) - 1, j = V - 1 - low;
         uint32_t w;
@@ -298,11 +330,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
       n += __popcll(m);
     }
   };
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i)
-    if (__builtin_amdgcn_ballot_w64(key(most[i]) >= bound_key))
-      collect(i, [&](int j) { return value(i, j) >= bound; });
-  if (n > CAP) {
+  if (n > CAP || chunks > CHUNKS) {
     // (sorted or equal logits: the bound is loose)  The width-th largest value, bit by bit
     // from above; then those above it, and as many of its equals as are missing, the
     // lowest places first: load by load, lane by lane.
@@ -318,7 +346,7 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
       }
       return c;
     };
-    // (more than CAP reach `bound`, so the value is not below it)
+    // (more than `width` reach `bound`, so the value is not below it)
     int64_t least = order_key(__float_as_uint(bound));
 #pragma unroll 1
     for (int64_t bit = 1ll << 31; bit >= STEP; bit >>= 1)
