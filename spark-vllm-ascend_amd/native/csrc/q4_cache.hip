@@ -2,7 +2,7 @@
 // a step's keys and values, the same behind q/k RMSNorm and RoPE, and tokens' values.
 // Bound by memory: 2 bytes a value in, 4.5 bits out (read: 4.5 bits in, 4 bytes out).  8000
 // tokens of 8 heads of 128: written in 10.8 us (3.9 TB/s; 12.0 with one load a lane), read in
-// 18.1 (4.1 TB/s, most of it stores); 16 tokens 2.8 and 2.7.
+// 14.5 (5.2 TB/s; 18.1 with K or V of a lane); 16 tokens 2.8 and 3.2 (2.7).
 #include <math.h>
 
 #include "q4_cache.h"
@@ -62,8 +62,7 @@ __global__ __launch_bounds__(256) void q4_qknorm_rope_write_kernel(
   stores_done();
 }
 
-// A lane 4 channels (one 16-byte store), K's values and then V's; 0 for a slot outside
-// the cache.
+// A lane 4 channels of K and of V (a 16-byte store each); 0 for a slot outside the cache.
 template <int HD>
 __global__ __launch_bounds__(256) void q4_read_kernel(Q4Cache c, const int64_t* __restrict__ slots,
                                                       float* __restrict__ key,
@@ -71,28 +70,34 @@ __global__ __launch_bounds__(256) void q4_read_kernel(Q4Cache c, const int64_t* 
                                                       int64_t cache_slots) {
   constexpr int LANES = HD / 4, PER = 256 / LANES;
   const int j = threadIdx.x % LANES;
-  const int64_t at = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
-  if (at < 2 * pairs) {
-    const int plane = at >= pairs;
-    const int64_t pair = plane ? at - pairs : at;
+  const int64_t pair = (int64_t)blockIdx.x * PER + threadIdx.x / LANES;
+  if (pair < pairs) {
     const int64_t t = (uint32_t)pair / (uint32_t)c.n_kv;
     const int head = (int)(pair - t * c.n_kv);
     const int64_t slot = slots[t];
-    u32x4 out = {0u, 0u, 0u, 0u};
-    if (slot >= 0 && slot < cache_slots) {
-      const int64_t row = q4_row(c, plane, slot, head);
-      const int b = j / 8, g = (j & 7) / 2, half = j & 1;  // channels 4 j .. of block b
-      const int dword = plane == 0 ? g * (HD / 32) + b : j / 2;
-      const uint32_t w = reinterpret_cast<const uint32_t*>(c.codes + row * (HD / 2))[dword];
-      const float d = f16_bits_to_f32(c.scales[row * (HD / 32) + b]);
+    const bool in = slot >= 0 && slot < cache_slots;
+    const int b = j / 8, g = (j & 7) / 2, half = j & 1;  // channels 4 j .. of block b
+    uint32_t w[2] = {0u, 0u};
+    float d[2] = {0.f, 0.f};
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane)
+      if (in) {
+        const int64_t row = q4_row(c, plane, slot, head);
+        const int dword = plane == 0 ? g * (HD / 32) + b : j / 2;
+        w[plane] = reinterpret_cast<const uint32_t*>(c.codes + row * (HD / 2))[dword];
+        d[plane] = f16_bits_to_f32(c.scales[row * (HD / 32) + b]);
+      }
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+      u32x4 out = {0u, 0u, 0u, 0u};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int ch = 4 * half + i;
         const int bit = plane == 0 ? 4 * (ch / 2) + 16 * (ch & 1) : 4 * ch;
-        out[i] = __float_as_uint(d * (float)((int)((w >> bit) & 15u) - 8));
+        if (in) out[i] = __float_as_uint(d[plane] * (float)((int)((w[plane] >> bit) & 15u) - 8));
       }
+      st_agent_b128((plane ? value : key) + pair * HD + 4 * j, out);
     }
-    st_agent_b128((plane ? value : key) + pair * HD + 4 * j, out);
   }
   stores_done();
 }
@@ -186,7 +191,7 @@ extern "C" int smx_q4_kv_read(void* stream, const void* codes, const void* scale
               "key and value must be 16-byte aligned");
   const smx::Q4Cache c = q4_cache(codes, scales, num_blocks, block_size, n_kv);
   const int64_t pairs = (int64_t)num_tokens * n_kv, per = 256 * 4 / head_dim;
-  const dim3 grid((unsigned)((2 * pairs + per - 1) / per));
+  const dim3 grid((unsigned)((pairs + per - 1) / per));
   SMX_LAUNCH((head_dim == 128 ? smx::q4_read_kernel<128> : smx::q4_read_kernel<64>), grid,
              dim3(256), 0, (hipStream_t)stream, c, slot_mapping, (float*)key, (float*)value, pairs,
              (int64_t)num_blocks * block_size);
