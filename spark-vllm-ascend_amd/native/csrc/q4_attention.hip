@@ -413,7 +413,7 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
 // and first tile, and the join), as much as BEGIN rounds.  So every tile begins a new part
 // where parts no longer than that allow it.  Grid: kv heads, parts.
 template <int HD>
-__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(HD == 64 ? 4 : 2)))
 void q4_attention_kernel(Q4Args A) {
   constexpr int M = 16;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES * 2 * Tile<HD>::BYTES];
@@ -523,7 +523,13 @@ void q4_attention_kernel(Q4Args A) {
 
 // How a call is cut, from its sizes (lengths are on the device).  512 workgroups fill the
 // chip once (two a compute unit, by their registers).  Twice as many parts, 48 sequences
-// behind 2000 to 32000 152 us for 155, but 16 behind 300 to 8000 22 for 19.
+// behind 2000 to 32000 152 us for 155, but 16 behind 300 to 8000 22 for 19.  Heads of 64
+// leave registers for four, which few rows a sequence are cut for from 16 rounds (of the
+// tables' capacity) a part of 512 on: us with 512 / 768 / 1024 parts, 32 / 8 heads, 48
+// sequences behind 2000 to 32000 92 / 90 / 85, 128 behind 500 to 4000 50 / 44 / 41, 32 behind 500
+// to 8000 24.3 / 21.2 / 20.6, 8 behind 32000 42 / 40 / 40, 64 behind 300 to 2000 (21 rounds) 20 /
+// 19 / 17, 24 behind 1000 to 20000, 16 / 4 18.8 / 18.0 / 19.1, but 2 behind 32000 (12) 15.7 and
+// 16.9 with 1024.
 constexpr int FILL = 512, MAX_PARTS = 64;
 
 int tune(const char* name, int v) {
@@ -555,10 +561,13 @@ bool is_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int
   return work > tune("SMX_Q4_WORK", hd == 64 ? 9600 : 5500);
 }
 
-Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv) {
+Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv, int hd) {
   Q4Choice c{};
   const int64_t rounds = (cap + ROUND - 1) / ROUND;  // the most of a tile
-  c.target = std::max(1, FILL / n_kv);
+  const bool few = num_tokens * group <= 32 * num_seqs;
+  const int64_t work = q4_tiles(num_tokens, num_seqs, group) * rounds * n_kv;
+  const int fill = hd == 64 && few && work > 16 * FILL ? 2 * FILL : FILL;
+  c.target = std::max(1, fill / n_kv);
   // uneven lengths: the longest may take four times the parts of even ones
   const int64_t even = (c.target + num_seqs - 1) / num_seqs;
   c.splits = (int)std::clamp<int64_t>(4 * even + 2, 3, MAX_PARTS);
@@ -595,7 +604,7 @@ extern "C" int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_se
     return smx::q4_prompt_workspace(p);
   }
   const smx::Q4Choice c = smx::choose_q4(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
-                                         n_q / n_kv, n_kv);
+                                         n_q / n_kv, n_kv, head_dim);
   return smx::q4_workspace((int64_t)num_tokens * n_q, c.splits, head_dim);
 }
 
@@ -645,7 +654,7 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
     return smx::q4_prompt((hipStream_t)stream, p);
   }
   const smx::Q4Choice c = smx::choose_q4(num_tokens, num_seqs, (int64_t)max_blocks * block_size,
-                                         n_q / n_kv, n_kv);
+                                         n_q / n_kv, n_kv, head_dim);
   SMX_REQUIRE(smx::q4_tiles(num_tokens, num_seqs, n_q / n_kv) *
                       (((int64_t)max_blocks * block_size + smx::ROUND - 1) / smx::ROUND) <
                   (1ll << 28),
