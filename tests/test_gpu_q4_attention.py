@@ -349,3 +349,19 @@ def test_blocks_of_v_without_a_value(n, ctx, n_q, n_kv, hd, bs):
         assert torch.isfinite(got).all()
         # (the weights of a tile are rescaled or not by rows that are NaN now: one rounding)
         torch.testing.assert_close(got, clean, rtol=2.0 ** -7, atol=2.0 ** -9)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("most", [900, 3000])
+def test_wide_tables(hd, most):
+    """Tables much wider than their sequences are long (a model's full width): calls are cut
+    into more parts, most of which have nothing."""
+    n = [1] * 19 + [3, 0]
+    ctx = [0, 31, 32, 127, 128, 129, 255, 500] + [most - 83 * i % most for i in range(13)]
+    c = Case(12, n, ctx, 8, 4, hd, 32)
+    narrow = c.run()
+    wide = torch.full((len(n), 500 - c.table.shape[1]), -1, dtype=torch.int32)
+    c.table = torch.cat((c.table, wide), 1)
+    got = c.run()
+    c.check(got)
+    c.check(narrow)
