@@ -44,6 +44,9 @@ Kernel sequence (HIP launches):
           tokens; any T): prompt_layer (integration/prompt.py), its positions
           the argument, its slots metadata.slot_mapping -> add +
           RMSNorm(next norm).
+  A cache in 4 bits (the layer's kv_cache a torch_ops.Q4KVCache): prompt_layer
+          as well, of packed rows or of one decode token per sequence, without
+          a plan.
 Other calls -- no published metadata, more than 16 rows, rows that are not
 one decode token per sequence (prefill), or a shared prefix (the metadata's
 prefix_table) -- go to the stock layer, as the reference's op runs vLLM's
@@ -165,7 +168,8 @@ def _check_plan_positions(md: SplitKVDecodeMetadata, positions: torch.Tensor) ->
 
 def _packed_rows(e: _Entry, md: SplitKVDecodeMetadata, x: torch.Tensor, residual: torch.Tensor,
                  positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """The layer over packed rows (the metadata has a query_start_loc)."""
+    """The layer over packed rows (the metadata has a query_start_loc), or a decode step
+    over a cache in 4 bits."""
     c = e.cfg
     if x.dim() != 2 or x.shape[1] != c.hidden or x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bf16 [T, {c.hidden}], got {x.dtype} {tuple(x.shape)}")
@@ -196,8 +200,11 @@ def layer_run(x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor,
         if shared:
             raise ValueError("packed query rows and a shared prefix do not go together")
         return _packed_rows(e, md, x, residual, positions)
+    if (md is not None and not shared and isinstance(e.layer.kv_cache, torch_ops.Q4KVCache)
+            and md.seq_lens.numel() == T):
+        return _packed_rows(e, md, x, residual, positions)
     decode = md is not None and not shared and 1 <= T <= 16 and md.seq_lens.numel() == T
-    if not decode:
+    if not decode or isinstance(e.layer.kv_cache, torch_ops.Q4KVCache):
         if e.stock is not None:  # prefill, unpublished metadata, a shared prefix
             return e.stock(e.index, x, residual, positions)
         if md is None:
@@ -206,6 +213,10 @@ def layer_run(x: torch.Tensor, residual: torch.Tensor, positions: torch.Tensor,
         if shared:
             raise ValueError("layer_run does not decode under a shared prefix "
                              "(SplitKVDecodeImpl.forward does); install a stock layer for it")
+        if isinstance(e.layer.kv_cache, torch_ops.Q4KVCache):
+            raise ValueError(f"the metadata describes {md.seq_lens.numel()} sequences, x has {T} "
+                             "rows: a cache in 4 bits takes one decode token a sequence, or "
+                             "packed rows with a query_start_loc")
     c, L = e.cfg, e.layer
     if x.dim() != 2 or x.shape[1] != c.hidden or x.dtype != torch.bfloat16:
         raise ValueError(f"x must be bf16 [T, {c.hidden}], got {x.dtype} {tuple(x.shape)}")

@@ -92,7 +92,8 @@ class DecoderLayer:
     post_norm: torch.Tensor
     q_norm: torch.Tensor
     k_norm: torch.Tensor
-    kv_cache: torch.Tensor  # [2, num_blocks, block_size, n_kv, head_dim]
+    kv_cache: torch.Tensor  # [2, num_blocks, block_size, n_kv, head_dim] (layer_run and
+    #                         prompt_layer: or a torch_ops.Q4KVCache)
     name: str = ""
 
 
