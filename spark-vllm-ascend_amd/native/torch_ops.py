@@ -1023,8 +1023,8 @@ def qknorm_rope_kv_write_q4(qkv: torch.Tensor, q_gamma: torch.Tensor, k_gamma: t
 
 def q4_attention_workspace(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
                            query_start_loc: torch.Tensor | None = None) -> torch.Tensor | None:
-    """The workspace q4_attention uses for these sizes (uint8; None where it uses none).
-    Calls that can overlap need one each."""
+    """The workspace q4_attention uses for these sizes (uint8; None where it uses none),
+    with or without offsets.  Calls that can overlap need one each."""
     return _workspace(load().smx_q4_attention_workspace(
         q.shape[0], block_table.shape[0], block_table.shape[1], cache.block_size, q.shape[1],
         cache.n_kv, cache.head_dim), q.device)
