@@ -451,7 +451,7 @@ void q4_attention_kernel(Q4Args A) {
   // tile of `top` rounds must lie in at most (top - 2) / chunk + 2 <= splits parts
   int chunk = (int)(all * A.target_inv + 0.999f);
   if (A.splits > 2) chunk = max(chunk, (int)((float)top * A.splits_inv) + 1);
-  chunk = max(chunk, 1);
+  chunk = max(chunk, A.splits == 1 ? top : 1);
   const int equal = chunk;
   float inv = __builtin_amdgcn_rcpf((float)chunk);
   bool apart = A.num_seqs <= 64;
@@ -571,8 +571,12 @@ Q4Choice choose_q4(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group,
   // uneven lengths: the longest may take four times the parts of even ones
   const int64_t even = (c.target + num_seqs - 1) / num_seqs;
   c.splits = (int)std::clamp<int64_t>(4 * even + 2, 3, MAX_PARTS);
-  // (a tile of one round is never cut)
-  c.splits = rounds == 1 ? 1 : (int)std::min<int64_t>(c.splits, rounds + 1);
+  // Tiles of few rounds are not cut (up to 64 sequences, each can begin a part of its own): the
+  // merge takes longer than they do.  us cut / whole, 32 / 8 heads of 128: 200 tokens (3 rounds
+  // of capacity) 8.0 / 6.5, 100 queries 7.7 / 5.9, 16 sequences of 100 to 500 (5) 9.4 / 8.5, 48
+  // 13.9 / 12.0, 512 tokens (6) 9.2 / 9.25, but 700 (7) 9.3 / 10.3.
+  const bool whole = rounds == 1 || (num_seqs <= 64 && rounds <= 6);
+  c.splits = whole ? 1 : (int)std::min<int64_t>(c.splits, rounds + 1);
   return c;
 }
 
