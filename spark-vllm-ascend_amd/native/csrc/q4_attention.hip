@@ -31,7 +31,7 @@
 //
 // 32 / 8 heads of 128, us: 48 sequences behind 2000 to 32000 tokens 130 to 150 (635 MB, 4.9 to
 // 4.2 TB/s; the same loads without the arithmetic 135, a copy's rate 124), 16 behind 300 to
-// 8000 19 (2.4 TB/s), 8 of 5 tokens behind them 20, 1 behind 512 9.3 (6.9 and the merge).
+// 8000 19 (2.4 TB/s), 8 of 5 tokens behind them 20, 1 behind 512 9.3.
 #include <math.h>
 
 #include <algorithm>
