@@ -309,3 +309,29 @@ def test_refusals():
             ops.copy_pages(s, pairs)
     with pytest.raises(ValueError):
         ops.copy_pages([cache], _i32([[0, 1]]))
+
+
+@pytest.mark.parametrize("rows", [3, 20, 90])
+def test_any_tables(rows):
+    """Pages listed in any way: twice in a row, as the full page of one and the last of another,
+    none at all, entries outside the pool; lengths below and above what rows hold."""
+    rng = random.Random(rows)
+    for _ in range(25):
+        bs, width = rng.choice([1, 4, 16]), rng.randint(1, 6)
+        blocks = rng.randint(2, 3 * rows)
+        table = [[rng.choice([rng.randrange(blocks), rng.randrange(blocks), -1, blocks])
+                  for _ in range(width)] for _ in range(rows)]
+        pages = [rng.randint(-1, width + 1) for _ in range(rows)]
+        lens = [rng.randint(-2, (width + 1) * bs) for _ in range(rows)]
+        listed = {p for r, n in zip(table, pages) for p in r[:max(n, 0)]}
+        free = [p for p in range(blocks) if p not in listed]
+        rng.shuffle(free)
+        parents = [rng.randint(-1, rows) for _ in range(rows)]
+        _check(_fork(parents, lens, pages, table, free, blocks, bs),
+               fork(parents, lens, pages, free, table, blocks, bs), blocks)
+        got = _ops().compact_pages(_i32(pages), _i32(table), blocks)
+        out, left, moves = compact(pages, table, blocks)
+        assert got.block_table.tolist() == out
+        assert got.free_count.item() == len(left)
+        assert got.free_pages.tolist() == left + [-1] * (blocks - len(left))
+        assert got.moves.tolist() == (moves + [[-1, -1]] * blocks)[:blocks // 2]
