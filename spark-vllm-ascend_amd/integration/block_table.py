@@ -149,7 +149,12 @@ class DeviceBlockTables:
             num_pages=self.num_pages, free_count=self.free_count)
         self._ends = torch.zeros(max_seqs + 1, **i32)
         self._room = torch.zeros(max_seqs, **i32)
-        self._forked = self._moves = None
+        # fork()'s and compact()'s, from here on: either may be captured first
+        self._forked = None
+        self._fork_out = tuple(torch.empty_like(t) for t in (self.block_table, self.num_pages,
+                                                             self.lens))
+        self._copies = torch.empty((max_seqs, 2), **i32)
+        self._moves = torch.empty((num_blocks // 2, 2), **i32)
 
     def step(self, query_lens: torch.Tensor) -> torch_ops.RequestTables:
         """query_lens (int32 [max_seqs], on the device) more tokens a request: takes
@@ -188,10 +193,8 @@ class DeviceBlockTables:
         valid until the next fork).  A row for whose copy there is no page is cut to its
         whole pages."""
         if self._forked is None:
-            self._forked = torch_ops.ForkedPages(
-                torch.empty_like(self.block_table), torch.empty_like(self.num_pages),
-                torch.empty_like(self.lens), self.free_pages, self.free_count,
-                self.num_pages.new_empty((self.num_pages.numel(), 2)))
+            self._forked = torch_ops.ForkedPages(*self._fork_out, self.free_pages,
+                                                 self.free_count, self._copies)
         out = torch_ops.fork_pages(parents, self.lens, self.num_pages, self.free_pages,
                                    self.free_count, self.block_table, self.free_pages.numel(),
                                    self.block_size, out=self._forked)
@@ -205,8 +208,6 @@ class DeviceBlockTables:
         """Moves the pages in use to the front of the pool: the moves are returned, int32
         [num_blocks // 2, 2], to be done by torch_ops.copy_pages before the cache is used
         again (a buffer of this object, valid until the next compact)."""
-        if self._moves is None:
-            self._moves = self.num_pages.new_empty((self.free_pages.numel() // 2, 2))
         torch_ops.compact_pages(
             self.num_pages, self.block_table, self.free_pages.numel(),
             out=torch_ops.CompactedPages(self.block_table, self.free_pages, self.free_count,

@@ -172,3 +172,44 @@ def test_a_cache_in_4_bits_has_no_plan():
     with pytest.raises(ValueError, match="4 bits"):
         impl.forward(None, torch.zeros((1, N_Q * HD), dtype=BF16, device="cuda"), None, None,
                      cache, m)
+
+
+@pytest.mark.gpu
+def test_a_captured_fork_and_compaction():
+    """DeviceBlockTables.fork and compact captured before any other call of theirs, with the
+    copies, and replayed; against the same calls one by one."""
+    ops, tab = pkg("native.torch_ops"), pkg("integration.block_table")
+    rows, blocks = 4, 24
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def fresh():
+        t = tab.DeviceBlockTables(blocks, BS, rows, 4, 200, "cuda")
+        cache = ops.q4_kv_cache(blocks, BS, N_KV, HD, "cuda")
+        cache.codes.copy_(torch.arange(cache.codes.numel(), device="cuda").view(cache.codes.shape))
+        return t, cache, ops.PageSet(cache.planes())
+
+    (a, ca, pa), (b, cb, pb) = fresh(), fresh()
+    parents = torch.zeros(rows, **i32)
+    ones = torch.ones(rows, **i32)
+
+    def turn(t, pages):
+        ops.copy_pages(pages, t.fork(parents))
+        ops.copy_pages(pages, t.compact())
+
+    for t in (a, b):
+        t.step(torch.tensor([40, 64, 1, 0], **i32))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        turn(a, pa)
+    for p in ([0, 0, 1, 2], [1, 1, 1, 2], [3, 2, -1, 0], [0, 0, 0, 0], [2, 1, 0, 3]):
+        parents.copy_(torch.tensor(p))
+        graph.replay()
+        turn(b, pb)
+        for t in (a, b):
+            t.step(ones)
+        torch.cuda.synchronize()
+        for x, y in ((a.block_table, b.block_table), (a.num_pages, b.num_pages), (a.lens, b.lens),
+                     (a.free_pages, b.free_pages), (a.free_count, b.free_count),
+                     (ca.codes, cb.codes)):
+            assert torch.equal(x, y), p

@@ -1,5 +1,7 @@
 """Beam search's selection (torch_ops.beam_select) against float64 log-softmaxes and a
 sort: rows and tokens equal, scores to half a step of fp32."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -202,3 +204,37 @@ def test_refusals():
             print("not refused:", i)
     with pytest.raises(pkg("native").SmxError):
         f(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("shift,scale", [(15.0, 1.0), (16.0, 0.0), (40.0, 1.0), (-60.0, 1.0),
+                                         (0.0, 10.0), (-300.0, 30.0), (1e4, 100.0), (3e38, 0.0),
+                                         (-3e38, 0.0), (0.0, 1e-4)])
+def test_logits_of_any_size(shift, scale, dtype):
+    """Near 0, where exponentials are taken as they are, on the border, and far from it."""
+    for seqs, beams, width, vocab in ((2, 3, 4, 5000), (1, 2, 16, 40001)):
+        x, c = _inputs(9, seqs, beams, vocab, torch.float32, std=1.0)
+        x = (x * scale + shift).to(dtype)
+        x[:, ::7] = -math.inf
+        check(_ops().beam_select(x, c, beams, width), reference(x, c, beams, width),
+              f"{shift} {scale}")
+
+
+@pytest.mark.parametrize("dtype,bits", [
+    (BF16, [0x7fc0, 0x7f81, 0xffc0 - 65536, 0xff81 - 65536, 0xffff - 65536, 0x7fff]),
+    (torch.float32, [0x7fc00000, 0x7f800001, 0xffc00000 - 2 ** 32, 0xff800001 - 2 ** 32, -1,
+                     0x7fffffff])])
+def test_every_kind_of_nan(dtype, bits):
+    """Quiet and signalling, with and without a sign: never chosen, nothing in the sum."""
+    x, c = _inputs(10, 2, 3, 9001, dtype)
+    clean = x.clone()
+    clean[:, 5::11] = -math.inf
+    raw = x.view(torch.int16 if dtype is BF16 else torch.int32)
+    for i, b in enumerate(bits):
+        at = torch.arange(5, 9001, 11, device="cuda")[i::len(bits)]
+        raw[:, at] = b
+    assert x[:, 5::11].isnan().all()
+    got, want = _ops().beam_select(x, c, 3, 8), _ops().beam_select(clean, c, 3, 8)
+    for a, b in ((got.parents, want.parents), (got.tokens, want.tokens), (got.scores, want.scores)):
+        assert torch.equal(a, b)
+    check(got, reference(clean, c, 3, 8))
