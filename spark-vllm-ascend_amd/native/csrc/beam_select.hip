@@ -253,7 +253,8 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     if (least_key + bit <= INF_KEY &&
         __popcll(__builtin_amdgcn_ballot_w64(best >= (int)(least_key + bit))) >= A.width)
       least_key += bit;
-  const int bound_key = (int)least_key;
+  // (0 and -0 are the same value, but not the same key: a bound of 0 is -0's)
+  const int bound_key = least_key == 0 ? -STEP : (int)least_key;
   const float bound = key_value<BITS>(bound_key);
   const float top = key_value<BITS>(max(top_key, NO_KEY));
   uint64_t* const mine = list[wave];
