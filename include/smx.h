@@ -722,7 +722,8 @@ int smx_q4_attention(void* stream, const void* q, int64_t q_stride, const void* 
  * by element_size 2 or 4, rows stride elements apart) and of scores (fp32).  Its
  * continuations score
  *   scores[b] + logits[b][v] - log sum_u exp(logits[b][u])
- * taken in 64 bits; the best `width` in order, ties to the lowest b * vocab + v, go to
+ * taken in 64 bits (good to 3e-12, rows that differ by a constant exactly alike); the best
+ * `width` in order, ties to the lowest b * vocab + v, go to
  * parents (the row), tokens and out_scores [seqs, width].  Where there are fewer the rest
  * is -1, -1 and -inf.  A logit of -inf or NaN is never chosen; logits of +inf share the
  * probability; a row whose score is -inf or NaN offers nothing.  A row with done[row] != 0

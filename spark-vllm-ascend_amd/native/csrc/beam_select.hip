@@ -6,14 +6,17 @@
 // One pass over the logits.  A beam's best are its largest logits, so a workgroup keeps
 // the `width` largest of its part of a row and the part's maximum and sum of exponentials
 // (beam_parts_kernel); a workgroup a sequence then takes the best of the parts'
-// (beam_merge_kernel).  Beams are compared by their sums, so these are good to about 2e-9
-// and joined in 64 bits: two beams' candidates whose scores differ by less than that might
-// be taken in the wrong order, where fp32 sums would confuse those within 1e-6.
+// (beam_merge_kernel).  Beams are compared by their sums, so these are of exponentials in
+// 64 bits, each good to 8e-13 of itself, relative to a part's maximum: a score is good to
+// 3e-12, and rows that differ by a constant have the same sums.  (The transcendental unit's
+// exponentials with a correction for most of a peaked row's sum were 1.4 times as fast, but
+// their error of some 1e-8 is a function of the value: in a row of few distinct logits it
+// does not average out.)
 //
 // Bound by vector instructions where there are many rows: 512 rows of 151936 bf16 values,
-// a tenth of them done, 16 best of 8 beams: 52 us, the parts 41 (3.4 TB/s; about 14
-// instructions a value, an exponential and a 64-bit sum among them), the merge 9.  4 rows
-// 10.7 us: two launches of short latencies one after another.
+// a tenth of them done, 16 best of 8 beams: 75 us, the parts 67 (2.1 TB/s; about 25
+// instructions a value, 18 of them in 64 bits), the merge 7.4.  4 rows 10.8 us: two launches
+// of short latencies one after another.
 //
 // A NaN logit counts as -inf, a token that is never chosen; of several logits of +inf each
 // has an equal share.
@@ -35,11 +38,11 @@ constexpr int MAX_WIDTH = 64, MAX_BEAMS = 64;
 constexpr int CAP = 128;     // candidates of a wave
 constexpr int CHUNKS = 128;  // loads of a wave that hold candidates
 constexpr int NT = 256, WAVES = NT / 64;
-// Of 16 bytes, a lane: a part is 32 KB of a row.  us with 2 / 4 / 8 of them, rows of 151936
-// bf16 values: 1 row 9.2 / 9.3 / 10.0, 16 rows 11.2 / 10.9 / 10.8, 128 rows 25 / 21 / 20,
-// 512 rows (an eighth done) 77 / 58 / 56; 64 rows of 32000 10.0 / 10.1 / 10.9, 512 rows 22 /
-// 19 / 19.
-constexpr int LOADS = 8;
+// Of 16 bytes, a lane: a part is 16 KB of a row.  us with 2 / 4 / 8 of them, rows of 151936
+// bf16 values: 1 row 9.5 / 10.0 / 11.4, 16 rows 11.4 / 11.7 / 12.0, 128 rows 33 / 27 / 26,
+// 512 rows (a tenth done) 94 / 75 / 75; 64 rows of 32000 10.7 / 10.9 / 12.3, 512 rows 27 /
+// 24 / 24.
+constexpr int LOADS = 4;
 
 struct BeamArgs {
   const void* logits;
@@ -73,7 +76,9 @@ __device__ __forceinline__ double exp_any(double a) {
   p = fma(p, r, 0x1.ffffffffd55a3p-1);
   p = fma(p, r, 0x1.ffffffffff79dp-1);
   const uint64_t bits = __builtin_bit_cast(uint64_t, p);
-  const uint32_t hi = (uint32_t)(bits >> 32) + ((uint32_t)__builtin_bit_cast(uint64_t, t) << 20);
+  uint32_t hi = (uint32_t)(bits >> 32);
+  asm("" : "+v"(hi));  // (so that 32 bits are added in one instruction, not 64 in five)
+  hi += (uint32_t)__builtin_bit_cast(uint64_t, t) << 20;
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)bits);
 }
 
@@ -141,11 +146,6 @@ __device__ __forceinline__ double wave_sum64(double v) {
 // maximum, the values that reach a bound which `width` of the part do (found from maxima
 // over a lane of each wave), and its sum of exponentials; the few collected of all waves are ranked
 // by counting.
-//
-// The sum, in 64 bits: exp by the transcendental unit, whose errors are a few 1e-8 of each
-// term, and again in 64 bits for the collected values, which are most of a peaked row's
-// sum.  So what is left is 1e-9 of it, and less where many terms' errors average out; equal
-// logits of two beams have equal errors.
 template <typename L>
 __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   constexpr int V = 16 / sizeof(L);  // logits of a load
@@ -373,69 +373,18 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
     }
   }
 
-  // ---- the sum of exponentials: as they are, relative to `top` where that is large
-  const bool near = top > -16.f && top < 16.f;
+  // ---- the sum of exponentials relative to `top` (-inf and NaN with a sign: below -700)
   double sum = 0.0;
-  // exp f = 2^(f HI) (1 + f REST), HI log2(e) to 16 bits, so that a bf16 value's product with
-  // it is exact, and REST what is missing, times log 2; the next term, half of (f REST)^2, is
-  // below 4e-9 at 16 and less below.  Other products' rounding is made good.  The first
-  // factor is `p`, the second 1 + `more` REST.
-  constexpr float HI = 0x1.7154p+0f, REST = 0x1.480fb6p-18f;
-  auto quick = [&](auto relative, float f, float& more) -> float {
-    const float t = f * HI;
-    more = V == 8 && !relative ? f : fmaf(fmaf(f, HI, -t), 0x1.62e430p-1f / REST, f);
-    return __builtin_amdgcn_exp2f(t);
-  };
-  // (exact where it is small: v is half of `top` at least, or exp(v - top) below e^-8)
-  auto from_top = [&](float v) {
-    const float f = v - top;
-    return f > -200.f ? f : -200.f;
-  };
-  auto add = [&](auto relative) {
-    // (values below -200, -inf and NaN with a sign are larger as unsigned numbers)
-    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-    typedef typename std::conditional<V == 8, u16x2, uint32_t>::type Bits;
+  if (top_key < INF_KEY && top_key > NO_KEY) {
     double s[2] = {0.0, 0.0};
-    float small = 0.f;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
+      opaque(i);
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        float f;
-        if constexpr (relative) {
-          f = from_top(value(i, j));
-        } else {
-          if (j % (V / 4) == 0) {
-            const uint32_t u = x[i][j / (V / 4)];
-            x[i][j / (V / 4)] = __builtin_bit_cast(
-                uint32_t, __builtin_elementwise_min(__builtin_bit_cast(Bits, u),
-                                                    (Bits)(V == 8 ? 0xc348u : 0xc3480000u)));
-          }
-          f = value(i, j);
-        }
-        float more;
-        const float p = quick(relative, f, more);
-        small = fmaf(p, more, small);
-        s[j & 1] += (double)p;
-      }
-      asm volatile("" : "+v"(small));  // (its products here, not all of them at the end)
+      for (int j = 0; j < V; ++j)
+        s[j & 1] += exp_any(fmax((double)value(i, j) - (double)top, -700.0));
     }
-    sum = s[0] + s[1] + (double)(small * REST);
-    // the collected ones' in 64 bits
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the wave's list
-    for (int i = lane; i < n; i += 64) {
-      const float v = order_value((int)((uint32_t)(mine[i] >> 32) ^ 0x80000000u));
-      const float f = relative ? from_top(v) : fmaxf(v, -200.f);
-      float more;
-      const double p = (double)quick(relative, f, more);
-      sum += (exp_any(relative ? fmax((double)v - (double)top, -700.0) : (double)f) - p) -
-             p * (double)(more * REST);
-    }
-  };
-  if (near) {
-    add(std::false_type());
-  } else if (top_key < INF_KEY && top_key > NO_KEY) {
-    add(std::true_type());
+    sum = s[0] + s[1];
   } else if (top_key == INF_KEY) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
@@ -474,7 +423,6 @@ __global__ __launch_bounds__(NT) void beam_parts_kernel(BeamArgs A) {
   if (tid == 0) {
     double s = 0.0;
     for (int w = 0; w < WAVES; ++w) s += sum_s[w];
-    if (near) s /= exp_any((double)top);
     st_agent(A.part_max + (int64_t)row * A.parts + part, top);
     st_agent(reinterpret_cast<uint64_t*>(A.part_sum) + (int64_t)row * A.parts + part,
              __builtin_bit_cast(uint64_t, s));
