@@ -26,7 +26,15 @@ class BeamSearch:
     """The beams of several sequences: row s * beams + b of `tables` is sequence s's beam b,
     the best first; `pages` are the caches that the tables' pages are of.  A sequence
     starts with one beam, its prompt in row s * beams.  A beam ends with eos_id (-1: none
-    does) and keeps its score and place among the others; it takes no more tokens."""
+    does) and keeps its score and place among the others; it takes no more tokens, and its
+    pages are given up.
+
+    Nothing is read back, so that a step is not refused where the pool has no page left for
+    a beam: one whose tokens the cache does not hold all (there was no page for its copy of
+    a last page or for its new token, or the tables' max_tokens are fewer than the rows)
+    offers nothing in the next step.  A sequence none of whose beams had room has scores
+    of -inf alone.  (Whether the tables held the prompts is for the caller to see:
+    tables.lens before the first step.)"""
 
     def __init__(self, tables: DeviceBlockTables, pages: torch_ops.PageSet, beams: int,
                  eos_id: int = -1, pad_id: int = 0):
@@ -44,18 +52,26 @@ class BeamSearch:
         self.scores[:, 1:] = float("-inf")
         self.done = torch.zeros(rows, dtype=torch.bool, device=dev)
         self._history: list = []
+        self._held = None  # the tokens that each row of the tables must hold
 
     def step(self, logits: torch.Tensor) -> torch.Tensor:
         """Goes on from the rows' logits [rows, vocab] (those of a row without a score, or
         done, are not looked at): the rows' next tokens, int64 [rows], pad_id where a beam is
-        done or there is none.  The tables' rows are those of the new beams."""
-        best = torch_ops.beam_select(logits, self.scores.view(-1), self.beams, self.beams,
-                                     done=self.done, pad_id=self.pad_id)
+        done or there is none.  The tables' rows are those of the new beams, and
+        tables.step(query_lens()) takes their tokens before the next step."""
+        lens = self.tables.lens
+        if self._held is None:
+            self._held = lens.clone()
+        scores = torch.where(lens < self._held, float("-inf"), self.scores.view(-1))
+        best = torch_ops.beam_select(logits, scores, self.beams, self.beams, done=self.done,
+                                     pad_id=self.pad_id)
         parents, tokens = best.parents.view(-1), best.tokens.view(-1)
-        was_done = self.done[parents.clamp(min=0).long()]
+        at = parents.clamp(min=0).long()
         self.scores = best.scores
-        self.done = (tokens == self.eos_id) | was_done | (parents < 0)
-        torch_ops.copy_pages(self.pages, self.tables.fork(parents))
+        self.done = (tokens == self.eos_id) | self.done[at] | (parents < 0)
+        self._held = torch.where(self.done, 0, self._held[at] + 1)
+        going_on = torch.where(self.done, -1, parents)
+        torch_ops.copy_pages(self.pages, self.tables.fork(going_on))
         self._history.append((parents, torch.where(parents < 0, self.pad_id, tokens)))
         return self._history[-1][1]
 
