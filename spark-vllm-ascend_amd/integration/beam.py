@@ -58,7 +58,12 @@ class BeamSearch:
         """Goes on from the rows' logits [rows, vocab] (those of a row without a score, or
         done, are not looked at): the rows' next tokens, int64 [rows], pad_id where a beam is
         done or there is none.  The tables' rows are those of the new beams, and
-        tables.step(query_lens()) takes their tokens before the next step."""
+        tables.step(query_lens()) takes their tokens before the next step.  Not in a graph's
+        capture: a step's scores and tokens are buffers of their own, that a replay would
+        not go on from (beam_select, tables.fork and copy_pages can be captured)."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a step of BeamSearch cannot be captured: replays would start from "
+                               "the same scores")
         lens = self.tables.lens
         if self._held is None:
             self._held = lens.clone()
