@@ -6,12 +6,13 @@ head.py:12-31).  Here a step of logits becomes the next step's rows without the 
 the pages that they share and ``torch_ops.copy_pages`` the last pages that they write to.
 
     search = BeamSearch(tables, torch_ops.PageSet(cache.planes()), beams, eos_id)
-    tables.step(lens)               # the prompts, in each sequence's first row
-    ... logits of the prompts' last tokens ...
+    t = tables.step(lens)           # the prompts, in each sequence's first row
+    ... logits [rows, vocab] of the prompts' last tokens ...
     for _ in range(n):
-        tokens = search.step(logits)
-        step = tables.step(search.query_lens())
-        ... logits of the rows' new tokens ...
+        search.step(logits)
+        t = tables.step(search.query_lens())
+        ... packed [rows, vocab] of packed_tokens(), at t's positions and slots ...
+        logits = packed[search.last_rows(t)]
     search.sequences()
 """
 from __future__ import annotations
@@ -81,8 +82,26 @@ class BeamSearch:
         return self._history[-1][1]
 
     def query_lens(self) -> torch.Tensor:
-        """The tokens a row takes in the next step, 1 or 0: tables.step's argument."""
+        """The tokens a row takes in the next step, 1 or 0: tables.step's argument.  What the
+        model is given for them is packed_tokens(), not step's tokens, once a beam is done."""
         return (~self.done).to(torch.int32)
+
+    def packed_tokens(self) -> torch.Tensor:
+        """The rows' next tokens as tables.step(query_lens()) packs them, int64 [rows]: row
+        after row those of the beams that go on, pad_id behind them (of no sequence: their
+        slots are -1)."""
+        if not self._history:
+            raise RuntimeError("there is no token before the first step")
+        rows, tokens = self.done.numel(), self._history[-1][1]
+        out = tokens.new_full((rows + 1,), self.pad_id)
+        out[torch.where(self.done, rows, torch.cumsum(~self.done, 0) - 1)] = tokens
+        return out[:rows]
+
+    def last_rows(self, tables: torch_ops.RequestTables) -> torch.Tensor:
+        """Where the rows' last tokens stand in the packed tokens of a tables.step, int64
+        [rows]: step's logits are those there.  (Any of a row that takes no tokens, whose
+        logits are not looked at.)"""
+        return (tables.query_start_loc[1:].long() - 1).clamp(min=0)
 
     def sequences(self) -> torch.Tensor:
         """The beams' tokens so far, int64 [seqs, beams, steps], the best first (`scores`;
