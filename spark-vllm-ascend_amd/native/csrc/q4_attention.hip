@@ -454,7 +454,9 @@ void q4_attention_kernel(Q4Args A) {
   chunk = max(chunk, A.splits == 1 ? top : 1);
   const int equal = chunk;
   float inv = __builtin_amdgcn_rcpf((float)chunk);
-  bool apart = A.num_seqs <= 64;
+  // (so much work that a part's length is nothing beside it: the sums below stay in int32,
+  // and so do a part's tokens, where parts end past the tokens of a tile)
+  bool apart = A.num_seqs <= 64 && all < 0x1p22f;
   auto padded = [&](int r) {
     if (!apart) return r;
     const int q = small_div(r, chunk, inv);

@@ -69,3 +69,21 @@ def test_every_token_has_its_weight(case):
                               1 / math.sqrt(hd))
     assert mine.all()
     assert_rows(got, ref, mag, str(case))
+
+
+def test_sequences_of_2_31_tokens():
+    """Three of the longest tables, of one page again and again (K and V 0) but for a page at the
+    front, in the middle or at the end, whose tokens have all the weight.  Parts of equal
+    length would end past 2^31 tokens here."""
+    ops = pkg("native.torch_ops")
+    bs, hd, n_kv, width = 4096, 64, 4, 524286
+    cache = ops.q4_kv_cache(2, bs, n_kv, hd, "cuda")
+    ones = torch.ones((bs, n_kv, hd), dtype=BF16, device="cuda")
+    ops.reshape_and_cache_q4(8 * ones, 3 * ones, cache, torch.arange(bs, 2 * bs, device="cuda"))
+    table = torch.zeros((3, width), dtype=torch.int32, device="cuda")
+    table[[0, 1, 2], [0, width // 2, width - 1]] = 1
+    lens = torch.full((3,), width * bs, dtype=torch.int32, device="cuda")
+    q = torch.ones((3, n_kv, hd), dtype=BF16, device="cuda")
+    # scores 64 against 0: e^-64 2^31 / 4096 of the weight is elsewhere
+    got = ops.q4_attention(q, cache, table, lens, hd ** -0.5)
+    assert torch.equal(got, torch.full_like(got, 3.0))
