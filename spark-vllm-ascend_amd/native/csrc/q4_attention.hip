@@ -664,7 +664,7 @@ extern "C" int smx_q4_attention(void* stream, const void* q, int64_t q_stride, c
   SMX_REQUIRE(smx::q4_tiles(num_tokens, num_seqs, n_q / n_kv) *
                       (((int64_t)max_blocks * block_size + smx::ROUND - 1) / smx::ROUND) <
                   (1ll << 28),
-              "row tiles times the sequences' capacity / 256 must be below 2^28");
+              "row tiles times the sequences' capacity / 128 must be below 2^28");
   const int64_t rows = (int64_t)num_tokens * n_q;
   SMX_REQUIRE(c.splits == 1 || (workspace && (uintptr_t)workspace % 16 == 0 &&
                                 workspace_bytes >= smx::q4_workspace(rows, c.splits, head_dim)),
