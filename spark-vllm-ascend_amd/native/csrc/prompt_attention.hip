@@ -40,6 +40,9 @@ typedef __attribute__((address_space(3))) uint16_t lds_u16;
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(4))) int32_t constant_i32;
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 // A dword of two bf16 values with those that are infinite or NaN replaced by 0.
 __device__ __forceinline__ uint32_t finite_bf16x2(uint32_t w) {
@@ -99,7 +102,7 @@ struct Shape {
   static constexpr int M = 32 * WM, NT = 64 * WM * WN;
   static constexpr int CH = HD / 8;                  // 16-byte chunks of a row
   static constexpr int TILE = KT * CH;               // chunks of a K or V tile
-  static constexpr int BUFFER = 2 * TILE + (Q4 ? KT / 4 : 0);  // K, V (Q4: and its flags)
+  static constexpr int BUFFER = 2 * TILE + (Q4 ? KT / 4 + 1 : 0);  // K, V (Q4: and flags)
   static constexpr int GROUP = ST * BUFFER;
   static constexpr int JOIN = WN > 1 ? (WN - 1) * WM * (32 * HD + 64) / 4 : 0;
   static constexpr int LDS = WN * GROUP > JOIN ? WN * GROUP : JOIN;
@@ -130,13 +133,59 @@ __device__ __forceinline__ void meet() {
   __asm__ volatile("" ::: "memory");
 }
 
+// Two values' product with the matrix in c: bf16 numbers, or fp16 ones over a cache in 4 bits.
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// A row's bf16 values (this lane's, the rest lane ^ 32's) as fp16 numbers, the largest
+// between 2^15 and 2^16: exact but for those 2^-29 of it and less.  The power of two that
+// makes them what they were; NaN for a row with an infinity or a NaN.
+template <int N>
+__device__ __forceinline__ float row_as_f16(u32x4 (&x)[N]) {
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = x[i][j] & 0x7fff7fffu;
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w));
+    }
+  const uint32_t half = max((uint32_t)m[0], (uint32_t)m[1]);
+  const auto both = __builtin_amdgcn_permlane32_swap(half, half, false, false);
+  const uint32_t top = max((uint32_t)both[0], (uint32_t)both[1]);
+  // bf16's exponent bits become fp16's, the row's largest 30, three places further up
+  const int exponent = max((int)(top >> 7), 30);
+  const uint16_t less = (uint16_t)((exponent - 30) << 7);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t w = x[i][j], mag = w & 0x7fff7fffu;
+      const u16x2 v = __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, mag),
+                                                    u16x2{less, less}) << 3;
+      x[i][j] = __builtin_bit_cast(uint32_t, v) | (w & 0x80008000u);
+    }
+  return top >= 0x7f80u ? __builtin_nanf("") : __uint_as_float((uint32_t)(exponent - 15) << 23);
+}
+
 // BS: the least block_size, 32 or 64: a tile is looked up and addressed by NP pieces
 // of BT tokens that are within a page.
 // Q4: the cache is held in 4 bits; tiles are loaded into registers a round ahead and
-// written to LDS as bf16 values.  (These are rounded, to 8 significant bits of the 15 of d
-// (c - 8): with codes multiplied as they are, as decode steps do, the scales' products take
-// as many instructions for every row as the rest of its softmax, which would be most of
-// a prompt's time.)
+// written to LDS as fp16 values, with which q and the weights are multiplied as fp16 numbers
+// too: of the 15 significant bits of d (c - 8) 11 are left, of a weight 11, of q all 8.  (With
+// codes multiplied as they are, as decode steps do, the scales' products take as many
+// instructions for every row as the rest of its softmax, which would be most of a prompt's
+// time; as bf16 numbers, of 8 bits, the outputs' error was 1.8 times their own rounding's,
+// and five instructions a pair of values, not four.)  d (c - 8) is a multiple of 2^-24, so
+// that no value is too small for fp16; 16 tokens among which one is too large, a |d| of 2^13
+// or more, are divided by BIG.
 template <int HD, int WM, int WN, int KT, int ST, int BS, bool Q4 = false>
 __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kvh, u32x4* smem) {
   using S = Shape<HD, WM, WN, KT, ST, Q4>;
@@ -169,6 +218,8 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       qf[ks] = *reinterpret_cast<const u32x4*>(A.q + (int64_t)tok * A.q_stride + head * HD +
                                                16 * ks + 8 * h);
   }
+  float scale_log2 = A.scale_log2;
+  if constexpr (Q4) scale_log2 *= row_as_f16(qf);
   const int lim_min = __builtin_amdgcn_readfirstlane(-wave_max_i32(-lim));
 
   // ---- staging: wave wm of a group loads every WM-th kilobyte of its tile, by
@@ -268,32 +319,59 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       }
     }
   };
-  // Eight values of scale d as bf16: bytes of half-bytes 0, 2, 4, 6 (lo) and 1, 3, 5, 7 (hi).
-  auto widen = [](uint32_t w, float d, bool key) -> u32x4 {
-    uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
-    // (so that a byte's conversion is one instruction, not a bit field's and one)
-    __asm__("" : "+v"(lo), "+v"(hi));
-    const float off = -8.f * d;
-    auto val = [&](uint32_t x, int i) { return fmaf((float)((x >> (8 * i)) & 0xffu), d, off); };
-    if (key)
-      return u32x4{cvt_pk_bf16(val(lo, 0), val(lo, 2)), cvt_pk_bf16(val(hi, 0), val(hi, 2)),
-                   cvt_pk_bf16(val(lo, 1), val(lo, 3)), cvt_pk_bf16(val(hi, 1), val(hi, 3))};
-    return u32x4{cvt_pk_bf16(val(lo, 0), val(hi, 0)), cvt_pk_bf16(val(lo, 1), val(hi, 1)),
-                 cvt_pk_bf16(val(lo, 2), val(hi, 2)), cvt_pk_bf16(val(lo, 3), val(hi, 3))};
+  // Eight values of scale d as fp16: a code behind 0x64 is the number 1024 + code, of which
+  // 1032 is taken off exactly.  (The mask and 0x64 come in registers, so that they are one
+  // instruction.)
+  constexpr float BIG = 32.f, BIG_LOG2 = 5.f;
+  uint32_t code_mask = 0x000f000fu, thousand = 0x64006400u;
+  if constexpr (Q4) {
+    __asm__("" : "+s"(code_mask));
+    __asm__("" : "+v"(thousand));
+  }
+  auto widen = [&](uint32_t w, f16x2 d, bool key) -> u32x4 {
+    auto val = [&](uint32_t x) {
+      return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2, x) - (_Float16)1032.f) * d);
+    };
+    u32x4 out;
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      out[j] = val(key ? ((w >> (4 * j)) & code_mask) | thousand
+                       : __builtin_amdgcn_perm(hi, lo, 0x0c040c00u + 0x00010001u * j) | thousand);
+    return out;
+  };
+  // Whether a finite scale among a wave's (in either half of w) is 2^13 or more.
+  auto too_large = [](const auto&... w) {
+    uint32_t least = ~0u;
+    auto look = [&](uint32_t x) {
+      const u16x2 v = __builtin_bit_cast(u16x2, x & 0x7fff7fffu) - (uint16_t)0x7000;
+      least = __builtin_bit_cast(uint32_t, __builtin_elementwise_min(
+                                               __builtin_bit_cast(u16x2, least), v));
+    };
+    (look(w), ...);
+    return __builtin_amdgcn_ballot_w64(min(least & 0xffffu, least >> 16) < 0x0c00u) != 0;
   };
   auto fill_k = [&](lds_u32x4* dst) {
+    bool big;
+    if constexpr (NB == 4)
+      big = too_large(kd[0], kd[1]);
+    else
+      big = too_large(kd[0]);
+    if (lane == 0) ((lds_u32*)(dst + 2 * S::TILE))[KT + qwave] = big;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const float d = f16_bits_to_f32(kd[b / 2] >> (16 * (b & 1)) & 0xffffu);
-      dst[qtok * CH + ((4 * b + qg) ^ k_swz<HD>(qtok))] = widen(kq[b], d, true);
+      const uint32_t w = kd[b / 2];
+      const _Float16 d = __builtin_bit_cast(f16x2, w)[b & 1] * (_Float16)(big ? 1 / BIG : 1.f);
+      dst[qtok * CH + ((4 * b + qg) ^ k_swz<HD>(qtok))] = widen(kq[b], f16x2{d, d}, true);
     }
   };
   auto fill_v = [&](lds_u32x4* dst) {
     // A token's block without a value (its scale is not finite) is 0 here, so that it does
     // not reach the rows that do not see the token, and a flag for those that do.
-    const bool none = (vd & 0x7fffu) >= 0x7c00u;
-    const float d = none ? 0.f : f16_bits_to_f32(vd);
-    ((lds_u8*)(dst + 2 * S::TILE))[4 * qtok + qg] = none;
+    const bool none = (vd & 0x7fffu) >= 0x7c00u, big = too_large(vd);
+    const uint16_t bits = none ? 0 : (uint16_t)vd;
+    const _Float16 d = __builtin_bit_cast(_Float16, bits) * (_Float16)(big ? 1 / BIG : 1.f);
+    ((lds_u8*)(dst + 2 * S::TILE))[4 * qtok + qg] = (uint8_t)(none | big << 1);
     // V's swizzle goes by two bits of the token: the others turn the order of the dwords
     const int turn = (qtok >> 2) & (NB - 1);
     Dwords w = vq;
@@ -306,7 +384,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
     for (int j = 0; j < NB; ++j)
       dst[S::TILE + qtok * CH + ((NB * qg + ((j + turn) & (NB - 1))) ^ v_swz<HD>(qtok))] =
-          widen(w[j], d, false);
+          widen(w[j], f16x2{d, d}, false);
   };
   auto bad_pages = [&](const int (&page)[NP]) {
     int bad = 0;
@@ -325,7 +403,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   f32x16 s[NU];       // scores: s[u][4 a + b] is token 32 u + 8 a + 4 h + b of row n
-  uint32_t p[NU][8];  // and their 2^(score - ref), bf16 pairs
+  uint32_t p[NU][8];  // and their 2^(score - ref), pairs of bf16 (Q4: fp16) numbers
 
   auto scores = [&](const lds_u32x4* kt) {
 #pragma unroll
@@ -337,9 +415,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         const u32x4 a = kt[(32 * u + n) * CH + ((2 * ks + h) ^ k_swz<HD>(n))];
-        s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                       __builtin_bit_cast(bf16x8, qf[ks]), s[u],
-                                                       0, 0, 0);
+        s[u] = mfma<Q4>(a, qf[ks], s[u]);
       }
   };
   // A plain tile: every row of the wave sees all of it, and its pages are known.  The
@@ -348,7 +424,20 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   auto is_plain = [&](int base, int bad) {
     return base >= it.from && base + KT <= lim_min && !bad;
   };
-  auto softmax = [&](auto plain, int base, int bad, uint32_t flags) {
+  // (of 11 significant bits a weight is to be at least 2^-14: the largest is up to 2^15 there)
+  constexpr float LIFT = Q4 ? 7.f : 0.f;
+  // Q4: tokens 16 g .. of a tile have V divided by BIG, or are weighed less by as much, where
+  // another 16 of the tile are divided (o is divided then); `shift` is what a score has
+  // added for that, beside -ref, `whole` what makes their weights' sum what it is.
+  constexpr int NG = Q4 ? KT / 16 : 1;
+  float shift[NG], whole[NG];
+  bool divided = false;
+#pragma unroll
+  for (int g = 0; g < NG; ++g) {
+    shift[g] = -ref;
+    whole[g] = 1.f;
+  }
+  auto softmax = [&](auto plain, int base, int bad, uint32_t flags, uint32_t k_flag) {
     // the scores of tokens without a page are NaN, and so is every row that sees one
     if constexpr (!plain) {
 #pragma unroll
@@ -365,15 +454,42 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-    mx = xor_max<32>(mx) * A.scale_log2;
+    mx = xor_max<32>(mx) * scale_log2;
     // The reference follows the maximum only once that has grown by LAG: p is then
     // at most 2^LAG, which neither fp32 nor bf16 minds, and most tiles leave o and
     // l as they are.
-    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG || (Q4 && flags != 0))) {
-      const float next = fmaxf(ref, mx);
-      const float alpha = __builtin_amdgcn_exp2f(ref - next);
+    if (__builtin_amdgcn_ballot_w64(mx > ref + (LAG + LIFT) || (Q4 && (flags | k_flag) != 0)) |
+        (uint64_t)divided) {
+      if constexpr (Q4) {
+        // (lane g % NG has the flag of K's tokens 16 g ..)
+        if (const uint64_t k_big = __builtin_amdgcn_ballot_w64(k_flag != 0)) {
+          mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[u][i] *= k_big >> (2 * u + i / 8) & 1 ? BIG : 1.f;
+              mx = fmaxf(mx, s[u][i]);
+            }
+          mx = xor_max<32>(mx) * scale_log2;
+        }
+      }
+      const float next = fmaxf(ref, mx - LIFT);
+      float alpha = __builtin_amdgcn_exp2f(ref - next);
       ref = next;
       l *= alpha;
+      if constexpr (Q4) {
+        const uint64_t v_big = __builtin_amdgcn_ballot_w64((flags & 0x02020202u) != 0);
+        alpha *= divided ? BIG : 1.f;
+        divided = v_big != 0;
+        alpha *= divided ? 1 / BIG : 1.f;
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+          const bool less = divided && !(v_big >> (16 * g) & 0xffff);
+          shift[g] = less ? -ref - BIG_LOG2 : -ref;
+          whole[g] = less ? BIG : 1.f;
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -393,18 +509,25 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
         }
       }
     }
-    float part[4] = {0.f, 0.f, 0.f, 0.f};
+    float part[Q4 ? 2 * NG : 4] = {};
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], A.scale_log2, -ref));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], A.scale_log2, -ref));
-        part[2 * (i & 1)] += p0;
-        part[2 * (i & 1) + 1] += p1;
-        p[u][i] = cvt_pk_bf16(p0, p1);
+        const int g = Q4 ? 2 * u + i / 4 : 0, at = Q4 ? 2 * g : 2 * (i & 1);
+        const float less = Q4 ? shift[g] : -ref;
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i], scale_log2, less));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[u][2 * i + 1], scale_log2, less));
+        part[at] += p0;
+        part[at + 1] += p1;
+        p[u][i] = Q4 ? cvt_pk_f16(p0, p1) : cvt_pk_bf16(p0, p1);
       }
-    l += (part[0] + part[1]) + (part[2] + part[3]);
+    if constexpr (Q4) {
+#pragma unroll
+      for (int g = 0; g < NG; ++g) l = fmaf(part[2 * g] + part[2 * g + 1], whole[g], l);
+    } else {
+      l += (part[0] + part[1]) + (part[2] + part[3]);
+    }
   };
   // O^T += V^T P^T
   const int vr = 4 * h + ((lane & 15) >> 2), vcol = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -451,10 +574,7 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              __builtin_bit_cast(bf16x8, v_operand(vt, kk, d)),
-              __builtin_bit_cast(bf16x8, p_operand(kk)), o[d], 0, 0, 0);
+        for (int d = 0; d < DT; ++d) o[d] = mfma<Q4>(v_operand(vt, kk, d), p_operand(kk), o[d]);
     } else {
 #pragma unroll
       for (int kk = 0; kk < 2 * NU; ++kk)
@@ -536,10 +656,14 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
       }
     }
     if (!(!plain && tile >= ntiles) && 32 * wm < it.rows) {
-      uint32_t flags = 0;  // Q4: of token lane % KT
-      if constexpr (Q4) flags = ((const lds_u32*)(cur + 2 * S::TILE))[lane % KT];
+      uint32_t flags = 0, k_flag = 0;  // Q4: of token lane % KT, of 16 tokens
+      if constexpr (Q4) {
+        const lds_u32* const f = (const lds_u32*)(cur + 2 * S::TILE);
+        flags = f[lane % KT];
+        k_flag = f[KT + lane % (KT / 16)];
+      }
       scores(cur);
-      softmax(plain, base, bad[0], flags);
+      softmax(plain, base, bad[0], flags, k_flag);
       weigh(plain, cur + S::TILE, base);
     }
     if constexpr (Q4 && WM > SHARE) {
@@ -574,6 +698,13 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
     while (rd * WN + wn < ntiles && is_plain(first + (rd * WN + wn) * KT, bad[0]))
       step(std::true_type{});
     if (rd < rounds) step(std::false_type{});
+  }
+
+  if (Q4 && divided) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] *= BIG;
   }
 
   // ---- the lane pair's sums, then the WN groups' states (of one tile the first's only)
@@ -992,10 +1123,10 @@ struct Choice {
 // vector instructions with 128 of them, so that 256 (one workgroup a compute unit, eight
 // waves) are the faster where they fill the chip: cut, or behind a context from nine
 // tenths of a filling on, or from twice that on.  us, rows of 64 / 128 / 256: 500 tokens
-// behind 4000 85 / 71 / 64, 300 behind 30000 324 / 225 / 194, 2000 behind 8000 520 / 369 /
-// 335, 16 x 100 behind 1000 78 / 58 / 52, 4000 236 / 182 / 165, 8000 874 / 639 / 588; but
-// 1000 behind 3000 111 / 130 / 139, 2000 82 / 73 / 79, 4000, 16 / 4 heads of 64 82 / 91 /
-// 102.
+// behind 4000 91 / 76 / 71, 300 behind 30000 332 / 227 / 201, 2000 behind 8000 532 / 377 /
+// 353, 16 x 100 behind 1000 81 / 58 / 52, 4000 246 / 185 / 171, 8000 910 / 657 / 621; but
+// 1000 behind 3000 117 / 118 / 138, 2000 78 / 67 / 77, 4000, 16 / 4 heads of 64 77 / 91 /
+// 105.
 Choice choose_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv,
                      bool q4 = false) {
   Choice c{};

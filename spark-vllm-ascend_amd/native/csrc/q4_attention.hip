@@ -552,11 +552,11 @@ int64_t q4_tiles(int64_t num_tokens, int64_t num_seqs, int group) {
 // more work altogether than tiles of 16 rows, which widen every code and scale again,
 // are done with first (the tables' capacity stands for the lengths, and a tile's
 // beginning counts as three rounds).  us by tiles / by the prompt kernels, and the work, 32
-// / 8 heads of 128: 100 tokens 8.0 / 9.7 (0.8k), 8 x 20 behind 1000 22 / 31 (3.5k), 300
-// tokens 14.8 / 14.3 (3.6k), 40 behind 8000 27 / 30 (5.3k), 16 x 60 25 / 13 (7.7k), 8 x 60
-// behind 1000 37 / 33 (12k), 60 behind 15000 54 / 47 (15k); heads of 64: 1000 tokens, 14 / 2
-// heads 19 / 23 (9.6k), 8 x 100 behind 500, 16 / 4 18 / 16 (6.4k), 500 behind 4000, 14 / 2
-// 45 / 40 (17k).
+// / 8 heads of 128: 100 tokens 6.0 / 10.3 (0.8k), 8 x 20 behind 1000 24 / 31 (3.5k), 300
+// tokens 12.5 / 14.7 (3.6k), 40 behind 8000 26 / 29 (5.3k), 16 x 60 21 / 14 (7.7k), 8 x 60
+// behind 1000 38 / 33 (12k), 60 behind 15000 53 / 43 (15k); heads of 64: 1000 tokens, 14 / 2
+// heads 19 / 24 (9.6k), 8 x 100 behind 500, 16 / 4 15.8 / 17.6 (6.4k), 500 behind 4000, 14 / 2
+// 44 / 34 (17k).
 bool is_prompt(int64_t num_tokens, int64_t num_seqs, int64_t cap, int group, int n_kv, int hd) {
   if (num_tokens * group <= 32 * num_seqs) return false;
   const int64_t work = q4_tiles(num_tokens, num_seqs, group) * ((cap + ROUND - 1) / ROUND + 3) * n_kv;

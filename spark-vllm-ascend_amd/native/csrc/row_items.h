@@ -45,6 +45,13 @@ __device__ __forceinline__ uint32_t cvt_pk_bf16(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), bf16x2));
 }
 
+// (lo, hi) as one v_cvt_pk_f16_f32
+__device__ __forceinline__ uint32_t cvt_pk_f16(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), f16x2));
+}
+
 // The largest of a wave's values, for every lane.
 __device__ __forceinline__ int wave_max_i32(int v) {
   auto dpp = [](int x, auto ctrl) {

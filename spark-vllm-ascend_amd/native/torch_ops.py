@@ -1039,7 +1039,8 @@ def q4_attention(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
     query_start_loc[r]..query_start_loc[r + 1] of q [tokens, n_q, hd] (tokens may be
     strided), the last of its seq_lens[r] tokens.  Without query_start_loc row r is
     sequence r's newest token: a decode step.  Of few rows the cache's values are not
-    rounded; prompts round them to bf16.  Rows of no sequence are left as they are in `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
+    rounded; prompts round them to fp16.  Rows of no sequence are left as they are in
+    `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
     needs it."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is BF16 and q.dim() == 3):
         raise ValueError("q must be a bf16 GPU tensor [tokens, n_q, hd]")
