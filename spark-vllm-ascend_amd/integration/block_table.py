@@ -178,16 +178,18 @@ class DeviceBlockTables:
         """Takes every request back to its first lens[r] tokens (int32 [max_seqs]; one
         past its length keeps it, 0 ends it): pages no longer needed are free again.
         Not after a fork, since it takes a row's pages for its own: fork() ends requests
-        then, by not continuing them."""
+        then, by not continuing them, and takes them back by its lens."""
         if self._forked is not None:
-            raise RuntimeError("keep() frees a row's pages, which rows share after a fork()")
+            raise RuntimeError("keep() frees a row's pages, which rows share after a fork(): "
+                               "fork(parents, lens) takes rows back then")
         torch_ops.release_pages(lens, self.num_pages, self.free_pages, self.free_count,
                                 self.block_table, self.block_size)
         torch.minimum(self.lens, lens.clamp(min=0), out=self.lens)
 
-    def fork(self, parents: torch.Tensor) -> torch.Tensor:
+    def fork(self, parents: torch.Tensor, lens: torch.Tensor | None = None) -> torch.Tensor:
         """Row r goes on with what row parents[r] holds (int32 [max_seqs]; -1: with
-        nothing).  Full pages are shared, a last page that is not full is one row's: the
+        nothing), or with the first lens[parents[r]] tokens of it (int32 [max_seqs]; one past
+        its length keeps it).  Full pages are shared, a last page that is not full is one row's: the
         copies that this takes are returned, int32 [max_seqs, 2], to be done by
         torch_ops.copy_pages before the next tokens are written (a buffer of this object,
         valid until the next fork).  A row for whose copy there is no page is cut to its
@@ -195,7 +197,12 @@ class DeviceBlockTables:
         if self._forked is None:
             self._forked = torch_ops.ForkedPages(*self._fork_out, self.free_pages,
                                                  self.free_count, self._copies)
-        out = torch_ops.fork_pages(parents, self.lens, self.num_pages, self.free_pages,
+        held = self.lens
+        if lens is not None:
+            if lens.shape != held.shape or lens.dtype != held.dtype or lens.device != held.device:
+                raise ValueError("lens must be int32 [max_seqs] on the tables' device")
+            held = torch.minimum(held, lens.clamp(min=0))
+        out = torch_ops.fork_pages(parents, held, self.num_pages, self.free_pages,
                                    self.free_count, self.block_table, self.free_pages.numel(),
                                    self.block_size, out=self._forked)
         # (in place: graphs hold the tables' addresses)
