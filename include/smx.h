@@ -667,7 +667,7 @@ int smx_decode_advance(void* stream, int64_t* next_ids,
  * an fp16 scale d and hold codes c of 0..15 for the values d (c - 8), the block format of
  * the Q4_0 weights (src/spark_vllm_ascend/integration/weights.py:34-40): m the block's
  * first value of largest magnitude, d = fp16(m / -8) kept within +-65504, c =
- * floor(x / d + 8.5) kept within 0..15 (8 where d is 0: |m| below 2^-22); a block with a
+ * floor(x / d + 8.5) kept within 0..15 (8 where d is 0: |m| up to 2^-22); a block with a
  * NaN has the scale NaN and codes 0, an infinity becomes the block's largest value.
  *   codes  [2][num_blocks][n_kv][block_size][head_dim / 2] bytes, K first
  *   scales [2][num_blocks][n_kv][block_size][head_dim / 32] fp16
