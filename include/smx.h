@@ -703,10 +703,10 @@ int smx_q4_kv_read(void* stream, const void* codes, const void* scales,
  * none 0, rows of no sequence stay as they are).  query_start_loc may be NULL where
  * num_tokens is num_seqs: row r is sequence r's newest token, a decode step.  Scores,
  * sums and outputs are fp32.  Of few rows the cache's values are not rounded, and the
- * weights of the second product (softmax weight times V's scale) are rounded to bf16; of
+ * weights of the second product (softmax weight times V's scale) are rounded to fp16; of
  * prompts (more than 32 pairs of a token and a head of a group a sequence, and enough of
- * them times the tables' capacity) the values and the weights are rounded to fp16.  A row
- * of q with an infinity or a NaN is NaN of prompts.
+ * them times the tables' capacity) the values are too.  A row of q with an infinity or a
+ * NaN is NaN of prompts.
  */
 int64_t smx_q4_attention_workspace(int32_t num_tokens, int32_t num_seqs, int32_t max_blocks,
                                    int32_t block_size, int32_t n_q, int32_t n_kv,

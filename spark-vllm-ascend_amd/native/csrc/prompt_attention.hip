@@ -424,8 +424,9 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
   auto is_plain = [&](int base, int bad) {
     return base >= it.from && base + KT <= lim_min && !bad;
   };
-  // (of 11 significant bits a weight is to be at least 2^-14: the largest is up to 2^15 there)
-  constexpr float LIFT = Q4 ? 7.f : 0.f;
+  // Q4: the largest weight is between 2^LIFT and 2^15, so that those down to 2^-25 of it have
+  // 11 significant bits, and all are off by 2^-36 of it at most.
+  constexpr float LIFT = Q4 ? 11.f : 0.f, GROWTH = Q4 ? 15.f : LAG;
   // Q4: tokens 16 g .. of a tile have V divided by BIG, or are weighed less by as much, where
   // another 16 of the tile are divided (o is divided then); `shift` is what a score has
   // added for that, beside -ref, `whole` what makes their weights' sum what it is.
@@ -455,10 +456,10 @@ __device__ __forceinline__ void attend(const RowsArgs& A, const Item& it, int kv
 #pragma unroll
       for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
     mx = xor_max<32>(mx) * scale_log2;
-    // The reference follows the maximum only once that has grown by LAG: p is then
-    // at most 2^LAG, which neither fp32 nor bf16 minds, and most tiles leave o and
+    // The reference follows the maximum only once that has grown by LAG (Q4: by 4): p is
+    // then at most 2^GROWTH, which neither fp32 nor bf16 minds, and most tiles leave o and
     // l as they are.
-    if (__builtin_amdgcn_ballot_w64(mx > ref + (LAG + LIFT) || (Q4 && (flags | k_flag) != 0)) |
+    if (__builtin_amdgcn_ballot_w64(mx > ref + GROWTH || (Q4 && (flags | k_flag) != 0)) |
         (uint64_t)divided) {
       if constexpr (Q4) {
         // (lane g % NG has the flag of K's tokens 16 g ..)

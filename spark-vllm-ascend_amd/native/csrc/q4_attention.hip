@@ -2,15 +2,16 @@
 // paged KV cache held in 4 bits (q4_cache.h), for gfx950.
 //
 // A value is d (c - 8): c the code, d the scale of its block of 32 channels.  Codes are
-// multiplied as they are, as the bf16 numbers 16 + c (exact: two instructions a pair,
-// with no conversion), and what that adds is taken off again:
+// multiplied as they are, as the numbers 16 + c (exact: two instructions a pair, with no
+// conversion), and what that adds is taken off again:
 //   s_t = sum_b dk[t][b] (sum_{c in b} q_c (16 + code) - 24 sum_{c in b} q_c)
-//   o_c = sum_t p'[t][b] (16 + code[t][c]) - 24 sum_t p'[t][b],  p' = bf16(p_t dv[t][b])
-// with v_mfma_f32_16x16x32_bf16, whose 32 channels are one block b of K: -24 sum q is its
-// initial accumulator, and dk multiplies its result.  V's scale goes into the weights,
-// which are rounded to bf16 once, as they are over a bf16 cache; sum p' is a product
-// with ones.  So no value of the cache is rounded.  Scores, the running maximum, sums
-// and outputs are fp32.  (Calls of many rows, is_prompt below, go to the kernels of
+//   o_c = sum_t p'[t][b] (16 + code[t][c]) - 24 sum_t p'[t][b],  p' = fp16(p_t dv[t][b])
+// with v_mfma_f32_16x16x32, of bf16 numbers and then of fp16 ones, whose 32 channels are one
+// block b of K: -24 sum q is its initial accumulator, and dk multiplies its result.  V's
+// scale goes into the weights, which are rounded to fp16 once, an eighth of the outputs' own
+// rounding (as bf16 numbers, as much as it; 2 to 7% less time but for the longest); sum p'
+// is a product with ones.  So no value of the cache is rounded.  Scores, the running maximum,
+// sums and outputs are fp32.  (Calls of many rows, is_prompt below, go to the kernels of
 // prompt_attention.hip instead, which widen a tile once for all of its rows.)
 //
 // Products are transposed, S^T = K Q^T and O^T = V^T P^T: a row (a token's q head; "row =
@@ -31,7 +32,7 @@
 //
 // 32 / 8 heads of 128, us: 48 sequences behind 2000 to 32000 tokens 130 to 150 (635 MB, 4.9 to
 // 4.2 TB/s; the same loads without the arithmetic 135, a copy's rate 124), 16 behind 300 to
-// 8000 19 (2.4 TB/s), 8 of 5 tokens behind them 20, 1 behind 512 9.3.
+// 8000 19.4 (2.3 TB/s), 8 of 5 tokens behind them 21, 1 behind 512 9.7.
 #include <math.h>
 
 #include <algorithm>
@@ -47,15 +48,21 @@ namespace {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
 typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 typedef __attribute__((address_space(4))) int32_t constant_i32;
 
-constexpr float LAG = 8.f;        // log2 units
+// Log2 units: the largest weight times V's largest scale is between 2^TOP and 2^(TOP + LAG) by
+// the reference.  (fp16 holds up to 65504, and 11 significant bits of 2^-14 or more: weights
+// times scales down to 2^-25 of the largest; all are off by 2^-36 of it at most.)
+constexpr float LAG = 4.f, TOP = 11.f;
 constexpr float NO_REF = -3e38f;  // before the first token: below the scores of any use
 constexpr int KT = 32;            // tokens of a tile
 constexpr int WAVES = 4;
@@ -88,26 +95,37 @@ struct Tile {
   static constexpr int BYTES = 2 * (CODES + SCALES);
 };
 
-// Eight codes (the half-bytes of w) as bf16 numbers 16 + code, pairs of half-bytes j and
-// j + 4: bits 3..6 of a bf16 with exponent 4 are whole units.  The mask and the exponents
-// come in registers, of which the compiler does not know the value: as literals they
-// would make two instructions of v_and_or_b32 (three a pair of codes, not two).
+// Eight codes (the half-bytes of w) as numbers 16 + code, pairs of half-bytes j and j + 4:
+// bits 3..6 of a bf16, or 6..9 of an fp16, with exponent 4 are whole units.  The masks and the
+// exponents come in registers, of which the compiler does not know the value: as literals
+// they would make two instructions of v_and_or_b32 (three a pair of codes, not two).
 struct CodeBits {
   uint32_t mask = 0x00780078u, one = 0x41804180u;
+  uint32_t mask16 = 0x03c003c0u, one16 = 0x4c004c00u;
   float zero = 0.f;  // likewise, for products that are one instruction with a sum only
   __device__ __forceinline__ CodeBits() {
     __asm__("" : "+s"(mask));
     __asm__("" : "+v"(one));
+    __asm__("" : "+s"(mask16));
+    __asm__("" : "+v"(one16));
     __asm__("" : "+s"(zero));
   }
-  __device__ __forceinline__ bf16x8 operator()(uint32_t w) const {
+  __device__ __forceinline__ bf16x8 bf16(uint32_t w) const {
     return __builtin_bit_cast(bf16x8, u32x4{((w << 3) & mask) | one, ((w >> 1) & mask) | one,
                                             ((w >> 5) & mask) | one, ((w >> 9) & mask) | one});
+  }
+  __device__ __forceinline__ f16x8 f16(uint32_t w) const {
+    return __builtin_bit_cast(f16x8, u32x4{((w << 6) & mask16) | one16, ((w << 2) & mask16) | one16,
+                                           ((w >> 2) & mask16) | one16, ((w >> 6) & mask16) | one16});
   }
 };
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 __device__ __forceinline__ float half_of(uint32_t w, int i) {
@@ -195,8 +213,8 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
       }
   };
 
-  // ---- the row's state: the exponents' reference (log2 units: the running maximum, or up
-  // to LAG below it), the sum of 2^(score - ref) over this lane's tokens, the output's
+  // ---- the row's state: the exponents' reference (log2 units: TOP below the running maximum
+  // and V's largest scale together, or up to LAG less than that), the sum of 2^(score - ref) over this lane's tokens, the output's
   // products with 16 + code and, block by block, the sums of their weights (in every register
   // the same; of its own for each block, so that one that is NaN stays among its dims).
   float ref = NO_REF, l = 0.f;
@@ -206,15 +224,21 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
 #pragma unroll
   for (int b = 0; b < NB; ++b) w_sum[b] = f32x4{0.f, 0.f, 0.f, 0.f};
   bf16x8 qf[NB];
-  const uint32_t one2 = 0x3f803f80u;
-  const bf16x8 ones = __builtin_bit_cast(bf16x8, u32x4{one2, one2, one2, one2});
+  const uint32_t one2 = 0x3c003c00u;
+  const f16x8 ones = __builtin_bit_cast(f16x8, u32x4{one2, one2, one2, one2});
   f32x4 c0[NB];
-  const CodeBits codes_bf16;
+  const CodeBits codes;
   const int k_addr = HD == 128 ? n * RB + 16 * (g ^ k_swz(n))
                                : n * RB + 16 * ((g >> 1) ^ k_swz(n)) + 8 * (g & 1);
   const int vt = 16 * (n >> 2 & 1) + 4 * g + (n & 3);
   const int v_addr = T::CODES + vt * RB + 8 * (n >> 3), v_place = v_swz(vt);
   const int s_addr = 2 * T::CODES + 4 * g * 2 * NB;  // scales of tokens 4 g ..
+
+  // Scales of V are below the fp16 number of the bits v_limit, a power of two 2^e, and so
+  // weights times them below 2^(score - ref + e): scores up to ref + room leave ref where it is.
+  constexpr int PAIRS = T::SCALES / 4;
+  uint16_t v_limit = 0x400;
+  float room = TOP + LAG + 14.f;
 
   auto compute = [&](auto plain, const lds_u8* __restrict__ buf, int base, bool bad) {
     // scales of tokens 16 t + 4 g + i, block b: fp16 i * NB + b
@@ -244,7 +268,7 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
       for (int i = 0; i < 4; ++i) p[t][i] = 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const f32x4 s = mfma(codes_bf16(kw[b]), qf[b], c0[b]);
+        const f32x4 s = mfma(codes.bf16(kw[b]), qf[b], c0[b]);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           p[t][i] = fmaf(half_of(dk[(i * NB + b) / 2], (i * NB + b) & 1), s[i], p[t][i]);
@@ -260,14 +284,26 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
           p[t][i] = 16 * t + i < left ? x : -INFINITY;
         }
     }
+    // Two of V's scales a lane, those of the tile once: whether one is past the largest so far
+    // (an unseen token's, an infinity and a NaN do not count).
+    uint32_t sizes = *(const lds_u32*)(buf + 2 * T::CODES + T::SCALES + 4 * (lane % PAIRS));
+    sizes &= 0x7fff7fffu;
+    if constexpr (!plain) sizes = lane % PAIRS * 2 / NB < it.to - base ? sizes : 0u;
+    const u16x2 past = __builtin_bit_cast(u16x2, sizes) - u16x2{v_limit, v_limit};
+    const bool larger = __builtin_elementwise_min(past[0], past[1]) < (uint16_t)(0x7c00 - v_limit);
     float mx = p[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) mx = fmaxf(mx, p[t][i]);
     mx = xor_max<32>(xor_max<16>(mx)) * A.scale_log2;
-    if (__builtin_amdgcn_ballot_w64(mx > ref + LAG)) {
-      const float next = fmaxf(ref, mx);
+    if (__builtin_amdgcn_ballot_w64(mx > ref + room || larger)) {
+      const int lo = sizes & 0xffff, hi = sizes >> 16;
+      const int most = wave_max_i32(max(lo < 0x7c00 ? lo : 0, hi < 0x7c00 ? hi : 0));
+      v_limit = (uint16_t)__builtin_amdgcn_readfirstlane(max((int)v_limit, (most & 0x7c00) + 0x400));
+      const float above = (float)(v_limit >> 10) - 15.f;
+      room = TOP + LAG - above;
+      const float next = fmaxf(ref, mx + above - TOP);
       const float alpha = __builtin_amdgcn_exp2f(ref - next);
       ref = next;
       l *= alpha;
@@ -300,15 +336,15 @@ __device__ __forceinline__ void q4_attend(const Q4Args& A, const Q4Item& it, int
       for (int i = 0; i < 4; ++i) {
         const int e = i * NB + b;
         // (one instruction with the conversion, where a product alone would be two)
-        x[i] = cvt_pk_bf16(fmaf(p[0][i], half_of(dv[0][e / 2], e & 1), codes_bf16.zero),
-                           fmaf(p[1][i], half_of(dv[1][e / 2], e & 1), codes_bf16.zero));
+        x[i] = cvt_pk_f16(fmaf(p[0][i], half_of(dv[0][e / 2], e & 1), codes.zero),
+                          fmaf(p[1][i], half_of(dv[1][e / 2], e & 1), codes.zero));
       }
-      const bf16x8 w = __builtin_bit_cast(bf16x8, x);
+      const f16x8 w = __builtin_bit_cast(f16x8, x);
       w_sum[b] = mfma(ones, w, w_sum[b]);
       const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
           (lds_i32x2*)(buf + v_addr + 16 * (b ^ v_place)));
-      o[2 * b] = mfma(codes_bf16((uint32_t)v[0]), w, o[2 * b]);
-      o[2 * b + 1] = mfma(codes_bf16((uint32_t)v[1]), w, o[2 * b + 1]);
+      o[2 * b] = mfma(codes.f16((uint32_t)v[0]), w, o[2 * b]);
+      o[2 * b + 1] = mfma(codes.f16((uint32_t)v[1]), w, o[2 * b + 1]);
     }
   };
 

@@ -1038,8 +1038,8 @@ def q4_attention(q: torch.Tensor, cache: Q4KVCache, block_table: torch.Tensor,
     """prompt_attention over a cache in 4 bits: sequence r's queries are the rows
     query_start_loc[r]..query_start_loc[r + 1] of q [tokens, n_q, hd] (tokens may be
     strided), the last of its seq_lens[r] tokens.  Without query_start_loc row r is
-    sequence r's newest token: a decode step.  Of few rows the cache's values are not
-    rounded; prompts round them to fp16.  Rows of no sequence are left as they are in
+    sequence r's newest token: a decode step.  Weights are rounded to fp16, and of
+    prompts the cache's values.  Rows of no sequence are left as they are in
     `out`.  Without `workspace` (q4_attention_workspace) one is allocated where the call
     needs it."""
     if not (isinstance(q, torch.Tensor) and q.is_cuda and q.dtype is BF16 and q.dim() == 3):

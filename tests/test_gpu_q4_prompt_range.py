@@ -80,7 +80,7 @@ class Rows:
         return [torch.cat(x) for x in zip(*outs)]
 
 
-@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
 def test_the_outputs_rounding_is_what_counts(case):
     """N(0, 1): roundings to fp16, of K, V and the weights, are an eighth of the outputs' own to
     bf16 each, and independent of them: together 1.03 times those alone, below 1.15."""
@@ -93,7 +93,7 @@ def test_the_outputs_rounding_is_what_counts(case):
 
 
 @pytest.mark.parametrize("kind", ["plain", "large", "small"])
-@pytest.mark.parametrize("case", CASES, ids=str)
+@pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
 def test_values_of_any_size(case, kind):
     """Element by element: the outputs' rounding; the weights' and V's to fp16 and what fp32 adds
     (FP32); K's, which moves a score by F16 top at most, and a weight with the sum's change by
